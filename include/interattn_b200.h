@@ -169,6 +169,11 @@ const char* ia_last_error_string(void);
 #define IA_DEV_STATUS_GEMM_WAIT 2
 #define IA_DEV_STATUS_PEER_WAIT 4
 #define IA_DEV_STATUS_BAD_INDEX 8
+/*   IA_DEV_STATUS_NO_PAGES     ia_pages_extend or ia_pages_fork found fewer free pages than the list wants: the
+ *                              entries from the first one on that does not fit were left as they were
+ *   IA_DEV_STATUS_ATTEND_WAIT  a bounded wait inside the dense attention kernels ran out: that output is invalid */
+#define IA_DEV_STATUS_NO_PAGES 16
+#define IA_DEV_STATUS_ATTEND_WAIT 32
 int ia_read_device_status(int* out);
 
 /* Replaces _build_prompt_blocks (IMPL/core.py:449-500): one pass over the K/V
@@ -513,6 +518,88 @@ int ia_llama_rope_append_parts(const void* parts, int k, const void* cos_table, 
 int ia_llama_silu_mul_parts(const void* parts, int k, void* out, int n_rows, int intermediate, ia_stream_t stream);
 int ia_llama_argmax_parts(const void* parts, int k, void* logits, int n_rows, int vocab, int64_t* out,
                           ia_stream_t stream);
+
+/* ---- dense attention: whole prompts, and single tokens of sequences that share a prefix --------------------------------
+ * No counterpart in the reference, whose prefill and dense layers are torch's scaled_dot_product_attention on one
+ * sequence at a time (IMPL/core.py:115-123, 1276-1290).  Scale 1 / sqrt(head_dim), softmax statistics and sums in fp32.
+ * Values in places that a row does not see never reach it, be they infinite or NaN. */
+
+/* The prompt's work, cut and spread over the SMs once for a batch (host arithmetic; q_lens, kv_lens and items are host
+ * memory).  Sequence i has q_lens[i] query tokens and kv_lens[i] >= 0 keys; its query token t sees the first
+ * kv_lens[i] - q_lens[i] + t + 1 keys (none: zeros come out).  Writes ia_prompt_plan_ints() int32 words that
+ * ia_prompt_attention reads on the device; the plan holds for one dtype, group size and number of kv heads, on devices
+ * with as many SMs as the current one. */
+int64_t ia_prompt_plan_ints(const int32_t* q_lens, const int32_t* kv_lens, int n_seqs, int n_kv_heads, int group_size, int head_dim,
+                            int dtype);
+int ia_prompt_plan(const int32_t* q_lens, const int32_t* kv_lens, int n_seqs, int n_kv_heads, int group_size, int head_dim,
+                   int dtype, int32_t* plan, int64_t plan_ints);
+
+typedef struct ia_prompt_tensors {
+  const void *q, *k, *v; /* [tokens, heads, head_dim], packed sequence after sequence; 16-byte aligned */
+  void* out;             /* [q tokens, query heads, head_dim] contiguous, 16-byte aligned */
+  float* lse;            /* [q tokens, query heads] natural log-sum-exp, -inf for rows without keys; may be null */
+  int64_t q_tok_stride, q_head_stride, k_tok_stride, k_head_stride, v_tok_stride, v_head_stride; /* elements; multiples of
+                            16 bytes, head_dim elements contiguous */
+  int32_t n_q_tokens, n_kv_tokens, n_kv_heads, group_size, head_dim, dtype;
+} ia_prompt_tensors;
+/* plan_host: the first 8 words of the plan (host memory); plan_device: all of it. */
+int ia_prompt_attention(const ia_prompt_tensors* tensors, const int32_t* plan_host, const int32_t* plan_device,
+                        ia_stream_t stream);
+
+/* One decode step in which consecutive sequences form groups whose first tokens lie in the same pages: those are read
+ * once for all query rows of the group.  Sequence b sees its first seq_lens[b] tokens through its own, complete table row;
+ * of group g the first shared_lens[g] tokens, rounded down to whole pages, are read through the row of the group's longest
+ * sequence (members may have left: a sequence of length 0 is never read and gives zeros).  An entry outside [0, n_pool_pages) is never dereferenced, reports
+ * IA_DEV_STATUS_BAD_INDEX and makes the output of the sequences that use it meaningless.
+ *   group_sizes  int32 [n_groups], host memory, adding up to geom->batch
+ *   plan         ia_shared_prefix_plan_ints() int32 words that ia_shared_prefix_plan fills (host); the step reads a device
+ *                copy.  Lengths are read on the device by every step.
+ *   workspace    ia_shared_prefix_workspace_bytes(), 16-byte aligned; calls that overlap on the GPU need their own. */
+int64_t ia_shared_prefix_plan_ints(const int32_t* group_sizes, int n_groups, const ia_geom* geom);
+int ia_shared_prefix_plan(const int32_t* group_sizes, int n_groups, const ia_geom* geom, int32_t* plan, int64_t plan_ints);
+int64_t ia_shared_prefix_workspace_bytes(int n_shared_parts, const ia_geom* geom);
+/* n_shared_parts: word 0 of the plan */
+int ia_shared_prefix_decode(const void* q, const void* k_pool, const void* v_pool, const int32_t* block_table,
+                            const int32_t* seq_lens, const int32_t* shared_lens, const int32_t* plan_device,
+                            int n_shared_parts, const ia_geom* geom, void* workspace, int64_t workspace_bytes, void* out,
+                            ia_stream_t stream);
+
+/* ---- pages of a cache that sequences share ---------------------------------------------------------------------------
+ * No counterpart in the reference (one sequence, one contiguous cache).  All state is device memory and every call is
+ * ordered by its stream alone, so a loop that admits, forks and frees sequences can be captured.  refs[p] counts the
+ * table entries that hold page p (plus whatever the caller added for its own purposes); 0 = free.  Free pages are handed
+ * out lowest first, in the order of the list.  A list names a row once: a second mention, a row or count out of range is
+ * refused for that entry alone with IA_DEV_STATUS_BAD_INDEX.  All layers share the table: pools holds the base
+ * addresses of every layer's key and value pool. */
+typedef struct ia_page_cache {
+  int32_t* block_table;  /* [n_rows, max_pages] */
+  int32_t* seq_lens;     /* [n_rows] */
+  int32_t* refs;         /* [n_pages] */
+  void* const* pools;    /* [n_pools] device array of device addresses, 16-byte aligned each */
+  void* scratch;         /* ia_pages_scratch_bytes(), 256-byte aligned; one per cache */
+  int64_t scratch_bytes;
+  int64_t page_stride, head_stride;  /* elements */
+  int32_t n_rows, max_pages, n_pages, n_pools, n_kv_heads, head_dim, dtype;
+  int32_t reserved;      /* 0 */
+} ia_page_cache;
+int64_t ia_pages_scratch_bytes(int n_rows, int n_pages);
+/* rows[i] gets n_tokens[i] more tokens: pages as needed, the new length.  The tokens themselves are written by
+ * ia_pages_write. */
+int ia_pages_extend(const ia_page_cache* cache, const int32_t* rows, const int32_t* n_tokens, int n, ia_stream_t stream);
+/* Keys and values of one layer: tokens [starts[i], starts[i + 1]) of k, v [n_tokens, n_kv_heads, head_dim] become the last
+ * tokens of rows[i].  starts int32 [n + 1] ascending.  Strides in elements, multiples of 16 bytes. */
+int ia_pages_write(const ia_page_cache* cache, const int32_t* rows, const int32_t* starts, int n, const void* k, const void* v,
+                   int64_t k_tok_stride, int64_t k_head_stride, int64_t v_tok_stride, int64_t v_head_stride, int n_tokens,
+                   void* k_pool, void* v_pool, ia_stream_t stream);
+/* children[i], an empty row, becomes a copy of parents[i] as it was before the call: with `share` its whole pages are the
+ * parent's and a partly filled last page is copied in all pools, otherwise every page is copied. */
+int ia_pages_fork(const ia_page_cache* cache, const int32_t* parents, const int32_t* children, int n, int share,
+                  ia_stream_t stream);
+/* The rows become empty; pages that no row holds any more are free. */
+int ia_pages_free(const ia_page_cache* cache, const int32_t* rows, int n, ia_stream_t stream);
+/* All pages in use move to the front of the pools: the i-th page in use at or past their number goes to the i-th free one
+ * below it, table entries follow. */
+int ia_pages_compact(const ia_page_cache* cache, ia_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -30,6 +30,7 @@ IA_REP_SPARSE_ONLY, IA_REP_HYBRID = 0, 1
 ABI_VERSION = 3
 # masks of the device status word (ia_read_device_status)
 IA_DEV_STATUS_SELECT_WAIT, IA_DEV_STATUS_GEMM_WAIT, IA_DEV_STATUS_PEER_WAIT, IA_DEV_STATUS_BAD_INDEX = 1, 2, 4, 8
+IA_DEV_STATUS_NO_PAGES, IA_DEV_STATUS_ATTEND_WAIT = 16, 32
 
 
 class Geom(Structure):
@@ -67,6 +68,21 @@ class PeerExchange(Structure):
 class SelectExchange(Structure):
     _fields_ = [("n_ranks", c_int32), ("my_rank", c_int32), ("norm", c_void_p * 8), ("cand", c_void_p * 8),
                 ("flags", c_void_p * 8), ("step_counter", c_void_p), ("grid_counter", c_void_p)]
+
+
+class PromptTensors(Structure):
+    _fields_ = [("q", c_void_p), ("k", c_void_p), ("v", c_void_p), ("out", c_void_p), ("lse", c_void_p),
+                ("q_tok_stride", c_int64), ("q_head_stride", c_int64), ("k_tok_stride", c_int64),
+                ("k_head_stride", c_int64), ("v_tok_stride", c_int64), ("v_head_stride", c_int64),
+                ("n_q_tokens", c_int32), ("n_kv_tokens", c_int32), ("n_kv_heads", c_int32), ("group_size", c_int32),
+                ("head_dim", c_int32), ("dtype", c_int32)]
+
+
+class PageCacheState(Structure):
+    _fields_ = [("block_table", c_void_p), ("seq_lens", c_void_p), ("refs", c_void_p), ("pools", c_void_p),
+                ("scratch", c_void_p), ("scratch_bytes", c_int64), ("page_stride", c_int64), ("head_stride", c_int64),
+                ("n_rows", c_int32), ("max_pages", c_int32), ("n_pages", c_int32), ("n_pools", c_int32),
+                ("n_kv_heads", c_int32), ("head_dim", c_int32), ("dtype", c_int32), ("reserved", c_int32)]
 
 
 # name -> (restype, argtypes); mirrors include/interattn_b200.h one to one
@@ -127,6 +143,21 @@ SIGNATURES = {
                                            c_int64, c_int64, c_int, c_void_p, c_int, c_int, c_int, c_int, c_void_p]),
     "ia_llama_silu_mul_parts": (c_int, [c_void_p, c_int, c_void_p, c_int, c_int, c_void_p]),
     "ia_llama_argmax_parts": (c_int, [c_void_p, c_int, c_void_p, c_int, c_int, c_void_p, c_void_p]),
+    "ia_prompt_plan_ints": (c_int64, [c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int]),
+    "ia_prompt_plan": (c_int, [c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p, c_int64]),
+    "ia_prompt_attention": (c_int, [POINTER(PromptTensors), c_void_p, c_void_p, c_void_p]),
+    "ia_shared_prefix_plan_ints": (c_int64, [c_void_p, c_int, POINTER(Geom)]),
+    "ia_shared_prefix_plan": (c_int, [c_void_p, c_int, POINTER(Geom), c_void_p, c_int64]),
+    "ia_shared_prefix_workspace_bytes": (c_int64, [c_int, POINTER(Geom)]),
+    "ia_shared_prefix_decode": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int,
+                                        POINTER(Geom), c_void_p, c_int64, c_void_p, c_void_p]),
+    "ia_pages_scratch_bytes": (c_int64, [c_int, c_int]),
+    "ia_pages_extend": (c_int, [POINTER(PageCacheState), c_void_p, c_void_p, c_int, c_void_p]),
+    "ia_pages_write": (c_int, [POINTER(PageCacheState), c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int64, c_int64,
+                               c_int64, c_int64, c_int, c_void_p, c_void_p, c_void_p]),
+    "ia_pages_fork": (c_int, [POINTER(PageCacheState), c_void_p, c_void_p, c_int, c_int, c_void_p]),
+    "ia_pages_free": (c_int, [POINTER(PageCacheState), c_void_p, c_int, c_void_p]),
+    "ia_pages_compact": (c_int, [POINTER(PageCacheState), c_void_p]),
     "ia_llama_gemm": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_int64, c_void_p]),
 }
 

@@ -6,8 +6,10 @@
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
+#include <exception>
 
-#include "ia_common.cuh"
+#include "dense_attention.cuh"
+#include "page_cache.cuh"
 
 namespace ia {
 
@@ -616,6 +618,228 @@ int ia_decode_attention_noalloc(const void* q, const void* k_pool, const void* v
   return decode_attention_impl(q, k_pool, v_pool, block_table, prefix_lens, seq_lens, summaries, geom, mode, top_k,
                                eps, max_sel, rep_mode, n_splits, scratch, need, nullptr, nullptr, out, nullptr,
                                stream);
+}
+
+// ---- dense attention --------------------------------------------------------------------------------------------------
+
+static int check_prompt_lens(const int32_t* q_lens, const int32_t* kv_lens, int n_seqs, int n_kv_heads, int group, int head_dim,
+                             int dtype) {
+  if (n_seqs < 0 || (n_seqs > 0 && (!q_lens || !kv_lens))) return fail(IA_ERR_BAD_ARG, "prompt_plan: lengths");
+  if (n_kv_heads <= 0 || n_kv_heads > 65535 || group <= 0) return fail(IA_ERR_BAD_ARG, "prompt_plan: %d kv heads, group %d", n_kv_heads, group);
+  if (group > 16) return fail(IA_ERR_UNSUPPORTED, "prompt_plan: group size %d (built: up to 16)", group);
+  if (head_dim != 64 && head_dim != 128) return fail(IA_ERR_UNSUPPORTED, "prompt_plan: head_dim %d (built: 64, 128)", head_dim);
+  if (dtype != IA_F32 && dtype != IA_BF16) return fail(IA_ERR_BAD_ARG, "prompt_plan: dtype %d", dtype);
+  int64_t q = 0, k = 0;
+  for (int i = 0; i < n_seqs; ++i) {
+    if (q_lens[i] < 0 || kv_lens[i] < 0)
+      return fail(IA_ERR_BAD_ARG, "prompt_plan: sequence %d has %d query tokens and %d keys", i, q_lens[i], kv_lens[i]);
+    q += q_lens[i];
+    k += kv_lens[i];
+  }
+  if (q > 0x7fffffff || k > 0x7fffffff) return fail(IA_ERR_UNSUPPORTED, "prompt_plan: more than 2^31 - 1 tokens");
+  return IA_OK;
+}
+
+int64_t ia_prompt_plan_ints(const int32_t* q_lens, const int32_t* kv_lens, int n_seqs, int n_kv_heads, int group_size,
+                            int head_dim, int dtype) {
+  if (check_prompt_lens(q_lens, kv_lens, n_seqs, n_kv_heads, group_size, head_dim, dtype)) return -1;
+  const int64_t n = prompt_plan_ints(q_lens, n_seqs, n_kv_heads, group_size, dtype);
+  if (n < 0) fail(IA_ERR_UNSUPPORTED, "prompt_plan: too many pieces");
+  return n;
+}
+
+int ia_prompt_plan(const int32_t* q_lens, const int32_t* kv_lens, int n_seqs, int n_kv_heads, int group_size, int head_dim,
+                   int dtype, int32_t* plan, int64_t plan_ints) {
+  if (int s = check_prompt_lens(q_lens, kv_lens, n_seqs, n_kv_heads, group_size, head_dim, dtype)) return s;
+  if (!plan) return fail(IA_ERR_BAD_ARG, "prompt_plan: null argument");
+  try {
+    return make_prompt_plan(q_lens, kv_lens, n_seqs, n_kv_heads, group_size, head_dim, dtype, plan, plan_ints);
+  } catch (const std::exception&) {
+    return fail(IA_ERR_UNSUPPORTED, "prompt_plan: out of host memory");
+  }
+}
+
+static bool strides_ok(int64_t tok, int64_t head, int head_dim, int size) {
+  return tok >= head_dim && head >= head_dim && (tok * size) % 16 == 0 && (head * size) % 16 == 0;
+}
+
+int ia_prompt_attention(const ia_prompt_tensors* t, const int32_t* plan_host, const int32_t* plan_device, ia_stream_t stream) {
+  if (!t || !plan_host || !plan_device) return fail(IA_ERR_BAD_ARG, "prompt_attention: null argument");
+  if (plan_host[4] != t->group_size * 1000 + t->head_dim || plan_host[5] != t->n_kv_heads * 16 + t->dtype)
+    return fail(IA_ERR_BAD_ARG, "prompt_attention: the plan was made for other heads or another dtype");
+  if (plan_host[6] != t->n_q_tokens || plan_host[7] != t->n_kv_tokens)
+    return fail(IA_ERR_BAD_ARG, "prompt_attention: %d query tokens and %d keys, the plan has %d and %d", t->n_q_tokens,
+                t->n_kv_tokens, plan_host[6], plan_host[7]);
+  if (plan_host[0] == 0) return IA_OK;
+  if (!t->q || !t->out || (t->n_kv_tokens > 0 && (!t->k || !t->v)))
+    return fail(IA_ERR_BAD_ARG, "prompt_attention: null argument");
+  if (!aligned16(t->q) || !aligned16(t->k) || !aligned16(t->v) || !aligned16(t->out))
+    return fail(IA_ERR_BAD_ARG, "prompt_attention: tensors must be 16-byte aligned");
+  const int size = t->dtype == IA_BF16 ? 2 : 4;
+  if (!strides_ok(t->q_tok_stride, t->q_head_stride, t->head_dim, size) ||
+      (t->n_kv_tokens > 0 && (!strides_ok(t->k_tok_stride, t->k_head_stride, t->head_dim, size) ||
+                              !strides_ok(t->v_tok_stride, t->v_head_stride, t->head_dim, size))))
+    return fail(IA_ERR_BAD_ARG, "prompt_attention: token and head strides are multiples of 16 bytes and hold a head");
+  const PromptTensors p{t->q, t->k, t->v, t->out, t->lse, t->q_tok_stride, t->q_head_stride, t->k_tok_stride, t->k_head_stride,
+                        t->v_tok_stride, t->v_head_stride, t->n_q_tokens, t->n_kv_tokens, t->n_kv_heads, t->group_size};
+  return launch_prompt_fma(p, t->dtype, t->head_dim, reinterpret_cast<const PromptItem*>(plan_device + plan_host[3]),
+                           plan_host[0], plan_host[2] != 0, (cudaStream_t)stream);
+}
+
+static int check_groups(const int32_t* group_sizes, int n_groups, const ia_geom* g) {
+  if (int s = check_geom(g)) return s;
+  if (n_groups < 0 || (n_groups > 0 && !group_sizes)) return fail(IA_ERR_BAD_ARG, "shared_prefix: groups");
+  int64_t n = 0;
+  for (int i = 0; i < n_groups; ++i) {
+    if (group_sizes[i] <= 0) return fail(IA_ERR_BAD_ARG, "shared_prefix: group %d has %d sequences", i, group_sizes[i]);
+    n += group_sizes[i];
+  }
+  if (n != g->batch) return fail(IA_ERR_BAD_ARG, "shared_prefix: the groups hold %lld sequences, the batch %d", (long long)n, g->batch);
+  if ((int64_t)g->max_pages * g->page_size > 0x7fffffff) return fail(IA_ERR_UNSUPPORTED, "shared_prefix: max_pages %d", g->max_pages);
+  return IA_OK;
+}
+
+int64_t ia_shared_prefix_plan_ints(const int32_t* group_sizes, int n_groups, const ia_geom* geom) {
+  if (check_groups(group_sizes, n_groups, geom)) return -1;
+  return 8 + 8 * (shared_parts(group_sizes, n_groups, geom->group_size) + geom->batch) + 2 * (int64_t)geom->batch;
+}
+
+int ia_shared_prefix_plan(const int32_t* group_sizes, int n_groups, const ia_geom* geom, int32_t* plan, int64_t plan_ints) {
+  const int64_t need = ia_shared_prefix_plan_ints(group_sizes, n_groups, geom);
+  if (need < 0) return IA_ERR_BAD_ARG;
+  if (!plan || plan_ints < need) return fail(IA_ERR_BAD_ARG, "shared_prefix_plan: %lld words, %lld needed", (long long)plan_ints, (long long)need);
+  make_shared_plan(group_sizes, n_groups, geom->batch, geom->group_size, plan);
+  return IA_OK;
+}
+
+// partial outputs and their log-sum-exps: a slot per (item, CTA) that can occur
+static int64_t carve_shared(int n_shared, const ia_geom& g, char* base, SharedParams* p) {
+  const int64_t slots_shared = n_shared > 0 ? (int64_t)n_shared * g.n_kv_heads + shared_ctas() : 0;
+  const int64_t slots_own = (int64_t)g.batch * g.n_kv_heads + shared_ctas();
+  int64_t off = 0;
+  auto take = [&](int64_t bytes) {
+    char* r = base ? base + off : nullptr;
+    off += align256(bytes);
+    return r;
+  };
+  char* a[4] = {take(slots_shared * shared_row_block() * g.head_dim * 4), take(slots_shared * shared_row_block() * 4),
+                take(slots_own * g.group_size * g.head_dim * 4), take(slots_own * g.group_size * 4)};
+  if (p) {
+    p->o_shared = (float*)a[0];
+    p->lse_shared = (float*)a[1];
+    p->o_own = (float*)a[2];
+    p->lse_own = (float*)a[3];
+  }
+  return off;
+}
+
+int64_t ia_shared_prefix_workspace_bytes(int n_shared_parts, const ia_geom* geom) {
+  if (check_geom(geom)) return -1;
+  if (n_shared_parts < 0 || n_shared_parts > geom->batch) {
+    fail(IA_ERR_BAD_ARG, "shared_prefix: %d shared parts for %d sequences", n_shared_parts, geom->batch);
+    return -1;
+  }
+  return carve_shared(n_shared_parts, *geom, nullptr, nullptr);
+}
+
+int ia_shared_prefix_decode(const void* q, const void* k_pool, const void* v_pool, const int32_t* block_table,
+                            const int32_t* seq_lens, const int32_t* shared_lens, const int32_t* plan_device, int n_shared_parts,
+                            const ia_geom* geom, void* workspace, int64_t workspace_bytes, void* out, ia_stream_t stream) {
+  if (int s = check_geom(geom)) return s;
+  if (geom->batch == 0) return IA_OK;
+  const int64_t need = ia_shared_prefix_workspace_bytes(n_shared_parts, geom);
+  if (need < 0) return IA_ERR_BAD_ARG;
+  if (!q || !k_pool || !v_pool || !block_table || !seq_lens || !shared_lens || !plan_device || !workspace || !out)
+    return fail(IA_ERR_BAD_ARG, "shared_prefix_decode: null argument");
+  if (!aligned16(q) || !aligned16(k_pool) || !aligned16(v_pool) || !aligned16(workspace) || !aligned16(out))
+    return fail(IA_ERR_BAD_ARG, "shared_prefix_decode: tensors must be 16-byte aligned");
+  if (workspace_bytes < need)
+    return fail(IA_ERR_BAD_ARG, "shared_prefix_decode: workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)need);
+  SharedParams p{};
+  p.q = q; p.k_pool = k_pool; p.v_pool = v_pool;
+  p.block_table = block_table; p.seq_lens = seq_lens; p.shared_lens = shared_lens;
+  p.entities = reinterpret_cast<const SharedEntity*>(plan_device + 8);
+  carve_shared(n_shared_parts, *geom, static_cast<char*>(workspace), &p);
+  p.status = device_status_address();
+  if (p.status == nullptr) return IA_ERR_LAUNCH;
+  p.page_stride = geom->pool_page_stride; p.head_stride = geom->pool_head_stride;
+  p.n_shared = n_shared_parts; p.batch = geom->batch; p.n_kv_heads = geom->n_kv_heads; p.group = geom->group_size;
+  p.max_pages = geom->max_pages; p.n_pool_pages = geom->n_pool_pages; p.row_block = shared_row_block();
+  if (int s = launch_shared_fma(p, geom->dtype, geom->head_dim, shared_ctas(), (cudaStream_t)stream)) return s;
+  return launch_shared_merge(p, plan_device + 8 + 8 * ((int64_t)n_shared_parts + geom->batch), geom->head_dim, geom->dtype,
+                             shared_ctas(), out, (cudaStream_t)stream);
+}
+
+// ---- pages of a cache -------------------------------------------------------------------------------------------------
+
+static int check_cache(const ia_page_cache* c, int n, const char* what) {
+  if (!c || !c->block_table || !c->seq_lens || !c->refs || !c->scratch || (c->n_pools > 0 && !c->pools))
+    return fail(IA_ERR_BAD_ARG, "%s: null argument", what);
+  if (c->n_rows <= 0 || c->max_pages <= 0 || c->n_pages <= 0 || c->n_pools < 0 || c->n_kv_heads <= 0 || c->reserved != 0)
+    return fail(IA_ERR_BAD_ARG, "%s: %d rows of %d pages, pool of %d, %d pools, %d kv heads", what, c->n_rows, c->max_pages,
+                c->n_pages, c->n_pools, c->n_kv_heads);
+  if ((int64_t)c->n_rows * c->max_pages > 0x7fffffff || c->max_pages > 0x7fffffff / 16)
+    return fail(IA_ERR_UNSUPPORTED, "%s: a table of %d x %d entries", what, c->n_rows, c->max_pages);
+  if (c->dtype != IA_F32 && c->dtype != IA_BF16) return fail(IA_ERR_BAD_ARG, "%s: dtype %d", what, c->dtype);
+  if (c->head_dim != 64 && c->head_dim != 128) return fail(IA_ERR_UNSUPPORTED, "%s: head_dim %d (built: 64, 128)", what, c->head_dim);
+  const int64_t run = 16 * (int64_t)c->head_dim, size = c->dtype == IA_BF16 ? 2 : 4;
+  if (c->page_stride < run || c->head_stride < run || (c->page_stride * size) % 16 != 0 || (c->head_stride * size) % 16 != 0)
+    return fail(IA_ERR_BAD_ARG, "%s: pool strides (%lld, %lld)", what, (long long)c->page_stride, (long long)c->head_stride);
+  if ((reinterpret_cast<uintptr_t>(c->scratch) & 255u) != 0 || c->scratch_bytes < page_cache_scratch_bytes(c->n_rows, c->n_pages))
+    return fail(IA_ERR_BAD_ARG, "%s: scratch", what);
+  if (n < 0 || n > c->n_rows) return fail(IA_ERR_BAD_ARG, "%s: a list of %d entries for %d rows", what, n, c->n_rows);
+  return IA_OK;
+}
+
+int64_t ia_pages_scratch_bytes(int n_rows, int n_pages) {
+  if (n_rows <= 0 || n_pages <= 0) {
+    fail(IA_ERR_BAD_ARG, "pages_scratch_bytes: %d rows, %d pages", n_rows, n_pages);
+    return -1;
+  }
+  return page_cache_scratch_bytes(n_rows, n_pages);
+}
+
+int ia_pages_extend(const ia_page_cache* c, const int32_t* rows, const int32_t* n_tokens, int n, ia_stream_t stream) {
+  if (int s = check_cache(c, n, "pages_extend")) return s;
+  if (n == 0) return IA_OK;
+  if (!rows || !n_tokens) return fail(IA_ERR_BAD_ARG, "pages_extend: null argument");
+  return launch_pages_extend(*c, rows, n_tokens, n, (cudaStream_t)stream);
+}
+
+int ia_pages_write(const ia_page_cache* c, const int32_t* rows, const int32_t* starts, int n, const void* k, const void* v,
+                   int64_t k_tok_stride, int64_t k_head_stride, int64_t v_tok_stride, int64_t v_head_stride, int n_tokens,
+                   void* k_pool, void* v_pool, ia_stream_t stream) {
+  if (int s = check_cache(c, n, "pages_write")) return s;
+  if (n_tokens < 0) return fail(IA_ERR_BAD_ARG, "pages_write: %d tokens", n_tokens);
+  if (n == 0 || n_tokens == 0) return IA_OK;
+  if (!rows || !starts || !k || !v || !k_pool || !v_pool) return fail(IA_ERR_BAD_ARG, "pages_write: null argument");
+  if (!aligned16(k) || !aligned16(v) || !aligned16(k_pool) || !aligned16(v_pool))
+    return fail(IA_ERR_BAD_ARG, "pages_write: tensors must be 16-byte aligned");
+  const int size = c->dtype == IA_BF16 ? 2 : 4;
+  if (!strides_ok(k_tok_stride, k_head_stride, c->head_dim, size) || !strides_ok(v_tok_stride, v_head_stride, c->head_dim, size))
+    return fail(IA_ERR_BAD_ARG, "pages_write: token and head strides are multiples of 16 bytes and hold a head");
+  return launch_pages_write(*c, rows, starts, n,
+                            PagesWrite{k, v, k_pool, v_pool, k_tok_stride, k_head_stride, v_tok_stride, v_head_stride, n_tokens},
+                            (cudaStream_t)stream);
+}
+
+int ia_pages_fork(const ia_page_cache* c, const int32_t* parents, const int32_t* children, int n, int share, ia_stream_t stream) {
+  if (int s = check_cache(c, n, "pages_fork")) return s;
+  if (n == 0) return IA_OK;
+  if (!parents || !children) return fail(IA_ERR_BAD_ARG, "pages_fork: null argument");
+  return launch_pages_fork(*c, parents, children, n, share != 0, (cudaStream_t)stream);
+}
+
+int ia_pages_free(const ia_page_cache* c, const int32_t* rows, int n, ia_stream_t stream) {
+  if (int s = check_cache(c, n, "pages_free")) return s;
+  if (n == 0) return IA_OK;
+  if (!rows) return fail(IA_ERR_BAD_ARG, "pages_free: null argument");
+  return launch_pages_free(*c, rows, n, (cudaStream_t)stream);
+}
+
+int ia_pages_compact(const ia_page_cache* c, ia_stream_t stream) {
+  if (int s = check_cache(c, 0, "pages_compact")) return s;
+  return launch_pages_compact(*c, (cudaStream_t)stream);
 }
 
 }  // extern "C"

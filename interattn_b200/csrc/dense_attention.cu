@@ -1,0 +1,538 @@
+// Dense attention on the CUDA cores, the merge of the shared-prefix decode step, and the host side of the prompt's plan.
+//
+//   o_r = sum_{j < limit_r} softmax_j(q_r . k_j / sqrt(D)) v_j
+//
+// One pass over the keys in tiles of 64 with the running maximum m and sum l of each row: a tile's logits go from
+// registers through shared memory into the second product, the accumulator is rescaled by exp(m_old - m_new) when the
+// maximum moves.  All of it in fp32.  A thread owns RPT rows x 4 keys of the logits and RPT rows x D / 16 output columns;
+// 16 neighbouring lanes share a row, so the row's statistics are four shuffles.  Rows of 132 floats keep the key reads of
+// 8 lanes on 32 banks.
+#include <algorithm>
+#include <atomic>
+#include <vector>
+
+#include "dense_attention.cuh"
+
+namespace ia {
+namespace {
+
+constexpr int kThreads = 256, kKeys = 64, kPLd = kKeys + 4;
+
+template <int D, int RPT> struct Smem {
+  static constexpr int rows = 16 * RPT, ld = D + 4;
+  static constexpr int q = 0, k = q + rows * ld, v = k + kKeys * ld, p = v + kKeys * D, floats = p + rows * kPLd;
+  static constexpr size_t bytes = (size_t)floats * 4 + rows * 8;  // + limits and flags
+};
+
+__device__ __forceinline__ void cp_async16(void* dst, const void* src, bool valid) {
+  const int n = valid ? 16 : 0;  // 0: sixteen zero bytes, nothing is read
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src),
+               "r"(n)
+               : "memory");
+}
+// four elements as floats; zeros where not valid
+__device__ __forceinline__ void put4(float* dst, const float* src, bool valid) { cp_async16(dst, src, valid); }
+__device__ __forceinline__ void put4(float* dst, const __nv_bfloat16* src, bool valid) {
+  float x[4] = {0.f, 0.f, 0.f, 0.f};
+  if (valid) load_vec<4>(src, x);
+  store_vec<4>(dst, x);
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// rows of a [kKeys, D] tile from key j0 on; rows at or past `hi`, and rows without an address, are zero
+template <bool VALUES, int D, int LD, typename T, typename Key>
+__device__ __forceinline__ void load_tile(float* dst, const T* any, int j0, int hi, const Key& key) {
+#pragma unroll 4
+  for (int i = threadIdx.x; i < kKeys * D / 4; i += kThreads) {
+    const int row = i / (D / 4), c = i % (D / 4) * 4;
+    const T *k = any, *v = any;
+    const bool ok = j0 + row < hi && key(j0 + row, k, v);
+    put4(dst + row * LD + c, (VALUES ? v : k) + (ok ? c : 0), ok);
+  }
+}
+
+// Rows [0, n_rows) of one piece over the keys [lo, hi).  q_row(r): the row's query; limit(r): the keys below it are seen;
+// sink.row(r) -> where its outputs go.
+template <typename T, int D, int RPT, typename Key, typename QRow, typename Limit, typename Sink>
+__device__ void attend(float* sm, int n_rows, int lo, int hi, float scale_log2, const Key& key, const QRow& q_row,
+                       const Limit& limit, const Sink& sink) {
+  using S = Smem<D, RPT>;
+  constexpr int ROWS = S::rows, LD = S::ld, NO = D / 64;
+  const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
+  float *qs = sm + S::q, *ks = sm + S::k, *vs = sm + S::v, *ps = sm + S::p;
+  int* lim = reinterpret_cast<int*>(sm + S::floats);
+  int* bad = lim + ROWS;
+  const T* any = q_row(0);
+  __syncthreads();  // the piece before is done with the shared memory
+  for (int i = tid; i < ROWS * D / 4; i += kThreads) {
+    const int row = i / (D / 4), c = i % (D / 4) * 4;
+    put4(qs + row * LD + c, row < n_rows ? q_row(row) + c : any, row < n_rows);
+  }
+  load_tile<false, D, LD>(ks, any, lo, hi, key);
+  cp_commit();
+  load_tile<true, D, D>(vs, any, lo, hi, key);
+  cp_commit();
+  if (tid < ROWS) {
+    lim[tid] = tid < n_rows ? limit(tid) : 0;
+    bad[tid] = 0;
+  }
+  float o[RPT][NO][4], m[RPT], l[RPT];
+#pragma unroll
+  for (int i = 0; i < RPT; ++i) {
+    m[i] = -INFINITY;
+    l[i] = 0.f;
+#pragma unroll
+    for (int a = 0; a < NO; ++a)
+#pragma unroll
+      for (int b = 0; b < 4; ++b) o[i][a][b] = 0.f;
+  }
+  for (int j0 = lo; j0 < hi; j0 += kKeys) {
+    cp_wait<1>();
+    __syncthreads();
+    float s[RPT][4];
+#pragma unroll
+    for (int i = 0; i < RPT; ++i)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) s[i][c] = 0.f;
+#pragma unroll 2
+    for (int d = 0; d < D; d += 4) {
+      float4 kv[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) kv[c] = *reinterpret_cast<const float4*>(ks + (tx + 16 * c) * LD + d);
+#pragma unroll
+      for (int i = 0; i < RPT; ++i) {
+        const float4 qv = *reinterpret_cast<const float4*>(qs + (ty * RPT + i) * LD + d);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          s[i][c] += qv.x * kv[c].x;
+          s[i][c] += qv.y * kv[c].y;
+          s[i][c] += qv.z * kv[c].z;
+          s[i][c] += qv.w * kv[c].w;
+        }
+      }
+    }
+    __syncthreads();
+    if (j0 + kKeys < hi) load_tile<false, D, LD>(ks, any, j0 + kKeys, hi, key);
+    cp_commit();
+#pragma unroll
+    for (int i = 0; i < RPT; ++i) {
+      const int end = lim[ty * RPT + i] - j0;
+      float top = -INFINITY;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        s[i][c] = tx + 16 * c < end ? s[i][c] * scale_log2 : -INFINITY;
+        top = fmaxf(top, s[i][c]);
+      }
+#pragma unroll
+      for (int w = 8; w > 0; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+      const float m_new = fmaxf(m[i], top), base = m_new == -INFINITY ? 0.f : m_new;
+      const float keep = exp2f(m[i] - base);
+      m[i] = m_new;
+      l[i] *= keep;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const float w = exp2f(s[i][c] - base);
+        l[i] += w;
+        ps[(ty * RPT + i) * kPLd + tx + 16 * c] = w;
+      }
+#pragma unroll
+      for (int a = 0; a < NO; ++a)
+#pragma unroll
+        for (int b = 0; b < 4; ++b) o[i][a][b] *= keep;
+    }
+    cp_wait<1>();
+    __syncthreads();  // also: the row's weights are written
+#pragma unroll 2
+    for (int n = 0; n < kKeys; n += 4) {
+      float4 w[RPT];
+#pragma unroll
+      for (int i = 0; i < RPT; ++i) w[i] = *reinterpret_cast<const float4*>(ps + (ty * RPT + i) * kPLd + n);
+#pragma unroll
+      for (int k4 = 0; k4 < 4; ++k4) {
+#pragma unroll
+        for (int a = 0; a < NO; ++a) {
+          const float4 vv = *reinterpret_cast<const float4*>(vs + (n + k4) * D + tx * 4 + 64 * a);
+#pragma unroll
+          for (int i = 0; i < RPT; ++i) {
+            const float wi = k4 == 0 ? w[i].x : k4 == 1 ? w[i].y : k4 == 2 ? w[i].z : w[i].w;
+            o[i][a][0] += wi * vv.x;
+            o[i][a][1] += wi * vv.y;
+            o[i][a][2] += wi * vv.z;
+            o[i][a][3] += wi * vv.w;
+          }
+        }
+      }
+    }
+    __syncthreads();
+    if (j0 + kKeys < hi) load_tile<true, D, D>(vs, any, j0 + kKeys, hi, key);
+    cp_commit();
+  }
+  cp_wait<0>();
+  __syncthreads();  // lim is written also where there was no tile
+  bool some_bad = false;
+#pragma unroll
+  for (int i = 0; i < RPT; ++i) {
+    const int row = ty * RPT + i;
+#pragma unroll
+    for (int w = 8; w > 0; w >>= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], w);
+    if (row >= n_rows) continue;
+    const bool empty = lim[row] <= lo;
+    const float inv = empty ? 0.f : 1.f / l[i];
+    bool finite = true;
+#pragma unroll
+    for (int a = 0; a < NO; ++a) {
+      float e[4];
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        e[b] = empty ? 0.f : o[i][a][b] * inv;
+        finite &= fabsf(e[b]) <= 3.4028235e38f;
+      }
+      store_vec<4>(sink.row(row) + tx * 4 + 64 * a, e);
+    }
+    if (tx == 0 && sink.lse(row) != nullptr)
+      *sink.lse(row) = empty ? -INFINITY : (m[i] + log2f(l[i])) * kLn2;
+    if (!finite) bad[row] = 1;
+    some_bad |= !finite;
+  }
+  if (!__syncthreads_or(some_bad)) return;
+  for (int row = tid >> 5; row < n_rows; row += kThreads / 32) {
+    if (!bad[row] || last_not_finite<T, D>(max(lo, lim[row]), hi, key) < 0) continue;
+    float x[D / 32], mx, lx;
+    exact_row<T, D>(q_row(row), lo, lim[row], scale_log2, key, x, mx, lx);
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) from_f32(sink.row(row)[(tid & 31) + 32 * i], x[i] / lx);
+    if ((tid & 31) == 0 && sink.lse(row) != nullptr) *sink.lse(row) = (mx + log2f(lx)) * kLn2;
+  }
+}
+
+template <typename O> struct RowSink {  // rows r = token * group + g of one kv head
+  O* o;
+  float* l;
+  int64_t o_tok, o_g, l_tok;
+  int group;
+  __device__ __forceinline__ O* row(int r) const { return o + r / group * o_tok + r % group * o_g; }
+  __device__ __forceinline__ float* lse(int r) const { return l == nullptr ? nullptr : l + r / group * l_tok + r % group; }
+};
+
+template <typename T, int D, int RPT>
+__global__ void __launch_bounds__(kThreads) prompt_attention_kernel(const PromptTensors t, const PromptItem* items) {
+  extern __shared__ __align__(16) float sm[];
+  grid_dependency_wait();
+  grid_launch_dependents();
+  const PromptItem it = items[blockIdx.x];
+  const int G = t.group, hq = t.n_kv_heads * G;
+  const PackedKeys<T> key{(const T*)t.k + it.kv_tok * t.k_tok_stride + it.head * t.k_head_stride,
+                              (const T*)t.v + it.kv_tok * t.v_tok_stride + it.head * t.v_head_stride, t.k_tok_stride,
+                              t.v_tok_stride, it.kv_len};
+  const T* q = (const T*)t.q + it.q_tok * t.q_tok_stride + (int64_t)it.head * G * t.q_head_stride;
+  const auto q_row = [&](int r) { return q + r / G * t.q_tok_stride + r % G * t.q_head_stride; };
+  const auto limit = [&](int r) { return max(0, min(it.limit0 + r / G, it.kv_len)); };
+  const RowSink<T> sink{(T*)t.out + ((int64_t)it.q_tok * hq + it.head * G) * D,
+                     t.lse == nullptr ? nullptr : t.lse + (int64_t)it.q_tok * hq + it.head * G, (int64_t)hq * D, D, hq, G};
+  attend<T, D, RPT>(sm, it.n_tok * G, 0, limit(it.n_tok * G - 1), kLog2e * rsqrtf((float)D), key, q_row, limit, sink);
+}
+
+// The decode step: this CTA's share of all units, segment by segment.
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads) shared_attention_kernel(const SharedParams p) {
+  extern __shared__ __align__(16) float sm[];
+  __shared__ unsigned long long scratch[kThreads / 32];
+  grid_dependency_wait();
+  grid_launch_dependents();
+  const int G = p.group, hq = p.n_kv_heads * G, cta = blockIdx.x;
+  SharedCursor c = find_share<kKeys, kThreads>(p, cta, gridDim.x, scratch);
+  while (c.left > 0) {
+    const SharedEntity ent = p.entities[c.e];
+    int lo, hi;
+    entity_keys(p, c.e, ent, lo, hi);
+    const int n = (int)min((int64_t)(c.units - c.k), c.left);
+    const int2 lead = entity_lead(p, ent, hi);
+    const int32_t* table = p.block_table + (int64_t)lead.x * p.max_pages;
+    const int from = lo + c.k * kKeys, to = max(from, min(lead.y, from + n * kKeys));
+    const bool own = c.e >= p.n_shared;
+    const int64_t slot = (int64_t)(own ? c.e - p.n_shared : c.e) * p.n_kv_heads + c.h + cta;
+    const int slot_rows = own ? G : p.row_block;
+    const PagedKeys<T> key{(const T*)p.k_pool + c.h * p.head_stride, (const T*)p.v_pool + c.h * p.head_stride,
+                               table, p.page_stride, D, p.n_pool_pages, p.max_pages};
+    const T* q = (const T*)p.q + ((int64_t)ent.first_seq * hq + c.h * G) * D;
+    const auto q_row = [&](int r) { return q + (int64_t)(r / G) * hq * D + r % G * D; };
+    const auto limit = [&](int r) { return min(to, shared_seq_len(p, ent.first_seq + r / G)); };
+    const RowSink<float> sink{(own ? p.o_own : p.o_shared) + slot * slot_rows * D, (own ? p.lse_own : p.lse_shared) + slot * slot_rows,
+                       (int64_t)G * D, D, G, G};
+    for (int j = (from >> 4) + threadIdx.x; j < (to + 15) >> 4; j += kThreads) {
+      const int page = table[j];
+      if (page < 0 || (p.n_pool_pages > 0 && page >= p.n_pool_pages)) atomicOr(p.status, DEV_STATUS_BAD_INDEX);
+    }
+    // a single sequence has at most 16 rows: the narrow form, which spends the threads on keys instead of empty rows
+    if (ent.n_seqs * G <= 16)
+      attend<T, D, 1>(sm, ent.n_seqs * G, from, to, kLog2e * rsqrtf((float)D), key, q_row, limit, sink);
+    else
+      attend<T, D, 8>(sm, ent.n_seqs * G, from, to, kLog2e * rsqrtf((float)D), key, q_row, limit, sink);
+    c.left -= n;
+    c.k = 0;
+    if (++c.h == p.n_kv_heads) {
+      c.h = 0;
+      if (c.left > 0)  // some entity behind this one has units: they were counted
+        do c.units = entity_units<kKeys>(p, ++c.e);
+        while (c.units == 0);
+    }
+  }
+}
+
+// out[row] = sum_s o_s 2^(lse_s - M) / sum_s 2^(lse_s - M) over the segments of the row's shared and own item.  A warp per
+// query row; every block first finds where its sequence's two items lie on the line of units.
+template <typename T, int D, int kUnit>
+__global__ void __launch_bounds__(256) shared_merge_kernel(const SharedParams p, const int2* seq_info, int ctas, T* out) {
+  __shared__ long long sums[8][3];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int G = p.group, hq = p.n_kv_heads * G;
+  const int per_seq = (hq + 7) / 8, seq = blockIdx.x / per_seq, head = blockIdx.x % per_seq * 8 + warp;
+  grid_launch_dependents();
+  const int2 info = seq_info[seq];  // shared entity, the sequence's place in it
+  const int own_e = p.n_shared + seq;
+  // the lengths belong to the caller and were there before the attention kernel; its partials were not
+  grid_dependency_wait();
+  long long before_shared = 0, before_own = 0, total = 0;
+  for (int e = tid; e < p.n_shared + p.batch; e += 256) {
+    const long long n = (long long)entity_units<kUnit>(p, e) * p.n_kv_heads;
+    if (e < info.x) before_shared += n;
+    if (e < own_e) before_own += n;
+    total += n;
+  }
+#pragma unroll
+  for (int w = 16; w > 0; w >>= 1) {
+    before_shared += __shfl_xor_sync(0xffffffffu, before_shared, w);
+    before_own += __shfl_xor_sync(0xffffffffu, before_own, w);
+    total += __shfl_xor_sync(0xffffffffu, total, w);
+  }
+  if (lane == 0) {
+    sums[warp][0] = before_shared;
+    sums[warp][1] = before_own;
+    sums[warp][2] = total;
+  }
+  __syncthreads();
+  before_shared = before_own = total = 0;
+  for (int w = 0; w < 8; ++w) {
+    before_shared += sums[w][0];
+    before_own += sums[w][1];
+    total += sums[w][2];
+  }
+  if (head >= hq) return;
+  ctas = shares_of(total, ctas);
+  const int h = head / G, g = head % G;
+  float acc[D / 32], M = -INFINITY, L = 0.f;
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i) acc[i] = 0.f;
+#pragma unroll
+  for (int part = 0; part < 2; ++part) {
+    const int e = part == 0 ? info.x : own_e;
+    const int units = entity_units<kUnit>(p, e);
+    if (units == 0) continue;
+    const long long u0 = (part == 0 ? before_shared : before_own) + (long long)h * units;
+    const int c0 = share_owner(u0, total, ctas), c1 = share_owner(u0 + units - 1, total, ctas);
+    const int64_t slot = (int64_t)(part == 0 ? e : seq) * p.n_kv_heads + h;
+    const int rows = part == 0 ? p.row_block : G, row = part == 0 ? info.y * G + g : g;
+    const float *ob = part == 0 ? p.o_shared : p.o_own, *lb = part == 0 ? p.lse_shared : p.lse_own;
+#pragma unroll 4
+    for (int c = c0; c <= c1; ++c) {
+      const int64_t at = (slot + c) * rows + row;
+      const float lse = __ldcg(lb + at) * kLog2e;
+      float v[D / 32];
+      if constexpr (D == 128) {
+        const float4 x = __ldcg(reinterpret_cast<const float4*>(ob + at * D) + lane);
+        v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+      } else {
+        const float2 x = __ldcg(reinterpret_cast<const float2*>(ob + at * D) + lane);
+        v[0] = x.x; v[1] = x.y;
+      }
+      const float m = fmaxf(M, lse), base = m == -INFINITY ? 0.f : m;
+      const float keep = exp2f(M - base), w = exp2f(lse - base);
+      if (lse == -INFINITY) continue;  // a segment without a visible key
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) acc[i] = acc[i] * keep + w * v[i];
+      L = L * keep + w;
+      M = m;
+    }
+  }
+  const float inv = L == 0.f ? 0.f : 1.f / L;  // a sequence without keys: zeros
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i) acc[i] *= inv;
+  store_vec<D / 32>(out + ((int64_t)seq * hq + head) * D + lane * (D / 32), acc);
+}
+
+template <typename Kern> int set_smem(Kern kern, size_t bytes, const char* what) {
+  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  return e == cudaSuccess ? IA_OK : fail(IA_ERR_LAUNCH, "%s: cudaFuncSetAttribute: %s", what, cudaGetErrorString(e));
+}
+
+template <typename... Args, typename... Given>
+int launch(void (*kern)(Args...), unsigned grid, size_t smem, cudaStream_t stream, const char* what, Given... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = overlapped_launch_enabled() ? 1 : 0;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, args...);
+  return e == cudaSuccess ? check_launch(what) : fail(IA_ERR_LAUNCH, "%s: %s", what, cudaGetErrorString(e));
+}
+
+template <typename T, int D, int RPT>
+int launch_prompt(const PromptTensors& t, const PromptItem* items, int n_items, cudaStream_t stream) {
+  auto kern = prompt_attention_kernel<T, D, RPT>;
+  if (int s = set_smem(kern, Smem<D, RPT>::bytes, "prompt_attention")) return s;
+  return launch(kern, (unsigned)n_items, Smem<D, RPT>::bytes, stream, "prompt_attention_kernel", t, items);
+}
+template <typename T, int D> int launch_shared(const SharedParams& p, int ctas, cudaStream_t stream) {
+  auto kern = shared_attention_kernel<T, D>;
+  if (int s = set_smem(kern, Smem<D, 8>::bytes, "shared_attention")) return s;
+  return launch(kern, (unsigned)ctas, Smem<D, 8>::bytes, stream, "shared_attention_kernel", p);
+}
+template <typename T, int D, int kUnit>
+int launch_merge(const SharedParams& p, const int2* seq_info, int ctas, T* out, cudaStream_t stream) {
+  const int per_seq = (p.n_kv_heads * p.group + 7) / 8;
+  return launch(shared_merge_kernel<T, D, kUnit>, (unsigned)(p.batch * per_seq), 0, stream, "shared_merge_kernel", p, seq_info,
+                ctas, out);
+}
+
+}  // namespace
+
+int sm_count() {
+  constexpr int kMaxDevices = 64;
+  static std::atomic<int> cached[kMaxDevices];
+  int dev = 0, sms = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return 148;
+  if (int n = cached[dev].load(std::memory_order_relaxed)) return n;
+  if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || sms <= 0) return 148;
+  cached[dev].store(sms, std::memory_order_relaxed);
+  return sms;
+}
+
+template <typename T>
+static int prompt_of(const PromptTensors& t, int head_dim, const PromptItem* items, int n_items, bool few_rows, cudaStream_t stream) {
+  if (head_dim == 128)
+    return few_rows ? launch_prompt<T, 128, 2>(t, items, n_items, stream) : launch_prompt<T, 128, 8>(t, items, n_items, stream);
+  return few_rows ? launch_prompt<T, 64, 2>(t, items, n_items, stream) : launch_prompt<T, 64, 8>(t, items, n_items, stream);
+}
+int launch_prompt_fma(const PromptTensors& t, int dtype, int head_dim, const PromptItem* items, int n_items, bool few_rows,
+                      cudaStream_t stream) {
+  return dtype == IA_F32 ? prompt_of<float>(t, head_dim, items, n_items, few_rows, stream)
+                         : prompt_of<__nv_bfloat16>(t, head_dim, items, n_items, few_rows, stream);
+}
+
+int launch_shared_fma(const SharedParams& p, int dtype, int head_dim, int ctas, cudaStream_t stream) {
+  if (dtype == IA_F32) return head_dim == 128 ? launch_shared<float, 128>(p, ctas, stream) : launch_shared<float, 64>(p, ctas, stream);
+  return head_dim == 128 ? launch_shared<__nv_bfloat16, 128>(p, ctas, stream) : launch_shared<__nv_bfloat16, 64>(p, ctas, stream);
+}
+
+int launch_shared_merge(const SharedParams& p, const int32_t* seq_info, int head_dim, int dtype, int ctas, void* out,
+                        cudaStream_t stream) {
+  const int2* info = reinterpret_cast<const int2*>(seq_info);
+  if (dtype == IA_F32)
+    return head_dim == 128 ? launch_merge<float, 128, kKeys>(p, info, ctas, (float*)out, stream)
+                           : launch_merge<float, 64, kKeys>(p, info, ctas, (float*)out, stream);
+  return head_dim == 128 ? launch_merge<__nv_bfloat16, 128, kKeys>(p, info, ctas, (__nv_bfloat16*)out, stream)
+                         : launch_merge<__nv_bfloat16, 64, kKeys>(p, info, ctas, (__nv_bfloat16*)out, stream);
+}
+
+// ---- the prompt's plan ----------------------------------------------------------------------------------------------
+// Words: a header of 8, where each CTA's items begin (ctas + 1 words, padded to whole items), the items.
+namespace {
+constexpr int kRowsFew = 32, kRowsFull = 128;
+struct PlanShape {
+  int n_items, ctas, item_tokens;
+  bool few_rows;
+  int64_t ints() const { return 8 + (int64_t)(ctas + 1 + 7) / 8 * 8 + (int64_t)n_items * 8; }
+};
+int64_t count_items(const int32_t* q_lens, int n_seqs, int tokens) {
+  int64_t n = 0;
+  for (int i = 0; i < n_seqs; ++i) n += ((int64_t)q_lens[i] + tokens - 1) / tokens;
+  return n;
+}
+bool plan_shape(const int32_t* q_lens, int n_seqs, int n_kv_heads, int group, int dtype, PlanShape* s) {
+  (void)dtype;
+  int64_t items = count_items(q_lens, n_seqs, kRowsFull / group) * n_kv_heads;
+  s->few_rows = items < 2 * sm_count();
+  s->item_tokens = (s->few_rows ? kRowsFew : kRowsFull) / group;
+  items = count_items(q_lens, n_seqs, s->item_tokens) * n_kv_heads;
+  if (items > 0x7fffffff / 64) return false;
+  s->n_items = (int)items;
+  s->ctas = (int)items;
+  return true;
+}
+}  // namespace
+
+int64_t prompt_plan_ints(const int32_t* q_lens, int n_seqs, int n_kv_heads, int group, int dtype) {
+  PlanShape s;
+  return plan_shape(q_lens, n_seqs, n_kv_heads, group, dtype, &s) ? s.ints() : -1;
+}
+
+int make_prompt_plan(const int32_t* q_lens, const int32_t* kv_lens, int n_seqs, int n_kv_heads, int group, int head_dim, int dtype,
+                     int32_t* plan, int64_t plan_ints) {
+  PlanShape s;
+  if (!plan_shape(q_lens, n_seqs, n_kv_heads, group, dtype, &s) || plan_ints < s.ints())
+    return fail(IA_ERR_BAD_ARG, "prompt_plan: %lld words", (long long)plan_ints);
+  std::vector<PromptItem> items;
+  items.reserve(s.n_items);
+  int64_t q0 = 0, k0 = 0;
+  for (int i = 0; i < n_seqs; ++i) {
+    for (int t = 0; t < q_lens[i]; t += s.item_tokens)
+      for (int h = 0; h < n_kv_heads; ++h)
+        items.push_back(PromptItem{(int)(q0 + t), std::min(s.item_tokens, q_lens[i] - t), (int)k0,
+                                   kv_lens[i] - q_lens[i] + t + 1, kv_lens[i], h, {0, 0}});
+    q0 += q_lens[i];
+    k0 += kv_lens[i];
+  }
+  const auto keys = [](const PromptItem& it) { return std::max(0, std::min(it.limit0 + it.n_tok - 1, it.kv_len)); };
+  // the longest first, so that what is started last is short
+  std::stable_sort(items.begin(), items.end(), [&](const PromptItem& a, const PromptItem& b) { return keys(a) > keys(b); });
+  const int64_t first = s.ints() - (int64_t)s.n_items * 8;
+  const int32_t head[8] = {s.n_items, s.ctas, s.few_rows, (int32_t)first, group * 1000 + head_dim, n_kv_heads * 16 + dtype,
+                           (int32_t)q0, (int32_t)k0};
+  std::copy(head, head + 8, plan);
+  for (int64_t i = 8; i < first; ++i) plan[i] = std::min<int64_t>(i - 8, s.n_items);
+  if (s.n_items > 0) std::copy((const int32_t*)items.data(), (const int32_t*)(items.data() + s.n_items), plan + first);
+  return IA_OK;
+}
+
+// ---- the plan of the shared-prefix step: a header of 8 words, the entities, then (shared entity, place in it) per sequence
+namespace {
+int row_block() { return kRowsFull; }
+}  // namespace
+int shared_row_block() { return row_block(); }
+int shared_ctas() { return sm_count(); }
+int64_t shared_parts(const int32_t* group_sizes, int n_groups, int group) {
+  const int per = row_block() / group;
+  int64_t n = 0;
+  for (int i = 0; i < n_groups; ++i) n += ((int64_t)group_sizes[i] + per - 1) / per;
+  return n;
+}
+void make_shared_plan(const int32_t* group_sizes, int n_groups, int batch, int group, int32_t* plan) {
+  const int per = row_block() / group;
+  const int n_shared = (int)shared_parts(group_sizes, n_groups, group);
+  SharedEntity* ent = reinterpret_cast<SharedEntity*>(plan + 8);
+  int32_t* info = plan + 8 + 8 * ((int64_t)n_shared + batch);
+  std::fill(plan, plan + 8, 0);
+  plan[0] = n_shared;
+  int seq = 0, e = 0;
+  for (int g = 0; g < n_groups; ++g) {
+    const int lead = seq;
+    for (int m = 0; m < group_sizes[g]; m += per, ++e) {
+      const int n = std::min(per, group_sizes[g] - m);
+      ent[e] = SharedEntity{lead + m, n, lead, group_sizes[g], g, {0, 0, 0}};
+      for (int i = 0; i < n; ++i) {
+        info[2 * (lead + m + i)] = e;
+        info[2 * (lead + m + i) + 1] = i;
+        ent[n_shared + lead + m + i] = SharedEntity{lead + m + i, 1, lead + m + i, 1, g, {0, 0, 0}};
+      }
+    }
+    seq += group_sizes[g];
+  }
+}
+
+}  // namespace ia

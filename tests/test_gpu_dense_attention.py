@@ -1,0 +1,329 @@
+"""Prompt attention and the shared-prefix decode step against the formula in float64."""
+
+import pytest
+import torch
+
+from tests.dense_util import PAGE, decode_reference, prompt_reference
+from interattn_b200 import _lib, dense_attention, ops, page_cache
+
+pytestmark = pytest.mark.gpu
+BF16, F32 = torch.bfloat16, torch.float32
+GEOMETRIES = [(8, 2, 64, BF16), (8, 2, 128, BF16), (8, 2, 64, F32), (4, 1, 128, F32), (3, 3, 64, BF16), (6, 2, 128, BF16),
+              (16, 1, 128, BF16), (14, 2, 64, BF16), (5, 1, 64, F32), (16, 1, 64, F32), (2, 2, 128, BF16)]
+
+
+def randn(shape, dtype, seed, scale=1.0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(shape, generator=g) * scale).to(dtype).cuda()
+
+
+def i32(values):
+    return torch.tensor(values, dtype=torch.int32, device="cuda")
+
+
+def prompt_case(hq, hkv, d, dtype, q_lens, kv_lens, seed=0):
+    q = randn((sum(q_lens), hq, d), dtype, seed, 1.5)
+    k, v = randn((sum(kv_lens), hkv, d), dtype, seed + 1), randn((sum(kv_lens), hkv, d), dtype, seed + 2)
+    plan = dense_attention.PromptAttention(q_lens, hq, hkv, d, kv_lens=kv_lens, dtype=dtype)
+    return q, k, v, plan
+
+
+@pytest.mark.parametrize("hq,hkv,d,dtype", GEOMETRIES)
+@pytest.mark.parametrize("q_lens,kv_lens", [
+    ([1], [1]), ([0, 3, 0], [0, 3, 0]), ([127, 1, 128, 129], None), ([300, 17], None),
+    ([5, 64, 1, 2], [200, 64, 129, 257]),          # continued prompts
+    ([40, 3, 7], [10, 0, 6]),                      # rows that see nothing
+])
+def test_prompt(hq, hkv, d, dtype, q_lens, kv_lens):
+    kv_lens = q_lens if kv_lens is None else kv_lens
+    q, k, v, plan = prompt_case(hq, hkv, d, dtype, q_lens, kv_lens)
+    ref = prompt_reference(q, k, v, q_lens, kv_lens)
+    out, lse = plan.run(q, k, v, return_lse=True)
+    assert ops.device_status() == 0
+    ref.check(out, dtype)
+    ref.check_lse(lse)
+    assert torch.equal(plan.run(q, k, v), out)      # the same bits again, and without the log-sum-exp
+
+
+@pytest.mark.parametrize("hq,hkv,d,dtype", [(8, 2, 128, BF16), (8, 2, 64, BF16), (4, 4, 64, F32)])
+def test_prompt_of_many_tiles(hq, hkv, d, dtype):
+    """Enough pieces that a CTA takes several, with a rising score that moves the running maximum often."""
+    q_lens, kv_lens = [900, 1, 450, 513], [900, 1, 1450, 513]
+    q, k, v, plan = prompt_case(hq, hkv, d, dtype, q_lens, kv_lens, seed=5)
+    k = (k.float() * torch.linspace(0.05, 6.0, k.shape[0], device="cuda")[:, None, None]).to(dtype)
+    ref = prompt_reference(q, k, v, q_lens, kv_lens)
+    out = plan.run(q, k, v)
+    assert ops.device_status() == 0
+    ref.check(out, dtype)
+
+
+@pytest.mark.parametrize("dtype,d", [(BF16, 128), (F32, 64)])
+def test_prompt_strided_views(dtype, d):
+    """Queries, keys and values as views of one fused projection."""
+    hq, hkv, lens = 8, 2, [70, 33]
+    fused = randn((sum(lens), (hq + 2 * hkv) * d), dtype, 3).view(sum(lens), hq + 2 * hkv, d)
+    q, k, v = fused[:, :hq], fused[:, hq:hq + hkv], fused[:, hq + hkv:]
+    plan = dense_attention.PromptAttention(lens, hq, hkv, d, dtype=dtype)
+    out = plan.run(q, k, v)
+    assert torch.equal(out, plan.run(q.contiguous(), k.contiguous(), v.contiguous()))
+    prompt_reference(q, k, v, lens, lens).check(out, dtype)
+    heads_first = q.transpose(0, 1).contiguous().transpose(0, 1)
+    assert torch.equal(out, plan.run(heads_first, k, v))
+
+
+@pytest.mark.parametrize("dtype,d,hq,hkv", [(BF16, 128, 8, 2), (BF16, 64, 2, 2), (F32, 64, 4, 2), (F32, 128, 2, 2)])
+@pytest.mark.parametrize("poison", [float("nan"), float("inf"), float("-inf"), 3.0e38])
+def test_prompt_rows_do_not_see_the_future_or_the_neighbour(dtype, d, hq, hkv, poison):
+    lens = [150, 20, 1, 140]
+    q, k, v, plan = prompt_case(hq, hkv, d, dtype, lens, lens, seed=11)
+    clean, clean_lse = plan.run(q, k, v, return_lse=True)
+    at = 100                                          # a token of the first sequence, and the whole second one
+    k2, v2 = k.clone(), v.clone()
+    k2[at], v2[at] = poison, poison
+    k2[150:170], v2[150:170] = poison, poison
+    out, lse = plan.run(q, k2, v2, return_lse=True)
+    assert ops.device_status() == 0
+    keep = list(range(at)) + list(range(170, sum(lens)))
+    ref = prompt_reference(q, k, v, lens, lens)
+    got = clean.clone()
+    got[keep] = out[keep]
+    ref.check(got, dtype)
+    got_lse = clean_lse.clone()
+    got_lse[keep] = lse[keep]
+    ref.check_lse(got_lse)
+    if poison != poison:
+        assert bool(torch.isnan(out[at:170].float()).all())
+
+
+def test_prompt_graph_streams_and_threads():
+    q_lens = [200, 31]
+    q, k, v, plan = prompt_case(8, 2, 128, BF16, q_lens, q_lens, seed=7)
+    want = plan.run(q, k, v)
+    q2 = torch.randn_like(q)
+    want2 = plan.run(q2, k, v)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        a = plan.run(q, k, v)
+    b = plan.run(q2, k, v)                            # at the same time on this stream
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(a, want) and torch.equal(b, want2)
+    graph, buf, out = torch.cuda.CUDAGraph(), q.clone(), torch.empty_like(q)
+    with torch.cuda.graph(graph):
+        plan.run(buf, k, v, out=out)
+    buf.copy_(q2)
+    graph.replay()
+    assert torch.equal(out, want2)
+    buf.copy_(q)
+    graph.replay()
+    assert torch.equal(out, want)
+
+
+# ---- the decode step ------------------------------------------------------------------------------------------------
+
+def paged_case(hq, hkv, d, dtype, groups, shared, lens, seed=0, spare=3):
+    """Random pages; the sequences of a group have the same leading pages, and a prefix that ends inside a page is copied."""
+    g = torch.Generator().manual_seed(seed)
+    rows, n_pages, b, copies = [], 0, 0, []
+    for n, s in zip(groups, shared):
+        full = s // PAGE
+        base = n_pages
+        n_pages += full
+        for i in range(n):
+            pages = -(-lens[b] // PAGE)
+            own = max(0, pages - full)
+            rows.append(list(range(base, base + full))[:max(pages, 0)] + list(range(n_pages, n_pages + own)))
+            if s % PAGE and own:
+                copies.append((b, n, full, s % PAGE))
+            n_pages += own
+            b += 1
+    total = n_pages + spare
+    perm = torch.randperm(total, generator=g)
+    width = max([len(r) for r in rows] + [1]) + 2
+    table = torch.full((len(rows), width), -1, dtype=torch.int32)
+    for i, r in enumerate(rows):
+        table[i, :len(r)] = perm[torch.tensor(r, dtype=torch.long)].int()
+    k_pool, v_pool = randn((total, hkv, PAGE, d), dtype, seed + 1), randn((total, hkv, PAGE, d), dtype, seed + 2)
+    lead = 0
+    for n, s in zip(groups, shared):
+        if s % PAGE:
+            have = [i for i in range(lead, lead + n) if lens[i] > s // PAGE * PAGE]
+            for i in have[1:]:
+                for pool in (k_pool, v_pool):
+                    pool[table[i, s // PAGE].long(), :, :s % PAGE] = pool[table[have[0], s // PAGE].long(), :, :s % PAGE]
+        lead += n
+    kv = ops.PagedKV(k_pool, v_pool, table.cuda(), i32(lens), i32(lens))
+    q = randn((len(rows), hq, d), dtype, seed + 3, 1.5)
+    return q, kv, table
+
+
+DECODES = [
+    ([1], [0], [1]), ([2], [16], [17, 16]), ([3], [40], [41, 40, 100]), ([1, 4, 2], [0, 300, 129], [77, 301, 300, 420, 555, 129, 130]),
+    ([5], [1000], [1000, 1001, 1016, 0, 1500]),      # one row is idle
+    ([40], [256], [256 + i for i in range(40)]),     # more rows than one block holds
+    ([2, 2], [64, 0], [30, 70, 5, 0]),               # a member shorter than what the others share
+    ([3, 2], [200, 50], [0, 210, 333, 0, 0]),        # the first members have left; a whole group has
+    ([3], [100], [40, 70, 20]),                      # nobody holds all of it
+]
+
+
+@pytest.mark.parametrize("hq,hkv,d,dtype", GEOMETRIES)
+@pytest.mark.parametrize("groups,shared,lens", DECODES)
+def test_shared_prefix(hq, hkv, d, dtype, groups, shared, lens):
+    q, kv, table = paged_case(hq, hkv, d, dtype, groups, shared, lens)
+    step = dense_attention.SharedPrefixAttention(kv, groups, i32(shared), hq)
+    out = step.step(q)
+    assert ops.device_status() == 0
+    decode_reference(q, kv.k_pool, kv.v_pool, table, lens).check(out, dtype)
+    assert torch.equal(step.step(q), out)
+    alone = dense_attention.SharedPrefixAttention(kv, [1] * len(lens), i32([0] * len(lens)), hq)
+    decode_reference(q, kv.k_pool, kv.v_pool, table, lens).check(alone.step(q), dtype)
+
+
+@pytest.mark.parametrize("hq,hkv,d,dtype", [(32, 8, 128, BF16), (8, 2, 64, F32)])
+def test_shared_prefix_long(hq, hkv, d, dtype):
+    """Cut over all SMs; lengths that end inside tiles."""
+    groups, shared = [3, 1, 6], [9001, 0, 4444]
+    lens = [9001 + 5, 9001 + 700, 9001, 2777, 4444 + 1, 4444 + 16, 4445 + 31, 4444 + 333, 5000, 4460]
+    q, kv, table = paged_case(hq, hkv, d, dtype, groups, shared, lens, seed=3)
+    step = dense_attention.SharedPrefixAttention(kv, groups, i32(shared), hq)
+    out = step.step(q)
+    assert ops.device_status() == 0
+    decode_reference(q, kv.k_pool, kv.v_pool, table, lens).check(out, dtype)
+
+
+@pytest.mark.parametrize("dtype,d", [(BF16, 128), (BF16, 64), (F32, 64)])
+@pytest.mark.parametrize("poison", [float("nan"), float("inf")])
+def test_shared_prefix_unwritten_places_do_not_count(dtype, d, poison):
+    """Fresh cache memory behind the last token, and whole pages that no sequence holds, may hold anything."""
+    groups, shared, lens = [3, 1], [150, 0], [151, 150, 200, 33]
+    q, kv, table = paged_case(8, 2, d, dtype, groups, shared, lens, seed=9)
+    want = decode_reference(q, kv.k_pool, kv.v_pool, table, lens)
+    seen = torch.zeros(kv.k_pool.shape[:1] + (PAGE,), dtype=torch.bool)
+    for b, n in enumerate(lens):
+        for t in range(n):
+            seen[int(table[b, t // PAGE]), t % PAGE] = True
+    for pool in (kv.k_pool, kv.v_pool):
+        pool.transpose(1, 2)[~seen.cuda()] = poison
+    out = dense_attention.SharedPrefixAttention(kv, groups, i32(shared), 8).step(q)
+    assert ops.device_status() == 0
+    want.check(out, dtype)
+
+
+@pytest.mark.parametrize("dtype,d", [(BF16, 128), (F32, 64)])
+def test_shared_prefix_shorter_member_next_to_poison(dtype, d):
+    """A member that ends inside the shared part must not see what the longer ones see there."""
+    groups, shared, lens = [3], [160], [170, 70, 161]
+    q, kv, table = paged_case(8, 2, d, dtype, groups, shared, lens, seed=10)
+    want = decode_reference(q, kv.k_pool, kv.v_pool, table, lens)
+    kv.v_pool[table[0, 6].long(), :, 3] = float("nan")
+    out = dense_attention.SharedPrefixAttention(kv, groups, i32(shared), 8).step(q)
+    assert bool(torch.isnan(out[[0, 2]].float()).all())
+    want.out[[0, 2]], want.mean_abs[[0, 2]] = 0, 0
+    out[[0, 2]] = 0
+    want.check(out, dtype)
+
+
+def test_shared_prefix_bad_entries_are_reported():
+    groups, shared, lens = [2], [64], [100, 90]
+    for dtype in (BF16, F32):
+        for bad in (-1, 10 ** 6):
+            for at in (1, 5, 6):                       # a shared page, an own page, the last page of the first sequence
+                q, kv, table = paged_case(8, 2, 64, dtype, groups, shared, lens, seed=12)
+                kv.block_table[0, at] = bad
+                dense_attention.SharedPrefixAttention(kv, groups, i32(shared), 8).step(q)
+                assert ops.device_status() == _lib.IA_DEV_STATUS_BAD_INDEX
+                if at >= 4:                            # the other sequence is not concerned
+                    got = dense_attention.SharedPrefixAttention(kv, groups, i32(shared), 8).step(q)
+                    ref = decode_reference(q, kv.k_pool, kv.v_pool, table, lens)
+                    ref.out[0], ref.mean_abs[0] = 0, 0
+                    got[0] = 0
+                    ref.check(got, dtype)
+                    ops.device_status()
+
+
+def test_shared_prefix_captured_steps_follow_the_lengths():
+    groups, shared, lens = [2, 1], [48, 0], [60, 49, 33]
+    q, kv, table = paged_case(8, 2, 128, BF16, groups, shared, lens, seed=13)
+    step = dense_attention.SharedPrefixAttention(kv, groups, i32(shared), 8)
+    out = torch.empty_like(q)
+    step.step(q, out=out)
+    graphs = []
+    for _ in range(2):                                 # two graphs of one object on two streams
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = step.step(q)
+        graphs.append((graph, y))
+    shorter = [50, 48, 20]
+    kv.seq_lens.copy_(i32(shorter))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    for _ in range(3):
+        graphs[0][0].replay()
+        with torch.cuda.stream(side):
+            graphs[1][0].replay()
+    torch.cuda.current_stream().wait_stream(side)
+    ref = decode_reference(q, kv.k_pool, kv.v_pool, table, shorter)
+    for _, y in graphs:
+        ref.check(y, BF16)
+    assert ops.device_status() == 0
+
+
+# ---- together -------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype,hq,hkv,d", [(BF16, 8, 2, 128), (F32, 8, 2, 64)])
+def test_prompts_forks_and_steps_together(dtype, hq, hkv, d):
+    """Two prompts are read and written into pages, answered several times each; an answer leaves, the pages close up."""
+    layers, lens, answers = 2, [75, 32], [3, 2]
+    cache = page_cache.PageCache.empty(layers, 64, hkv, d, 5, 12, dtype=dtype)
+    total, leaders = sum(lens), [0, 3]
+    starts = i32([0, lens[0], total])
+    plan = dense_attention.PromptAttention(lens, hq, hkv, d, dtype=dtype)
+    history = [[[], []] for _ in range(5)]            # keys and values of every row, layer 1
+    cache.extend(i32(leaders), i32(lens))
+    for layer in range(layers):
+        q, k, v = randn((total, hq, d), dtype, 20 + layer), randn((total, hkv, d), dtype, 30 + layer), randn((total, hkv, d), dtype, 40 + layer)
+        out = plan.run(q, k, v)
+        prompt_reference(q, k, v, lens, lens).check(out, dtype)
+        cache.write(layer, i32(leaders), starts, k, v)
+    cache.fork(i32([0, 0, 3]), i32([1, 2, 4]))
+    for row in range(5):
+        s = slice(0, lens[0]) if row < 3 else slice(lens[0], total)
+        history[row] = [[k[s]], [v[s]]]
+    kv = cache.kv(1)
+    shared = i32(lens)
+    step = dense_attention.SharedPrefixAttention(kv, answers, shared, hq)
+    everyone, ones, each = i32([0, 1, 2, 3, 4]), i32([1] * 5), i32(list(range(6)))
+
+    def token(seed):
+        cache.extend(everyone, ones)
+        k, v = randn((5, hkv, d), dtype, seed), randn((5, hkv, d), dtype, seed + 1)
+        for layer in range(layers):
+            cache.write(layer, everyone, each, k, v)
+        for row in range(5):
+            history[row][0].append(k[row:row + 1])
+            history[row][1].append(v[row:row + 1])
+        q = randn((5, hq, d), dtype, seed + 2)
+        out = step.step(q)
+        keys, values = [torch.cat(h[0]) for h in history], [torch.cat(h[1]) for h in history]
+        n = [len(x) for x in keys]
+        ref = prompt_reference(q, torch.cat(keys), torch.cat(values), [1] * 5, n)
+        ref.check(out, dtype)
+
+    for i in range(20):
+        token(100 + 3 * i)
+    cache.free(i32([1]))
+    cache.compact()
+    cache.fork(i32([2]), i32([1]))
+    history[1] = [list(history[2][0]), list(history[2][1])]
+    for i in range(3):
+        token(200 + 3 * i)
+    assert int((cache.refs > 0).sum()) == len(set(cache.block_table.flatten().tolist()) - {-1})
+    # and the block-sparse step of the framework reads the same pages
+    summ = ops.build_summaries(cache.kv(1), 64, max_blocks=3)
+    sparse = ops.DecodeAttention(cache.kv(1), summ, hq, top_k=3)
+    q = randn((5, hq, d), dtype, 300)
+    keys, values = [torch.cat(h[0]) for h in history], [torch.cat(h[1]) for h in history]
+    prompt_reference(q, torch.cat(keys), torch.cat(values), [1] * 5, [len(x) for x in keys])
+    torch.testing.assert_close(sparse.step(q).float(), step.step(q).float(), rtol=2e-2, atol=2e-2)
+    assert ops.device_status() == 0
