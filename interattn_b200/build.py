@@ -25,7 +25,8 @@ SOURCES = ["capi.cu", "summaries.cu", "prompt_blocks.cu", "select.cu", "select_i
            "select_inst_bf16_d64.cu", "select_inst_f32_d128.cu", "select_inst_f32_d64.cu",
            "select_inst_kbar16_d128.cu", "select_inst_kbar16_d64.cu", "select_inst_bf16_d128_packed.cu",
            "select_inst_bf16_d64_packed.cu", "select_inst_f32_packed.cu", "select_inst_kbar16_packed.cu", "sparse_decode.cu", "sparse_decode_mma.cu",
-           "finalize.cu", "llama_step.cu", "skinny_gemm.cu", "dense_attention.cu", "page_cache.cu"]
+           "finalize.cu", "llama_step.cu", "skinny_gemm.cu", "dense_attention.cu", "dense_attention_tc.cu",
+           "page_cache.cu"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
     "-Xcompiler", "-fPIC",

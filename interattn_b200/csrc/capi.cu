@@ -682,8 +682,9 @@ int ia_prompt_attention(const ia_prompt_tensors* t, const int32_t* plan_host, co
     return fail(IA_ERR_BAD_ARG, "prompt_attention: token and head strides are multiples of 16 bytes and hold a head");
   const PromptTensors p{t->q, t->k, t->v, t->out, t->lse, t->q_tok_stride, t->q_head_stride, t->k_tok_stride, t->k_head_stride,
                         t->v_tok_stride, t->v_head_stride, t->n_q_tokens, t->n_kv_tokens, t->n_kv_heads, t->group_size};
-  return launch_prompt_fma(p, t->dtype, t->head_dim, reinterpret_cast<const PromptItem*>(plan_device + plan_host[3]),
-                           plan_host[0], plan_host[2] != 0, (cudaStream_t)stream);
+  const PromptItem* items = reinterpret_cast<const PromptItem*>(plan_device + plan_host[3]);
+  if (t->dtype == IA_BF16) return launch_prompt_tc(p, t->head_dim, items, plan_device + 8, plan_host[1], (cudaStream_t)stream);
+  return launch_prompt_fma(p, t->dtype, t->head_dim, items, plan_host[0], plan_host[2] != 0, (cudaStream_t)stream);
 }
 
 static int check_groups(const int32_t* group_sizes, int n_groups, const ia_geom* g) {
@@ -701,14 +702,14 @@ static int check_groups(const int32_t* group_sizes, int n_groups, const ia_geom*
 
 int64_t ia_shared_prefix_plan_ints(const int32_t* group_sizes, int n_groups, const ia_geom* geom) {
   if (check_groups(group_sizes, n_groups, geom)) return -1;
-  return 8 + 8 * (shared_parts(group_sizes, n_groups, geom->group_size) + geom->batch) + 2 * (int64_t)geom->batch;
+  return 8 + 8 * (shared_parts(group_sizes, n_groups, geom->group_size, geom->dtype) + geom->batch) + 2 * (int64_t)geom->batch;
 }
 
 int ia_shared_prefix_plan(const int32_t* group_sizes, int n_groups, const ia_geom* geom, int32_t* plan, int64_t plan_ints) {
   const int64_t need = ia_shared_prefix_plan_ints(group_sizes, n_groups, geom);
   if (need < 0) return IA_ERR_BAD_ARG;
   if (!plan || plan_ints < need) return fail(IA_ERR_BAD_ARG, "shared_prefix_plan: %lld words, %lld needed", (long long)plan_ints, (long long)need);
-  make_shared_plan(group_sizes, n_groups, geom->batch, geom->group_size, plan);
+  make_shared_plan(group_sizes, n_groups, geom->batch, geom->group_size, geom->dtype, plan);
   return IA_OK;
 }
 
@@ -722,7 +723,7 @@ static int64_t carve_shared(int n_shared, const ia_geom& g, char* base, SharedPa
     off += align256(bytes);
     return r;
   };
-  char* a[4] = {take(slots_shared * shared_row_block() * g.head_dim * 4), take(slots_shared * shared_row_block() * 4),
+  char* a[4] = {take(slots_shared * shared_row_block(g.dtype) * g.head_dim * 4), take(slots_shared * shared_row_block(g.dtype) * 4),
                 take(slots_own * g.group_size * g.head_dim * 4), take(slots_own * g.group_size * 4)};
   if (p) {
     p->o_shared = (float*)a[0];
@@ -764,8 +765,10 @@ int ia_shared_prefix_decode(const void* q, const void* k_pool, const void* v_poo
   if (p.status == nullptr) return IA_ERR_LAUNCH;
   p.page_stride = geom->pool_page_stride; p.head_stride = geom->pool_head_stride;
   p.n_shared = n_shared_parts; p.batch = geom->batch; p.n_kv_heads = geom->n_kv_heads; p.group = geom->group_size;
-  p.max_pages = geom->max_pages; p.n_pool_pages = geom->n_pool_pages; p.row_block = shared_row_block();
-  if (int s = launch_shared_fma(p, geom->dtype, geom->head_dim, shared_ctas(), (cudaStream_t)stream)) return s;
+  p.max_pages = geom->max_pages; p.n_pool_pages = geom->n_pool_pages; p.row_block = shared_row_block(geom->dtype);
+  const int s = geom->dtype == IA_BF16 ? launch_shared_tc(p, geom->head_dim, shared_ctas(), (cudaStream_t)stream)
+                                       : launch_shared_fma(p, geom->dtype, geom->head_dim, shared_ctas(), (cudaStream_t)stream);
+  if (s) return s;
   return launch_shared_merge(p, plan_device + 8 + 8 * ((int64_t)n_shared_parts + geom->batch), geom->head_dim, geom->dtype,
                              shared_ctas(), out, (cudaStream_t)stream);
 }

@@ -9,6 +9,10 @@
 // 8 lanes on 32 banks.
 #include <algorithm>
 #include <atomic>
+#include <cstring>
+#include <functional>
+#include <queue>
+#include <utility>
 #include <vector>
 
 #include "dense_attention.cuh"
@@ -436,14 +440,15 @@ int launch_shared_merge(const SharedParams& p, const int32_t* seq_info, int head
   if (dtype == IA_F32)
     return head_dim == 128 ? launch_merge<float, 128, kKeys>(p, info, ctas, (float*)out, stream)
                            : launch_merge<float, 64, kKeys>(p, info, ctas, (float*)out, stream);
-  return head_dim == 128 ? launch_merge<__nv_bfloat16, 128, kKeys>(p, info, ctas, (__nv_bfloat16*)out, stream)
-                         : launch_merge<__nv_bfloat16, 64, kKeys>(p, info, ctas, (__nv_bfloat16*)out, stream);
+  return head_dim == 128 ? launch_merge<__nv_bfloat16, 128, 128>(p, info, ctas, (__nv_bfloat16*)out, stream)
+                         : launch_merge<__nv_bfloat16, 64, 128>(p, info, ctas, (__nv_bfloat16*)out, stream);
 }
 
 // ---- the prompt's plan ----------------------------------------------------------------------------------------------
 // Words: a header of 8, where each CTA's items begin (ctas + 1 words, padded to whole items), the items.
 namespace {
 constexpr int kRowsFew = 32, kRowsFull = 128;
+constexpr int kPieceCost = 256;  // what starting and ending a piece costs, in keys
 struct PlanShape {
   int n_items, ctas, item_tokens;
   bool few_rows;
@@ -455,14 +460,16 @@ int64_t count_items(const int32_t* q_lens, int n_seqs, int tokens) {
   return n;
 }
 bool plan_shape(const int32_t* q_lens, int n_seqs, int n_kv_heads, int group, int dtype, PlanShape* s) {
-  (void)dtype;
-  int64_t items = count_items(q_lens, n_seqs, kRowsFull / group) * n_kv_heads;
+  // query rows of a piece: large ones read K and V less often, small ones spread over more SMs
+  const int full = dtype == IA_F32 ? kRowsFull / group : 2 * (kRowsFull / group);
+  const int few = dtype == IA_F32 ? kRowsFew / group : kRowsFull / group;
+  int64_t items = count_items(q_lens, n_seqs, full) * n_kv_heads;
   s->few_rows = items < 2 * sm_count();
-  s->item_tokens = (s->few_rows ? kRowsFew : kRowsFull) / group;
+  s->item_tokens = s->few_rows ? few : full;
   items = count_items(q_lens, n_seqs, s->item_tokens) * n_kv_heads;
   if (items > 0x7fffffff / 64) return false;
   s->n_items = (int)items;
-  s->ctas = (int)items;
+  s->ctas = dtype == IA_F32 ? (int)items : (int)std::min<int64_t>(items, sm_count());
   return true;
 }
 }  // namespace
@@ -491,30 +498,48 @@ int make_prompt_plan(const int32_t* q_lens, const int32_t* kv_lens, int n_seqs, 
   const auto keys = [](const PromptItem& it) { return std::max(0, std::min(it.limit0 + it.n_tok - 1, it.kv_len)); };
   // the longest first, so that what is started last is short
   std::stable_sort(items.begin(), items.end(), [&](const PromptItem& a, const PromptItem& b) { return keys(a) > keys(b); });
+  std::vector<int> order(s.n_items), begin(s.ctas + 1, 0);
+  if (dtype == IA_F32) {  // a CTA each, in this order
+    for (int i = 0; i < s.n_items; ++i) order[i] = begin[i] = i;
+    begin[s.ctas] = s.n_items;
+  } else {  // a list for each SM: the next longest piece goes to the SM with the least to do so far
+    std::vector<int> cta_of(s.n_items);
+    using Load = std::pair<int64_t, int>;
+    std::priority_queue<Load, std::vector<Load>, std::greater<Load>> loads;
+    for (int c = 0; c < s.ctas; ++c) loads.push({0, c});
+    for (int i = 0; i < s.n_items; ++i) {
+      const Load at = loads.top();
+      loads.pop();
+      cta_of[i] = at.second;
+      ++begin[at.second + 1];
+      loads.push({at.first + keys(items[i]) + kPieceCost, at.second});
+    }
+    for (int c = 0; c < s.ctas; ++c) begin[c + 1] += begin[c];
+    std::vector<int> next(begin.begin(), begin.end() - 1);
+    for (int i = 0; i < s.n_items; ++i) order[next[cta_of[i]]++] = i;
+  }
   const int64_t first = s.ints() - (int64_t)s.n_items * 8;
   const int32_t head[8] = {s.n_items, s.ctas, s.few_rows, (int32_t)first, group * 1000 + head_dim, n_kv_heads * 16 + dtype,
                            (int32_t)q0, (int32_t)k0};
   std::copy(head, head + 8, plan);
-  for (int64_t i = 8; i < first; ++i) plan[i] = std::min<int64_t>(i - 8, s.n_items);
-  if (s.n_items > 0) std::copy((const int32_t*)items.data(), (const int32_t*)(items.data() + s.n_items), plan + first);
+  for (int64_t i = 8; i < first; ++i) plan[i] = begin[std::min<int64_t>(i - 8, s.ctas)];
+  for (int i = 0; i < s.n_items; ++i) std::memcpy(plan + first + 8 * (int64_t)i, &items[order[i]], sizeof(PromptItem));
   return IA_OK;
 }
 
 // ---- the plan of the shared-prefix step: a header of 8 words, the entities, then (shared entity, place in it) per sequence
-namespace {
-int row_block() { return kRowsFull; }
-}  // namespace
-int shared_row_block() { return row_block(); }
+int shared_row_block(int dtype) { return dtype == IA_F32 ? kRowsFull : 2 * kRowsFull; }
+static int shared_members(int dtype, int group) { return shared_row_block(dtype) / kRowsFull * (kRowsFull / group); }
 int shared_ctas() { return sm_count(); }
-int64_t shared_parts(const int32_t* group_sizes, int n_groups, int group) {
-  const int per = row_block() / group;
+int64_t shared_parts(const int32_t* group_sizes, int n_groups, int group, int dtype) {
+  const int per = shared_members(dtype, group);
   int64_t n = 0;
   for (int i = 0; i < n_groups; ++i) n += ((int64_t)group_sizes[i] + per - 1) / per;
   return n;
 }
-void make_shared_plan(const int32_t* group_sizes, int n_groups, int batch, int group, int32_t* plan) {
-  const int per = row_block() / group;
-  const int n_shared = (int)shared_parts(group_sizes, n_groups, group);
+void make_shared_plan(const int32_t* group_sizes, int n_groups, int batch, int group, int dtype, int32_t* plan) {
+  const int per = shared_members(dtype, group);
+  const int n_shared = (int)shared_parts(group_sizes, n_groups, group, dtype);
   SharedEntity* ent = reinterpret_cast<SharedEntity*>(plan + 8);
   int32_t* info = plan + 8 + 8 * ((int64_t)n_shared + batch);
   std::fill(plan, plan + 8, 0);

@@ -234,14 +234,17 @@ int sm_count();
 int64_t prompt_plan_ints(const int32_t* q_lens, int n_seqs, int n_kv_heads, int group, int dtype);  // -1: too large
 int make_prompt_plan(const int32_t* q_lens, const int32_t* kv_lens, int n_seqs, int n_kv_heads, int group, int head_dim, int dtype,
                      int32_t* plan, int64_t plan_ints);
-int shared_row_block();  // query rows of a shared part, at most
+int shared_row_block(int dtype);  // query rows of a shared part, at most
 int shared_ctas();
-int64_t shared_parts(const int32_t* group_sizes, int n_groups, int group);
-void make_shared_plan(const int32_t* group_sizes, int n_groups, int batch, int group, int32_t* plan);
+int64_t shared_parts(const int32_t* group_sizes, int n_groups, int group, int dtype);
+void make_shared_plan(const int32_t* group_sizes, int n_groups, int batch, int group, int dtype, int32_t* plan);
 
 int launch_prompt_fma(const PromptTensors& t, int dtype, int head_dim, const PromptItem* items, int n_items, bool few_rows,
                       cudaStream_t stream);
 int launch_shared_fma(const SharedParams& p, int dtype, int head_dim, int ctas, cudaStream_t stream);
+int launch_prompt_tc(const PromptTensors& t, int head_dim, const PromptItem* items, const int32_t* cta_begin, int ctas,
+                     cudaStream_t stream);
+int launch_shared_tc(const SharedParams& p, int head_dim, int ctas, cudaStream_t stream);
 int launch_shared_merge(const SharedParams& p, const int32_t* seq_info, int head_dim, int dtype, int ctas, void* out,
                         cudaStream_t stream);
 
