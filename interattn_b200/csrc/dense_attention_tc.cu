@@ -7,7 +7,12 @@
 // A query row is a (token, query head of the kv head): the G heads of a token share its keys, so a tile of 128 / G tokens
 // needs K and V once for all of them, and a decode step over a shared prefix is the same computation with sequences in
 // the place of tokens.
-// The two tiles take turns: while the tensor core works on one tile's products the other's warps take exponentials.
+// The two sets of softmax warps take turns with the tensor core: while it works on one's products the other takes
+// exponentials.  Where a piece fills both row tiles each set has a tile and both see every key tile; where it fills only one
+// (a decode step of few rows, a short prompt) the key tiles alternate between the sets, each with its own running maximum,
+// sum and O, which are merged at the end: row and lane are the same in both, so either set reads the other's O from
+// tensor memory.  In both cases the key tiles' steps run 0, 1, 0, 1, ... over the sets and across pieces, so the next
+// piece's first products start while the last one's outputs are written.
 // The running maximum follows the true one only when it has moved by more than 2^8 (weights then stay below 256, exact in
 // the sums' fp32 and the same relative rounding in bf16): O is rescaled then, by the warps that own it, which is rare after
 // the first tiles.  The weights are rounded to bf16 for the second product, half a step = 2^-8 relative each; their
@@ -15,7 +20,12 @@
 //
 // Warps 0-3 and 4-7: softmax, rescaling and output of tile 0 and 1.  Warp 8: copies - it alone knows where work comes from
 // (a list for prompts, an equal share of all units for the decode step) and hands the others descriptors through a small
-// ring.  Warp 9: one thread issues every MMA.  Tensor memory: S_0, S_1, O_0, O_1 of 128 columns each.
+// ring.  Warps 9 and 10 issue the MMAs of set 0 and 1, each set's second product and next first product as one block, and
+// pass the turn on: issuing holds a thread until the tensor core takes the instruction, so what one warp decides and waits
+// for between its blocks is hidden behind the other's, and the fixed order keeps the sets half a period apart.  Tensor
+// memory: S_0, S_1, O_0, O_1 of 128 columns each.
+#include <type_traits>
+
 #include <cuda.h>  // CUtensorMap (types only; the encoder is fetched through the runtime)
 
 #include "dense_attention.cuh"
@@ -23,22 +33,58 @@
 namespace ia {
 namespace {
 
-constexpr int kThreads = 320, kRows = 128, kKeys = 128, kWorkSlots = 4;
-constexpr int kCopyWarp = 8, kMmaWarp = 9;
+constexpr int kThreads = 384, kRows = 128, kKeys = 128, kWorkSlots = 8;
+constexpr int kCopyWarp = 8, kMmaWarp = 9;  // and 10; 11 only makes up the third warpgroup
+// The block is launched with 168 registers a thread (64,512 in all).  A softmax thread holds a row of 128 logits.
+constexpr int kSoftmaxRegs = 208, kOtherRegs = 88;
+static_assert(256 * kSoftmaxRegs + 128 * kOtherRegs <= kThreads * 168, "what the block was launched with");
 
 template <int D> struct Tc {
   static constexpr int halves = D / 64;                 // 128-byte wide column blocks
   static constexpr int block = kRows * 128;             // bytes of one [128 rows][128 bytes] block
   static constexpr int tile = halves * block;           // a Q, K or V tile
-  static constexpr int stages = D == 128 ? 5 : 10;      // ring of K and V tiles
-  static constexpr size_t smem = (size_t)(2 + stages) * tile + 1024;
+  static constexpr int stages = D == 128 ? 4 : 8;       // ring of K and V tiles
+  static constexpr int out_warp = 4096;                 // a warp's 32 rows of 128 bytes on their way out
+  static constexpr size_t tiles = (size_t)(2 + stages) * tile, control = tiles + 8 * out_warp, smem = control + 3072;
 };
+
+// Step i of a piece belongs to set (first + i) % 2 of softmax warps.  Split: key tile i.  Else: key tile i / 2, row tile i % 2.
+struct Order {
+  int split;          // one row tile, key tiles alternate between the sets
+  int tiles[2];       // key tiles of each row tile; the second sees no fewer
+  int first;
+  __device__ __forceinline__ int steps() const { return split ? tiles[0] : 2 * tiles[1]; }
+};
+struct Step {
+  int tile, rt;
+  bool valid, first_use;  // of the key tile
+  bool opens, closes;               // the row tile's first and last (split: the set's)
+};
+__device__ __forceinline__ Step step_of(const Order& o, int i) {
+  Step st;
+  if (o.split) {
+    st.tile = i;
+    st.rt = 0;
+    st.valid = st.first_use = true;
+    st.opens = i < 2;
+    st.closes = i + 2 >= o.tiles[0];
+  } else {
+    st.tile = i >> 1;
+    st.rt = i & 1;
+    const int n = st.rt ? o.tiles[1] : o.tiles[0];
+    st.valid = st.tile < n;
+    st.first_use = st.valid && (st.rt == 0 || st.tile >= o.tiles[0]);
+    st.opens = st.tile == 0;
+    st.closes = st.tile + 1 == n;
+  }
+  return st;
+}
 
 // one piece of work, as the copy warp hands it to the others
 struct Work {
   int q_tok, n_tok;   // query tokens (prompt) or sequences (decode step)
   int head;
-  int tiles[2];       // key tiles for each row tile; 0: none
+  Order order;
   int key0;           // first key: an index into the packed keys, or the position in the sequence
   int limit0;         // prompt: keys that the first query token sees
   int n_keys;         // keys from key0 on that anyone sees
@@ -86,7 +132,7 @@ __device__ __forceinline__ unsigned long long global_timer_ns() {
   return t;
 }
 constexpr unsigned long long kWaitNs = 2000000000ull;
-__device__ __noinline__ bool mbar_wait_slow(uint64_t* bar, uint32_t parity) {
+__device__ __forceinline__ bool mbar_wait_slow(uint64_t* bar, uint32_t parity) {
   const unsigned long long start = global_timer_ns();
   do {
     if (mbar_try(bar, parity)) return true;
@@ -140,6 +186,15 @@ __device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b, uint
       "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
       : "memory");
 }
+// true in one lane of a whole warp
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(p));
+  return p != 0;
+}
+// the same value in all lanes, and the compiler knows
+__device__ __forceinline__ uint32_t uniform(uint32_t x) { return __shfl_sync(0xffffffffu, x, 0); }
+
 // one arrival when every MMA issued so far by this thread has completed
 __device__ __forceinline__ void umma_commit(uint64_t* bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
@@ -159,6 +214,13 @@ __device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[32]) {
                  "=r"(r[30]), "=r"(r[31])
                : "r"(taddr));
 }
+__device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+               :
+                 "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+                 "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+               : "r"(taddr));
+}
 // After the wait the registers of the loads before it may be read.  Naming them ties every use to this point.
 __device__ __forceinline__ void tmem_wait_ld(uint32_t (&r)[32]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;"
@@ -171,6 +233,14 @@ __device__ __forceinline__ void tmem_wait_ld(uint32_t (&r)[32]) {
                :
                : "memory");
 }
+__device__ __forceinline__ void tmem_wait_ld(uint32_t (&r)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               :
+                 "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+               :
+               : "memory");
+}
 __device__ __forceinline__ void tmem_st(uint32_t taddr, const uint32_t (&r)[16]) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, "
                "%12, %13, %14, %15, %16};"
@@ -178,18 +248,6 @@ __device__ __forceinline__ void tmem_st(uint32_t taddr, const uint32_t (&r)[16])
                :
                  "r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
                  "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
-               : "memory");
-}
-__device__ __forceinline__ void tmem_st(uint32_t taddr, const uint32_t (&r)[32]) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, "
-               "%12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, "
-               "%31, %32};"
-               :
-               :
-                 "r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
-                 "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
-                 "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
-                 "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
                : "memory");
 }
 __device__ __forceinline__ float exp2_fast(float x) {
@@ -203,9 +261,61 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   return w;
 }
 
+// two fp32 numbers in a register pair
+__device__ __forceinline__ uint64_t pair(float lo, float hi) {
+  uint64_t v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi));
+  return v;
+}
+__device__ __forceinline__ void unpair(uint64_t v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+// the larger of three, NaN if one is
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float m;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(a), "f"(b), "f"(c));
+  return m;
+}
+
+// 32 columns of a row
+__device__ __forceinline__ void mask_row(uint32_t (&s)[32], int seen) {
+#pragma unroll
+  for (int k = 0; k < 32; ++k)
+    if (k >= seen) s[k] = 0xff800000u;  // -inf
+}
+__device__ __forceinline__ void max_row(const uint32_t (&s)[32], float (&top)[4]) {
+#pragma unroll
+  for (int k = 0; k < 32; k += 8)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) top[i] = max3(top[i], __uint_as_float(s[k + 2 * i]), __uint_as_float(s[k + 2 * i + 1]));
+}
+// exp2(s c - mc), added up, and as bf16 pairs to 16 columns of tensor memory
+__device__ __forceinline__ void weights(const uint32_t (&s)[32], uint64_t c, uint64_t minus_mc, uint64_t (&sum)[2], uint32_t to) {
+  uint32_t packed[16];
+#pragma unroll
+  for (int k = 0; k < 16; ++k) {
+    const uint64_t x = fma2(pair(__uint_as_float(s[2 * k]), __uint_as_float(s[2 * k + 1])), c, minus_mc);
+    float a, b;
+    unpair(x, a, b);
+    a = exp2_fast(a);
+    b = exp2_fast(b);
+    sum[k & 1] = add2(sum[k & 1], pair(a, b));
+    packed[k] = pack_bf16(a, b);
+  }
+  tmem_st(to, packed);
+}
+
 struct Bars {
-  uint64_t full[10], empty[10], q_full, q_empty, s_full[2], p_full[2], o_full[2], work_full[kWorkSlots], work_empty[kWorkSlots],
-      drain;
+  uint64_t full[8], empty[8], q_full[2], q_empty[2], s_full[2], p_full[2], o_full[2], stats, read, work_full[kWorkSlots],
+      work_empty[kWorkSlots], turn[2], drain;
 };
 
 // keys that the row's token sees, counted from the piece's first key
@@ -213,247 +323,362 @@ template <bool PAGED> __device__ __forceinline__ int row_limit(const TcParams& p
   if constexpr (PAGED) return max(0, min(shared_seq_len(p.s, wk.q_tok + tok) - wk.key0, wk.n_keys));
   return max(0, min(wk.limit0 + tok, wk.n_keys));
 }
+__device__ __forceinline__ int key_tiles(int keys) { return max(1, (keys + kKeys - 1) / kKeys); }
 
 // ---- copy warp: finds the work, fetches Q, K and V --------------------------------------------------------------------
-template <int D, bool PAGED>
-__device__ __forceinline__ void copy_role(const TcParams& p, Bars* bars, Work* ring, unsigned char* base, SharedCursor cur) {
+// Tiles are fetched in the order in which the MMA thread first needs them: S runs two steps ahead of the second product.
+template <int D, bool PAGED> struct CopyRole {
   using C = Tc<D>;
-  const int lane = threadIdx.x & 31, G = p.group, tpm = kRows / G;
-  unsigned char* stage0 = base + 2 * C::tile;
-  uint32_t it = 0, q_it = 0, w_it = 0;
-  bool alive = true;
-  int next_item = 0, end_item = 0;
-  if constexpr (!PAGED) {
-    next_item = p.cta_begin[blockIdx.x];
-    end_item = p.cta_begin[blockIdx.x + 1];
+  const TcParams& p;
+  Bars* bars;
+  Work* ring;
+  unsigned char* base;
+  SharedCursor cur;
+  int next_item, end_item;
+  uint32_t it = 0, q_it = 0;                    // ring stages and Q tiles used so far
+  uint32_t s_work = 0, p_work = 0;              // pieces opened
+  int s_step = 0, s_n = 0, p_step = 0, p_n = 0; // steps of the piece at hand
+  int parity = 0;
+  Work s_wk, p_wk;                              // in registers: shared memory is slow for a chain of decisions
+  bool alive = true, ended = false;
+
+  __device__ __forceinline__ CopyRole(const TcParams& p_, Bars* b, Work* r, unsigned char* base_, const SharedCursor& c)
+      : p(p_), bars(b), ring(r), base(base_), cur(c) {
+    next_item = PAGED ? 0 : p.cta_begin[blockIdx.x];
+    end_item = PAGED ? 0 : p.cta_begin[blockIdx.x + 1];
   }
-  const auto give_up = [&] {
-    alive = false;
-    if (lane == 0) atomicOr(p.status, IA_DEV_STATUS_ATTEND_WAIT);
-  };
-  while (alive) {
-    Work wk{};
+  __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity_) {
+    if (alive && !__all_sync(0xffffffffu, mbar_wait(bar, parity_))) {
+      alive = false;
+      if ((threadIdx.x & 31) == 0) atomicOr(p.status, IA_DEV_STATUS_ATTEND_WAIT);
+    }
+    return alive;
+  }
+  __device__ __forceinline__ void find(Work& wk) {
+    const int tpm = kRows / p.group;
     if constexpr (PAGED) {
       wk.last = cur.left <= 0;
-      if (!wk.last) {
-        const SharedParams& s = p.s;
-        const SharedEntity ent = s.entities[cur.e];
-        int lo, hi;
-        entity_keys(s, cur.e, ent, lo, hi);
-        const int n = (int)min((int64_t)(cur.units - cur.k), cur.left);
-        const int2 lead = entity_lead(s, ent, hi);
-        wk.q_tok = ent.first_seq;
-        wk.n_tok = ent.n_seqs;
-        wk.head = cur.h;
-        wk.key0 = lo + cur.k * kKeys;
-        wk.n_keys = max(0, min(lead.y, wk.key0 + n * kKeys) - wk.key0);
-        wk.own = cur.e >= s.n_shared;
-        wk.row = lead.x;
-        wk.slot = (int64_t)(wk.own ? cur.e - s.n_shared : cur.e) * s.n_kv_heads + cur.h + blockIdx.x;
-        wk.tiles[0] = (wk.n_keys + kKeys - 1) / kKeys;
-        wk.tiles[1] = ent.n_seqs > tpm ? wk.tiles[0] : 0;
-        cur.left -= n;
-        cur.k = 0;
-        if (++cur.h == s.n_kv_heads) {
-          cur.h = 0;
-          if (cur.left > 0)  // some entity behind this one has units: they were counted
-            do cur.units = entity_units<kKeys>(s, ++cur.e);
-            while (cur.units == 0);
-        }
+      if (wk.last) return;
+      const SharedParams& s = p.s;
+      const SharedEntity ent = s.entities[cur.e];
+      int lo, hi;
+      entity_keys(s, cur.e, ent, lo, hi);
+      const int n = (int)min((int64_t)(cur.units - cur.k), cur.left);
+      const int2 lead = entity_lead(s, ent, hi);
+      wk.q_tok = ent.first_seq;
+      wk.n_tok = ent.n_seqs;
+      wk.head = cur.h;
+      wk.key0 = lo + cur.k * kKeys;
+      wk.n_keys = max(0, min(lead.y, wk.key0 + n * kKeys) - wk.key0);
+      wk.own = cur.e >= s.n_shared;
+      wk.row = lead.x;
+      wk.slot = (int64_t)(wk.own ? cur.e - s.n_shared : cur.e) * s.n_kv_heads + cur.h + blockIdx.x;
+      wk.order.split = ent.n_seqs <= tpm;
+      wk.order.tiles[0] = wk.order.tiles[1] = key_tiles(wk.n_keys);
+      cur.left -= n;
+      cur.k = 0;
+      if (++cur.h == s.n_kv_heads) {
+        cur.h = 0;
+        if (cur.left > 0)  // some entity behind this one has units: they were counted
+          do cur.units = entity_units<kKeys>(s, ++cur.e);
+          while (cur.units == 0);
       }
     } else {
       wk.last = next_item >= end_item;
-      if (!wk.last) {
-        const PromptItem item = p.items[next_item++];
-        wk.q_tok = item.q_tok;
-        wk.n_tok = item.n_tok;
-        wk.head = item.head;
-        wk.key0 = item.kv_tok;
-        wk.limit0 = item.limit0;
-        wk.n_keys = item.kv_len;
-#pragma unroll
-        for (int w = 0; w < 2; ++w) {
-          const int toks = min(item.n_tok - w * tpm, tpm);
-          if (toks > 0) wk.tiles[w] = (row_limit<false>(p, wk, w * tpm + toks - 1) + kKeys - 1) / kKeys;
-        }
-      }
-    }
-    const int slot = w_it % kWorkSlots;
-    if (!mbar_wait(&bars->work_empty[slot], ((w_it / kWorkSlots) & 1) ^ 1)) {
-      give_up();
-      break;
-    }
-    if (lane == 0) {
-      ring[slot] = wk;
-      mbar_arrive(&bars->work_full[slot]);
-    }
-    ++w_it;
-    if (wk.last) break;
-    const int tiles = max(wk.tiles[0], wk.tiles[1]);
-    for (int j = 0; j < tiles; ++j) {
-#pragma unroll
-      for (int which = 0; which < 2; ++which) {  // K, then V
-        if (which == 1 && j == 0) {              // Q behind the first K tile: the ring may be ahead of the last piece's end
-          if (!mbar_wait(&bars->q_empty, (q_it & 1) ^ 1)) {
-            give_up();
-            break;
-          }
-          if (lane == 0) {
-            const int active = (wk.tiles[0] > 0) + (wk.tiles[1] > 0);
-            mbar_arrive_expect_tx(&bars->q_full, (uint32_t)(active * C::halves * tpm * G * 128));
-#pragma unroll
-            for (int w = 0; w < 2; ++w)
-              for (int h = 0; wk.tiles[w] > 0 && h < C::halves; ++h)
-                tma_load_5d(smem_u32(base + w * C::tile + h * C::block), &p.tm_q, 0, 0, wk.q_tok + w * tpm, h, wk.head,
-                            &bars->q_full);
-          }
-          ++q_it;
-        }
-        const uint32_t st = it % C::stages;
-        unsigned char* dst = stage0 + (size_t)st * C::tile;
-        if (!mbar_wait(&bars->empty[st], ((it / C::stages) & 1) ^ 1)) {
-          give_up();
-          break;
-        }
-        ++it;
-        uint64_t* full = &bars->full[st];
-        if constexpr (!PAGED) {
-          if (lane == 0) {
-            mbar_arrive_expect_tx(full, C::tile);
-            tma_load_4d(smem_u32(dst), which == 0 ? &p.tm_k : &p.tm_v, 0, wk.key0 + j * kKeys, 0, wk.head, full);
-          }
-        } else {
-          const int valid = min(kKeys, wk.n_keys - j * kKeys);
-          const int pages = which == 0 ? (valid + 15) >> 4 : valid >> 4;
-          const int32_t* table = p.s.block_table + (int64_t)wk.row * p.s.max_pages + ((wk.key0 + j * kKeys) >> 4);
-          const int page = lane < (valid + 15) >> 4 ? table[lane] : 0;
-          const bool bad = page < 0 || (p.s.n_pool_pages > 0 && page >= p.s.n_pool_pages);
-          if (bad) atomicOr(p.status, DEV_STATUS_BAD_INDEX);
-          if (which == 1 && valid < kKeys) {
-            // The last tile of a sequence: behind its last token the page may hold anything, and the tile's other pages
-            // whatever the stage held before.  Zero times that must be zero, so the rows are written here.
-            const int tail = __shfl_sync(0xffffffffu, bad ? -1 : page, pages & 7);
-            const __nv_bfloat16* src = (const __nv_bfloat16*)p.s.v_pool + (int64_t)tail * p.s.page_stride + wk.head * p.s.head_stride;
-            for (int i = lane; i < (kKeys - pages * 16) * (D / 8); i += 32) {
-              const int row = i / (D / 8), c = i % (D / 8);
-              uint4 x = make_uint4(0, 0, 0, 0);
-              if (pages * 16 + row < valid && tail >= 0) x = *reinterpret_cast<const uint4*>(src + row * D + c * 8);
-              const int pg = pages + (row >> 4), t = row & 15;
-              *reinterpret_cast<uint4*>(dst + pg * (C::halves * 2048) + (c >> 3) * 2048 + t * 128 + (((c & 7) ^ (t & 7)) << 4)) = x;
-            }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-          }
-          if (lane == 0) mbar_arrive_expect_tx(full, (uint32_t)pages * (C::halves * 2048));
-          __syncwarp();
-          if (lane < pages) {
-            if (which == 0) {  // [128 keys][128 bytes] per half
-#pragma unroll
-              for (int h = 0; h < C::halves; ++h)
-                tma_load_5d(smem_u32(dst + h * C::block + lane * 2048), &p.tm_k, 0, 0, h, wk.head, page, full);
-            } else {           // page by page: a k step of the second product is one page
-              tma_load_5d(smem_u32(dst + lane * (C::halves * 2048)), &p.tm_v, 0, 0, 0, wk.head, page, full);
-            }
-          }
-          __syncwarp();
-        }
-      }
-      if (!alive) break;
+      if (wk.last) return;
+      const PromptItem item = p.items[next_item++];
+      wk.q_tok = item.q_tok;
+      wk.n_tok = item.n_tok;
+      wk.head = item.head;
+      wk.key0 = item.kv_tok;
+      wk.limit0 = item.limit0;
+      wk.n_keys = item.kv_len;
+      wk.order.split = item.n_tok <= tpm;
+      wk.order.tiles[0] = key_tiles(row_limit<false>(p, wk, min(item.n_tok, tpm) - 1));
+      wk.order.tiles[1] = key_tiles(row_limit<false>(p, wk, item.n_tok - 1));
     }
   }
-  if (!alive) {  // no copy may be in flight when the CTA ends
-    for (uint32_t i = it > C::stages ? it - C::stages : 0; i < it; ++i)
-      mbar_wait(&bars->full[i % C::stages], (i / C::stages) & 1);
-    if (q_it > 0) mbar_wait(&bars->q_full, (q_it - 1) & 1);
+  __device__ __forceinline__ unsigned char* stage(uint64_t*& full, bool alone) {
+    const uint32_t st = it % C::stages;
+    full = &bars->full[st];
+    if (!wait(&bars->empty[st], ((it / C::stages) & 1) ^ 1)) return nullptr;
+    if (alone && (threadIdx.x & 31) == 0) mbar_arrive(&bars->empty[st]);  // in the place of the set that does not read it
+    ++it;
+    return base + (2 + (size_t)st) * C::tile;
   }
-}
+  // key tile j of K (which = 0) or V
+  __device__ __forceinline__ void fetch(const Work& wk, int j, int which) {
+    const int lane = threadIdx.x & 31;
+    uint64_t* full;
+    unsigned char* dst = stage(full, wk.order.split || j >= wk.order.tiles[0]);
+    if (dst == nullptr) return;
+    if constexpr (!PAGED) {
+      if (lane == 0) {
+        mbar_arrive_expect_tx(full, C::tile);
+        tma_load_4d(smem_u32(dst), which == 0 ? &p.tm_k : &p.tm_v, 0, wk.key0 + j * kKeys, 0, wk.head, full);
+      }
+    } else {
+      const int valid = min(kKeys, wk.n_keys - j * kKeys);
+      const int held = (valid + 15) >> 4, pages = which == 0 ? held : valid >> 4;
+      const int32_t* table = p.s.block_table + (int64_t)wk.row * p.s.max_pages + ((wk.key0 + j * kKeys) >> 4);
+      const int page = lane < held ? table[lane] : 0;
+      const bool bad = page < 0 || (p.s.n_pool_pages > 0 && page >= p.s.n_pool_pages);
+      if (bad) atomicOr(p.status, DEV_STATUS_BAD_INDEX);
+      if (which == 1 && valid < kKeys) {
+        // The last tile of a sequence: behind its last token the page may hold anything, and the tile's other pages
+        // whatever the stage held before.  Zero times that must be zero, so the rows are written here.
+        const int tail = __shfl_sync(0xffffffffu, bad ? -1 : page, pages & 7);
+        const __nv_bfloat16* src = (const __nv_bfloat16*)p.s.v_pool + (int64_t)tail * p.s.page_stride + wk.head * p.s.head_stride;
+        for (int i = lane; i < (kKeys - pages * 16) * (D / 8); i += 32) {
+          const int row = i / (D / 8), c = i % (D / 8);
+          uint4 x = make_uint4(0, 0, 0, 0);
+          if (pages * 16 + row < valid && tail >= 0) x = *reinterpret_cast<const uint4*>(src + row * D + c * 8);
+          const int pg = pages + (row >> 4), t = row & 15;
+          *reinterpret_cast<uint4*>(dst + pg * (C::halves * 2048) + (c >> 3) * 2048 + t * 128 + (((c & 7) ^ (t & 7)) << 4)) = x;
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+      }
+      if (lane == 0) mbar_arrive_expect_tx(full, (uint32_t)pages * (C::halves * 2048));
+      __syncwarp();
+      if (lane < pages) {
+        if (which == 0) {  // [128 keys][128 bytes] per half
+#pragma unroll
+          for (int h = 0; h < C::halves; ++h)
+            tma_load_5d(smem_u32(dst + h * C::block + lane * 2048), &p.tm_k, 0, 0, h, wk.head, page, full);
+        } else {           // page by page: a k step of the second product is one page
+          tma_load_5d(smem_u32(dst + lane * (C::halves * 2048)), &p.tm_v, 0, 0, 0, wk.head, page, full);
+        }
+      }
+      __syncwarp();
+    }
+  }
+  __device__ __forceinline__ void s_next() {
+    if (ended || !alive) return;
+    const int lane = threadIdx.x & 31;
+    if (s_step == s_n) {  // open the next piece
+      const int slot = s_work % kWorkSlots;
+      if (!wait(&bars->work_empty[slot], ((s_work / kWorkSlots) & 1) ^ 1)) return;
+      s_wk = Work{};
+      find(s_wk);
+      s_wk.order.first = parity;
+      s_step = 0;
+      s_n = s_wk.last ? 0 : s_wk.order.steps();
+      parity ^= s_n & 1;
+      ended = s_wk.last;
+      if (lane == 0) {
+        ring[slot] = s_wk;
+        mbar_arrive(&bars->work_full[slot]);
+      }
+      __syncwarp();
+      ++s_work;
+      if (ended) return;
+    }
+    const Work& wk = s_wk;
+    const Step st = step_of(wk.order, s_step);
+    if (st.valid && st.opens && (!wk.order.split || s_step == 0)) {  // Q of the row tile
+      const uint32_t buf = q_it & 1;
+      if (!wait(&bars->q_empty[buf], ((q_it >> 1) & 1) ^ 1)) return;
+      ++q_it;
+      const int tpm = kRows / p.group;
+      if (lane == 0) {
+        if (!wk.order.split || s_n == 1) mbar_arrive(&bars->q_empty[buf]);  // only one set reads it
+        mbar_arrive_expect_tx(&bars->q_full[buf], (uint32_t)(C::halves * tpm * p.group * 128));
+        for (int h = 0; h < C::halves; ++h)
+          tma_load_5d(smem_u32(base + buf * C::tile + h * C::block), &p.tm_q, 0, 0, wk.q_tok + st.rt * tpm, h, wk.head,
+                      &bars->q_full[buf]);
+      }
+    }
+    if (st.first_use) fetch(wk, st.tile, 0);
+    ++s_step;
+  }
+  __device__ __forceinline__ bool p_next() {  // false: no steps left
+    if (!alive) return false;
+    if (p_step == p_n) {
+      if (ended && p_work + 1 == s_work) return false;  // the one that says so is the last
+      p_step = 0;
+      p_wk = ring[p_work % kWorkSlots];
+      p_n = p_wk.order.steps();
+      ++p_work;
+    }
+    const Step st = step_of(p_wk.order, p_step++);
+    if (st.first_use) fetch(p_wk, st.tile, 1);
+    return alive;
+  }
+  __device__ __forceinline__ void run() {
+    s_next();
+    s_next();
+    while (p_next()) s_next();
+    if (!alive) {  // no copy may be in flight when the CTA ends
+      for (uint32_t i = it > C::stages ? it - C::stages : 0; i < it; ++i) mbar_wait(&bars->full[i % C::stages], (i / C::stages) & 1);
+      for (uint32_t i = q_it > 2 ? q_it - 2 : 0; i < q_it; ++i) mbar_wait(&bars->q_full[i & 1], (i >> 1) & 1);
+    }
+  }
+};
 
 // ---- MMA thread -------------------------------------------------------------------------------------------------------
-template <int D, bool PAGED>
-__device__ __forceinline__ void mma_role(const TcParams& p, Bars* bars, const Work* ring, unsigned char* base, uint32_t tmem) {
+template <int D, bool PAGED> struct MmaRole {
   using C = Tc<D>;
-  const uint32_t q0 = smem_u32(base), stage0 = q0 + 2 * C::tile;
-  constexpr uint32_t kNextCols = PAGED ? 2048 : C::block, kStepBytes = PAGED ? C::halves * 2048 : 2048;
-  uint32_t it = 0, q_it = 0, w_it = 0, p_it[2] = {0, 0};
-  bool alive = true;
-  const auto wait = [&](uint64_t* bar, uint32_t parity) {
-    if (alive && !mbar_wait(bar, parity)) {
+  static constexpr uint32_t kNextCols = PAGED ? 2048 : C::block, kStepBytes = PAGED ? C::halves * 2048 : 2048;
+  const TcParams& p;
+  Bars* bars;
+  const Work* ring;
+  uint32_t q0, tmem;
+  uint32_t me;  // the set
+  uint32_t it = 0, q_it = 0, s_work = 0, p_work = 0, turn_it = 0, p_count = 0, q_buf = 0, k_use = 0, v_use = 0;  // q_buf: a bit per row tile
+  int s_step = 0, s_n = 0, p_step = 0, p_n = 0;
+  Order so, po;
+  bool alive = true, ended = false;
+
+  __device__ __forceinline__ MmaRole(const TcParams& p_, Bars* b, const Work* r, uint32_t base, uint32_t t, uint32_t me_)
+      : p(p_), bars(b), ring(r), q0(base), tmem(t), me(me_) {}
+  __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity) {
+        if (alive && !__all_sync(0xffffffffu, mbar_wait(bar, parity))) {
       alive = false;
-      atomicOr(p.status, IA_DEV_STATUS_ATTEND_WAIT);
+      if ((threadIdx.x & 31) == 0) atomicOr(p.status, IA_DEV_STATUS_ATTEND_WAIT);
     }
     return alive;
-  };
-  const auto issue_s = [&](int w, uint32_t k) {
-    const uint64_t a = umma_desc(q0 + w * C::tile, 0), b = umma_desc(k, 0);
-#pragma unroll
-    for (int h = 0; h < C::halves; ++h)
-#pragma unroll
-      for (int s = 0; s < 4; ++s)  // 16 dims = 32 bytes further inside the swizzled row
-        umma_ss(tmem + w * 128, a + (h * C::block + s * 32) / 16, b + (h * C::block + s * 32) / 16, kIdesc<kKeys, false>, h + s > 0);
-    umma_commit(&bars->s_full[w]);
-  };
-  while (alive) {
-    const int slot = w_it % kWorkSlots;
-    if (!wait(&bars->work_full[slot], (w_it / kWorkSlots) & 1)) break;
-    const int n0 = ring[slot].tiles[0], n1 = ring[slot].tiles[1], last = ring[slot].last;
-    mbar_arrive(&bars->work_empty[slot]);
-    ++w_it;
-    if (last) break;
-    const int tiles = max(n0, n1);
-    if (tiles == 0) continue;
-    uint32_t st = it % C::stages;
-    if (!wait(&bars->full[st], (it / C::stages) & 1) || !wait(&bars->q_full, q_it & 1)) break;
-    ++q_it;
-    ++it;
-    tc_fence_after();
-    if (n0 > 0) issue_s(0, stage0 + st * C::tile);
-    if (n1 > 0) issue_s(1, stage0 + st * C::tile);
-    umma_commit(&bars->empty[st]);
-    if (tiles == 1) umma_commit(&bars->q_empty);
-    for (int j = 0; j < tiles && alive; ++j) {
-      const uint32_t vs = it % C::stages, ks = (it + 1) % C::stages;
-      const bool more = j + 1 < tiles;
-      if (!wait(&bars->full[vs], (it / C::stages) & 1)) break;
-#pragma unroll
-      for (int w = 0; w < 2; ++w) {
-        const int n = w == 0 ? n0 : n1;
-        if (j >= n) continue;
-        if (!wait(&bars->p_full[w], p_it[w] & 1)) break;
-        ++p_it[w];
-        tc_fence_after();
-        const uint64_t b = umma_desc(stage0 + vs * C::tile, kNextCols);
-#pragma unroll
-        for (int s = 0; s < kKeys / 16; ++s)  // 16 keys: 8 columns of packed weights, 16 rows of V
-          umma_ts(tmem + 256 + w * 128, tmem + w * 128 + s * 8, b + s * kStepBytes / 16, kIdesc<D, true>, j + s > 0);
-        if (j + 1 == n) umma_commit(&bars->o_full[w]);
-        if (j + 1 < n) {
-          if (!wait(&bars->full[ks], ((it + 1) / C::stages) & 1)) break;
-          tc_fence_after();
-          issue_s(w, stage0 + ks * C::tile);
-        }
-      }
-      if (!alive) break;
-      umma_commit(&bars->empty[vs]);
-      if (more) {
-        umma_commit(&bars->empty[ks]);
-        if (j + 2 == tiles) umma_commit(&bars->q_empty);
-      }
-      it += more ? 2 : 1;
-    }
   }
-  umma_commit(&bars->drain);  // no MMA, and no arrival of one, may be in flight when the CTA ends
-  if (!mbar_wait(&bars->drain, 0)) atomicOr(p.status, IA_DEV_STATUS_ATTEND_WAIT);
-}
+  __device__ __forceinline__ bool wait_stage(uint32_t use) { return wait(&bars->full[use % C::stages], (use / C::stages) & 1); }
+  // What there is to do for the next step, decided before anything is waited for: between its products this thread only
+  // issues.
+  struct First { bool mine, valid, opens, closes; uint32_t use, buf, q_parity; };
+  struct Second { bool mine, valid, opens, closes; uint32_t use; };
+  __device__ __forceinline__ First s_next() {
+    First f{};
+    if (ended || !alive) return f;
+    if (s_step == s_n) {
+      const uint32_t slot = s_work % kWorkSlots;
+      if (!wait(&bars->work_full[slot], (s_work / kWorkSlots) & 1)) return f;
+      ++s_work;
+      if (ring[slot].last) {
+        ended = true;
+        return f;
+      }
+      s_step = 0;
+      so = ring[slot].order;
+      s_n = so.steps();
+    }
+    const int i = s_step++;
+    const Step st = step_of(so, i);
+    f.mine = ((so.first + i) & 1) == me;
+    f.valid = st.valid;
+    if (!st.valid) return f;
+    if (st.first_use) k_use = it++;
+    if (st.opens && (!so.split || i == 0)) {
+      q_buf = (q_buf & ~(1u << st.rt)) | ((q_it & 1) << st.rt);
+      ++q_it;
+    }
+    f.opens = st.opens;
+    f.closes = st.closes;
+    f.use = k_use;
+    f.buf = (q_buf >> st.rt) & 1;
+    f.q_parity = ((q_it - 1 - (((q_it - 1) & 1) ^ f.buf)) >> 1) & 1;
+    return f;
+  }
+  __device__ __forceinline__ bool p_next(Second& f) {  // false: no steps left
+    f = Second{};
+    if (!alive) return false;
+    if (p_step == p_n) {
+      if (p_work > 0 && elect_one()) mbar_arrive(&bars->work_empty[(p_work - 1) % kWorkSlots]);
+      if (ended && p_work + 1 == s_work) return false;
+      p_step = 0;
+      po = ring[p_work % kWorkSlots].order;
+      p_n = po.steps();
+      ++p_work;
+    }
+    const int i = p_step++;
+    const Step st = step_of(po, i);
+    f.mine = ((po.first + i) & 1) == me;
+    f.valid = st.valid;
+    if (!st.valid) return true;
+    if (st.first_use) v_use = it++;
+    f.opens = st.opens;
+    f.closes = st.closes;
+    f.use = v_use;
+    return true;
+  }
+  // The descriptors' upper halves never change; what is added to the lower ones is known to the compiler.  The values have to
+  // be known as the same in all lanes, or every operand of every MMA is moved to the uniform registers anew.
+  __device__ __forceinline__ void first_product(const First& f, bool take) {
+    const uint32_t ks = uniform(f.use % C::stages), buf = uniform(f.buf), closes = uniform(f.closes);
+    const uint64_t a = umma_desc(q0 + buf * C::tile, 0), b = umma_desc(q0 + (2 + ks) * C::tile, 0);
+    if (f.opens && !wait(&bars->q_full[f.buf], f.q_parity)) return;
+    if (!wait_stage(f.use)) return;
+    if (take && !wait(&bars->turn[me], turn_it++ & 1)) return;
+    tc_fence_after();
+    if (elect_one()) {
+#pragma unroll
+      for (int h = 0; h < C::halves; ++h)
+#pragma unroll
+        for (int s = 0; s < 4; ++s)  // 16 dims = 32 bytes further inside the swizzled row
+          umma_ss(tmem + me * 128, a + (h * C::block + s * 32) / 16, b + (h * C::block + s * 32) / 16, kIdesc<kKeys, false>, h + s > 0);
+      umma_commit(&bars->s_full[me]);
+      umma_commit(&bars->empty[ks]);
+      if (closes) umma_commit(&bars->q_empty[buf]);
+    }
+    __syncwarp();
+  }
+  __device__ __forceinline__ void second_product(const Second& f) {
+    const uint32_t vs = uniform(f.use % C::stages), first = uniform(f.opens), closes = uniform(f.closes);
+    const uint64_t b = umma_desc(q0 + (2 + vs) * C::tile, kNextCols);
+    if (!wait_stage(f.use) || !wait(&bars->p_full[me], p_count & 1)) return;
+    if (!wait(&bars->turn[me], turn_it++ & 1)) return;
+    tc_fence_after();
+    if (elect_one()) {
+#pragma unroll
+      for (int s = 0; s < kKeys / 16; ++s)  // 16 keys: 8 columns of packed weights, 16 rows of V
+        umma_ts(tmem + 256 + me * 128, tmem + me * 128 + s * 8, b + s * kStepBytes / 16, kIdesc<D, true>, s > 0 ? 1u : first ^ 1u);
+      if (closes) umma_commit(&bars->o_full[me]);
+    }
+    __syncwarp();
+    ++p_count;
+  }
+  __device__ __forceinline__ void pass() {
+    if (elect_one()) mbar_arrive(&bars->turn[me ^ 1]);
+  }
+  __device__ __forceinline__ void release(uint32_t use) {
+    const uint32_t st = uniform(use % C::stages);
+    if (elect_one()) umma_commit(&bars->empty[st]);
+    __syncwarp();
+  }
+  __device__ __forceinline__ void run() {
+#pragma unroll 1
+    for (int i = 0; i < 2; ++i) {
+      const First s = s_next();
+      if (i != me) continue;
+      if (s.mine) first_product(s, true);  // set 0's turn was given at the start
+      else if (!wait(&bars->turn[me], turn_it++ & 1)) break;
+      pass();
+    }
+    Second v;
+    while (p_next(v)) {
+      const First s = s_next();  // two steps ahead: the same set's
+      if (!v.mine) continue;
+      if (v.valid) second_product(v);
+      else wait(&bars->turn[me], turn_it++ & 1);
+      if (s.mine && s.valid && alive) first_product(s, false);
+      pass();
+      if (v.valid && alive) release(v.use);
+    }
+    if (elect_one()) umma_commit(&bars->drain);  // no MMA, and no arrival of one, may be in flight when the CTA ends
+    __syncwarp();
+    alive = true;
+    wait(&bars->drain, 0);
+  }
+};
 
 // ---- softmax warps ----------------------------------------------------------------------------------------------------
 template <int D, bool PAGED>
-__device__ __forceinline__ void softmax_role(const TcParams& p, Bars* bars, const Work* ring, uint32_t tmem) {
+__device__ __forceinline__ void softmax_role(const TcParams& p, Bars* bars, const Work* ring, uint32_t tmem, unsigned char* out_base,
+                                             float2 (*stats)[kRows]) {
+  using Out = std::conditional_t<PAGED, float, __nv_bfloat16>;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, w = warp >> 2, row = (warp & 3) * 32 + lane;
-  const int G = p.group, tpm = kRows / G, tok = w * tpm + row / G, g = row % G;
+  const int G = p.group, tpm = kRows / G, row_tok = row / G, g = row % G;
   const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-  const uint32_t s_addr = tmem + lanes + w * 128, o_addr = tmem + lanes + 256 + w * 128;
+  const uint32_t s_addr = tmem + lanes + w * 128, o_addr = tmem + lanes + 256;
   const float c = kLog2e * rsqrtf((float)D);
-  uint32_t s_it = 0, o_it = 0;
+  uint32_t s_it = 0, o_it = 0, x_it = 0;
   const auto wait = [&](uint64_t* bar, uint32_t parity) {  // the whole warp goes on or none of it
     const bool ok = __all_sync(0xffffffffu, mbar_wait(bar, parity));
     if (!ok && lane == 0) atomicOr(p.status, IA_DEV_STATUS_ATTEND_WAIT);
@@ -462,220 +687,276 @@ __device__ __forceinline__ void softmax_role(const TcParams& p, Bars* bars, cons
   for (uint32_t w_it = 0;; ++w_it) {
     const int slot = w_it % kWorkSlots;
     if (!wait(&bars->work_full[slot], (w_it / kWorkSlots) & 1)) return;
-    const Work wk = ring[slot];
-    __syncwarp();
-    if (lane == 0) mbar_arrive(&bars->work_empty[slot]);
+    const Work& wk = ring[slot];  // read where it is needed: registers are scarce in the loop below
     if (wk.last) return;
-    const int n = wk.tiles[w];
+    const auto done = [&] {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars->work_empty[slot]);
+    };
+    const bool split = wk.order.split;
+    const int me = w ^ wk.order.first;  // row tile, or place in the order of key tiles
+    const int total = wk.order.tiles[split ? 0 : me], stride = split ? 2 : 1, begin = split ? me : 0;
+    const int tok = (split ? 0 : me * tpm) + row_tok;
     const bool valid = row < tpm * G && tok < wk.n_tok;
     const bool busy = __any_sync(0xffffffffu, valid);
     const int limit = valid ? row_limit<PAGED>(p, wk, tok) : 0;
-    const int least = __reduce_min_sync(0xffffffffu, limit);  // below it nothing is masked for the warp
+    const int least = __reduce_min_sync(0xffffffffu, valid ? limit : 0x7fffffff);  // below it nothing is masked
+    if (begin >= total) {  // the other set has the only key tile
+      done();
+      continue;
+    }
     float m = -INFINITY, l = 0.f;
-    for (int j = 0; j < n; ++j) {
-      if (!wait(&bars->s_full[w], s_it & 1)) return;
+    for (int j = begin; j < total; j += stride) {
+            if (!wait(&bars->s_full[w], s_it & 1)) return;
       ++s_it;
       if (busy) {
         tc_fence_after();
-        uint32_t s[4][32];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) tmem_ld(s_addr + 32 * i, s[i]);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) tmem_wait_ld(s[i]);
-        const int seen = limit - j * kKeys;
-        if (least < (j + 1) * kKeys) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int k = 0; k < 32; ++k)
-              if (32 * i + k >= seen) s[i][k] = 0xff800000u;  // -inf
-        }
-        float top[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          top[i] = __uint_as_float(s[i][0]);
-#pragma unroll
-          for (int k = 1; k < 31; k += 2) top[i] = fmaxf(fmaxf(top[i], __uint_as_float(s[i][k])), __uint_as_float(s[i][k + 1]));
-          top[i] = fmaxf(top[i], __uint_as_float(s[i][31]));
-        }
-        const float t = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-        if (j == 0) {
+        const int seen = limit - j * kKeys, all_seen = least - j * kKeys;
+        uint32_t ra[32], rb[32], rc[32], rd[32];
+        tmem_ld(s_addr, ra);
+        tmem_ld(s_addr + 32, rb);
+        tmem_ld(s_addr + 64, rc);
+        tmem_ld(s_addr + 96, rd);
+        tmem_wait_ld(ra);
+        tmem_wait_ld(rb);
+        tmem_wait_ld(rc);
+        tmem_wait_ld(rd);
+        if (all_seen < 32) mask_row(ra, seen);
+        if (all_seen < 64) mask_row(rb, seen - 32);
+        if (all_seen < 96) mask_row(rc, seen - 64);
+        if (all_seen < 128) mask_row(rd, seen - 96);
+        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        max_row(ra, top);
+        max_row(rb, top);
+        max_row(rc, top);
+        max_row(rd, top);
+        const float t = max3(top[0], top[1], max3(top[2], top[3], -INFINITY));
+        if (j == begin) {
           m = t;
         } else {
-          const bool far = (t - m) * c > 8.f;  // also where m is still -inf
+          const bool far = !((t - m) * c <= 8.f) && t != -INFINITY;  // also where m is still -inf, or t is NaN
           if (__any_sync(0xffffffffu, far)) {
             const float keep = far ? exp2_fast((m - t) * c) : 1.f;
             if (far) {
               m = t;
               l *= keep;
             }
-            uint32_t o[32];
-#pragma unroll
-            for (int i = 0; i < D / 32; ++i) {  // the products of the tile before are complete: S of this one came after them
-              tmem_ld(o_addr + 32 * i, o);
+#pragma unroll 1
+            for (int i = 0; i < D; i += 16) {  // the products of the tile before are complete: S of this one came after them
+              uint32_t o[16];
+              tmem_ld(o_addr + w * 128 + i, o);
               tmem_wait_ld(o);
 #pragma unroll
-              for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * keep);
-              tmem_st(o_addr + 32 * i, o);
+              for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * keep);
+              tmem_st(o_addr + w * 128 + i, o);
             }
           }
         }
-        const float mc = m == -INFINITY ? 0.f : m * c;
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          uint32_t packed[16];
-#pragma unroll
-          for (int k = 0; k < 32; k += 2) {
-            const float a = exp2_fast(fmaf(__uint_as_float(s[i][k]), c, -mc)), b = exp2_fast(fmaf(__uint_as_float(s[i][k + 1]), c, -mc));
-            sum[(k >> 1) & 3] += a + b;
-            packed[k >> 1] = pack_bf16(a, b);
-          }
-          tmem_st(s_addr + 16 * i, packed);
-        }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        float mc = m == -INFINITY ? 0.f : m * c;
+        mc = fmaf(mc, 0.f, mc);  // infinite: NaN, as infinity - infinity in the weights
+        const uint64_t c2 = pair(c, c), mc2 = pair(-mc, -mc);
+        uint64_t sum[2] = {0, 0};
+        weights(ra, c2, mc2, sum, s_addr);
+        weights(rb, c2, mc2, sum, s_addr + 16);
+        weights(rc, c2, mc2, sum, s_addr + 32);
+        weights(rd, c2, mc2, sum, s_addr + 48);
+        float la, lb;
+        unpair(add2(sum[0], sum[1]), la, lb);
+        l += la + lb;
         tmem_wait_st();
         tc_fence_before();
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars->p_full[w]);
     }
-    if (n > 0) {
-      if (!wait(&bars->o_full[w], o_it & 1)) return;
-      ++o_it;
+    if (!wait(&bars->o_full[w], o_it & 1)) return;
+    ++o_it;
+    tc_fence_after();
+    // ---- output: this set's O scaled, or over half of the columns both sets' ----
+    float scale = 0.f, its_scale = 0.f, lse = -INFINITY;
+    const bool merge = split && total > 1, empty = limit <= 0;
+    if (merge) {
+      stats[w][row] = make_float2(m, l);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars->stats);
+      if (!wait(&bars->stats, x_it & 1)) return;
       tc_fence_after();
+      const float2 other = stats[w ^ 1][row];
+      const float top = fmaxf(m, other.x), at = top == -INFINITY ? 0.f : top;
+      const float mine = exp2_fast((m - at) * c), its = exp2_fast((other.x - at) * c), sum = l * mine + other.y * its;
+      if (!empty) {
+        scale = mine / sum;
+        its_scale = its / sum;
+        lse = (top * c + __log2f(sum)) * kLn2;
+      }
+    } else if (!empty) {
+      scale = 1.f / l;
+      lse = (m * c + __log2f(l)) * kLn2;
     }
-    if (!busy) continue;
-    // ---- output ----
-    const int hq = p.group * (PAGED ? p.s.n_kv_heads : p.t.n_kv_heads);
-    const bool empty = limit <= 0;
-    const float inv = empty ? 0.f : 1.f / l;
-    const float lse = empty ? -INFINITY : (m * c + __log2f(l)) * kLn2;
-    __nv_bfloat16* out = nullptr;
-    float* part = nullptr;
-    float* lse_out = nullptr;
+    const int64_t hq = (int64_t)G * (PAGED ? p.s.n_kv_heads : p.t.n_kv_heads);
+    Out* out;          // of the piece's first row
+    float* lse_out;    // of this row
+    int at;            // this row, in elements from `out`; -1: none
     if constexpr (PAGED) {
-      const int64_t at = wk.slot * (wk.own ? G : p.s.row_block) + tok * G + g;
-      part = (wk.own ? p.s.o_own : p.s.o_shared) + at * D;
-      lse_out = (wk.own ? p.s.lse_own : p.s.lse_shared) + at;
+      const int64_t first = wk.slot * (wk.own ? G : p.s.row_block);
+      out = (wk.own ? p.s.o_own : p.s.o_shared) + first * D;
+      at = (tok * G + g) * D;
+      lse_out = (wk.own ? p.s.lse_own : p.s.lse_shared) + first + tok * G + g;
     } else {
-      const int64_t at = (int64_t)(wk.q_tok + tok) * hq + wk.head * G + g;
-      out = (__nv_bfloat16*)p.t.out + at * D;
-      lse_out = p.t.lse == nullptr ? nullptr : p.t.lse + at;
+      const int64_t first = wk.q_tok * hq + wk.head * G;
+      out = (Out*)p.t.out + first * D;
+      at = (int)(tok * hq + g) * D;
+      lse_out = p.t.lse == nullptr ? nullptr : p.t.lse + first + tok * hq + g;
     }
+    if (!valid) at = -1;
+    const int col0 = merge ? w * (D / 2) : 0, col1 = merge ? col0 + D / 2 : D;
+    unsigned char* rows = out_base + warp * Tc<D>::out_warp;  // [32 rows][32 columns], 16-byte words swizzled
+    constexpr int kWords = 32 * sizeof(Out) / 16;             // words of a row: 8 or 4
     bool finite = true;
+    if (busy) {
+#pragma unroll 1
+      for (int col = col0; col < col1; col += 32) {
+        float x[32];
+        {
+          uint32_t o[32];
+          tmem_ld(o_addr + w * 128 + col, o);
+          tmem_wait_ld(o);
 #pragma unroll
-    for (int i = 0; i < D / 32; ++i) {
-      uint32_t o[32];
-      if (n > 0) {
-        tmem_ld(o_addr + 32 * i, o);
-        tmem_wait_ld(o);
-      }
-      float x[32];
+          for (int k = 0; k < 32; ++k) x[k] = empty ? 0.f : __uint_as_float(o[k]) * scale;
+          if (merge) {
+            tmem_ld(o_addr + (w ^ 1) * 128 + col, o);
+            tmem_wait_ld(o);
 #pragma unroll
-      for (int k = 0; k < 32; ++k) {
-        x[k] = empty ? 0.f : __uint_as_float(o[k]) * inv;
-        finite &= fabsf(x[k]) <= 3.4028235e38f;
-      }
-      if (valid) {
-        if constexpr (PAGED) {
-#pragma unroll
-          for (int k = 0; k < 32; k += 4)
-            *reinterpret_cast<float4*>(part + 32 * i + k) = make_float4(x[k], x[k + 1], x[k + 2], x[k + 3]);
-        } else {
-#pragma unroll
-          for (int k = 0; k < 32; k += 8)
-            *reinterpret_cast<uint4*>(out + 32 * i + k) = make_uint4(pack_bf16(x[k], x[k + 1]), pack_bf16(x[k + 2], x[k + 3]),
-                                                                     pack_bf16(x[k + 4], x[k + 5]), pack_bf16(x[k + 6], x[k + 7]));
+            for (int k = 0; k < 32; ++k) x[k] = empty ? 0.f : fmaf(__uint_as_float(o[k]), its_scale, x[k]);
+          }
         }
+#pragma unroll
+        for (int k = 0; k < 32; ++k) finite &= fabsf(x[k]) <= 3.4028235e38f;
+#pragma unroll
+        for (int k = 0; k < kWords; ++k) {
+          uint4 v;
+          if constexpr (PAGED)
+            v = make_uint4(__float_as_uint(x[4 * k]), __float_as_uint(x[4 * k + 1]), __float_as_uint(x[4 * k + 2]), __float_as_uint(x[4 * k + 3]));
+          else
+            v = make_uint4(pack_bf16(x[8 * k], x[8 * k + 1]), pack_bf16(x[8 * k + 2], x[8 * k + 3]), pack_bf16(x[8 * k + 4], x[8 * k + 5]),
+                           pack_bf16(x[8 * k + 6], x[8 * k + 7]));
+          *reinterpret_cast<uint4*>(rows + lane * 128 + ((k ^ (lane & 7)) << 4)) = v;
+        }
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) {  // kWords neighbouring lanes write a row's run
+          const int r = i * (32 / kWords) + lane / kWords, k = lane % kWords;
+          const int to = __shfl_sync(0xffffffffu, at, r);
+          const uint4 v = *reinterpret_cast<const uint4*>(rows + r * 128 + ((k ^ (r & 7)) << 4));
+          if (to >= 0) *reinterpret_cast<uint4*>(out + to + col + k * (16 / (int)sizeof(Out))) = v;
+        }
+        __syncwarp();
       }
+      if (valid && lse_out != nullptr && (!merge || me == 0)) *lse_out = lse;
     }
-    if (valid && lse_out != nullptr) *lse_out = lse;
+    if (merge) {  // the other set has read O before the next piece's products may overwrite it
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars->read);
+      if (!wait(&bars->read, x_it & 1)) return;
+      ++x_it;
+    }
     const unsigned bad = __ballot_sync(0xffffffffu, valid && !finite);
     if (bad != 0) {  // see exact_row
-      const auto redo = [&](const auto& key, const __nv_bfloat16* q) {
-        const int end = PAGED ? wk.n_keys : n * kKeys;
-        const int last = last_not_finite<__nv_bfloat16, D>(least, end, key);
+      using T = __nv_bfloat16;
+      const auto redo = [&](const auto& key, const T* q, int64_t tok_stride, int64_t head_stride) {
+        const int last = last_not_finite<T, D>(least, PAGED ? wk.n_keys : total * kKeys, key);
         for (int r = 0; r < 32; ++r) {
-          const int lim = __shfl_sync(0xffffffffu, limit, r);
+          const int lim = __shfl_sync(0xffffffffu, limit, r), to = __shfl_sync(0xffffffffu, at, r);
+          const int q_tok = __shfl_sync(0xffffffffu, tok, r), q_head = __shfl_sync(0xffffffffu, g, r);
           if (!((bad >> r) & 1) || last < lim) continue;
-          const uint64_t q_row = __shfl_sync(0xffffffffu, (unsigned long long)q, r);
           float x[D / 32], mx, lx;
-          exact_row<__nv_bfloat16, D>((const __nv_bfloat16*)q_row, 0, lim, c, key, x, mx, lx);
-          const uint64_t to = __shfl_sync(0xffffffffu, PAGED ? (unsigned long long)part : (unsigned long long)out, r);
-          float* lse_to = (float*)__shfl_sync(0xffffffffu, (unsigned long long)lse_out, r);
+          exact_row<T, D>(q + q_tok * tok_stride + q_head * head_stride, 0, lim, c, key, x, mx, lx);
 #pragma unroll
-          for (int i = 0; i < D / 32; ++i) {
-            if constexpr (PAGED) ((float*)to)[lane + 32 * i] = x[i] / lx;
-            else ((__nv_bfloat16*)to)[lane + 32 * i] = __float2bfloat16_rn(x[i] / lx);
-          }
-          if (lane == 0 && lse_to != nullptr) *lse_to = (mx + __log2f(lx)) * kLn2;
+          for (int i = 0; i < D / 32; ++i)
+            if (lane + 32 * i >= col0 && lane + 32 * i < col1) from_f32(out[to + lane + 32 * i], x[i] / lx);
         }
       };
       __syncwarp();
-      using T = __nv_bfloat16;
       if constexpr (PAGED) {
         const PagedKeys<T> key{(const T*)p.s.k_pool + wk.head * p.s.head_stride, (const T*)p.s.v_pool + wk.head * p.s.head_stride,
                                p.s.block_table + (int64_t)wk.row * p.s.max_pages + (wk.key0 >> 4), p.s.page_stride, D,
                                p.s.n_pool_pages, p.s.max_pages - (wk.key0 >> 4)};
-        redo(key, (const T*)p.s.q + ((int64_t)(wk.q_tok + tok) * hq + wk.head * G + g) * D);
+        redo(key, (const T*)p.s.q + (wk.q_tok * hq + wk.head * G) * D, hq * D, D);
       } else {
         const PackedKeys<T> key{(const T*)p.t.k + wk.key0 * p.t.k_tok_stride + wk.head * p.t.k_head_stride,
                                 (const T*)p.t.v + wk.key0 * p.t.v_tok_stride + wk.head * p.t.v_head_stride, p.t.k_tok_stride,
                                 p.t.v_tok_stride, p.t.n_kv_tok - wk.key0};
-        redo(key, (const T*)p.t.q + (int64_t)(wk.q_tok + tok) * p.t.q_tok_stride + (int64_t)(wk.head * G + g) * p.t.q_head_stride);
+        redo(key, (const T*)p.t.q + (int64_t)wk.q_tok * p.t.q_tok_stride + (int64_t)wk.head * G * p.t.q_head_stride, p.t.q_tok_stride,
+             p.t.q_head_stride);
       }
     }
+    done();
   }
 }
+
+struct Control {
+  Bars bars;
+  Work ring[kWorkSlots];
+  float2 stats[2][kRows];  // (m, l) of either set, for the merge
+  unsigned long long scratch[kThreads / 32];
+  uint32_t tmem;
+};
 
 template <int D, bool PAGED>
 __global__ void __launch_bounds__(kThreads, 1) attend_tc_kernel(const __grid_constant__ TcParams p) {
   using C = Tc<D>;
-  extern __shared__ __align__(1024) unsigned char smem_raw[];
-  unsigned char* base = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  __shared__ Bars bars;
-  __shared__ Work ring[kWorkSlots];
-  __shared__ uint32_t tmem_s;
-  __shared__ unsigned long long scratch[kThreads / 32];
+  extern __shared__ __align__(1024) unsigned char base[];
+  static_assert(sizeof(Control) <= 3072, "the whole of an SM's shared memory is spoken for");
+  Control& ctl = *reinterpret_cast<Control*>(base + C::control);
+  Bars& bars = ctl.bars;
   const int warp = threadIdx.x >> 5;
+  if ((smem_u32(base) & 1023u) != 0) {  // swizzled tiles start on 1024 bytes; there is no room to round up
+    if (threadIdx.x == 0) atomicOr(p.status, IA_DEV_STATUS_ATTEND_WAIT);
+    return;
+  }
   if (threadIdx.x == 0) {
     for (int i = 0; i < C::stages; ++i) {
       mbar_init(&bars.full[i], 1);
-      mbar_init(&bars.empty[i], 1);
+      mbar_init(&bars.empty[i], 2);  // both sets, or one and the copy warp
     }
-    mbar_init(&bars.q_full, 1);
-    mbar_init(&bars.q_empty, 1);
+    mbar_init(&bars.stats, 8);  // a lane of each softmax warp
+    mbar_init(&bars.read, 8);
     for (int w = 0; w < 2; ++w) {
+      mbar_init(&bars.q_full[w], 1);
+      mbar_init(&bars.q_empty[w], 2);
       mbar_init(&bars.s_full[w], 1);
       mbar_init(&bars.p_full[w], 4);  // a lane of each warp
+      mbar_init(&bars.turn[w], 1);
       mbar_init(&bars.o_full[w], 1);
     }
     for (int i = 0; i < kWorkSlots; ++i) {
       mbar_init(&bars.work_full[i], 1);
-      mbar_init(&bars.work_empty[i], 9);  // eight softmax warps and the MMA thread
+      mbar_init(&bars.work_empty[i], 10);  // eight softmax warps and two MMA threads
     }
-    mbar_init(&bars.drain, 1);
+    mbar_init(&bars.drain, 2);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    mbar_arrive(&bars.turn[0]);  // set 0 begins
   }
   if (warp == kMmaWarp) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_s)), "r"(512) : "memory");
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&ctl.tmem)), "r"(512) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = tmem_s;
+  const uint32_t tmem = ctl.tmem;
   grid_dependency_wait();
   grid_launch_dependents();
   SharedCursor cur{};
-  if constexpr (PAGED) cur = find_share<kKeys, kThreads>(p.s, blockIdx.x, gridDim.x, scratch);
-  if (warp == kCopyWarp) {
-    copy_role<D, PAGED>(p, &bars, ring, base, cur);
-  } else if (warp == kMmaWarp) {
-    if ((threadIdx.x & 31) == 0) mma_role<D, PAGED>(p, &bars, ring, base, tmem);
+  if constexpr (PAGED) cur = find_share<kKeys, kThreads>(p.s, blockIdx.x, gridDim.x, ctl.scratch);
+  if (warp < kCopyWarp) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
+    softmax_role<D, PAGED>(p, &bars, ctl.ring, tmem, base + C::tiles, ctl.stats);
   } else {
-    softmax_role<D, PAGED>(p, &bars, ring, tmem);
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+    if (warp == kCopyWarp) CopyRole<D, PAGED>(p, &bars, ctl.ring, base, cur).run();
+    if (warp >= kMmaWarp && warp < kMmaWarp + 2) MmaRole<D, PAGED>(p, &bars, ctl.ring, smem_u32(base), uniform(tmem), uniform(warp - kMmaWarp)).run();
   }
   __syncwarp();
   tc_fence_before();
@@ -743,7 +1024,12 @@ int launch_prompt_tc(const PromptTensors& t, int head_dim, const PromptItem* ite
   p.status = device_status_address();
   if (p.status == nullptr) return IA_ERR_LAUNCH;
   if (int s = encode_q(&p.tm_q, t.q, head_dim, t.group, t.n_kv_heads, t.n_q_tok, t.q_tok_stride, t.q_head_stride)) return s;
-  if (t.n_kv_tok > 0) {
+  if (t.n_kv_tok == 0) {  // every row is empty, but still has a tile of keys that it does not see: let it be the queries
+    p.t.k = p.t.v = t.q;
+    const int64_t dims[4] = {64, t.n_q_tok, head_dim / 64, t.n_kv_heads}, strides[3] = {t.q_tok_stride, 64, t.q_head_stride};
+    if (int s = encode<4>(&p.tm_k, t.q, dims, strides, {64, kKeys, head_dim / 64, 1})) return s;
+    p.tm_v = p.tm_k;
+  } else {
     const int64_t dims[4] = {64, t.n_kv_tok, head_dim / 64, t.n_kv_heads};
     const int box[4] = {64, kKeys, head_dim / 64, 1};
     const int64_t ks[3] = {t.k_tok_stride, 64, t.k_head_stride}, vs[3] = {t.v_tok_stride, 64, t.v_head_stride};

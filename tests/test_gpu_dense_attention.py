@@ -95,6 +95,23 @@ def test_prompt_rows_do_not_see_the_future_or_the_neighbour(dtype, d, hq, hkv, p
         assert bool(torch.isnan(out[at:170].float()).all())
 
 
+@pytest.mark.parametrize("dtype,d", [(BF16, 128), (BF16, 64), (F32, 64)])
+@pytest.mark.parametrize("poison", [float("nan"), float("inf")])
+@pytest.mark.parametrize("at", [0, 15, 24, 31, 63, 100, 127, 129, 158])
+def test_prompt_a_bad_key_spoils_exactly_the_rows_that_see_it(dtype, d, poison, at):
+    """Wherever in a tile the key lies; a logit of +infinity gives NaN too (infinity minus infinity), one of -infinity does
+    not, so the key's sign is taken from the query."""
+    lens = [160]
+    q, k, v, plan = prompt_case(2, 1, d, dtype, lens, lens, seed=17)
+    q = q.abs()
+    k[at] = 0
+    k[at, :, 0] = poison
+    out = plan.run(q, k, v).float()
+    bad = torch.isnan(out).flatten(1).all(dim=1).cpu()
+    assert ops.device_status() == 0
+    assert not bool(torch.isnan(out[:at]).any()) and bool(bad[at:].all())
+
+
 def test_prompt_graph_streams_and_threads():
     q_lens = [200, 31]
     q, k, v, plan = prompt_case(8, 2, 128, BF16, q_lens, q_lens, seed=7)
