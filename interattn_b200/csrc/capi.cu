@@ -723,13 +723,15 @@ static int64_t carve_shared(int n_shared, const ia_geom& g, char* base, SharedPa
     off += align256(bytes);
     return r;
   };
-  char* a[4] = {take(slots_shared * shared_row_block(g.dtype) * g.head_dim * 4), take(slots_shared * shared_row_block(g.dtype) * 4),
-                take(slots_own * g.group_size * g.head_dim * 4), take(slots_own * g.group_size * 4)};
+  char* a[5] = {take(slots_shared * shared_row_block(g.dtype) * g.head_dim * 4), take(slots_shared * shared_row_block(g.dtype) * 4),
+                take(slots_own * g.group_size * g.head_dim * 4), take(slots_own * g.group_size * 4),
+                take(((int64_t)n_shared + g.batch + 1) * 8)};
   if (p) {
     p->o_shared = (float*)a[0];
     p->lse_shared = (float*)a[1];
     p->o_own = (float*)a[2];
     p->lse_own = (float*)a[3];
+    p->unit_begin = (long long*)a[4];
   }
   return off;
 }

@@ -247,7 +247,7 @@ __global__ void __launch_bounds__(kThreads) shared_attention_kernel(const Shared
   const int G = p.group, hq = p.n_kv_heads * G, cta = blockIdx.x;
   SharedCursor c = find_share<kKeys, kThreads>(p, cta, gridDim.x, scratch);
   while (c.left > 0) {
-    const SharedEntity ent = p.entities[c.e];
+    const SharedEntity ent = load_entity(p, c.e);
     int lo, hi;
     entity_keys(p, c.e, ent, lo, hi);
     const int n = (int)min((int64_t)(c.units - c.k), c.left);
@@ -284,82 +284,62 @@ __global__ void __launch_bounds__(kThreads) shared_attention_kernel(const Shared
   }
 }
 
-// out[row] = sum_s o_s 2^(lse_s - M) / sum_s 2^(lse_s - M) over the segments of the row's shared and own item.  A warp per
-// query row; every block first finds where its sequence's two items lie on the line of units.
-template <typename T, int D, int kUnit>
+// out[row] = sum_s o_s 2^(lse_s - M) / sum_s 2^(lse_s - M) over the segments of the row's shared and own item, a warp per
+// query row.  Lane i fetches the i-th log-sum-exp, so the weights are there before the first partial row, whose loads
+// then do not depend on one another.
+template <typename T, int D>
 __global__ void __launch_bounds__(256) shared_merge_kernel(const SharedParams p, const int2* seq_info, int ctas, T* out) {
-  __shared__ long long sums[8][3];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int G = p.group, hq = p.n_kv_heads * G;
   const int per_seq = (hq + 7) / 8, seq = blockIdx.x / per_seq, head = blockIdx.x % per_seq * 8 + warp;
-  grid_launch_dependents();
   const int2 info = seq_info[seq];  // shared entity, the sequence's place in it
   const int own_e = p.n_shared + seq;
-  // the lengths belong to the caller and were there before the attention kernel; its partials were not
   grid_dependency_wait();
-  long long before_shared = 0, before_own = 0, total = 0;
-  for (int e = tid; e < p.n_shared + p.batch; e += 256) {
-    const long long n = (long long)entity_units<kUnit>(p, e) * p.n_kv_heads;
-    if (e < info.x) before_shared += n;
-    if (e < own_e) before_own += n;
-    total += n;
-  }
-#pragma unroll
-  for (int w = 16; w > 0; w >>= 1) {
-    before_shared += __shfl_xor_sync(0xffffffffu, before_shared, w);
-    before_own += __shfl_xor_sync(0xffffffffu, before_own, w);
-    total += __shfl_xor_sync(0xffffffffu, total, w);
-  }
-  if (lane == 0) {
-    sums[warp][0] = before_shared;
-    sums[warp][1] = before_own;
-    sums[warp][2] = total;
-  }
-  __syncthreads();
-  before_shared = before_own = total = 0;
-  for (int w = 0; w < 8; ++w) {
-    before_shared += sums[w][0];
-    before_own += sums[w][1];
-    total += sums[w][2];
-  }
+  grid_launch_dependents();
   if (head >= hq) return;
+  const long long total = __ldcg(p.unit_begin + p.n_shared + p.batch);
+  const long long begin[2] = {__ldcg(p.unit_begin + info.x), __ldcg(p.unit_begin + own_e)};
+  const long long end[2] = {__ldcg(p.unit_begin + info.x + 1), __ldcg(p.unit_begin + own_e + 1)};
   ctas = shares_of(total, ctas);
   const int h = head / G, g = head % G;
+  int n[2], c0[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const long long units = (end[i] - begin[i]) / p.n_kv_heads, u0 = begin[i] + h * units;
+    c0[i] = units > 0 ? share_owner(u0, total, ctas) : 0;
+    n[i] = units > 0 ? share_owner(u0 + units - 1, total, ctas) - c0[i] + 1 : 0;
+  }
+  const int64_t row0[2] = {(((int64_t)info.x * p.n_kv_heads + h + c0[0]) * p.row_block) + info.y * G + g,
+                           ((int64_t)seq * p.n_kv_heads + h + c0[1]) * G + g};
   float acc[D / 32], M = -INFINITY, L = 0.f;
 #pragma unroll
   for (int i = 0; i < D / 32; ++i) acc[i] = 0.f;
+  for (int s0 = 0; s0 < n[0] + n[1]; s0 += 32) {
+    const int mine = s0 + lane, count = min(32, n[0] + n[1] - s0);
+    const bool own = mine >= n[0];
+    const int64_t row = own ? row0[1] + (int64_t)(mine - n[0]) * G : row0[0] + (int64_t)mine * p.row_block;
+    const float lse = lane < count ? __ldcg((own ? p.lse_own : p.lse_shared) + row) * kLog2e : -INFINITY;
+    const float* src = (own ? p.o_own : p.o_shared) + row * D;
+    const float m = fmaxf(M, warp_max(lse)), base = m == -INFINITY ? 0.f : m;
+    const float keep = exp2f(M - base), w = exp2f(lse - base);  // a segment without a visible key: weight 0, o is 0
+    L = L * keep + warp_sum(w);
+    M = m;
 #pragma unroll
-  for (int part = 0; part < 2; ++part) {
-    const int e = part == 0 ? info.x : own_e;
-    const int units = entity_units<kUnit>(p, e);
-    if (units == 0) continue;
-    const long long u0 = (part == 0 ? before_shared : before_own) + (long long)h * units;
-    const int c0 = share_owner(u0, total, ctas), c1 = share_owner(u0 + units - 1, total, ctas);
-    const int64_t slot = (int64_t)(part == 0 ? e : seq) * p.n_kv_heads + h;
-    const int rows = part == 0 ? p.row_block : G, row = part == 0 ? info.y * G + g : g;
-    const float *ob = part == 0 ? p.o_shared : p.o_own, *lb = part == 0 ? p.lse_shared : p.lse_own;
-#pragma unroll 4
-    for (int c = c0; c <= c1; ++c) {
-      const int64_t at = (slot + c) * rows + row;
-      const float lse = __ldcg(lb + at) * kLog2e;
-      float v[D / 32];
+    for (int i = 0; i < D / 32; ++i) acc[i] *= keep;
+#pragma unroll 8
+    for (int s = 0; s < count; ++s) {
+      const float ws = __shfl_sync(0xffffffffu, w, s);
+      const float* from = (const float*)__shfl_sync(0xffffffffu, (unsigned long long)src, s) + lane * (D / 32);
       if constexpr (D == 128) {
-        const float4 x = __ldcg(reinterpret_cast<const float4*>(ob + at * D) + lane);
-        v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+        const float4 x = __ldcg(reinterpret_cast<const float4*>(from));
+        acc[0] += ws * x.x; acc[1] += ws * x.y; acc[2] += ws * x.z; acc[3] += ws * x.w;
       } else {
-        const float2 x = __ldcg(reinterpret_cast<const float2*>(ob + at * D) + lane);
-        v[0] = x.x; v[1] = x.y;
+        const float2 x = __ldcg(reinterpret_cast<const float2*>(from));
+        acc[0] += ws * x.x; acc[1] += ws * x.y;
       }
-      const float m = fmaxf(M, lse), base = m == -INFINITY ? 0.f : m;
-      const float keep = exp2f(M - base), w = exp2f(lse - base);
-      if (lse == -INFINITY) continue;  // a segment without a visible key
-#pragma unroll
-      for (int i = 0; i < D / 32; ++i) acc[i] = acc[i] * keep + w * v[i];
-      L = L * keep + w;
-      M = m;
     }
   }
-  const float inv = L == 0.f ? 0.f : 1.f / L;  // a sequence without keys: zeros
+  const float inv = n[0] + n[1] == 0 || M == -INFINITY ? 0.f : 1.f / L;  // a sequence without keys: zeros
 #pragma unroll
   for (int i = 0; i < D / 32; ++i) acc[i] *= inv;
   store_vec<D / 32>(out + ((int64_t)seq * hq + head) * D + lane * (D / 32), acc);
@@ -397,10 +377,10 @@ template <typename T, int D> int launch_shared(const SharedParams& p, int ctas, 
   if (int s = set_smem(kern, Smem<D, 8>::bytes, "shared_attention")) return s;
   return launch(kern, (unsigned)ctas, Smem<D, 8>::bytes, stream, "shared_attention_kernel", p);
 }
-template <typename T, int D, int kUnit>
+template <typename T, int D>
 int launch_merge(const SharedParams& p, const int2* seq_info, int ctas, T* out, cudaStream_t stream) {
   const int per_seq = (p.n_kv_heads * p.group + 7) / 8;
-  return launch(shared_merge_kernel<T, D, kUnit>, (unsigned)(p.batch * per_seq), 0, stream, "shared_merge_kernel", p, seq_info,
+  return launch(shared_merge_kernel<T, D>, (unsigned)(p.batch * per_seq), 0, stream, "shared_merge_kernel", p, seq_info,
                 ctas, out);
 }
 
@@ -438,10 +418,10 @@ int launch_shared_merge(const SharedParams& p, const int32_t* seq_info, int head
                         cudaStream_t stream) {
   const int2* info = reinterpret_cast<const int2*>(seq_info);
   if (dtype == IA_F32)
-    return head_dim == 128 ? launch_merge<float, 128, kKeys>(p, info, ctas, (float*)out, stream)
-                           : launch_merge<float, 64, kKeys>(p, info, ctas, (float*)out, stream);
-  return head_dim == 128 ? launch_merge<__nv_bfloat16, 128, 128>(p, info, ctas, (__nv_bfloat16*)out, stream)
-                         : launch_merge<__nv_bfloat16, 64, 128>(p, info, ctas, (__nv_bfloat16*)out, stream);
+    return head_dim == 128 ? launch_merge<float, 128>(p, info, ctas, (float*)out, stream)
+                           : launch_merge<float, 64>(p, info, ctas, (float*)out, stream);
+  return head_dim == 128 ? launch_merge<__nv_bfloat16, 128>(p, info, ctas, (__nv_bfloat16*)out, stream)
+                         : launch_merge<__nv_bfloat16, 64>(p, info, ctas, (__nv_bfloat16*)out, stream);
 }
 
 // ---- the prompt's plan ----------------------------------------------------------------------------------------------

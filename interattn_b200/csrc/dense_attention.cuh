@@ -51,6 +51,7 @@ struct SharedParams {
   const SharedEntity* entities;  // [n_shared + batch]
   float *o_shared, *lse_shared;  // slots of row_block rows
   float *o_own, *lse_own;        // slots of `group` rows
+  long long* unit_begin;         // [n_shared + batch + 1] where the entities' units begin; written for the merge
   int* status;
   int64_t page_stride, head_stride;  // elements
   int32_t n_shared, batch, n_kv_heads, group, max_pages, n_pool_pages, row_block;
@@ -87,8 +88,17 @@ __device__ __forceinline__ int2 entity_lead(const SharedParams& p, const SharedE
   who = __reduce_min_sync(0xffffffffu, best == top ? who : 0x7fffffff);
   return make_int2(ent.group_first + who, top);
 }
+__device__ __forceinline__ SharedEntity load_entity(const SharedParams& p, int e) {  // two 16-byte loads
+  union {
+    int4 v[2];
+    SharedEntity e;
+  } u;
+  u.v[0] = reinterpret_cast<const int4*>(p.entities + e)[0];
+  u.v[1] = reinterpret_cast<const int4*>(p.entities + e)[1];
+  return u.e;
+}
 template <int kUnit> __device__ __forceinline__ int entity_units(const SharedParams& p, int e) {
-  const SharedEntity ent = p.entities[e];
+  const SharedEntity ent = load_entity(p, e);
   int lo, hi;
   entity_keys(p, e, ent, lo, hi);
   return (hi - lo + kUnit - 1) / kUnit;
@@ -131,6 +141,14 @@ __device__ __forceinline__ SharedCursor find_share(const SharedParams& p, int ct
     total += x;
   }
   __syncthreads();
+  if (cta == 0) {
+    long long at = before;
+    for (int e = e0; e < e1; ++e) {
+      p.unit_begin[e] = at;
+      at += (long long)entity_units<kUnit>(p, e) * p.n_kv_heads;
+    }
+    if (tid == 0) p.unit_begin[n] = total;
+  }
   ctas = shares_of(total, ctas);
   const long long u0 = cta < ctas ? share_begin(total, cta, ctas) : 0, u1 = cta < ctas ? share_begin(total, cta + 1, ctas) : 0;
   SharedCursor* found = reinterpret_cast<SharedCursor*>(scratch);

@@ -36,7 +36,7 @@ namespace {
 constexpr int kThreads = 384, kRows = 128, kKeys = 128, kWorkSlots = 8;
 constexpr int kCopyWarp = 8, kMmaWarp = 9;  // and 10; 11 only makes up the third warpgroup
 // The block is launched with 168 registers a thread (64,512 in all).  A softmax thread holds a row of 128 logits.
-constexpr int kSoftmaxRegs = 208, kOtherRegs = 88;
+constexpr int kSoftmaxRegs = 184, kOtherRegs = 136;
 static_assert(256 * kSoftmaxRegs + 128 * kOtherRegs <= kThreads * 168, "what the block was launched with");
 
 template <int D> struct Tc {
@@ -51,14 +51,16 @@ template <int D> struct Tc {
 // Step i of a piece belongs to set (first + i) % 2 of softmax warps.  Split: key tile i.  Else: key tile i / 2, row tile i % 2.
 struct Order {
   int split;          // one row tile, key tiles alternate between the sets
-  int tiles[2];       // key tiles of each row tile; the second sees no fewer
+  int keys[2];        // keys that each row tile sees, at least 1; the second sees no fewer
   int first;
-  __device__ __forceinline__ int steps() const { return split ? tiles[0] : 2 * tiles[1]; }
+  __device__ __forceinline__ int tiles(int rt) const { return ((rt ? keys[1] : keys[0]) + kKeys - 1) / kKeys; }
+  __device__ __forceinline__ int steps() const { return split ? tiles(0) : 2 * tiles(1); }
 };
 struct Step {
   int tile, rt;
   bool valid, first_use;  // of the key tile
   bool opens, closes;               // the row tile's first and last (split: the set's)
+  int k16;                          // sixteens of keys of the tile that the row tile sees, 1 to 8
 };
 __device__ __forceinline__ Step step_of(const Order& o, int i) {
   Step st;
@@ -67,16 +69,17 @@ __device__ __forceinline__ Step step_of(const Order& o, int i) {
     st.rt = 0;
     st.valid = st.first_use = true;
     st.opens = i < 2;
-    st.closes = i + 2 >= o.tiles[0];
+    st.closes = i + 2 >= o.tiles(0);
   } else {
     st.tile = i >> 1;
     st.rt = i & 1;
-    const int n = st.rt ? o.tiles[1] : o.tiles[0];
+    const int n = o.tiles(st.rt);
     st.valid = st.tile < n;
-    st.first_use = st.valid && (st.rt == 0 || st.tile >= o.tiles[0]);
+    st.first_use = st.valid && (st.rt == 0 || st.tile >= o.tiles(0));
     st.opens = st.tile == 0;
     st.closes = st.tile + 1 == n;
   }
+  st.k16 = (min(kKeys, (st.rt ? o.keys[1] : o.keys[0]) - st.tile * kKeys) + 15) >> 4;
   return st;
 }
 
@@ -323,7 +326,6 @@ template <bool PAGED> __device__ __forceinline__ int row_limit(const TcParams& p
   if constexpr (PAGED) return max(0, min(shared_seq_len(p.s, wk.q_tok + tok) - wk.key0, wk.n_keys));
   return max(0, min(wk.limit0 + tok, wk.n_keys));
 }
-__device__ __forceinline__ int key_tiles(int keys) { return max(1, (keys + kKeys - 1) / kKeys); }
 
 // ---- copy warp: finds the work, fetches Q, K and V --------------------------------------------------------------------
 // Tiles are fetched in the order in which the MMA thread first needs them: S runs two steps ahead of the second product.
@@ -339,8 +341,13 @@ template <int D, bool PAGED> struct CopyRole {
   uint32_t s_work = 0, p_work = 0;              // pieces opened
   int s_step = 0, s_n = 0, p_step = 0, p_n = 0; // steps of the piece at hand
   int parity = 0;
-  Work s_wk, p_wk;                              // in registers: shared memory is slow for a chain of decisions
+  Work s_wk, p_wk, next;                        // in registers: shared memory is slow for a chain of decisions
   bool alive = true, ended = false;
+  // Decode step.  Lane l knows the entity window + l; page numbers are fetched a tile ahead, and the next piece is found
+  // while the last one's tiles are under way: a chain of loads per piece would be longer than the piece.
+  int window = -1, w_first, w_n, w_lo, w_hi, w_units, lead_of = -1;
+  int2 lead;
+  int ids, next_ids, fifo[3], n_fifo = 0;       // lane l: page l of a tile; the tiles whose K is fetched and V not yet
 
   __device__ __forceinline__ CopyRole(const TcParams& p_, Bars* b, Work* r, unsigned char* base_, const SharedCursor& c)
       : p(p_), bars(b), ring(r), base(base_), cur(c) {
@@ -354,34 +361,69 @@ template <int D, bool PAGED> struct CopyRole {
     }
     return alive;
   }
+  __device__ __forceinline__ void see(int e) {  // the window holds entity e
+    if (window >= 0 && e >= window && e < window + 32) return;
+    window = e;
+    const int mine = e + (threadIdx.x & 31);
+    w_first = w_n = w_lo = w_hi = w_units = 0;
+    if (mine < p.s.n_shared + p.s.batch) {
+      const SharedEntity ent = load_entity(p.s, mine);
+      entity_keys(p.s, mine, ent, w_lo, w_hi);
+      w_first = ent.first_seq;
+      w_n = ent.n_seqs;
+      w_units = (w_hi - w_lo + kKeys - 1) / kKeys;
+    }
+  }
+  // this lane's page of key tile j
+  __device__ __forceinline__ int page_of(const Work& wk, int j) {
+    const int lane = threadIdx.x & 31, held = (min(kKeys, wk.n_keys - j * kKeys) + 15) >> 4;
+    return lane < held ? p.s.block_table[(int64_t)wk.row * p.s.max_pages + ((wk.key0 + j * kKeys) >> 4) + lane] : 0;
+  }
+  __device__ __forceinline__ void look_ahead() {
+    next = Work{};
+    find(next);
+    if constexpr (PAGED)
+      if (!next.last) next_ids = page_of(next, 0);
+  }
   __device__ __forceinline__ void find(Work& wk) {
     const int tpm = kRows / p.group;
     if constexpr (PAGED) {
       wk.last = cur.left <= 0;
       if (wk.last) return;
       const SharedParams& s = p.s;
-      const SharedEntity ent = s.entities[cur.e];
-      int lo, hi;
-      entity_keys(s, cur.e, ent, lo, hi);
-      const int n = (int)min((int64_t)(cur.units - cur.k), cur.left);
-      const int2 lead = entity_lead(s, ent, hi);
-      wk.q_tok = ent.first_seq;
-      wk.n_tok = ent.n_seqs;
+      see(cur.e);
+      const int at = cur.e - window, lo = __shfl_sync(0xffffffffu, w_lo, at), hi = __shfl_sync(0xffffffffu, w_hi, at);
+      const int units = __shfl_sync(0xffffffffu, w_units, at), n = (int)min((int64_t)(units - cur.k), cur.left);
+      wk.q_tok = __shfl_sync(0xffffffffu, w_first, at);
+      wk.n_tok = __shfl_sync(0xffffffffu, w_n, at);
+      wk.own = cur.e >= s.n_shared;
+      if (wk.own) {
+        wk.row = wk.q_tok;
+      } else if (lead_of != cur.e) {
+        lead_of = cur.e;
+        lead = entity_lead(s, load_entity(s, cur.e), hi);
+      }
+      if (!wk.own) wk.row = lead.x;
       wk.head = cur.h;
       wk.key0 = lo + cur.k * kKeys;
-      wk.n_keys = max(0, min(lead.y, wk.key0 + n * kKeys) - wk.key0);
-      wk.own = cur.e >= s.n_shared;
-      wk.row = lead.x;
+      wk.n_keys = max(0, min(wk.own ? hi : lead.y, wk.key0 + n * kKeys) - wk.key0);
       wk.slot = (int64_t)(wk.own ? cur.e - s.n_shared : cur.e) * s.n_kv_heads + cur.h + blockIdx.x;
-      wk.order.split = ent.n_seqs <= tpm;
-      wk.order.tiles[0] = wk.order.tiles[1] = key_tiles(wk.n_keys);
+      wk.order.split = wk.n_tok <= tpm;
+      wk.order.keys[0] = wk.order.keys[1] = max(1, wk.n_keys);  // a tile of keys that nobody sees, where there are none
       cur.left -= n;
       cur.k = 0;
       if (++cur.h == s.n_kv_heads) {
         cur.h = 0;
-        if (cur.left > 0)  // some entity behind this one has units: they were counted
-          do cur.units = entity_units<kKeys>(s, ++cur.e);
-          while (cur.units == 0);
+        ++cur.e;
+        while (cur.left > 0) {  // some entity behind this one has units: they were counted
+          see(cur.e);
+          const unsigned some = __ballot_sync(0xffffffffu, w_units > 0) & ~((1u << (cur.e - window)) - 1u);
+          if (some != 0) {
+            cur.e = window + __ffs(some) - 1;
+            break;
+          }
+          cur.e = window + 32;
+        }
       }
     } else {
       wk.last = next_item >= end_item;
@@ -394,8 +436,8 @@ template <int D, bool PAGED> struct CopyRole {
       wk.limit0 = item.limit0;
       wk.n_keys = item.kv_len;
       wk.order.split = item.n_tok <= tpm;
-      wk.order.tiles[0] = key_tiles(row_limit<false>(p, wk, min(item.n_tok, tpm) - 1));
-      wk.order.tiles[1] = key_tiles(row_limit<false>(p, wk, item.n_tok - 1));
+      wk.order.keys[0] = max(1, row_limit<false>(p, wk, min(item.n_tok, tpm) - 1));
+      wk.order.keys[1] = max(1, row_limit<false>(p, wk, item.n_tok - 1));
     }
   }
   __device__ __forceinline__ unsigned char* stage(uint64_t*& full, bool alone) {
@@ -410,7 +452,7 @@ template <int D, bool PAGED> struct CopyRole {
   __device__ __forceinline__ void fetch(const Work& wk, int j, int which) {
     const int lane = threadIdx.x & 31;
     uint64_t* full;
-    unsigned char* dst = stage(full, wk.order.split || j >= wk.order.tiles[0]);
+    unsigned char* dst = stage(full, wk.order.split || j >= wk.order.tiles(0));
     if (dst == nullptr) return;
     if constexpr (!PAGED) {
       if (lane == 0) {
@@ -420,21 +462,40 @@ template <int D, bool PAGED> struct CopyRole {
     } else {
       const int valid = min(kKeys, wk.n_keys - j * kKeys);
       const int held = (valid + 15) >> 4, pages = which == 0 ? held : valid >> 4;
-      const int32_t* table = p.s.block_table + (int64_t)wk.row * p.s.max_pages + ((wk.key0 + j * kKeys) >> 4);
-      const int page = lane < held ? table[lane] : 0;
+      int page;
+      if (which == 0) {
+        page = ids;
+        if (n_fifo == 0) fifo[0] = page;
+        else if (n_fifo == 1) fifo[1] = page;
+        else fifo[2] = page;
+        ++n_fifo;
+        if ((j + 1) * kKeys < wk.n_keys) ids = page_of(wk, j + 1);
+      } else {
+        page = fifo[0];
+        fifo[0] = fifo[1];
+        fifo[1] = fifo[2];
+        --n_fifo;
+      }
       const bool bad = page < 0 || (p.s.n_pool_pages > 0 && page >= p.s.n_pool_pages);
-      if (bad) atomicOr(p.status, DEV_STATUS_BAD_INDEX);
-      if (which == 1 && valid < kKeys) {
-        // The last tile of a sequence: behind its last token the page may hold anything, and the tile's other pages
-        // whatever the stage held before.  Zero times that must be zero, so the rows are written here.
+      if (bad && which == 0) atomicOr(p.status, DEV_STATUS_BAD_INDEX);
+      if (which == 1 && (valid & 15 || valid == 0)) {
+        // The last page of a sequence: behind its last token it may hold anything, and zero times that must be zero, so its
+        // rows are written here.  What the second product does not read is left as it is.
         const int tail = __shfl_sync(0xffffffffu, bad ? -1 : page, pages & 7);
         const __nv_bfloat16* src = (const __nv_bfloat16*)p.s.v_pool + (int64_t)tail * p.s.page_stride + wk.head * p.s.head_stride;
-        for (int i = lane; i < (kKeys - pages * 16) * (D / 8); i += 32) {
-          const int row = i / (D / 8), c = i % (D / 8);
-          uint4 x = make_uint4(0, 0, 0, 0);
-          if (pages * 16 + row < valid && tail >= 0) x = *reinterpret_cast<const uint4*>(src + row * D + c * 8);
-          const int pg = pages + (row >> 4), t = row & 15;
-          *reinterpret_cast<uint4*>(dst + pg * (C::halves * 2048) + (c >> 3) * 2048 + t * 128 + (((c & 7) ^ (t & 7)) << 4)) = x;
+        const int c = lane % (D / 8);
+        unsigned char* to = dst + pages * (C::halves * 2048) + (c >> 3) * 2048;
+        uint4 x[D / 16];
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) {
+          const int row = i * (256 / D) + lane / (D / 8);
+          x[i] = make_uint4(0, 0, 0, 0);
+          if (pages * 16 + row < valid && tail >= 0) x[i] = *reinterpret_cast<const uint4*>(src + row * D + c * 8);
+        }
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) {
+          const int row = i * (256 / D) + lane / (D / 8);
+          *reinterpret_cast<uint4*>(to + row * 128 + (((c & 7) ^ (row & 7)) << 4)) = x[i];
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
@@ -459,8 +520,8 @@ template <int D, bool PAGED> struct CopyRole {
     if (s_step == s_n) {  // open the next piece
       const int slot = s_work % kWorkSlots;
       if (!wait(&bars->work_empty[slot], ((s_work / kWorkSlots) & 1) ^ 1)) return;
-      s_wk = Work{};
-      find(s_wk);
+      s_wk = next;
+      ids = next_ids;
       s_wk.order.first = parity;
       s_step = 0;
       s_n = s_wk.last ? 0 : s_wk.order.steps();
@@ -490,7 +551,7 @@ template <int D, bool PAGED> struct CopyRole {
       }
     }
     if (st.first_use) fetch(wk, st.tile, 0);
-    ++s_step;
+    if (s_step++ == 0) look_ahead();
   }
   __device__ __forceinline__ bool p_next() {  // false: no steps left
     if (!alive) return false;
@@ -506,6 +567,7 @@ template <int D, bool PAGED> struct CopyRole {
     return alive;
   }
   __device__ __forceinline__ void run() {
+    look_ahead();
     s_next();
     s_next();
     while (p_next()) s_next();
@@ -542,8 +604,8 @@ template <int D, bool PAGED> struct MmaRole {
   __device__ __forceinline__ bool wait_stage(uint32_t use) { return wait(&bars->full[use % C::stages], (use / C::stages) & 1); }
   // What there is to do for the next step, decided before anything is waited for: between its products this thread only
   // issues.
-  struct First { bool mine, valid, opens, closes; uint32_t use, buf, q_parity; };
-  struct Second { bool mine, valid, opens, closes; uint32_t use; };
+  struct First { bool mine, valid, opens, closes; uint32_t use, buf, q_parity, k16; };
+  struct Second { bool mine, valid, opens, closes; uint32_t use, k16; };
   __device__ __forceinline__ First s_next() {
     First f{};
     if (ended || !alive) return f;
@@ -572,6 +634,7 @@ template <int D, bool PAGED> struct MmaRole {
     f.opens = st.opens;
     f.closes = st.closes;
     f.use = k_use;
+    f.k16 = st.k16;
     f.buf = (q_buf >> st.rt) & 1;
     f.q_parity = ((q_it - 1 - (((q_it - 1) & 1) ^ f.buf)) >> 1) & 1;
     return f;
@@ -596,12 +659,13 @@ template <int D, bool PAGED> struct MmaRole {
     f.opens = st.opens;
     f.closes = st.closes;
     f.use = v_use;
+    f.k16 = st.k16;
     return true;
   }
   // The descriptors' upper halves never change; what is added to the lower ones is known to the compiler.  The values have to
   // be known as the same in all lanes, or every operand of every MMA is moved to the uniform registers anew.
   __device__ __forceinline__ void first_product(const First& f, bool take) {
-    const uint32_t ks = uniform(f.use % C::stages), buf = uniform(f.buf), closes = uniform(f.closes);
+    const uint32_t ks = uniform(f.use % C::stages), buf = uniform(f.buf), closes = uniform(f.closes), idesc = uniform(kIdesc<0, false> | (f.k16 << 18));  // N = 16 k16
     const uint64_t a = umma_desc(q0 + buf * C::tile, 0), b = umma_desc(q0 + (2 + ks) * C::tile, 0);
     if (f.opens && !wait(&bars->q_full[f.buf], f.q_parity)) return;
     if (!wait_stage(f.use)) return;
@@ -612,7 +676,7 @@ template <int D, bool PAGED> struct MmaRole {
       for (int h = 0; h < C::halves; ++h)
 #pragma unroll
         for (int s = 0; s < 4; ++s)  // 16 dims = 32 bytes further inside the swizzled row
-          umma_ss(tmem + me * 128, a + (h * C::block + s * 32) / 16, b + (h * C::block + s * 32) / 16, kIdesc<kKeys, false>, h + s > 0);
+          umma_ss(tmem + me * 128, a + (h * C::block + s * 32) / 16, b + (h * C::block + s * 32) / 16, idesc, h + s > 0);
       umma_commit(&bars->s_full[me]);
       umma_commit(&bars->empty[ks]);
       if (closes) umma_commit(&bars->q_empty[buf]);
@@ -620,7 +684,7 @@ template <int D, bool PAGED> struct MmaRole {
     __syncwarp();
   }
   __device__ __forceinline__ void second_product(const Second& f) {
-    const uint32_t vs = uniform(f.use % C::stages), first = uniform(f.opens), closes = uniform(f.closes);
+    const uint32_t vs = uniform(f.use % C::stages), first = uniform(f.opens), closes = uniform(f.closes), k16 = uniform(f.k16);
     const uint64_t b = umma_desc(q0 + (2 + vs) * C::tile, kNextCols);
     if (!wait_stage(f.use) || !wait(&bars->p_full[me], p_count & 1)) return;
     if (!wait(&bars->turn[me], turn_it++ & 1)) return;
@@ -628,7 +692,7 @@ template <int D, bool PAGED> struct MmaRole {
     if (elect_one()) {
 #pragma unroll
       for (int s = 0; s < kKeys / 16; ++s)  // 16 keys: 8 columns of packed weights, 16 rows of V
-        umma_ts(tmem + 256 + me * 128, tmem + me * 128 + s * 8, b + s * kStepBytes / 16, kIdesc<D, true>, s > 0 ? 1u : first ^ 1u);
+        if (s < k16) umma_ts(tmem + 256 + me * 128, tmem + me * 128 + s * 8, b + s * kStepBytes / 16, kIdesc<D, true>, s > 0 ? 1u : first ^ 1u);
       if (closes) umma_commit(&bars->o_full[me]);
     }
     __syncwarp();
@@ -695,16 +759,16 @@ __device__ __forceinline__ void softmax_role(const TcParams& p, Bars* bars, cons
     };
     const bool split = wk.order.split;
     const int me = w ^ wk.order.first;  // row tile, or place in the order of key tiles
-    const int total = wk.order.tiles[split ? 0 : me], stride = split ? 2 : 1, begin = split ? me : 0;
+    const int keys = wk.order.keys[split ? 0 : me], total = (keys + kKeys - 1) / kKeys, stride = split ? 2 : 1, begin = split ? me : 0;
+    if (begin >= total) {  // the other set has the only key tile
+      done();
+      continue;
+    }
     const int tok = (split ? 0 : me * tpm) + row_tok;
     const bool valid = row < tpm * G && tok < wk.n_tok;
     const bool busy = __any_sync(0xffffffffu, valid);
     const int limit = valid ? row_limit<PAGED>(p, wk, tok) : 0;
     const int least = __reduce_min_sync(0xffffffffu, valid ? limit : 0x7fffffff);  // below it nothing is masked
-    if (begin >= total) {  // the other set has the only key tile
-      done();
-      continue;
-    }
     float m = -INFINITY, l = 0.f;
     for (int j = begin; j < total; j += stride) {
             if (!wait(&bars->s_full[w], s_it & 1)) return;
@@ -721,15 +785,16 @@ __device__ __forceinline__ void softmax_role(const TcParams& p, Bars* bars, cons
         tmem_wait_ld(rb);
         tmem_wait_ld(rc);
         tmem_wait_ld(rd);
+        const int columns = keys - j * kKeys;  // behind them neither product reads or writes
         if (all_seen < 32) mask_row(ra, seen);
         if (all_seen < 64) mask_row(rb, seen - 32);
-        if (all_seen < 96) mask_row(rc, seen - 64);
-        if (all_seen < 128) mask_row(rd, seen - 96);
+        if (all_seen < 96 && columns > 64) mask_row(rc, seen - 64);
+        if (all_seen < 128 && columns > 96) mask_row(rd, seen - 96);
         float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
         max_row(ra, top);
         max_row(rb, top);
-        max_row(rc, top);
-        max_row(rd, top);
+        if (columns > 64) max_row(rc, top);
+        if (columns > 96) max_row(rd, top);
         const float t = max3(top[0], top[1], max3(top[2], top[3], -INFINITY));
         if (j == begin) {
           m = t;
@@ -758,8 +823,8 @@ __device__ __forceinline__ void softmax_role(const TcParams& p, Bars* bars, cons
         uint64_t sum[2] = {0, 0};
         weights(ra, c2, mc2, sum, s_addr);
         weights(rb, c2, mc2, sum, s_addr + 16);
-        weights(rc, c2, mc2, sum, s_addr + 32);
-        weights(rd, c2, mc2, sum, s_addr + 48);
+        if (columns > 64) weights(rc, c2, mc2, sum, s_addr + 32);
+        if (columns > 96) weights(rd, c2, mc2, sum, s_addr + 48);
         float la, lb;
         unpair(add2(sum[0], sum[1]), la, lb);
         l += la + lb;
@@ -843,13 +908,18 @@ __device__ __forceinline__ void softmax_role(const TcParams& p, Bars* bars, cons
           *reinterpret_cast<uint4*>(rows + lane * 128 + ((k ^ (lane & 7)) << 4)) = v;
         }
         __syncwarp();
+        // kWords neighbouring lanes write a row's run; all reads before the first write
+        uint4 v[kWords];
+        int to[kWords];
 #pragma unroll
-        for (int i = 0; i < kWords; ++i) {  // kWords neighbouring lanes write a row's run
+        for (int i = 0; i < kWords; ++i) {
           const int r = i * (32 / kWords) + lane / kWords, k = lane % kWords;
-          const int to = __shfl_sync(0xffffffffu, at, r);
-          const uint4 v = *reinterpret_cast<const uint4*>(rows + r * 128 + ((k ^ (r & 7)) << 4));
-          if (to >= 0) *reinterpret_cast<uint4*>(out + to + col + k * (16 / (int)sizeof(Out))) = v;
+          to[i] = __shfl_sync(0xffffffffu, at, r);
+          v[i] = *reinterpret_cast<const uint4*>(rows + r * 128 + ((k ^ (r & 7)) << 4));
         }
+#pragma unroll
+        for (int i = 0; i < kWords; ++i)
+          if (to[i] >= 0) *reinterpret_cast<uint4*>(out + to[i] + col + lane % kWords * (16 / (int)sizeof(Out))) = v[i];
         __syncwarp();
       }
       if (valid && lse_out != nullptr && (!merge || me == 0)) *lse_out = lse;
