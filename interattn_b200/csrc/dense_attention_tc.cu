@@ -144,7 +144,7 @@ __device__ __forceinline__ bool mbar_wait_slow(uint64_t* bar, uint32_t parity) {
 }
 // false: the phase did not complete in time
 __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity) {
-  return mbar_try(bar, parity) || mbar_try(bar, parity) || mbar_wait_slow(bar, parity);
+  return mbar_try(bar, parity) || mbar_wait_slow(bar, parity);
 }
 
 // ---- copies -----------------------------------------------------------------------------------------------------------
@@ -551,7 +551,7 @@ template <int D, bool PAGED> struct CopyRole {
       }
     }
     if (st.first_use) fetch(wk, st.tile, 0);
-    if (s_step++ == 0) look_ahead();
+    if (s_step++ == min(2, s_n - 1)) look_ahead();  // not before the first tiles are under way
   }
   __device__ __forceinline__ bool p_next() {  // false: no steps left
     if (!alive) return false;
@@ -568,9 +568,8 @@ template <int D, bool PAGED> struct CopyRole {
   }
   __device__ __forceinline__ void run() {
     look_ahead();
-    s_next();
-    s_next();
-    while (p_next()) s_next();
+#pragma unroll 1
+    for (int i = 0; i < 2 || p_next(); ++i) s_next();  // one copy of either in the instruction cache
     if (!alive) {  // no copy may be in flight when the CTA ends
       for (uint32_t i = it > C::stages ? it - C::stages : 0; i < it; ++i) mbar_wait(&bars->full[i % C::stages], (i / C::stages) & 1);
       for (uint32_t i = q_it > 2 ? q_it - 2 : 0; i < q_it; ++i) mbar_wait(&bars->q_full[i & 1], (i >> 1) & 1);
@@ -664,12 +663,11 @@ template <int D, bool PAGED> struct MmaRole {
   }
   // The descriptors' upper halves never change; what is added to the lower ones is known to the compiler.  The values have to
   // be known as the same in all lanes, or every operand of every MMA is moved to the uniform registers anew.
-  __device__ __forceinline__ void first_product(const First& f, bool take) {
+  __device__ __forceinline__ void first_product(const First& f) {
     const uint32_t ks = uniform(f.use % C::stages), buf = uniform(f.buf), closes = uniform(f.closes), idesc = uniform(kIdesc<0, false> | (f.k16 << 18));  // N = 16 k16
     const uint64_t a = umma_desc(q0 + buf * C::tile, 0), b = umma_desc(q0 + (2 + ks) * C::tile, 0);
     if (f.opens && !wait(&bars->q_full[f.buf], f.q_parity)) return;
     if (!wait_stage(f.use)) return;
-    if (take && !wait(&bars->turn[me], turn_it++ & 1)) return;
     tc_fence_after();
     if (elect_one()) {
 #pragma unroll
@@ -683,11 +681,10 @@ template <int D, bool PAGED> struct MmaRole {
     }
     __syncwarp();
   }
-  __device__ __forceinline__ void second_product(const Second& f) {
+  __device__ __forceinline__ bool second_product(const Second& f) {  // has taken the turn
     const uint32_t vs = uniform(f.use % C::stages), first = uniform(f.opens), closes = uniform(f.closes), k16 = uniform(f.k16);
     const uint64_t b = umma_desc(q0 + (2 + vs) * C::tile, kNextCols);
-    if (!wait_stage(f.use) || !wait(&bars->p_full[me], p_count & 1)) return;
-    if (!wait(&bars->turn[me], turn_it++ & 1)) return;
+    if (!wait_stage(f.use) || !wait(&bars->p_full[me], p_count & 1) || !wait(&bars->turn[me], turn_it++ & 1)) return true;
     tc_fence_after();
     if (elect_one()) {
 #pragma unroll
@@ -697,6 +694,7 @@ template <int D, bool PAGED> struct MmaRole {
     }
     __syncwarp();
     ++p_count;
+    return true;
   }
   __device__ __forceinline__ void pass() {
     if (elect_one()) mbar_arrive(&bars->turn[me ^ 1]);
@@ -707,21 +705,15 @@ template <int D, bool PAGED> struct MmaRole {
     __syncwarp();
   }
   __device__ __forceinline__ void run() {
+    Second v{};
 #pragma unroll 1
-    for (int i = 0; i < 2; ++i) {
-      const First s = s_next();
-      if (i != me) continue;
-      if (s.mine) first_product(s, true);  // set 0's turn was given at the start
-      else if (!wait(&bars->turn[me], turn_it++ & 1)) break;
-      pass();
-    }
-    Second v;
-    while (p_next(v)) {
-      const First s = s_next();  // two steps ahead: the same set's
-      if (!v.mine) continue;
-      if (v.valid) second_product(v);
-      else wait(&bars->turn[me], turn_it++ & 1);
-      if (s.mine && s.valid && alive) first_product(s, false);
+    for (uint32_t i = 0; i < 2 || p_next(v); ++i) {
+      const First s = s_next();  // two steps ahead of v: the same set's
+      if (i < 2 ? i != me : !v.mine) continue;
+      bool turn = false;
+      if (v.valid) turn = second_product(v);
+      if (!turn) wait(&bars->turn[me], turn_it++ & 1);  // set 0's first turn was given at the start
+      if (s.mine && s.valid && alive) first_product(s);
       pass();
       if (v.valid && alive) release(v.use);
     }
