@@ -661,13 +661,15 @@ template <int D, bool PAGED> struct MmaRole {
     f.k16 = st.k16;
     return true;
   }
+  __device__ __forceinline__ bool ready(const First& f) {
+    return (!f.opens || wait(&bars->q_full[f.buf], f.q_parity)) && wait_stage(f.use);
+  }
   // The descriptors' upper halves never change; what is added to the lower ones is known to the compiler.  The values have to
   // be known as the same in all lanes, or every operand of every MMA is moved to the uniform registers anew.
   __device__ __forceinline__ void first_product(const First& f) {
     const uint32_t ks = uniform(f.use % C::stages), buf = uniform(f.buf), closes = uniform(f.closes), idesc = uniform(kIdesc<0, false> | (f.k16 << 18));  // N = 16 k16
     const uint64_t a = umma_desc(q0 + buf * C::tile, 0), b = umma_desc(q0 + (2 + ks) * C::tile, 0);
-    if (f.opens && !wait(&bars->q_full[f.buf], f.q_parity)) return;
-    if (!wait_stage(f.use)) return;
+    if (PAGED && !ready(f)) return;
     tc_fence_after();
     if (elect_one()) {
 #pragma unroll
@@ -710,6 +712,7 @@ template <int D, bool PAGED> struct MmaRole {
     for (uint32_t i = 0; i < 2 || p_next(v); ++i) {
       const First s = s_next();  // two steps ahead of v: the same set's
       if (i < 2 ? i != me : !v.mine) continue;
+      if (!PAGED && s.mine && s.valid) ready(s);  // compute bound: the keys are there, and nothing is left to do between the products
       bool turn = false;
       if (v.valid) turn = second_product(v);
       if (!turn) wait(&bars->turn[me], turn_it++ & 1);  // set 0's first turn was given at the start
