@@ -20,10 +20,9 @@
 //
 // Warps 0-3 and 4-7: softmax, rescaling and output of tile 0 and 1.  Warp 8: copies - it alone knows where work comes from
 // (a list for prompts, an equal share of all units for the decode step) and hands the others descriptors through a small
-// ring.  Warps 9 and 10 issue the MMAs of set 0 and 1, each set's second product and next first product as one block, and
-// pass the turn on: issuing holds a thread until the tensor core takes the instruction, so what one warp decides and waits
-// for between its blocks is hidden behind the other's, and the fixed order keeps the sets half a period apart.  Tensor
-// memory: S_0, S_1, O_0, O_1 of 128 columns each.
+// ring.  Warps 9 and 10 issue the MMAs of set 0 and 1, a set's second product and its next first product together: issuing
+// holds a warp until the tensor core takes the instruction, so what one decides and waits for between them is hidden behind
+// the other's.  Tensor memory: S_0, S_1, O_0, O_1 of 128 columns each.
 #include <type_traits>
 
 #include <cuda.h>  // CUtensorMap (types only; the encoder is fetched through the runtime)
@@ -33,55 +32,29 @@
 namespace ia {
 namespace {
 
-constexpr int kThreads = 384, kRows = 128, kKeys = 128, kWorkSlots = 8;
-constexpr int kCopyWarp = 8, kMmaWarp = 9;  // and 10; 11 only makes up the third warpgroup
-// The block is launched with 168 registers a thread (64,512 in all).  A softmax thread holds a row of 128 logits.
-constexpr int kSoftmaxRegs = 184, kOtherRegs = 136;
-static_assert(256 * kSoftmaxRegs + 128 * kOtherRegs <= kThreads * 168, "what the block was launched with");
+constexpr int kThreads = 352, kRows = 128, kKeys = 128, kWorkSlots = 8;
+constexpr int kCopyWarp = 8, kMmaWarp = 9;  // and 10
 
 template <int D> struct Tc {
   static constexpr int halves = D / 64;                 // 128-byte wide column blocks
   static constexpr int block = kRows * 128;             // bytes of one [128 rows][128 bytes] block
-  static constexpr int tile = halves * block;           // a Q, K or V tile
-  static constexpr int stages = D == 128 ? 4 : 8;       // ring of K and V tiles
+  static constexpr int tile = halves * block;           // a Q tile
+  static constexpr int kv_block = kKeys * 128, kv_tile = halves * kv_block;
+  static constexpr int stages = D == 128 ? 4 : 8;      // ring of K and V tiles
   static constexpr int out_warp = 4096;                 // a warp's 32 rows of 128 bytes on their way out
-  static constexpr size_t tiles = (size_t)(2 + stages) * tile, control = tiles + 8 * out_warp, smem = control + 3072;
+  static constexpr size_t ring = 2 * (size_t)tile, tiles = ring + (size_t)stages * kv_tile, control = tiles + 8 * out_warp, smem = control + 3072;
 };
 
-// Step i of a piece belongs to set (first + i) % 2 of softmax warps.  Split: key tile i.  Else: key tile i / 2, row tile i % 2.
+// The key tiles of a piece and who takes them.  Split: one row tile, key tile j goes to set (first + j) % 2 of softmax warps.
+// Else: row tile r goes to set (first + r) % 2, with all its key tiles.  Tile j's K is fetch ring + 2 j, its V the one behind.
 struct Order {
-  int split;          // one row tile, key tiles alternate between the sets
+  int split;
   int keys[2];        // keys that each row tile sees, at least 1; the second sees no fewer
   int first;
-  __device__ __forceinline__ int tiles(int rt) const { return ((rt ? keys[1] : keys[0]) + kKeys - 1) / kKeys; }
-  __device__ __forceinline__ int steps() const { return split ? tiles(0) : 2 * tiles(1); }
+  uint32_t ring, q;   // uses of the K and V ring and of the Q tiles before this piece
+  __device__ __forceinline__ int keys_of(int rt) const { return rt ? keys[1] : keys[0]; }
+  __device__ __forceinline__ int tiles(int rt) const { return (keys_of(rt) + kKeys - 1) / kKeys; }
 };
-struct Step {
-  int tile, rt;
-  bool valid, first_use;  // of the key tile
-  bool opens, closes;               // the row tile's first and last (split: the set's)
-  int k16;                          // sixteens of keys of the tile that the row tile sees, 1 to 8
-};
-__device__ __forceinline__ Step step_of(const Order& o, int i) {
-  Step st;
-  if (o.split) {
-    st.tile = i;
-    st.rt = 0;
-    st.valid = st.first_use = true;
-    st.opens = i < 2;
-    st.closes = i + 2 >= o.tiles(0);
-  } else {
-    st.tile = i >> 1;
-    st.rt = i & 1;
-    const int n = o.tiles(st.rt);
-    st.valid = st.tile < n;
-    st.first_use = st.valid && (st.rt == 0 || st.tile >= o.tiles(0));
-    st.opens = st.tile == 0;
-    st.closes = st.tile + 1 == n;
-  }
-  st.k16 = (min(kKeys, (st.rt ? o.keys[1] : o.keys[0]) - st.tile * kKeys) + 15) >> 4;
-  return st;
-}
 
 // one piece of work, as the copy warp hands it to the others
 struct Work {
@@ -91,10 +64,10 @@ struct Work {
   int key0;           // first key: an index into the packed keys, or the position in the sequence
   int limit0;         // prompt: keys that the first query token sees
   int n_keys;         // keys from key0 on that anyone sees
-  int own;            // decode step: own part (slots of G rows)
   int row;            // decode step: table row
+  short own;          // decode step: own part (slots of G rows)
+  short last;         // nothing follows
   int64_t slot;
-  int last;           // nothing follows
 };
 
 struct TcParams {
@@ -123,6 +96,17 @@ __device__ __forceinline__ bool mbar_try(uint64_t* bar, uint32_t parity) {
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
       "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {  // without waiting
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
       "selp.u32 %0, 1, 0, p;\n\t}"
       : "=r"(ok)
       : "r"(smem_u32(bar)), "r"(parity)
@@ -318,7 +302,7 @@ __device__ __forceinline__ void weights(const uint32_t (&s)[32], uint64_t c, uin
 
 struct Bars {
   uint64_t full[8], empty[8], q_full[2], q_empty[2], s_full[2], p_full[2], o_full[2], stats, read, work_full[kWorkSlots],
-      work_empty[kWorkSlots], turn[2], drain;
+      work_empty[kWorkSlots], drain;
 };
 
 // keys that the row's token sees, counted from the piece's first key
@@ -328,7 +312,8 @@ template <bool PAGED> __device__ __forceinline__ int row_limit(const TcParams& p
 }
 
 // ---- copy warp: finds the work, fetches Q, K and V --------------------------------------------------------------------
-// Tiles are fetched in the order in which the MMA thread first needs them: S runs two steps ahead of the second product.
+// The code that a tile takes is kept short in all three roles that run beside the softmax: their warps do little else than
+// fetch instructions, past which the softmax warps stream their own.
 template <int D, bool PAGED> struct CopyRole {
   using C = Tc<D>;
   const TcParams& p;
@@ -337,17 +322,15 @@ template <int D, bool PAGED> struct CopyRole {
   unsigned char* base;
   SharedCursor cur;
   int next_item, end_item;
-  uint32_t it = 0, q_it = 0;                    // ring stages and Q tiles used so far
-  uint32_t s_work = 0, p_work = 0;              // pieces opened
-  int s_step = 0, s_n = 0, p_step = 0, p_n = 0; // steps of the piece at hand
-  int parity = 0;
-  Work s_wk, p_wk, next;                        // in registers: shared memory is slow for a chain of decisions
-  bool alive = true, ended = false;
+  uint32_t it = 0, q_it = 0, w_it = 0;  // ring stages, Q tiles, pieces so far
+  uint32_t parity = 0;
+  Work wk, next;
+  bool alive = true;
   // Decode step.  Lane l knows the entity window + l; page numbers are fetched a tile ahead, and the next piece is found
   // while the last one's tiles are under way: a chain of loads per piece would be longer than the piece.
   int window = -1, w_first, w_n, w_lo, w_hi, w_units, lead_of = -1;
   int2 lead;
-  int ids, next_ids, fifo[3], n_fifo = 0;       // lane l: page l of a tile; the tiles whose K is fetched and V not yet
+  int ids, next_ids;                    // lane l: page l of the next tile, of the next piece's first
 
   __device__ __forceinline__ CopyRole(const TcParams& p_, Bars* b, Work* r, unsigned char* base_, const SharedCursor& c)
       : p(p_), bars(b), ring(r), base(base_), cur(c) {
@@ -375,9 +358,9 @@ template <int D, bool PAGED> struct CopyRole {
     }
   }
   // this lane's page of key tile j
-  __device__ __forceinline__ int page_of(const Work& wk, int j) {
-    const int lane = threadIdx.x & 31, held = (min(kKeys, wk.n_keys - j * kKeys) + 15) >> 4;
-    return lane < held ? p.s.block_table[(int64_t)wk.row * p.s.max_pages + ((wk.key0 + j * kKeys) >> 4) + lane] : 0;
+  __device__ __forceinline__ int page_of(const Work& k, int j) {
+    const int lane = threadIdx.x & 31, held = (min(kKeys, k.n_keys - j * kKeys) + 15) >> 4;
+    return lane < held ? p.s.block_table[(int64_t)k.row * p.s.max_pages + ((k.key0 + j * kKeys) >> 4) + lane] : 0;
   }
   __device__ __forceinline__ void look_ahead() {
     next = Work{};
@@ -440,48 +423,29 @@ template <int D, bool PAGED> struct CopyRole {
       wk.order.keys[1] = max(1, row_limit<false>(p, wk, item.n_tok - 1));
     }
   }
-  __device__ __forceinline__ unsigned char* stage(uint64_t*& full, bool alone) {
-    const uint32_t st = it % C::stages;
-    full = &bars->full[st];
-    if (!wait(&bars->empty[st], ((it / C::stages) & 1) ^ 1)) return nullptr;
-    if (alone && (threadIdx.x & 31) == 0) mbar_arrive(&bars->empty[st]);  // in the place of the set that does not read it
-    ++it;
-    return base + (2 + (size_t)st) * C::tile;
-  }
-  // key tile j of K (which = 0) or V
-  __device__ __forceinline__ void fetch(const Work& wk, int j, int which) {
+  // K (which = 0) or V of key tile j into the next stage
+  __device__ __forceinline__ void fetch(int j, int which, int page) {
     const int lane = threadIdx.x & 31;
-    uint64_t* full;
-    unsigned char* dst = stage(full, wk.order.split || j >= wk.order.tiles(0));
-    if (dst == nullptr) return;
+    const uint32_t st = it % C::stages;
+    uint64_t* full = &bars->full[st];
+    unsigned char* dst = base + C::ring + (size_t)st * C::kv_tile;
+    if (!wait(&bars->empty[st], ((it / C::stages) & 1) ^ 1)) return;
+    ++it;
+    // in the place of the set that does not read the tile
+    if ((wk.order.split || j * kKeys >= wk.order.keys[0]) && lane == 0) mbar_arrive(&bars->empty[st]);
     if constexpr (!PAGED) {
       if (lane == 0) {
-        mbar_arrive_expect_tx(full, C::tile);
+        mbar_arrive_expect_tx(full, C::kv_tile);
         tma_load_4d(smem_u32(dst), which == 0 ? &p.tm_k : &p.tm_v, 0, wk.key0 + j * kKeys, 0, wk.head, full);
       }
     } else {
       const int valid = min(kKeys, wk.n_keys - j * kKeys);
-      const int held = (valid + 15) >> 4, pages = which == 0 ? held : valid >> 4;
-      int page;
-      if (which == 0) {
-        page = ids;
-        if (n_fifo == 0) fifo[0] = page;
-        else if (n_fifo == 1) fifo[1] = page;
-        else fifo[2] = page;
-        ++n_fifo;
-        if ((j + 1) * kKeys < wk.n_keys) ids = page_of(wk, j + 1);
-      } else {
-        page = fifo[0];
-        fifo[0] = fifo[1];
-        fifo[1] = fifo[2];
-        --n_fifo;
-      }
-      const bool bad = page < 0 || (p.s.n_pool_pages > 0 && page >= p.s.n_pool_pages);
-      if (bad && which == 0) atomicOr(p.status, DEV_STATUS_BAD_INDEX);
+      const int pages = which == 0 ? (valid + 15) >> 4 : valid >> 4;
       if (which == 1 && (valid & 15 || valid == 0)) {
         // The last page of a sequence: behind its last token it may hold anything, and zero times that must be zero, so its
         // rows are written here.  What the second product does not read is left as it is.
-        const int tail = __shfl_sync(0xffffffffu, bad ? -1 : page, pages & 7);
+        const int tail = __shfl_sync(0xffffffffu, page, pages & (kKeys / 16 - 1));
+        const bool good = tail >= 0 && (p.s.n_pool_pages == 0 || tail < p.s.n_pool_pages);
         const __nv_bfloat16* src = (const __nv_bfloat16*)p.s.v_pool + (int64_t)tail * p.s.page_stride + wk.head * p.s.head_stride;
         const int c = lane % (D / 8);
         unsigned char* to = dst + pages * (C::halves * 2048) + (c >> 3) * 2048;
@@ -490,7 +454,7 @@ template <int D, bool PAGED> struct CopyRole {
         for (int i = 0; i < D / 16; ++i) {
           const int row = i * (256 / D) + lane / (D / 8);
           x[i] = make_uint4(0, 0, 0, 0);
-          if (pages * 16 + row < valid && tail >= 0) x[i] = *reinterpret_cast<const uint4*>(src + row * D + c * 8);
+          if (pages * 16 + row < valid && good) x[i] = *reinterpret_cast<const uint4*>(src + row * D + c * 8);
         }
 #pragma unroll
         for (int i = 0; i < D / 16; ++i) {
@@ -503,10 +467,10 @@ template <int D, bool PAGED> struct CopyRole {
       if (lane == 0) mbar_arrive_expect_tx(full, (uint32_t)pages * (C::halves * 2048));
       __syncwarp();
       if (lane < pages) {
-        if (which == 0) {  // [128 keys][128 bytes] per half
+        if (which == 0) {  // [64 keys][128 bytes] per half
 #pragma unroll
           for (int h = 0; h < C::halves; ++h)
-            tma_load_5d(smem_u32(dst + h * C::block + lane * 2048), &p.tm_k, 0, 0, h, wk.head, page, full);
+            tma_load_5d(smem_u32(dst + h * C::kv_block + lane * 2048), &p.tm_k, 0, 0, h, wk.head, page, full);
         } else {           // page by page: a k step of the second product is one page
           tma_load_5d(smem_u32(dst + lane * (C::halves * 2048)), &p.tm_v, 0, 0, 0, wk.head, page, full);
         }
@@ -514,62 +478,56 @@ template <int D, bool PAGED> struct CopyRole {
       __syncwarp();
     }
   }
-  __device__ __forceinline__ void s_next() {
-    if (ended || !alive) return;
-    const int lane = threadIdx.x & 31;
-    if (s_step == s_n) {  // open the next piece
-      const int slot = s_work % kWorkSlots;
-      if (!wait(&bars->work_empty[slot], ((s_work / kWorkSlots) & 1) ^ 1)) return;
-      s_wk = next;
-      ids = next_ids;
-      s_wk.order.first = parity;
-      s_step = 0;
-      s_n = s_wk.last ? 0 : s_wk.order.steps();
-      parity ^= s_n & 1;
-      ended = s_wk.last;
-      if (lane == 0) {
-        ring[slot] = s_wk;
-        mbar_arrive(&bars->work_full[slot]);
-      }
-      __syncwarp();
-      ++s_work;
-      if (ended) return;
+  __device__ __forceinline__ void fetch_q(int rt) {
+    const uint32_t buf = q_it & 1;
+    const int tpm = kRows / p.group;
+    if (!wait(&bars->q_empty[buf], ((q_it >> 1) & 1) ^ 1)) return;
+    ++q_it;
+    if ((threadIdx.x & 31) == 0) {
+      if (!wk.order.split || wk.order.keys[0] <= kKeys) mbar_arrive(&bars->q_empty[buf]);  // only one set reads it
+      mbar_arrive_expect_tx(&bars->q_full[buf], (uint32_t)(C::halves * tpm * p.group * 128));
+      for (int h = 0; h < C::halves; ++h)
+        tma_load_5d(smem_u32(base + buf * C::tile + h * C::block), &p.tm_q, 0, 0, wk.q_tok + rt * tpm, h, wk.head,
+                    &bars->q_full[buf]);
     }
-    const Work& wk = s_wk;
-    const Step st = step_of(wk.order, s_step);
-    if (st.valid && st.opens && (!wk.order.split || s_step == 0)) {  // Q of the row tile
-      const uint32_t buf = q_it & 1;
-      if (!wait(&bars->q_empty[buf], ((q_it >> 1) & 1) ^ 1)) return;
-      ++q_it;
-      const int tpm = kRows / p.group;
-      if (lane == 0) {
-        if (!wk.order.split || s_n == 1) mbar_arrive(&bars->q_empty[buf]);  // only one set reads it
-        mbar_arrive_expect_tx(&bars->q_full[buf], (uint32_t)(C::halves * tpm * p.group * 128));
-        for (int h = 0; h < C::halves; ++h)
-          tma_load_5d(smem_u32(base + buf * C::tile + h * C::block), &p.tm_q, 0, 0, wk.q_tok + st.rt * tpm, h, wk.head,
-                      &bars->q_full[buf]);
-      }
-    }
-    if (st.first_use) fetch(wk, st.tile, 0);
-    if (s_step++ == min(2, s_n - 1)) look_ahead();  // not before the first tiles are under way
-  }
-  __device__ __forceinline__ bool p_next() {  // false: no steps left
-    if (!alive) return false;
-    if (p_step == p_n) {
-      if (ended && p_work + 1 == s_work) return false;  // the one that says so is the last
-      p_step = 0;
-      p_wk = ring[p_work % kWorkSlots];
-      p_n = p_wk.order.steps();
-      ++p_work;
-    }
-    const Step st = step_of(p_wk.order, p_step++);
-    if (st.first_use) fetch(p_wk, st.tile, 1);
-    return alive;
   }
   __device__ __forceinline__ void run() {
     look_ahead();
+    while (alive) {
+      const int slot = w_it % kWorkSlots;
+      if (!wait(&bars->work_empty[slot], ((w_it / kWorkSlots) & 1) ^ 1)) break;
+      wk = next;
+      ids = next_ids;
+      wk.order.first = (int)parity;
+      wk.order.ring = it;
+      wk.order.q = q_it;
+      const int tiles = wk.last ? 0 : wk.order.tiles(1);
+      if (wk.order.split) parity ^= tiles & 1;  // the sets take turns across pieces too
+      if ((threadIdx.x & 31) == 0) {
+        ring[slot] = wk;
+        mbar_arrive(&bars->work_full[slot]);
+      }
+      __syncwarp();
+      ++w_it;
+      if (wk.last) break;
 #pragma unroll 1
-    for (int i = 0; i < 2 || p_next(); ++i) s_next();  // one copy of either in the instruction cache
+      for (int j = 0; j < tiles && alive; ++j) {
+        const int page = ids;
+        if constexpr (PAGED) {
+          if (page < 0 || (p.s.n_pool_pages > 0 && page >= p.s.n_pool_pages)) atomicOr(p.status, DEV_STATUS_BAD_INDEX);
+          if ((j + 1) * kKeys < wk.n_keys) ids = page_of(wk, j + 1);
+        }
+#pragma unroll 1
+        for (int which = 0; which < 2; ++which) {
+          fetch(j, which, page);
+          if (j == 0 && which == 0) {  // Q behind the first K: the ring may be ahead of the end of the piece before
+            fetch_q(0);
+            if (!wk.order.split) fetch_q(1);
+          }
+        }
+        if (j == min(2, tiles - 1)) look_ahead();  // not before the first tiles are under way
+      }
+    }
     if (!alive) {  // no copy may be in flight when the CTA ends
       for (uint32_t i = it > C::stages ? it - C::stages : 0; i < it; ++i) mbar_wait(&bars->full[i % C::stages], (i / C::stages) & 1);
       for (uint32_t i = q_it > 2 ? q_it - 2 : 0; i < q_it; ++i) mbar_wait(&bars->q_full[i & 1], (i >> 1) & 1);
@@ -577,148 +535,119 @@ template <int D, bool PAGED> struct CopyRole {
   }
 };
 
-// ---- MMA thread -------------------------------------------------------------------------------------------------------
+// ---- MMA warps --------------------------------------------------------------------------------------------------------
 template <int D, bool PAGED> struct MmaRole {
   using C = Tc<D>;
-  static constexpr uint32_t kNextCols = PAGED ? 2048 : C::block, kStepBytes = PAGED ? C::halves * 2048 : 2048;
+  static constexpr uint32_t kNextCols = PAGED ? 2048 : C::kv_block, kStepBytes = PAGED ? C::halves * 2048 : 2048;
   const TcParams& p;
   Bars* bars;
   const Work* ring;
   uint32_t q0, tmem;
   uint32_t me;  // the set
-  uint32_t it = 0, q_it = 0, s_work = 0, p_work = 0, turn_it = 0, p_count = 0, q_buf = 0, k_use = 0, v_use = 0;  // q_buf: a bit per row tile
-  int s_step = 0, s_n = 0, p_step = 0, p_n = 0;
-  Order so, po;
-  bool alive = true, ended = false;
+  uint32_t p_count = 0;
+  bool alive = true;
+
+  // the set's key tiles, piece after piece
+  struct Cursor {
+    uint32_t work = 0, use = 0, step = 0, q = 0;  // pieces opened; ring use of the tile, its step; Q tile
+    int left = 0, keys = 0, width = 0;                       // tiles and keys from this one on, keys per step
+    bool opens = false, shared_q = false;
+  } s, v;
 
   __device__ __forceinline__ MmaRole(const TcParams& p_, Bars* b, const Work* r, uint32_t base, uint32_t t, uint32_t me_)
       : p(p_), bars(b), ring(r), q0(base), tmem(t), me(me_) {}
   __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity) {
-        if (alive && !__all_sync(0xffffffffu, mbar_wait(bar, parity))) {
+    if (alive && !__all_sync(0xffffffffu, mbar_wait(bar, parity))) {
       alive = false;
       if ((threadIdx.x & 31) == 0) atomicOr(p.status, IA_DEV_STATUS_ATTEND_WAIT);
     }
     return alive;
   }
-  __device__ __forceinline__ bool wait_stage(uint32_t use) { return wait(&bars->full[use % C::stages], (use / C::stages) & 1); }
-  // What there is to do for the next step, decided before anything is waited for: between its products this thread only
-  // issues.
-  struct First { bool mine, valid, opens, closes; uint32_t use, buf, q_parity, k16; };
-  struct Second { bool mine, valid, opens, closes; uint32_t use, k16; };
-  __device__ __forceinline__ First s_next() {
-    First f{};
-    if (ended || !alive) return f;
-    if (s_step == s_n) {
-      const uint32_t slot = s_work % kWorkSlots;
-      if (!wait(&bars->work_full[slot], (s_work / kWorkSlots) & 1)) return f;
-      ++s_work;
-      if (ring[slot].last) {
-        ended = true;
-        return f;
+  // On to the set's next tile; false: there is none.  The second product's cursor gives pieces back.
+  __device__ __forceinline__ bool next(Cursor& c, bool give_back) {
+    if (--c.left > 0) {
+      c.use += c.step;
+      c.keys -= c.width;
+      c.opens = false;
+      return true;
+    }
+    do {
+      if (give_back && c.work > 0 && elect_one()) mbar_arrive(&bars->work_empty[(c.work - 1) % kWorkSlots]);
+      const uint32_t slot = c.work % kWorkSlots;
+      if (!wait(&bars->work_full[slot], (c.work / kWorkSlots) & 1) || ring[slot].last) {
+        c.left = 1;  // and so it stays
+        return false;
       }
-      s_step = 0;
-      so = ring[slot].order;
-      s_n = so.steps();
-    }
-    const int i = s_step++;
-    const Step st = step_of(so, i);
-    f.mine = ((so.first + i) & 1) == me;
-    f.valid = st.valid;
-    if (!st.valid) return f;
-    if (st.first_use) k_use = it++;
-    if (st.opens && (!so.split || i == 0)) {
-      q_buf = (q_buf & ~(1u << st.rt)) | ((q_it & 1) << st.rt);
-      ++q_it;
-    }
-    f.opens = st.opens;
-    f.closes = st.closes;
-    f.use = k_use;
-    f.k16 = st.k16;
-    f.buf = (q_buf >> st.rt) & 1;
-    f.q_parity = ((q_it - 1 - (((q_it - 1) & 1) ^ f.buf)) >> 1) & 1;
+      ++c.work;
+      const Order o = ring[slot].order;
+      const int i = (int)me ^ o.first;
+      c.left = o.split ? (o.tiles(0) - i + 1) >> 1 : o.tiles(i);
+      c.use = o.ring + (o.split ? 2 * i : 0);
+      c.step = o.split ? 4 : 2;
+      c.keys = o.split ? o.keys[0] - i * kKeys : o.keys_of(i);
+      c.width = o.split ? 2 * kKeys : kKeys;
+      c.q = o.q + (o.split ? 0 : i);
+      c.opens = true;
+    } while (c.left <= 0);
+    return true;
+  }
+  // The values have to be known as the same in all lanes, or every operand of every MMA is moved to the uniform registers anew.
+  struct First { uint64_t a, b; uint32_t ks, buf, closes, idesc; };
+  __device__ __forceinline__ First first() const {
+    First f;
+    f.ks = uniform(s.use % C::stages);
+    f.buf = uniform(s.q & 1);
+    f.closes = uniform(s.left == 1);
+    f.idesc = uniform(kIdesc<0, false> | ((uint32_t)min(kKeys / 16, (s.keys + 15) >> 4) << 18));  // N = 16 for each 16 keys
+    f.a = umma_desc(q0 + f.buf * C::tile, 0);
+    f.b = umma_desc(q0 + (uint32_t)C::ring + f.ks * C::kv_tile, 0);
     return f;
   }
-  __device__ __forceinline__ bool p_next(Second& f) {  // false: no steps left
-    f = Second{};
-    if (!alive) return false;
-    if (p_step == p_n) {
-      if (p_work > 0 && elect_one()) mbar_arrive(&bars->work_empty[(p_work - 1) % kWorkSlots]);
-      if (ended && p_work + 1 == s_work) return false;
-      p_step = 0;
-      po = ring[p_work % kWorkSlots].order;
-      p_n = po.steps();
-      ++p_work;
-    }
-    const int i = p_step++;
-    const Step st = step_of(po, i);
-    f.mine = ((po.first + i) & 1) == me;
-    f.valid = st.valid;
-    if (!st.valid) return true;
-    if (st.first_use) v_use = it++;
-    f.opens = st.opens;
-    f.closes = st.closes;
-    f.use = v_use;
-    f.k16 = st.k16;
-    return true;
+  __device__ __forceinline__ bool first_ready() const {  // without waiting
+    return __all_sync(0xffffffffu, (!s.opens || mbar_test(&bars->q_full[s.q & 1], (s.q >> 1) & 1)) &&
+                                       mbar_test(&bars->full[s.use % C::stages], (s.use / C::stages) & 1));
   }
-  __device__ __forceinline__ bool ready(const First& f) {
-    return (!f.opens || wait(&bars->q_full[f.buf], f.q_parity)) && wait_stage(f.use);
-  }
-  // The descriptors' upper halves never change; what is added to the lower ones is known to the compiler.  The values have to
-  // be known as the same in all lanes, or every operand of every MMA is moved to the uniform registers anew.
-  __device__ __forceinline__ void first_product(const First& f) {
-    const uint32_t ks = uniform(f.use % C::stages), buf = uniform(f.buf), closes = uniform(f.closes), idesc = uniform(kIdesc<0, false> | (f.k16 << 18));  // N = 16 k16
-    const uint64_t a = umma_desc(q0 + buf * C::tile, 0), b = umma_desc(q0 + (2 + ks) * C::tile, 0);
-    if (PAGED && !ready(f)) return;
-    tc_fence_after();
-    if (elect_one()) {
+  __device__ __forceinline__ void issue_first(const First& f) const {
 #pragma unroll
-      for (int h = 0; h < C::halves; ++h)
+    for (int h = 0; h < C::halves; ++h)
 #pragma unroll
-        for (int s = 0; s < 4; ++s)  // 16 dims = 32 bytes further inside the swizzled row
-          umma_ss(tmem + me * 128, a + (h * C::block + s * 32) / 16, b + (h * C::block + s * 32) / 16, idesc, h + s > 0);
-      umma_commit(&bars->s_full[me]);
-      umma_commit(&bars->empty[ks]);
-      if (closes) umma_commit(&bars->q_empty[buf]);
-    }
-    __syncwarp();
-  }
-  __device__ __forceinline__ bool second_product(const Second& f) {  // has taken the turn
-    const uint32_t vs = uniform(f.use % C::stages), first = uniform(f.opens), closes = uniform(f.closes), k16 = uniform(f.k16);
-    const uint64_t b = umma_desc(q0 + (2 + vs) * C::tile, kNextCols);
-    if (!wait_stage(f.use) || !wait(&bars->p_full[me], p_count & 1) || !wait(&bars->turn[me], turn_it++ & 1)) return true;
-    tc_fence_after();
-    if (elect_one()) {
-#pragma unroll
-      for (int s = 0; s < kKeys / 16; ++s)  // 16 keys: 8 columns of packed weights, 16 rows of V
-        if (s < k16) umma_ts(tmem + 256 + me * 128, tmem + me * 128 + s * 8, b + s * kStepBytes / 16, kIdesc<D, true>, s > 0 ? 1u : first ^ 1u);
-      if (closes) umma_commit(&bars->o_full[me]);
-    }
-    __syncwarp();
-    ++p_count;
-    return true;
-  }
-  __device__ __forceinline__ void pass() {
-    if (elect_one()) mbar_arrive(&bars->turn[me ^ 1]);
-  }
-  __device__ __forceinline__ void release(uint32_t use) {
-    const uint32_t st = uniform(use % C::stages);
-    if (elect_one()) umma_commit(&bars->empty[st]);
-    __syncwarp();
+      for (int i = 0; i < 4; ++i)  // 16 dims = 32 bytes further inside the swizzled row
+        umma_ss(tmem + me * 128, f.a + (h * C::block + i * 32) / 16, f.b + (h * C::kv_block + i * 32) / 16, f.idesc, h + i > 0);
+    umma_commit(&bars->s_full[me]);
+    umma_commit(&bars->empty[f.ks]);
+    if (f.closes) umma_commit(&bars->q_empty[f.buf]);
   }
   __device__ __forceinline__ void run() {
-    Second v{};
+    s.left = v.left = 1;  // the first call opens a piece
 #pragma unroll 1
-    for (uint32_t i = 0; i < 2 || p_next(v); ++i) {
-      const First s = s_next();  // two steps ahead of v: the same set's
-      if (i < 2 ? i != me : !v.mine) continue;
-      if (!PAGED && s.mine && s.valid) ready(s);  // compute bound: the keys are there, and nothing is left to do between the products
-      bool turn = false;
-      if (v.valid) turn = second_product(v);
-      if (!turn) wait(&bars->turn[me], turn_it++ & 1);  // set 0's first turn was given at the start
-      if (s.mine && s.valid && alive) first_product(s);
-      pass();
-      if (v.valid && alive) release(v.use);
+    for (bool start = true; (start || next(v, true)) && alive; start = false) {
+      bool more = next(s, false);
+      const First f = first();
+      if (!start) {
+        const uint32_t vs = uniform((v.use + 1) % C::stages), old = uniform(!v.opens),
+                       k16 = uniform(min(kKeys / 16, (v.keys + 15) >> 4));
+        const uint64_t b = umma_desc(q0 + (uint32_t)C::ring + vs * C::kv_tile, kNextCols);
+        if (!wait(&bars->full[vs], ((v.use + 1) / C::stages) & 1) || !wait(&bars->p_full[me], p_count++ & 1)) break;
+        const bool both = more && first_ready();
+        tc_fence_after();
+        if (elect_one()) {
+#pragma unroll
+          for (int k = 0; k < kKeys / 16; ++k)  // 16 keys: 8 columns of packed weights, 16 rows of V
+            if (k < k16)
+              umma_ts(tmem + 256 + me * 128, tmem + me * 128 + k * 8, b + k * kStepBytes / 16, kIdesc<D, true>, k > 0 ? 1u : old);
+          umma_commit(&bars->o_full[me]);
+          umma_commit(&bars->empty[vs]);
+          if (both) issue_first(f);
+        }
+        __syncwarp();
+        if (both) more = false;
+      }
+      if (more && alive) {
+        if ((s.opens && !wait(&bars->q_full[s.q & 1], (s.q >> 1) & 1)) || !wait(&bars->full[s.use % C::stages], (s.use / C::stages) & 1)) break;
+        tc_fence_after();
+        if (elect_one()) issue_first(f);
+        __syncwarp();
+      }
     }
     if (elect_one()) umma_commit(&bars->drain);  // no MMA, and no arrival of one, may be in flight when the CTA ends
     __syncwarp();
@@ -737,7 +666,7 @@ __device__ __forceinline__ void softmax_role(const TcParams& p, Bars* bars, cons
   const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
   const uint32_t s_addr = tmem + lanes + w * 128, o_addr = tmem + lanes + 256;
   const float c = kLog2e * rsqrtf((float)D);
-  uint32_t s_it = 0, o_it = 0, x_it = 0;
+  uint32_t s_it = 0, x_it = 0;
   const auto wait = [&](uint64_t* bar, uint32_t parity) {  // the whole warp goes on or none of it
     const bool ok = __all_sync(0xffffffffu, mbar_wait(bar, parity));
     if (!ok && lane == 0) atomicOr(p.status, IA_DEV_STATUS_ATTEND_WAIT);
@@ -754,7 +683,7 @@ __device__ __forceinline__ void softmax_role(const TcParams& p, Bars* bars, cons
     };
     const bool split = wk.order.split;
     const int me = w ^ wk.order.first;  // row tile, or place in the order of key tiles
-    const int keys = wk.order.keys[split ? 0 : me], total = (keys + kKeys - 1) / kKeys, stride = split ? 2 : 1, begin = split ? me : 0;
+    const int keys = wk.order.keys_of(split ? 0 : me), total = wk.order.tiles(split ? 0 : me), stride = split ? 2 : 1, begin = split ? me : 0;
     if (begin >= total) {  // the other set has the only key tile
       done();
       continue;
@@ -771,25 +700,19 @@ __device__ __forceinline__ void softmax_role(const TcParams& p, Bars* bars, cons
       if (busy) {
         tc_fence_after();
         const int seen = limit - j * kKeys, all_seen = least - j * kKeys;
-        uint32_t ra[32], rb[32], rc[32], rd[32];
-        tmem_ld(s_addr, ra);
-        tmem_ld(s_addr + 32, rb);
-        tmem_ld(s_addr + 64, rc);
-        tmem_ld(s_addr + 96, rd);
-        tmem_wait_ld(ra);
-        tmem_wait_ld(rb);
-        tmem_wait_ld(rc);
-        tmem_wait_ld(rd);
+        uint32_t r[kKeys / 32][32];
+#pragma unroll
+        for (int i = 0; i < kKeys / 32; ++i) tmem_ld(s_addr + 32 * i, r[i]);
+#pragma unroll
+        for (int i = 0; i < kKeys / 32; ++i) tmem_wait_ld(r[i]);
         const int columns = keys - j * kKeys;  // behind them neither product reads or writes
-        if (all_seen < 32) mask_row(ra, seen);
-        if (all_seen < 64) mask_row(rb, seen - 32);
-        if (all_seen < 96 && columns > 64) mask_row(rc, seen - 64);
-        if (all_seen < 128 && columns > 96) mask_row(rd, seen - 96);
         float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-        max_row(ra, top);
-        max_row(rb, top);
-        if (columns > 64) max_row(rc, top);
-        if (columns > 96) max_row(rd, top);
+#pragma unroll
+        for (int i = 0; i < kKeys / 32; ++i) {
+          if (i * 32 >= columns) break;
+          if (all_seen < 32 * (i + 1)) mask_row(r[i], seen - 32 * i);
+          max_row(r[i], top);
+        }
         const float t = max3(top[0], top[1], max3(top[2], top[3], -INFINITY));
         if (j == begin) {
           m = t;
@@ -816,10 +739,11 @@ __device__ __forceinline__ void softmax_role(const TcParams& p, Bars* bars, cons
         mc = fmaf(mc, 0.f, mc);  // infinite: NaN, as infinity - infinity in the weights
         const uint64_t c2 = pair(c, c), mc2 = pair(-mc, -mc);
         uint64_t sum[2] = {0, 0};
-        weights(ra, c2, mc2, sum, s_addr);
-        weights(rb, c2, mc2, sum, s_addr + 16);
-        if (columns > 64) weights(rc, c2, mc2, sum, s_addr + 32);
-        if (columns > 96) weights(rd, c2, mc2, sum, s_addr + 48);
+#pragma unroll
+        for (int i = 0; i < kKeys / 32; ++i) {
+          if (i * 32 >= columns) break;
+          weights(r[i], c2, mc2, sum, s_addr + 16 * i);
+        }
         float la, lb;
         unpair(add2(sum[0], sum[1]), la, lb);
         l += la + lb;
@@ -829,8 +753,7 @@ __device__ __forceinline__ void softmax_role(const TcParams& p, Bars* bars, cons
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars->p_full[w]);
     }
-    if (!wait(&bars->o_full[w], o_it & 1)) return;
-    ++o_it;
+    if (!wait(&bars->o_full[w], (s_it - 1) & 1)) return;
     tc_fence_after();
     // ---- output: this set's O scaled, or over half of the columns both sets' ----
     float scale = 0.f, its_scale = 0.f, lse = -INFINITY;
@@ -964,7 +887,6 @@ struct Control {
   Bars bars;
   Work ring[kWorkSlots];
   float2 stats[2][kRows];  // (m, l) of either set, for the merge
-  unsigned long long scratch[kThreads / 32];
   uint32_t tmem;
 };
 
@@ -992,7 +914,6 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tc_kernel(const __grid_con
       mbar_init(&bars.q_empty[w], 2);
       mbar_init(&bars.s_full[w], 1);
       mbar_init(&bars.p_full[w], 4);  // a lane of each warp
-      mbar_init(&bars.turn[w], 1);
       mbar_init(&bars.o_full[w], 1);
     }
     for (int i = 0; i < kWorkSlots; ++i) {
@@ -1001,7 +922,6 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tc_kernel(const __grid_con
     }
     mbar_init(&bars.drain, 2);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    mbar_arrive(&bars.turn[0]);  // set 0 begins
   }
   if (warp == kMmaWarp) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&ctl.tmem)), "r"(512) : "memory");
@@ -1014,14 +934,12 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tc_kernel(const __grid_con
   grid_dependency_wait();
   grid_launch_dependents();
   SharedCursor cur{};
-  if constexpr (PAGED) cur = find_share<kKeys, kThreads>(p.s, blockIdx.x, gridDim.x, ctl.scratch);
+  if constexpr (PAGED) cur = find_share<kKeys, kThreads>(p.s, blockIdx.x, gridDim.x, reinterpret_cast<unsigned long long*>(ctl.stats));
   if (warp < kCopyWarp) {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
     softmax_role<D, PAGED>(p, &bars, ctl.ring, tmem, base + C::tiles, ctl.stats);
   } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
     if (warp == kCopyWarp) CopyRole<D, PAGED>(p, &bars, ctl.ring, base, cur).run();
-    if (warp >= kMmaWarp && warp < kMmaWarp + 2) MmaRole<D, PAGED>(p, &bars, ctl.ring, smem_u32(base), uniform(tmem), uniform(warp - kMmaWarp)).run();
+    if (warp >= kMmaWarp) MmaRole<D, PAGED>(p, &bars, ctl.ring, smem_u32(base), uniform(tmem), uniform(warp - kMmaWarp)).run();
   }
   __syncwarp();
   tc_fence_before();
