@@ -345,11 +345,6 @@ __global__ void __launch_bounds__(256) shared_merge_kernel(const SharedParams p,
   store_vec<D / 32>(out + ((int64_t)seq * hq + head) * D + lane * (D / 32), acc);
 }
 
-template <typename Kern> int set_smem(Kern kern, size_t bytes, const char* what) {
-  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-  return e == cudaSuccess ? IA_OK : fail(IA_ERR_LAUNCH, "%s: cudaFuncSetAttribute: %s", what, cudaGetErrorString(e));
-}
-
 template <typename... Args, typename... Given>
 int launch(void (*kern)(Args...), unsigned grid, size_t smem, cudaStream_t stream, const char* what, Given... args) {
   cudaLaunchConfig_t cfg{};
@@ -369,12 +364,14 @@ int launch(void (*kern)(Args...), unsigned grid, size_t smem, cudaStream_t strea
 template <typename T, int D, int RPT>
 int launch_prompt(const PromptTensors& t, const PromptItem* items, int n_items, cudaStream_t stream) {
   auto kern = prompt_attention_kernel<T, D, RPT>;
-  if (int s = set_smem(kern, Smem<D, RPT>::bytes, "prompt_attention")) return s;
+  static SmemOnce once;
+  if (int s = once.allow((const void*)kern, Smem<D, RPT>::bytes, "prompt_attention_kernel")) return s;
   return launch(kern, (unsigned)n_items, Smem<D, RPT>::bytes, stream, "prompt_attention_kernel", t, items);
 }
 template <typename T, int D> int launch_shared(const SharedParams& p, int ctas, cudaStream_t stream) {
   auto kern = shared_attention_kernel<T, D>;
-  if (int s = set_smem(kern, Smem<D, 8>::bytes, "shared_attention")) return s;
+  static SmemOnce once;
+  if (int s = once.allow((const void*)kern, Smem<D, 8>::bytes, "shared_attention_kernel")) return s;
   return launch(kern, (unsigned)ctas, Smem<D, 8>::bytes, stream, "shared_attention_kernel", p);
 }
 template <typename T, int D>
@@ -385,6 +382,17 @@ int launch_merge(const SharedParams& p, const int2* seq_info, int ctas, T* out, 
 }
 
 }  // namespace
+
+int SmemOnce::allow(const void* kern, size_t bytes, const char* what) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return fail(IA_ERR_LAUNCH, "%s: no current device", what);
+  const uint64_t bit = 1ull << (dev & 63);
+  if (dev < 64 && (done.load(std::memory_order_acquire) & bit)) return IA_OK;
+  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  if (e != cudaSuccess) return fail(IA_ERR_LAUNCH, "%s: cudaFuncSetAttribute: %s", what, cudaGetErrorString(e));
+  if (dev < 64) done.fetch_or(bit, std::memory_order_release);
+  return IA_OK;
+}
 
 int sm_count() {
   constexpr int kMaxDevices = 64;

@@ -3,6 +3,8 @@
 // the pieces of work, how the decode step is cut into equal shares, and the exact form of a single row.
 #pragma once
 
+#include <atomic>
+
 #include "ia_common.cuh"
 
 namespace ia {
@@ -249,6 +251,10 @@ template <typename T> struct PagedKeys {
 
 // ---- launchers ------------------------------------------------------------------------------------------------------
 int sm_count();
+struct SmemOnce {  // a kernel's shared memory, allowed once per device
+  std::atomic<uint64_t> done{0};
+  int allow(const void* kern, size_t bytes, const char* what);
+};
 int64_t prompt_plan_ints(const int32_t* q_lens, int n_seqs, int n_kv_heads, int group, int dtype);  // -1: too large
 int make_prompt_plan(const int32_t* q_lens, const int32_t* kv_lens, int n_seqs, int n_kv_heads, int group, int head_dim, int dtype,
                      int32_t* plan, int64_t plan_ints);

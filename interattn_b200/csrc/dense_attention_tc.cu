@@ -989,9 +989,9 @@ int encode_q(CUtensorMap* tm, const void* q, int head_dim, int group, int n_kv_h
 
 template <int D, bool PAGED> int launch_tc(const TcParams& p, int grid, cudaStream_t stream) {
   auto kern = attend_tc_kernel<D, PAGED>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Tc<D>::smem);
-  if (e != cudaSuccess) return fail(IA_ERR_LAUNCH, "dense attention: cudaFuncSetAttribute: %s", cudaGetErrorString(e));
-  e = launch_overlapped(kern, (unsigned)grid, (unsigned)kThreads, Tc<D>::smem, stream, p);
+  static SmemOnce once;
+  if (int s = once.allow((const void*)kern, Tc<D>::smem, "attend_tc_kernel")) return s;
+  const cudaError_t e = launch_overlapped(kern, (unsigned)grid, (unsigned)kThreads, Tc<D>::smem, stream, p);
   return e == cudaSuccess ? check_launch("attend_tc_kernel") : fail(IA_ERR_LAUNCH, "attend_tc_kernel: %s", cudaGetErrorString(e));
 }
 

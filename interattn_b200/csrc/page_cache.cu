@@ -3,11 +3,11 @@
 // number of table entries that hold it; a page is free when its count is zero.
 //
 // There is no free list: a page is handed out by its rank among the free ones, lowest first, so the result depends on the
-// counts alone and not on the order in which threads or earlier calls ran.  Ranks are prefix sums over the counts, which
-// one cluster of eight CTAs takes in one launch: 8192 threads, the cluster's hardware barrier between the phases, the
-// CTAs' totals through distributed shared memory.  Whatever moves data (the copies, the table rows of a fork, the
-// remapped entries) follows in a second launch on the whole GPU and reads what to do from the scratch that the cluster
-// left.
+// counts alone and not on the order in which threads or earlier calls ran.  Ranks are prefix sums over the counts, taken in
+// one launch: by one CTA where list and pool are short, a chain of barriers and round trips to memory either way, and by a
+// cluster of eight where they are long (8192 threads, the cluster's hardware barrier between the phases, the CTAs' totals
+// through distributed shared memory).  Whatever moves data (the copies, the table rows of a fork, the remapped entries)
+// follows in a second launch on the whole GPU and reads what to do from the scratch that the first left.
 #include <algorithm>
 
 #include "dense_attention.cuh"
@@ -17,7 +17,8 @@ namespace ia {
 namespace {
 
 constexpr int kPage = 16;
-constexpr int kPlanCtas = 8, kPlanThreads = 1024, kPlanAll = kPlanCtas * kPlanThreads;
+constexpr int kPlanCtas = 8, kPlanThreads = 1024;  // of the large plan; the small one is one CTA
+constexpr int kSmallList = 256, kSmallPool = 65536;
 constexpr int kMoveThreads = 256;
 
 // scratch: counters, then per entry of a list the inclusive sum of the pages wanted and what was granted, then the moves
@@ -57,9 +58,11 @@ __device__ __forceinline__ int len_of(const State& st, int row) {
 __device__ __forceinline__ void report(const State& st, int bits) { atomicOr(st.status, bits); }
 
 // ---- prefix sums over the whole cluster -----------------------------------------------------------------------------
-__device__ __forceinline__ void cluster_sync_all() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+template <int CTAS> __device__ __forceinline__ void sync_all() {
+  if constexpr (CTAS == 1) __syncthreads();
+  else asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
+template <int CTAS> __device__ __forceinline__ int cta_rank() { return CTAS == 1 ? 0 : (int)blockIdx.x; }
 __device__ __forceinline__ int peer_word(const int* smem, int rank) {
   uint32_t addr = (uint32_t)__cvta_generic_to_shared(smem), remote;
   int v;
@@ -68,8 +71,8 @@ __device__ __forceinline__ int peer_word(const int* smem, int rank) {
   return v;
 }
 struct Sums { int before, total; };
-// exclusive sum of v over all threads of the cluster in order of (CTA, thread), and the sum of all
-__device__ Sums cluster_scan(int v, int* warp_sums, int* cta_sum) {
+// exclusive sum of v over all threads in order of (CTA, thread), and the sum of all
+template <int CTAS> __device__ Sums scan(int v, int* warp_sums, int* cta_sum) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   int upto = v;
 #pragma unroll
@@ -91,15 +94,33 @@ __device__ Sums cluster_scan(int v, int* warp_sums, int* cta_sum) {
   }
   __syncthreads();
   int before = upto - v + (warp > 0 ? warp_sums[warp - 1] : 0), total = 0;
-  cluster_sync_all();  // every CTA's sum is there
+  if constexpr (CTAS == 1) {
+    total = *cta_sum;
+  } else {
+    sync_all<CTAS>();  // every CTA's sum is there
 #pragma unroll
-  for (int c = 0; c < kPlanCtas; ++c) {
-    const int x = peer_word(cta_sum, c);
-    if (c < (int)blockIdx.x) before += x;
-    total += x;
+    for (int c = 0; c < CTAS; ++c) {
+      const int x = peer_word(cta_sum, c);
+      if (c < cta_rank<CTAS>()) before += x;
+      total += x;
+    }
   }
-  cluster_sync_all();  // and has been read by all: the words may be used again
+  sync_all<CTAS>();  // and has been read by all: the words may be used again
   return {before, total};
+}
+
+// how many of the pages [p0, p1) are free; four counts at a time where the array allows it
+__device__ __forceinline__ int count_free(const int* refs, int p0, int p1) {
+  int n = 0, g = p0;
+  if ((reinterpret_cast<uintptr_t>(refs + p0) & 15) == 0) {
+#pragma unroll 4
+    for (; g + 4 <= p1; g += 4) {
+      const int4 r = *reinterpret_cast<const int4*>(refs + g);
+      n += (r.x == 0) + (r.y == 0) + (r.z == 0) + (r.w == 0);
+    }
+  }
+  for (; g < p1; ++g) n += refs[g] == 0;
+  return n;
 }
 
 // ---- who gets which page --------------------------------------------------------------------------------------------
@@ -112,29 +133,44 @@ struct PlanParams {
   int fork, share;
 };
 
-__global__ void __cluster_dims__(kPlanCtas, 1, 1) __launch_bounds__(kPlanThreads) pages_plan_kernel(const PlanParams p) {
+template <int CTAS> __global__ void __launch_bounds__(kPlanThreads) pages_plan_kernel(const PlanParams p) {
   __shared__ int warp_sums[32];
   __shared__ int cta_sum;
+  __shared__ int named[CTAS == 1 ? kSmallList : 1];
+  constexpr int kAll = CTAS * kPlanThreads;
   const State& st = p.st;
-  const int me = blockIdx.x * kPlanThreads + threadIdx.x;
-  const int per = (p.n + kPlanAll - 1) / kPlanAll, i0 = min(p.n, me * per), i1 = min(p.n, i0 + per);
-  cluster_sync_all();  // the whole cluster runs before anyone reads a peer's shared memory
+  const int me = cta_rank<CTAS>() * kPlanThreads + threadIdx.x;
+  const int per = (p.n + kAll - 1) / kAll, i0 = min(p.n, me * per), i1 = min(p.n, i0 + per);
+  if constexpr (CTAS > 1) sync_all<CTAS>();  // the whole cluster runs before anyone reads a peer's shared memory
   grid_dependency_wait();
   if (p.fork) grid_launch_dependents();  // the copies follow; what follows an extend is not known here
+  // free pages; a thread counts a run of them
+  const int run = ((st.n_pages + kAll - 1) / kAll + 3) & ~3, p0 = min(st.n_pages, me * run), p1 = min(st.n_pages, p0 + run);
+  const int n_free = count_free(st.refs, p0, p1);
   // a row that the list names twice belongs to its first entry
-  for (int i = i0; i < i1; ++i)
-    if ((unsigned)p.rows[i] < (unsigned)st.n_rows) p.sc.owner[p.rows[i]] = 0x7fffffff;
-  __threadfence();
-  cluster_sync_all();
-  for (int i = i0; i < i1; ++i)
-    if ((unsigned)p.rows[i] < (unsigned)st.n_rows) atomicMin(p.sc.owner + p.rows[i], i);
-  __threadfence();
-  cluster_sync_all();
+  bool again = false;
+  if constexpr (CTAS == 1) {
+    if (me < p.n) named[me] = p.rows[me];
+    __syncthreads();
+    if (me < p.n)
+      for (int i = 0; i < me; ++i) again |= named[i] == named[me];
+  } else {
+    for (int i = i0; i < i1; ++i)
+      if ((unsigned)p.rows[i] < (unsigned)st.n_rows) p.sc.owner[p.rows[i]] = 0x7fffffff;
+    __threadfence();
+    sync_all<CTAS>();
+    for (int i = i0; i < i1; ++i)
+      if ((unsigned)p.rows[i] < (unsigned)st.n_rows) atomicMin(p.sc.owner + p.rows[i], i);
+    __threadfence();
+    sync_all<CTAS>();
+  }
   int wanted = 0;
   for (int i = i0; i < i1; ++i) {
     const int row = p.rows[i], other = p.other[i];
     int kept = -1, need = 0;
-    if ((unsigned)row < (unsigned)st.n_rows && __ldcg(p.sc.owner + row) == i) {
+    if constexpr (CTAS > 1)
+      if ((unsigned)row < (unsigned)st.n_rows) again = __ldcg(p.sc.owner + row) != i;
+    if ((unsigned)row < (unsigned)st.n_rows && !again) {
       const int len = len_of(st, row);
       if (p.fork) {
         if ((unsigned)other < (unsigned)st.n_rows && other != row && len == 0) {
@@ -154,12 +190,8 @@ __global__ void __cluster_dims__(kPlanCtas, 1, 1) __launch_bounds__(kPlanThreads
     wanted += need;
     p.sc.upto[i] = need;
   }
-  const Sums want = cluster_scan(wanted, warp_sums, &cta_sum);
-  // free pages; a thread counts a run of them
-  const int run = ((st.n_pages + kPlanAll - 1) / kPlanAll + 3) & ~3, p0 = min(st.n_pages, me * run), p1 = min(st.n_pages, p0 + run);
-  int n_free = 0;
-  for (int g = p0; g < p1; ++g) n_free += st.refs[g] == 0;
-  const Sums free_pages = cluster_scan(n_free, warp_sums, &cta_sum);
+  const Sums want = scan<CTAS>(wanted, warp_sums, &cta_sum);
+  const Sums free_pages = scan<CTAS>(n_free, warp_sums, &cta_sum);
   // from the first entry on that does not fit, none is served
   int upto = want.before, granted = 0;
   for (int i = i0; i < i1; ++i) {
@@ -174,7 +206,7 @@ __global__ void __cluster_dims__(kPlanCtas, 1, 1) __launch_bounds__(kPlanThreads
     if (fits) granted += need;
   }
   __threadfence();
-  const Sums grants = cluster_scan(granted, warp_sums, &cta_sum);  // also: the sums above are visible to all
+  const Sums grants = scan<CTAS>(granted, warp_sums, &cta_sum);  // also: the sums above are visible to all
   // new lengths; all lengths were read before the barriers above
   for (int i = i0; i < i1; ++i)
     if (p.sc.kept[i] >= 0) st.lens[p.rows[i]] = p.sc.new_len[i];
@@ -198,22 +230,24 @@ __global__ void __cluster_dims__(kPlanCtas, 1, 1) __launch_bounds__(kPlanThreads
 }
 
 // Live pages at or past the number of live pages move into the holes below it, in order.
-__global__ void __cluster_dims__(kPlanCtas, 1, 1) __launch_bounds__(kPlanThreads) pages_compact_plan_kernel(const State st, const Scratch sc) {
+struct CompactParams { State st; Scratch sc; };
+template <int CTAS> __global__ void __launch_bounds__(kPlanThreads) pages_compact_plan_kernel(const CompactParams p) {
   __shared__ int warp_sums[32];
   __shared__ int cta_sum;
-  const int me = blockIdx.x * kPlanThreads + threadIdx.x;
-  cluster_sync_all();
+  constexpr int kAll = CTAS * kPlanThreads;
+  const State& st = p.st;
+  const Scratch& sc = p.sc;
+  const int me = cta_rank<CTAS>() * kPlanThreads + threadIdx.x;
+  if constexpr (CTAS > 1) sync_all<CTAS>();
   grid_dependency_wait();
   grid_launch_dependents();
-  const int run = ((st.n_pages + kPlanAll - 1) / kPlanAll + 3) & ~3, p0 = min(st.n_pages, me * run), p1 = min(st.n_pages, p0 + run);
-  int live = 0;
-  for (int g = p0; g < p1; ++g) live += st.refs[g] != 0;
-  const Sums all = cluster_scan(live, warp_sums, &cta_sum);
+  const int run = ((st.n_pages + kAll - 1) / kAll + 3) & ~3, p0 = min(st.n_pages, me * run), p1 = min(st.n_pages, p0 + run);
+  const Sums all = scan<CTAS>(p1 - p0 - count_free(st.refs, p0, p1), warp_sums, &cta_sum);
   const int n_live = all.total;
   // live pages before n_live: the sum up to the boundary; holes below it and movers above it pair off by rank
-  int hole = p0 - all.before, below = 0;
-  for (int g = p0; g < min(p1, n_live); ++g) below += st.refs[g] != 0;
-  const Sums low = cluster_scan(below, warp_sums, &cta_sum);
+  int hole = p0 - all.before;
+  const int upto = max(p0, min(p1, n_live));
+  const Sums low = scan<CTAS>(upto - p0 - count_free(st.refs, p0, upto), warp_sums, &cta_sum);
   int mover = all.before - min(all.before, low.total);
   if (p0 < n_live && p1 > n_live) mover = 0;
   for (int g = p0; g < p1; ++g) {
@@ -222,9 +256,9 @@ __global__ void __cluster_dims__(kPlanCtas, 1, 1) __launch_bounds__(kPlanThreads
     if (g >= n_live && is_live) sc.moves[mover++].x = g;
   }
   __threadfence();
-  cluster_sync_all();
+  sync_all<CTAS>();
   const int n = n_live - low.total;
-  for (int i = me; i < n; i += kPlanAll) {
+  for (int i = me; i < n; i += kAll) {
     const int2 mv = __ldcg(sc.moves + i);
     sc.remap[mv.x] = mv.y;
     st.refs[mv.y] = st.refs[mv.x];
@@ -277,17 +311,16 @@ __device__ __forceinline__ void copy_runs(const MoveParams& p) {
 __global__ void __launch_bounds__(kMoveThreads) pages_fork_kernel(const MoveParams p) {
   grid_dependency_wait();
   const State& st = p.st;
-  // table rows and counts of what parent and child share, a warp per entry of the list
-  for (int i = blockIdx.x * (kMoveThreads / 32) + (threadIdx.x >> 5); i < p.n; i += gridDim.x * (kMoveThreads / 32)) {
-    const int kept = p.sc.kept[i];
-    if (kept < 0) continue;
-    const int64_t child = p.children[i], parent = p.parents[i];
-    for (int j = threadIdx.x & 31; j < kept; j += 32) {
-      const int page = st.table[parent * st.max_pages + j];
-      st.table[child * st.max_pages + j] = page;
-      if ((unsigned)page < (unsigned)st.n_pages) atomicAdd(st.refs + page, 1);
-      else report(st, DEV_STATUS_BAD_INDEX);
-    }
+  // table rows and counts of what parent and child share: a warp takes 32 pages of an entry of the list
+  const int pieces = (st.max_pages + 31) / 32;
+  for (int64_t u = blockIdx.x * (kMoveThreads / 32) + (threadIdx.x >> 5); u < (int64_t)p.n * pieces;
+       u += gridDim.x * (kMoveThreads / 32)) {
+    const int i = (int)(u % p.n), j = (int)(u / p.n) * 32 + (threadIdx.x & 31);
+    if (j >= p.sc.kept[i]) continue;
+    const int page = st.table[(int64_t)p.parents[i] * st.max_pages + j];
+    st.table[(int64_t)p.children[i] * st.max_pages + j] = page;
+    if ((unsigned)page < (unsigned)st.n_pages) atomicAdd(st.refs + page, 1);
+    else report(st, DEV_STATUS_BAD_INDEX);
   }
   copy_runs(p);
 }
@@ -308,10 +341,12 @@ __global__ void __launch_bounds__(kMoveThreads) pages_compact_kernel(const MoveP
 }
 
 // One CTA per entry: whoever takes the row's length away gives its pages back, so a row named twice is freed once.
-__global__ void __launch_bounds__(512) pages_free_kernel(const State st, const int* rows) {
+struct FreeParams { State st; const int* rows; };
+__global__ void __launch_bounds__(512) pages_free_kernel(const FreeParams p) {
   __shared__ int len_s;
+  const State& st = p.st;
   grid_dependency_wait();
-  const int row = rows[blockIdx.x];
+  const int row = p.rows[blockIdx.x];
   if ((unsigned)row >= (unsigned)st.n_rows) {
     if (threadIdx.x == 0) report(st, DEV_STATUS_BAD_INDEX);
     return;
@@ -407,8 +442,8 @@ __global__ void __launch_bounds__(kMoveThreads) pages_write_kernel(const WritePa
 // None of the kernels that end a call lets its successor start early: that may be a kernel which reads tables, lengths
 // or pages before it waits.
 template <typename Params>
-int launch(void (*kern)(Params), unsigned grid, unsigned block, cudaStream_t stream, const char* what, const Params& p) {
-  const cudaError_t e = launch_overlapped(kern, grid, block, 0, stream, p);
+int launch(void (*kern)(Params), unsigned grid, unsigned block, cudaStream_t stream, const char* what, const Params& p, int cluster = 1) {
+  const cudaError_t e = launch_overlapped(kern, grid, block, 0, stream, p, cluster);
   return e == cudaSuccess ? check_launch(what) : fail(IA_ERR_LAUNCH, "%s: %s", what, cudaGetErrorString(e));
 }
 
@@ -443,8 +478,10 @@ static int plan(const ia_page_cache& c, const int32_t* rows, const int32_t* othe
                 Scratch* sc, cudaStream_t stream) {
   if (int s = state_of(c, st)) return s;
   *sc = scratch_of(c);
-  return launch(pages_plan_kernel, (unsigned)kPlanCtas, (unsigned)kPlanThreads, stream, "pages_plan_kernel",
-                PlanParams{*st, *sc, rows, other, n, fork, share});
+  const PlanParams p{*st, *sc, rows, other, n, fork, share};
+  if (n <= kSmallList && c.n_pages <= kSmallPool)
+    return launch(pages_plan_kernel<1>, 1u, (unsigned)kPlanThreads, stream, "pages_plan_kernel", p);
+  return launch(pages_plan_kernel<kPlanCtas>, (unsigned)kPlanCtas, (unsigned)kPlanThreads, stream, "pages_plan_kernel", p, kPlanCtas);
 }
 
 int launch_pages_extend(const ia_page_cache& c, const int32_t* rows, const int32_t* n_tokens, int n, cudaStream_t stream) {
@@ -468,16 +505,19 @@ int launch_pages_fork(const ia_page_cache& c, const int32_t* parents, const int3
 int launch_pages_free(const ia_page_cache& c, const int32_t* rows, int n, cudaStream_t stream) {
   State st;
   if (int s = state_of(c, &st)) return s;
-  pages_free_kernel<<<n, 512, 0, stream>>>(st, rows);
-  return check_launch("pages_free_kernel");
+  return launch(pages_free_kernel, (unsigned)n, 512u, stream, "pages_free_kernel", FreeParams{st, rows});
 }
 
 int launch_pages_compact(const ia_page_cache& c, cudaStream_t stream) {
   State st;
   if (int s = state_of(c, &st)) return s;
   const Scratch sc = scratch_of(c);
-  pages_compact_plan_kernel<<<kPlanCtas, kPlanThreads, 0, stream>>>(st, sc);
-  if (int s = check_launch("pages_compact_plan_kernel")) return s;
+  const CompactParams p{st, sc};
+  const int s = c.n_pages <= kSmallPool
+                    ? launch(pages_compact_plan_kernel<1>, 1u, (unsigned)kPlanThreads, stream, "pages_compact_plan_kernel", p)
+                    : launch(pages_compact_plan_kernel<kPlanCtas>, (unsigned)kPlanCtas, (unsigned)kPlanThreads, stream,
+                             "pages_compact_plan_kernel", p, kPlanCtas);
+  if (s) return s;
   return launch(pages_compact_kernel, (unsigned)sm_count() * 4, (unsigned)kMoveThreads, stream, "pages_compact_kernel",
                 moves_of(c, st, sc));
 }

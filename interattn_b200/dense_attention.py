@@ -19,6 +19,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import struct
 from typing import Optional, Sequence
 
 import torch
@@ -27,11 +28,13 @@ from . import _lib
 from .ops import PagedKV, _DTYPES, _need_cuda, _ptr, _q_geom
 
 
-def device_stream(device: torch.device):
-    """The raw current stream of ``device`` and a context in which kernels go to that device."""
-    index = device.index if device.index is not None else torch.cuda.current_device()
-    guard = contextlib.nullcontext() if index == torch.cuda.current_device() else torch.cuda.device(index)
-    return ctypes.c_void_p(torch._C._cuda_getCurrentRawStream(index)), guard
+_raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
+_NO_GUARD = contextlib.nullcontext()
+
+
+def device_guard(index: int):
+    """A context in which kernels go to the device."""
+    return _NO_GUARD if index == _current_device() else torch.cuda.device(index)
 
 
 def _same_device(device: torch.device, **tensors) -> None:
@@ -45,6 +48,9 @@ def _host_lens(name: str, lens) -> torch.Tensor:
     if t.dim() != 1 or (t.numel() and (int(t.min()) < 0 or int(t.max()) > 0x7fffffff)):
         raise ValueError(f"{name} is a list of lengths, one per sequence, none negative")
     return t.to(torch.int32).contiguous()
+
+
+_PROMPT_TENSORS = struct.Struct("=5Q6q6i").pack   # struct ia_prompt_tensors
 
 
 class PromptAttention:
@@ -86,41 +92,43 @@ class PromptAttention:
             _lib.check(lib.ia_prompt_plan(*args, _ptr(self._host), words))
             self._plan = self._host.to(self.device)
         self._host = self._host[:8].clone()
-        self._t = _lib.PromptTensors(n_q_tokens=self.n_q_tokens, n_kv_tokens=self.n_kv_tokens, n_kv_heads=self.n_kv_heads,
-                                     group_size=group, head_dim=self.head_dim, dtype=_DTYPES[dtype])
+        # run() is called once per layer: what it passes and checks against is made here
+        self._call, self._index = lib.ia_prompt_attention, self.device.index
+        self._plan_args = (self._host.data_ptr(), self._plan.data_ptr())
+        self._sizes = (self.n_q_tokens, self.n_kv_tokens, self.n_kv_heads, group, self.head_dim, _DTYPES[dtype])
+        self._q_shape = torch.Size((self.n_q_tokens, self.n_q_heads, self.head_dim))
+        self._kv_shape = torch.Size((self.n_kv_tokens, self.n_kv_heads, self.head_dim))
 
-    def _check(self, name: str, t: torch.Tensor, tokens: int, heads: int) -> None:
+    def _fits(self, t: torch.Tensor, shape: torch.Size) -> bool:
+        return t.shape == shape and t.dtype is self.dtype and t.get_device() == self._index and t.stride(2) == 1
+
+    def _refuse(self, name: str, t: torch.Tensor, shape: torch.Size) -> None:
         _need_cuda(t)
-        if t.shape != (tokens, heads, self.head_dim) or t.dtype != self.dtype:
-            raise ValueError(f"{name} must be a [{tokens}, {heads}, {self.head_dim}] {self.dtype} tensor")
+        if t.shape != shape or t.dtype != self.dtype:
+            raise ValueError(f"{name} must be a {list(shape)} {self.dtype} tensor")
         _same_device(self.device, **{name: t})
-        if t.stride(2) != 1:
-            raise ValueError(f"the {self.head_dim} elements of one head of {name} must be contiguous")
+        raise ValueError(f"the {self.head_dim} elements of one head of {name} must be contiguous")
 
     def run(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, out: Optional[torch.Tensor] = None,
             return_lse: bool = False):
         """q ``[sum(q_lens), Hq, D]``, k and v ``[sum(kv_lens), Hkv, D]`` (token and head strides of any multiple of 16 bytes)
         -> ``[sum(q_lens), Hq, D]``, with ``return_lse`` also the log-sum-exp ``[sum(q_lens), Hq]`` f32 (-inf for a
         row without keys) that ``ops.finalize`` merges by."""
-        self._check("q", q, self.n_q_tokens, self.n_q_heads)
-        self._check("k", k, self.n_kv_tokens, self.n_kv_heads)
-        self._check("v", v, self.n_kv_tokens, self.n_kv_heads)
+        for name, t, shape in (("q", q, self._q_shape), ("k", k, self._kv_shape), ("v", v, self._kv_shape)):
+            if not self._fits(t, shape):
+                self._refuse(name, t, shape)
         if out is None:
-            out = torch.empty(q.shape, dtype=self.dtype, device=self.device)
-        else:
-            self._check("out", out, self.n_q_tokens, self.n_q_heads)
-            if not out.is_contiguous():
-                raise ValueError("out must be contiguous")
-        lse = torch.empty(q.shape[:2], dtype=torch.float32, device=self.device) if return_lse else None
-        t = _lib.PromptTensors.from_buffer_copy(self._t)   # a copy: two threads may run the same plan
-        t.q, t.k, t.v, t.out = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
-        t.lse = None if lse is None else lse.data_ptr()
-        t.q_tok_stride, t.q_head_stride, _ = q.stride()
-        t.k_tok_stride, t.k_head_stride, _ = k.stride()
-        t.v_tok_stride, t.v_head_stride, _ = v.stride()
-        stream, guard = device_stream(self.device)
-        with guard:
-            _lib.check(_lib.load().ia_prompt_attention(ctypes.byref(t), _ptr(self._host), _ptr(self._plan), stream))
+            out = torch.empty(self._q_shape, dtype=self.dtype, device=self.device)
+        elif not self._fits(out, self._q_shape):
+            self._refuse("out", out, self._q_shape)
+        elif not out.is_contiguous():
+            raise ValueError("out must be contiguous")
+        lse = torch.empty(self._q_shape[:2], dtype=torch.float32, device=self.device) if return_lse else None
+        (qt, qh, _), (kt, kh, _), (vt, vh, _) = q.stride(), k.stride(), v.stride()
+        tensors = _PROMPT_TENSORS(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(),
+                                  qt, qh, kt, kh, vt, vh, *self._sizes)
+        with device_guard(self._index):
+            _lib.check(self._call(tensors, *self._plan_args, _raw_stream(self._index)))
         return (out, lse) if return_lse else out
 
 
@@ -159,22 +167,25 @@ class SharedPrefixAttention:
             _lib.check(lib.ia_shared_prefix_plan(_ptr(sizes), sizes.numel(), ctypes.byref(self.geom), _ptr(plan), words))
             self._plan, self._parts = plan.to(self.device), int(plan[0])
             self._ws_bytes = int(lib.ia_shared_prefix_workspace_bytes(self._parts, ctypes.byref(self.geom)))
+        self._call, self._index, self._q_shape = lib.ia_shared_prefix_decode, self.device.index, torch.Size(self._shape)
         self._args = (_ptr(kv.k_pool), _ptr(kv.v_pool), _ptr(kv.block_table), _ptr(kv.seq_lens), _ptr(shared_lens),
                       _ptr(self._plan), self._parts, ctypes.byref(self.geom))
 
     def step(self, q: torch.Tensor, *, out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """q ``[B, Hq, D]`` -> ``[B, Hq, D]``."""
-        if not q.is_cuda or q.shape != self._shape or q.dtype != self._dtype or not q.is_contiguous():
-            raise ValueError(f"q must be a contiguous CUDA {self._shape} {self._dtype} tensor")
+        if q.shape != self._q_shape or q.dtype is not self._dtype or q.get_device() != self._index or not q.is_contiguous():
+            self._refuse("q", q)
         if out is None:
             out = torch.empty_like(q)
-        elif not out.is_cuda or out.shape != self._shape or out.dtype != self._dtype or not out.is_contiguous():
-            raise ValueError(f"out must be a contiguous CUDA {self._shape} {self._dtype} tensor")
-        _same_device(self.device, q=q, out=out)
+        elif out.shape != self._q_shape or out.dtype is not self._dtype or out.get_device() != self._index or not out.is_contiguous():
+            self._refuse("out", out)
         ws = torch.empty((self._ws_bytes,), dtype=torch.uint8, device=self.device)
-        stream, guard = device_stream(self.device)
-        with guard:
-            _lib.check(_lib.load().ia_shared_prefix_decode(
-                ctypes.c_void_p(q.data_ptr()), *self._args, ctypes.c_void_p(ws.data_ptr()), self._ws_bytes,
-                ctypes.c_void_p(out.data_ptr()), stream))
+        with device_guard(self._index):
+            _lib.check(self._call(q.data_ptr(), *self._args, ws.data_ptr(), self._ws_bytes, out.data_ptr(),
+                                  _raw_stream(self._index)))
         return out
+
+    def _refuse(self, name: str, t: torch.Tensor) -> None:
+        if t.is_cuda and t.shape == self._q_shape and t.dtype == self._dtype and t.is_contiguous():
+            _same_device(self.device, **{name: t})
+        raise ValueError(f"{name} must be a contiguous CUDA {self._shape} {self._dtype} tensor")

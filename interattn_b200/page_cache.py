@@ -19,8 +19,8 @@ from typing import Optional, Sequence, Tuple
 import torch
 
 from . import _lib
-from .dense_attention import _same_device, device_stream
-from .ops import PagedKV, _DTYPES, _need_cuda, _ptr
+from .dense_attention import _raw_stream, _same_device, device_guard
+from .ops import PagedKV, _DTYPES, _need_cuda
 
 PAGE = 16
 
@@ -70,7 +70,9 @@ class PageCache:
             page_stride=k.stride(0), head_stride=k.stride(1), n_rows=int(block_table.shape[0]),
             max_pages=int(block_table.shape[1]), n_pages=int(k.shape[0]), n_pools=len(flat), n_kv_heads=int(k.shape[1]),
             head_dim=int(k.shape[3]), dtype=_DTYPES[k.dtype], reserved=0)
-        self._c = ctypes.byref(self._state)
+        self._c, self._index = ctypes.byref(self._state), self.device.index
+        self._lib = _lib.load()
+        self._token_shape = (int(k.shape[1]), int(k.shape[3]))
 
     @staticmethod
     def empty(n_layers: int, n_pages: int, n_kv_heads: int, head_dim: int, n_rows: int, max_pages: int, *,
@@ -89,51 +91,53 @@ class PageCache:
         k, v = self.pools[layer]
         return PagedKV(k, v, self.block_table, self.seq_lens if prefix_lens is None else prefix_lens, self.seq_lens)
 
-    def _list(self, name: str, t: torch.Tensor, n: Optional[int] = None) -> ctypes.c_void_p:
-        _need_cuda(t)
-        if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous():
-            raise ValueError(f"{name} must be a contiguous int32 list")
-        if n is not None and t.numel() != n:
-            raise ValueError(f"{name} must have {n} entries")
-        _same_device(self.device, **{name: t})
-        return ctypes.c_void_p(t.data_ptr())
+    def _list(self, name: str, t: torch.Tensor, n: Optional[int] = None) -> int:
+        if t.dtype is not torch.int32 or t.dim() != 1 or not t.is_contiguous() or t.get_device() != self._index \
+                or (n is not None and t.numel() != n):
+            _need_cuda(t)
+            _same_device(self.device, **{name: t})
+            raise ValueError(f"{name} must be a contiguous int32 list" + ("" if n is None else f" of {n} entries"))
+        return t.data_ptr()
 
-    def _call(self, name: str, *args) -> None:
-        stream, guard = device_stream(self.device)
-        with guard:
-            _lib.check(getattr(_lib.load(), name)(self._c, *args, stream))
+    def _call(self, function, *args) -> None:
+        with device_guard(self._index):
+            _lib.check(function(self._c, *args, _raw_stream(self._index)))
 
     def extend(self, rows: torch.Tensor, n_tokens: torch.Tensor) -> None:
         """``rows[i]`` becomes ``n_tokens[i]`` tokens longer and gets the pages for them."""
-        self._call("ia_pages_extend", self._list("rows", rows), self._list("n_tokens", n_tokens, rows.numel()), rows.numel())
+        n = rows.numel()
+        self._call(self._lib.ia_pages_extend, self._list("rows", rows), self._list("n_tokens", n_tokens, n), n)
 
     def write(self, layer: int, rows: torch.Tensor, starts: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> None:
         """Tokens ``[starts[i], starts[i + 1])`` of k and v ``[T, Hkv, D]`` (token and head strides of any multiple of 16 bytes)
         become the last tokens of ``rows[i]`` in this layer."""
         k_pool, v_pool = self.pools[layer]
-        _need_cuda(k, v)
-        for name, t in (("k", k), ("v", v)):
-            if t.dim() != 3 or t.shape[1:] != (k_pool.shape[1], k_pool.shape[3]) or t.dtype != k_pool.dtype or t.stride(2) != 1:
-                raise ValueError(f"{name} must be a [T, Hkv, D] tensor of the pools' dtype with contiguous heads")
         if k.shape != v.shape:
             raise ValueError("k and v hold the same tokens")
-        _same_device(self.device, k=k, v=v)
+        for name, t in (("k", k), ("v", v)):
+            if t.dim() != 3 or t.shape[1:] != self._token_shape or t.dtype is not k_pool.dtype or t.stride(2) != 1 \
+                    or t.get_device() != self._index:
+                _need_cuda(t)
+                _same_device(self.device, **{name: t})
+                raise ValueError(f"{name} must be a [T, Hkv, D] tensor of the pools' dtype with contiguous heads")
         n = rows.numel()
-        self._call("ia_pages_write", self._list("rows", rows), self._list("starts", starts, n + 1), n, _ptr(k), _ptr(v),
-                   k.stride(0), k.stride(1), v.stride(0), v.stride(1), int(k.shape[0]), _ptr(k_pool), _ptr(v_pool))
+        (kt, kh, _), (vt, vh, _) = k.stride(), v.stride()
+        self._call(self._lib.ia_pages_write, self._list("rows", rows), self._list("starts", starts, n + 1), n, k.data_ptr(),
+                   v.data_ptr(), kt, kh, vt, vh, k.shape[0], k_pool.data_ptr(), v_pool.data_ptr())
 
     def fork(self, parents: torch.Tensor, children: torch.Tensor, *, share: bool = True) -> None:
         """``children[i]``, an empty row, becomes a copy of ``parents[i]`` as it was before the call.  With ``share`` the two
         hold the same whole pages and a partly filled last page is copied, so both can be extended; without, every
         page is copied.  A parent may have any number of children."""
-        self._call("ia_pages_fork", self._list("parents", parents), self._list("children", children, parents.numel()),
-                   parents.numel(), int(bool(share)))
+        n = parents.numel()
+        self._call(self._lib.ia_pages_fork, self._list("parents", parents), self._list("children", children, n), n,
+                   1 if share else 0)
 
     def free(self, rows: torch.Tensor) -> None:
         """The rows become empty (they may be already); pages that no row holds any more are free."""
-        self._call("ia_pages_free", self._list("rows", rows), rows.numel())
+        self._call(self._lib.ia_pages_free, self._list("rows", rows), rows.numel())
 
     def compact(self) -> None:
         """The pages in use move to the front of the pools, in all layers, and the table follows.  Pages that the caller holds
         by a count of its own move too: it finds them nowhere in the table, so it should hold none."""
-        self._call("ia_pages_compact")
+        self._call(self._lib.ia_pages_compact)
