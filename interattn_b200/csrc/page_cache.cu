@@ -253,19 +253,13 @@ template <int CTAS> __global__ void __launch_bounds__(kPlanThreads) pages_compac
   for (int g = p0; g < p1; ++g) {
     const bool is_live = st.refs[g] != 0;
     if (g < n_live && !is_live) sc.moves[hole++].y = g;
-    if (g >= n_live && is_live) sc.moves[mover++].x = g;
-  }
-  __threadfence();
-  sync_all<CTAS>();
-  const int n = n_live - low.total;
-  for (int i = me; i < n; i += kAll) {
-    const int2 mv = __ldcg(sc.moves + i);
-    sc.remap[mv.x] = mv.y;
-    st.refs[mv.y] = st.refs[mv.x];
-    st.refs[mv.x] = 0;
+    if (g >= n_live && is_live) {
+      sc.remap[g] = mover;  // the move that takes this page
+      sc.moves[mover++].x = g;
+    }
   }
   if (me == 0) {
-    sc.n_moves[0] = n;
+    sc.n_moves[0] = n_live - low.total;
     sc.n_moves[1] = n_live;
   }
 }
@@ -334,8 +328,15 @@ __global__ void __launch_bounds__(kMoveThreads) pages_compact_kernel(const MoveP
     const int row = (int)(i / st.max_pages), j = (int)(i % st.max_pages);
     if (j >= pages_of(len_of(st, row))) continue;
     const int page = st.table[i];
-    if ((unsigned)page >= (unsigned)st.n_pages) report(st, DEV_STATUS_BAD_INDEX);
-    else if (page >= n_live) st.table[i] = p.sc.remap[page];
+    if (page >= 0 && page < n_live) continue;
+    const int move = (unsigned)page < (unsigned)st.n_pages ? p.sc.remap[page] : -1;
+    if ((unsigned)move < (unsigned)p.sc.n_moves[0] && p.sc.moves[move].x == page) st.table[i] = p.sc.moves[move].y;
+    else report(st, DEV_STATUS_BAD_INDEX);  // never a page, or one that the counts call free
+  }
+  for (int i = blockIdx.x * kMoveThreads + threadIdx.x; i < p.sc.n_moves[0]; i += gridDim.x * kMoveThreads) {
+    const int2 mv = p.sc.moves[i];
+    st.refs[mv.y] = st.refs[mv.x];
+    st.refs[mv.x] = 0;
   }
   copy_runs(p);
 }
