@@ -684,7 +684,7 @@ int ia_prompt_attention(const ia_prompt_tensors* t, const int32_t* plan_host, co
                         t->v_tok_stride, t->v_head_stride, t->n_q_tokens, t->n_kv_tokens, t->n_kv_heads, t->group_size};
   const PromptItem* items = reinterpret_cast<const PromptItem*>(plan_device + plan_host[3]);
   if (t->dtype == IA_BF16) return launch_prompt_tc(p, t->head_dim, items, plan_device + 8, plan_host[1], (cudaStream_t)stream);
-  return launch_prompt_fma(p, t->dtype, t->head_dim, items, plan_host[0], plan_host[2] != 0, (cudaStream_t)stream);
+  return launch_prompt_f32(p, t->head_dim, items, plan_host[0], plan_host[2] != 0, (cudaStream_t)stream);
 }
 
 static int check_groups(const int32_t* group_sizes, int n_groups, const ia_geom* g) {
@@ -769,7 +769,7 @@ int ia_shared_prefix_decode(const void* q, const void* k_pool, const void* v_poo
   p.n_shared = n_shared_parts; p.batch = geom->batch; p.n_kv_heads = geom->n_kv_heads; p.group = geom->group_size;
   p.max_pages = geom->max_pages; p.n_pool_pages = geom->n_pool_pages; p.row_block = shared_row_block(geom->dtype);
   const int s = geom->dtype == IA_BF16 ? launch_shared_tc(p, geom->head_dim, shared_ctas(), (cudaStream_t)stream)
-                                       : launch_shared_fma(p, geom->dtype, geom->head_dim, shared_ctas(), (cudaStream_t)stream);
+                                       : launch_shared_f32(p, geom->head_dim, shared_ctas(), (cudaStream_t)stream);
   if (s) return s;
   return launch_shared_merge(p, plan_device + 8 + 8 * ((int64_t)n_shared_parts + geom->batch), geom->head_dim, geom->dtype,
                              shared_ctas(), out, (cudaStream_t)stream);

@@ -22,9 +22,11 @@ namespace {
 
 constexpr int kThreads = 256, kKeys = 64, kPLd = kKeys + 4;
 
+// At most 16 rows: a ring of three tiles is under way.  More rows: the products take the time, and K and V of
+// the next tile replace each as soon as it has been used.
 template <int D, int RPT> struct Smem {
-  static constexpr int rows = 16 * RPT, ld = D + 4;
-  static constexpr int q = 0, k = q + rows * ld, v = k + kKeys * ld, p = v + kKeys * D, floats = p + rows * kPLd;
+  static constexpr int rows = 16 * RPT, ld = D + 4, stages = RPT == 1 ? 3 : 1;
+  static constexpr int q = 0, k = q + rows * ld, kv = kKeys * ld + kKeys * D, p = k + stages * kv, floats = p + rows * kPLd;
   static constexpr size_t bytes = (size_t)floats * 4 + rows * 8;  // + limits and flags
 };
 
@@ -34,49 +36,46 @@ __device__ __forceinline__ void cp_async16(void* dst, const void* src, bool vali
                "r"(n)
                : "memory");
 }
-// four elements as floats; zeros where not valid
-__device__ __forceinline__ void put4(float* dst, const float* src, bool valid) { cp_async16(dst, src, valid); }
-__device__ __forceinline__ void put4(float* dst, const __nv_bfloat16* src, bool valid) {
-  float x[4] = {0.f, 0.f, 0.f, 0.f};
-  if (valid) load_vec<4>(src, x);
-  store_vec<4>(dst, x);
-}
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 // rows of a [kKeys, D] tile from key j0 on; rows at or past `hi`, and rows without an address, are zero
-template <bool VALUES, int D, int LD, typename T, typename Key>
-__device__ __forceinline__ void load_tile(float* dst, const T* any, int j0, int hi, const Key& key) {
+template <bool VALUES, int D, int LD, typename Key>
+__device__ __forceinline__ void load_tile(float* dst, const float* any, int j0, int hi, const Key& key) {
 #pragma unroll 4
   for (int i = threadIdx.x; i < kKeys * D / 4; i += kThreads) {
     const int row = i / (D / 4), c = i % (D / 4) * 4;
-    const T *k = any, *v = any;
+    const float *k = any, *v = any;
     const bool ok = j0 + row < hi && key(j0 + row, k, v);
-    put4(dst + row * LD + c, (VALUES ? v : k) + (ok ? c : 0), ok);
+    cp_async16(dst + row * LD + c, (VALUES ? v : k) + (ok ? c : 0), ok);
   }
 }
 
 // Rows [0, n_rows) of one piece over the keys [lo, hi).  q_row(r): the row's query; limit(r): the keys below it are seen;
 // sink.row(r) -> where its outputs go.
-template <typename T, int D, int RPT, typename Key, typename QRow, typename Limit, typename Sink>
+template <int D, int RPT, typename Key, typename QRow, typename Limit, typename Sink>
 __device__ void attend(float* sm, int n_rows, int lo, int hi, float scale_log2, const Key& key, const QRow& q_row,
                        const Limit& limit, const Sink& sink) {
   using S = Smem<D, RPT>;
   constexpr int ROWS = S::rows, LD = S::ld, NO = D / 64;
   const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
-  float *qs = sm + S::q, *ks = sm + S::k, *vs = sm + S::v, *ps = sm + S::p;
+  float *qs = sm + S::q, *ps = sm + S::p;
   int* lim = reinterpret_cast<int*>(sm + S::floats);
   int* bad = lim + ROWS;
-  const T* any = q_row(0);
+  const float* any = q_row(0);
   __syncthreads();  // the piece before is done with the shared memory
   for (int i = tid; i < ROWS * D / 4; i += kThreads) {
     const int row = i / (D / 4), c = i % (D / 4) * 4;
-    put4(qs + row * LD + c, row < n_rows ? q_row(row) + c : any, row < n_rows);
+    cp_async16(qs + row * LD + c, row < n_rows ? q_row(row) + c : any, row < n_rows);
   }
-  load_tile<false, D, LD>(ks, any, lo, hi, key);
-  cp_commit();
-  load_tile<true, D, D>(vs, any, lo, hi, key);
-  cp_commit();
+#pragma unroll
+  for (int st = 0; st < S::stages; ++st) {  // a group each for K and V of a tile
+    float* to = sm + S::k + st * S::kv;
+    if (lo + st * kKeys < hi) load_tile<false, D, LD>(to, any, lo + st * kKeys, hi, key);
+    cp_commit();
+    if (lo + st * kKeys < hi) load_tile<true, D, D>(to + kKeys * LD, any, lo + st * kKeys, hi, key);
+    cp_commit();
+  }
   if (tid < ROWS) {
     lim[tid] = tid < n_rows ? limit(tid) : 0;
     bad[tid] = 0;
@@ -91,8 +90,12 @@ __device__ void attend(float* sm, int n_rows, int lo, int hi, float scale_log2, 
 #pragma unroll
       for (int b = 0; b < 4; ++b) o[i][a][b] = 0.f;
   }
+  int st = 0;
   for (int j0 = lo; j0 < hi; j0 += kKeys) {
-    cp_wait<1>();
+    float *ks = sm + S::k + st * S::kv, *vs = ks + kKeys * LD;
+    if (++st == S::stages) st = 0;
+    const int ahead = j0 + S::stages * kKeys;  // the tile that takes this one's place
+    cp_wait<2 * S::stages - 1>();
     __syncthreads();
     float s[RPT][4];
 #pragma unroll
@@ -117,7 +120,7 @@ __device__ void attend(float* sm, int n_rows, int lo, int hi, float scale_log2, 
       }
     }
     __syncthreads();
-    if (j0 + kKeys < hi) load_tile<false, D, LD>(ks, any, j0 + kKeys, hi, key);
+    if (ahead < hi) load_tile<false, D, LD>(ks, any, ahead, hi, key);
     cp_commit();
 #pragma unroll
     for (int i = 0; i < RPT; ++i) {
@@ -145,7 +148,7 @@ __device__ void attend(float* sm, int n_rows, int lo, int hi, float scale_log2, 
 #pragma unroll
         for (int b = 0; b < 4; ++b) o[i][a][b] *= keep;
     }
-    cp_wait<1>();
+    cp_wait<2 * S::stages - 1>();
     __syncthreads();  // also: the row's weights are written
 #pragma unroll 2
     for (int n = 0; n < kKeys; n += 4) {
@@ -169,7 +172,7 @@ __device__ void attend(float* sm, int n_rows, int lo, int hi, float scale_log2, 
       }
     }
     __syncthreads();
-    if (j0 + kKeys < hi) load_tile<true, D, D>(vs, any, j0 + kKeys, hi, key);
+    if (ahead < hi) load_tile<true, D, D>(vs, any, ahead, hi, key);
     cp_commit();
   }
   cp_wait<0>();
@@ -201,44 +204,43 @@ __device__ void attend(float* sm, int n_rows, int lo, int hi, float scale_log2, 
   }
   if (!__syncthreads_or(some_bad)) return;
   for (int row = tid >> 5; row < n_rows; row += kThreads / 32) {
-    if (!bad[row] || last_not_finite<T, D>(max(lo, lim[row]), hi, key) < 0) continue;
+    if (!bad[row] || last_not_finite<float, D>(max(lo, lim[row]), hi, key) < 0) continue;
     float x[D / 32], mx, lx;
-    exact_row<T, D>(q_row(row), lo, lim[row], scale_log2, key, x, mx, lx);
+    exact_row<float, D>(q_row(row), lo, lim[row], scale_log2, key, x, mx, lx);
 #pragma unroll
-    for (int i = 0; i < D / 32; ++i) from_f32(sink.row(row)[(tid & 31) + 32 * i], x[i] / lx);
+    for (int i = 0; i < D / 32; ++i) sink.row(row)[(tid & 31) + 32 * i] = x[i] / lx;
     if ((tid & 31) == 0 && sink.lse(row) != nullptr) *sink.lse(row) = (mx + log2f(lx)) * kLn2;
   }
 }
 
-template <typename O> struct RowSink {  // rows r = token * group + g of one kv head
-  O* o;
-  float* l;
+struct RowSink {  // rows r = token * group + g of one kv head
+  float *o, *l;
   int64_t o_tok, o_g, l_tok;
   int group;
-  __device__ __forceinline__ O* row(int r) const { return o + r / group * o_tok + r % group * o_g; }
+  __device__ __forceinline__ float* row(int r) const { return o + r / group * o_tok + r % group * o_g; }
   __device__ __forceinline__ float* lse(int r) const { return l == nullptr ? nullptr : l + r / group * l_tok + r % group; }
 };
 
-template <typename T, int D, int RPT>
+template <int D, int RPT>
 __global__ void __launch_bounds__(kThreads) prompt_attention_kernel(const PromptTensors t, const PromptItem* items) {
   extern __shared__ __align__(16) float sm[];
   grid_dependency_wait();
   grid_launch_dependents();
   const PromptItem it = items[blockIdx.x];
   const int G = t.group, hq = t.n_kv_heads * G;
-  const PackedKeys<T> key{(const T*)t.k + it.kv_tok * t.k_tok_stride + it.head * t.k_head_stride,
-                              (const T*)t.v + it.kv_tok * t.v_tok_stride + it.head * t.v_head_stride, t.k_tok_stride,
+  const PackedKeys<float> key{(const float*)t.k + it.kv_tok * t.k_tok_stride + it.head * t.k_head_stride,
+                              (const float*)t.v + it.kv_tok * t.v_tok_stride + it.head * t.v_head_stride, t.k_tok_stride,
                               t.v_tok_stride, it.kv_len};
-  const T* q = (const T*)t.q + it.q_tok * t.q_tok_stride + (int64_t)it.head * G * t.q_head_stride;
+  const float* q = (const float*)t.q + it.q_tok * t.q_tok_stride + (int64_t)it.head * G * t.q_head_stride;
   const auto q_row = [&](int r) { return q + r / G * t.q_tok_stride + r % G * t.q_head_stride; };
   const auto limit = [&](int r) { return max(0, min(it.limit0 + r / G, it.kv_len)); };
-  const RowSink<T> sink{(T*)t.out + ((int64_t)it.q_tok * hq + it.head * G) * D,
+  const RowSink sink{(float*)t.out + ((int64_t)it.q_tok * hq + it.head * G) * D,
                      t.lse == nullptr ? nullptr : t.lse + (int64_t)it.q_tok * hq + it.head * G, (int64_t)hq * D, D, hq, G};
-  attend<T, D, RPT>(sm, it.n_tok * G, 0, limit(it.n_tok * G - 1), kLog2e * rsqrtf((float)D), key, q_row, limit, sink);
+  attend<D, RPT>(sm, it.n_tok * G, 0, limit(it.n_tok * G - 1), kLog2e * rsqrtf((float)D), key, q_row, limit, sink);
 }
 
 // The decode step: this CTA's share of all units, segment by segment.
-template <typename T, int D>
+template <int D>
 __global__ void __launch_bounds__(kThreads) shared_attention_kernel(const SharedParams p) {
   extern __shared__ __align__(16) float sm[];
   __shared__ unsigned long long scratch[kThreads / 32];
@@ -257,12 +259,12 @@ __global__ void __launch_bounds__(kThreads) shared_attention_kernel(const Shared
     const bool own = c.e >= p.n_shared;
     const int64_t slot = (int64_t)(own ? c.e - p.n_shared : c.e) * p.n_kv_heads + c.h + cta;
     const int slot_rows = own ? G : p.row_block;
-    const PagedKeys<T> key{(const T*)p.k_pool + c.h * p.head_stride, (const T*)p.v_pool + c.h * p.head_stride,
+    const PagedKeys<float> key{(const float*)p.k_pool + c.h * p.head_stride, (const float*)p.v_pool + c.h * p.head_stride,
                                table, p.page_stride, D, p.n_pool_pages, p.max_pages};
-    const T* q = (const T*)p.q + ((int64_t)ent.first_seq * hq + c.h * G) * D;
+    const float* q = (const float*)p.q + ((int64_t)ent.first_seq * hq + c.h * G) * D;
     const auto q_row = [&](int r) { return q + (int64_t)(r / G) * hq * D + r % G * D; };
     const auto limit = [&](int r) { return min(to, shared_seq_len(p, ent.first_seq + r / G)); };
-    const RowSink<float> sink{(own ? p.o_own : p.o_shared) + slot * slot_rows * D, (own ? p.lse_own : p.lse_shared) + slot * slot_rows,
+    const RowSink sink{(own ? p.o_own : p.o_shared) + slot * slot_rows * D, (own ? p.lse_own : p.lse_shared) + slot * slot_rows,
                        (int64_t)G * D, D, G, G};
     for (int j = (from >> 4) + threadIdx.x; j < (to + 15) >> 4; j += kThreads) {
       const int page = table[j];
@@ -270,9 +272,9 @@ __global__ void __launch_bounds__(kThreads) shared_attention_kernel(const Shared
     }
     // a single sequence has at most 16 rows: the narrow form, which spends the threads on keys instead of empty rows
     if (ent.n_seqs * G <= 16)
-      attend<T, D, 1>(sm, ent.n_seqs * G, from, to, kLog2e * rsqrtf((float)D), key, q_row, limit, sink);
+      attend<D, 1>(sm, ent.n_seqs * G, from, to, kLog2e * rsqrtf((float)D), key, q_row, limit, sink);
     else
-      attend<T, D, 8>(sm, ent.n_seqs * G, from, to, kLog2e * rsqrtf((float)D), key, q_row, limit, sink);
+      attend<D, 8>(sm, ent.n_seqs * G, from, to, kLog2e * rsqrtf((float)D), key, q_row, limit, sink);
     c.left -= n;
     c.k = 0;
     if (++c.h == p.n_kv_heads) {
@@ -361,18 +363,19 @@ int launch(void (*kern)(Args...), unsigned grid, size_t smem, cudaStream_t strea
   return e == cudaSuccess ? check_launch(what) : fail(IA_ERR_LAUNCH, "%s: %s", what, cudaGetErrorString(e));
 }
 
-template <typename T, int D, int RPT>
+template <int D, int RPT>
 int launch_prompt(const PromptTensors& t, const PromptItem* items, int n_items, cudaStream_t stream) {
-  auto kern = prompt_attention_kernel<T, D, RPT>;
+  auto kern = prompt_attention_kernel<D, RPT>;
   static SmemOnce once;
   if (int s = once.allow((const void*)kern, Smem<D, RPT>::bytes, "prompt_attention_kernel")) return s;
   return launch(kern, (unsigned)n_items, Smem<D, RPT>::bytes, stream, "prompt_attention_kernel", t, items);
 }
-template <typename T, int D> int launch_shared(const SharedParams& p, int ctas, cudaStream_t stream) {
-  auto kern = shared_attention_kernel<T, D>;
+template <int D> int launch_shared(const SharedParams& p, int ctas, cudaStream_t stream) {
+  auto kern = shared_attention_kernel<D>;
   static SmemOnce once;
-  if (int s = once.allow((const void*)kern, Smem<D, 8>::bytes, "shared_attention_kernel")) return s;
-  return launch(kern, (unsigned)ctas, Smem<D, 8>::bytes, stream, "shared_attention_kernel", p);
+  constexpr size_t bytes = std::max(Smem<D, 8>::bytes, Smem<D, 1>::bytes);
+  if (int s = once.allow((const void*)kern, bytes, "shared_attention_kernel")) return s;
+  return launch(kern, (unsigned)ctas, bytes, stream, "shared_attention_kernel", p);
 }
 template <typename T, int D>
 int launch_merge(const SharedParams& p, const int2* seq_info, int ctas, T* out, cudaStream_t stream) {
@@ -405,21 +408,13 @@ int sm_count() {
   return sms;
 }
 
-template <typename T>
-static int prompt_of(const PromptTensors& t, int head_dim, const PromptItem* items, int n_items, bool few_rows, cudaStream_t stream) {
-  if (head_dim == 128)
-    return few_rows ? launch_prompt<T, 128, 2>(t, items, n_items, stream) : launch_prompt<T, 128, 8>(t, items, n_items, stream);
-  return few_rows ? launch_prompt<T, 64, 2>(t, items, n_items, stream) : launch_prompt<T, 64, 8>(t, items, n_items, stream);
-}
-int launch_prompt_fma(const PromptTensors& t, int dtype, int head_dim, const PromptItem* items, int n_items, bool few_rows,
-                      cudaStream_t stream) {
-  return dtype == IA_F32 ? prompt_of<float>(t, head_dim, items, n_items, few_rows, stream)
-                         : prompt_of<__nv_bfloat16>(t, head_dim, items, n_items, few_rows, stream);
+int launch_prompt_f32(const PromptTensors& t, int head_dim, const PromptItem* items, int n_items, bool few_rows, cudaStream_t stream) {
+  if (head_dim == 128) return few_rows ? launch_prompt<128, 2>(t, items, n_items, stream) : launch_prompt<128, 8>(t, items, n_items, stream);
+  return few_rows ? launch_prompt<64, 2>(t, items, n_items, stream) : launch_prompt<64, 8>(t, items, n_items, stream);
 }
 
-int launch_shared_fma(const SharedParams& p, int dtype, int head_dim, int ctas, cudaStream_t stream) {
-  if (dtype == IA_F32) return head_dim == 128 ? launch_shared<float, 128>(p, ctas, stream) : launch_shared<float, 64>(p, ctas, stream);
-  return head_dim == 128 ? launch_shared<__nv_bfloat16, 128>(p, ctas, stream) : launch_shared<__nv_bfloat16, 64>(p, ctas, stream);
+int launch_shared_f32(const SharedParams& p, int head_dim, int ctas, cudaStream_t stream) {
+  return head_dim == 128 ? launch_shared<128>(p, ctas, stream) : launch_shared<64>(p, ctas, stream);
 }
 
 int launch_shared_merge(const SharedParams& p, const int32_t* seq_info, int head_dim, int dtype, int ctas, void* out,

@@ -263,9 +263,9 @@ int shared_ctas();
 int64_t shared_parts(const int32_t* group_sizes, int n_groups, int group, int dtype);
 void make_shared_plan(const int32_t* group_sizes, int n_groups, int batch, int group, int dtype, int32_t* plan);
 
-int launch_prompt_fma(const PromptTensors& t, int dtype, int head_dim, const PromptItem* items, int n_items, bool few_rows,
+int launch_prompt_f32(const PromptTensors& t, int head_dim, const PromptItem* items, int n_items, bool few_rows,
                       cudaStream_t stream);
-int launch_shared_fma(const SharedParams& p, int dtype, int head_dim, int ctas, cudaStream_t stream);
+int launch_shared_f32(const SharedParams& p, int head_dim, int ctas, cudaStream_t stream);
 int launch_prompt_tc(const PromptTensors& t, int head_dim, const PromptItem* items, const int32_t* cta_begin, int ctas,
                      cudaStream_t stream);
 int launch_shared_tc(const SharedParams& p, int head_dim, int ctas, cudaStream_t stream);
