@@ -626,6 +626,8 @@ static int check_prompt_lens(const int32_t* q_lens, const int32_t* kv_lens, int 
                              int dtype) {
   if (n_seqs < 0 || (n_seqs > 0 && (!q_lens || !kv_lens))) return fail(IA_ERR_BAD_ARG, "prompt_plan: lengths");
   if (n_kv_heads <= 0 || n_kv_heads > 65535 || group <= 0) return fail(IA_ERR_BAD_ARG, "prompt_plan: %d kv heads, group %d", n_kv_heads, group);
+  if ((int64_t)n_kv_heads * group > 32768)  // a piece's outputs are addressed in 32 bits
+    return fail(IA_ERR_UNSUPPORTED, "prompt_plan: %d query heads", n_kv_heads * group);
   if (group > 16) return fail(IA_ERR_UNSUPPORTED, "prompt_plan: group size %d (built: up to 16)", group);
   if (head_dim != 64 && head_dim != 128) return fail(IA_ERR_UNSUPPORTED, "prompt_plan: head_dim %d (built: 64, 128)", head_dim);
   if (dtype != IA_F32 && dtype != IA_BF16) return fail(IA_ERR_BAD_ARG, "prompt_plan: dtype %d", dtype);
@@ -636,7 +638,7 @@ static int check_prompt_lens(const int32_t* q_lens, const int32_t* kv_lens, int 
     q += q_lens[i];
     k += kv_lens[i];
   }
-  if (q > 0x7fffffff || k > 0x7fffffff) return fail(IA_ERR_UNSUPPORTED, "prompt_plan: more than 2^31 - 1 tokens");
+  if (q > 1 << 30 || k > 1 << 30) return fail(IA_ERR_UNSUPPORTED, "prompt_plan: more than 2^30 tokens");
   return IA_OK;
 }
 
@@ -696,7 +698,7 @@ static int check_groups(const int32_t* group_sizes, int n_groups, const ia_geom*
     n += group_sizes[i];
   }
   if (n != g->batch) return fail(IA_ERR_BAD_ARG, "shared_prefix: the groups hold %lld sequences, the batch %d", (long long)n, g->batch);
-  if ((int64_t)g->max_pages * g->page_size > 0x7fffffff) return fail(IA_ERR_UNSUPPORTED, "shared_prefix: max_pages %d", g->max_pages);
+  if ((int64_t)g->max_pages * g->page_size > 1 << 30) return fail(IA_ERR_UNSUPPORTED, "shared_prefix: max_pages %d", g->max_pages);
   return IA_OK;
 }
 
@@ -750,6 +752,7 @@ int ia_shared_prefix_decode(const void* q, const void* k_pool, const void* v_poo
                             const ia_geom* geom, void* workspace, int64_t workspace_bytes, void* out, ia_stream_t stream) {
   if (int s = check_geom(geom)) return s;
   if (geom->batch == 0) return IA_OK;
+  if ((int64_t)geom->max_pages * geom->page_size > 1 << 30) return fail(IA_ERR_UNSUPPORTED, "shared_prefix_decode: max_pages %d", geom->max_pages);
   const int64_t need = ia_shared_prefix_workspace_bytes(n_shared_parts, geom);
   if (need < 0) return IA_ERR_BAD_ARG;
   if (!q || !k_pool || !v_pool || !block_table || !seq_lens || !shared_lens || !plan_device || !workspace || !out)

@@ -344,3 +344,78 @@ def test_prompts_forks_and_steps_together(dtype, hq, hkv, d):
     prompt_reference(q, torch.cat(keys), torch.cat(values), [1] * 5, [len(x) for x in keys])
     torch.testing.assert_close(sparse.step(q).float(), step.step(q).float(), rtol=2e-2, atol=2e-2)
     assert ops.device_status() == 0
+
+
+# ---- the ends of the ranges -------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype,d", [(BF16, 128), (BF16, 64), (F32, 64)])
+def test_nothing_to_do(dtype, d):
+    plan = dense_attention.PromptAttention([], 8, 2, d, dtype=dtype)
+    none_q, none_k = torch.empty((0, 8, d), dtype=dtype, device="cuda"), torch.empty((0, 2, d), dtype=dtype, device="cuda")
+    assert plan.run(none_q, none_k, none_k).shape == (0, 8, d)
+    plan = dense_attention.PromptAttention([3, 0], 8, 2, d, kv_lens=[0, 0], dtype=dtype)     # queries, but no key anywhere
+    out, lse = plan.run(randn((3, 8, d), dtype, 0), none_k, none_k, return_lse=True)
+    assert not out.any() and bool((lse == float("-inf")).all())
+    pool = torch.zeros((1, 2, PAGE, d), dtype=dtype, device="cuda")
+    kv = ops.PagedKV(pool, pool, torch.zeros((0, 1), dtype=torch.int32, device="cuda"), i32([]), i32([]))
+    assert dense_attention.SharedPrefixAttention(kv, [], i32([]), 8).step(none_q).shape == (0, 8, d)
+    kv = ops.PagedKV(pool, pool, torch.full((2, 1), -1, dtype=torch.int32, device="cuda"), i32([0, 0]), i32([0, 0]))
+    out = dense_attention.SharedPrefixAttention(kv, [2], i32([16]), 8).step(randn((2, 8, d), dtype, 1))
+    assert not out.any() and ops.device_status() == 0
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_offsets_past_32_bits(dtype):
+    """Tokens and pages far apart in large tensors: element offsets beyond 2^32, byte offsets beyond 2^33."""
+    hq, hkv, d, n = 4, 2, 64, 70
+    gap = 1 << 26                                            # elements between tokens, and between pages
+    flat = torch.empty((n * gap,), dtype=dtype, device="cuda")
+    far = lambda heads, at: flat[at:].as_strided((n, heads, d), (gap, d, 1))  # noqa: E731
+    q, k, v = far(hq, 0), far(hkv, hq * d), far(hkv, (hq + hkv) * d)
+    for i, t in enumerate((q, k, v)):
+        t.copy_(randn(t.shape, dtype, 50 + i))
+    lens = [n - 3, 3]
+    plan = dense_attention.PromptAttention(lens, hq, hkv, d, dtype=dtype)
+    prompt_reference(q, k, v, lens, lens).check(plan.run(q, k, v), dtype)
+    pages = n - 1
+    pools = [flat[at:].as_strided((pages, hkv, PAGE, d), (gap, PAGE * d, d, 1)) for at in (4096, 16384)]
+    for i, t in enumerate(pools):
+        t.copy_(randn(t.shape, dtype, 60 + i))
+    table = torch.arange(pages - 1, -1, -1, dtype=torch.int32).view(3, -1)
+    seq = [300, 301, 368]
+    kv = ops.PagedKV(*pools, table.cuda(), i32(seq), i32(seq))
+    q = randn((3, hq, d), dtype, 70)
+    out = dense_attention.SharedPrefixAttention(kv, [1, 1, 1], i32([100, 0, 368]), hq).step(q)
+    decode_reference(q, *pools, table, seq).check(out, dtype)
+    cache = page_cache.PageCache([tuple(pools)], torch.full((4, 30), -1, dtype=torch.int32, device="cuda"), i32([0] * 4),
+                                 i32([1] * 40 + [0] * (pages - 40)))
+    cache.extend(i32([0]), i32([40]))
+    kk, vv = randn((40, hkv, d), dtype, 71), randn((40, hkv, d), dtype, 72)
+    cache.write(0, i32([0]), i32([0, 40]), kk, vv)
+    cache.fork(i32([0]), i32([1]), share=False)
+    assert cache.block_table[:2, :3].tolist() == [[40, 41, 42], [43, 44, 45]]
+    got = pools[1][43:46].transpose(1, 2).reshape(48, hkv, d)[:40]
+    assert torch.equal(got, vv) and ops.device_status() == 0
+
+
+@pytest.mark.parametrize("seed", range(8))
+def test_random_batches(seed):
+    """Lengths, groups and heads as they come."""
+    import random
+    rng = random.Random(seed)
+    hq, hkv, d = rng.choice([(8, 2, 128), (6, 6, 64), (15, 3, 64), (16, 1, 128), (9, 1, 64)])
+    dtype = BF16 if seed % 4 else F32
+    n = rng.randint(1, 9)
+    q_lens = [rng.choice([0, 1, rng.randint(1, 40), rng.randint(1, 300)]) for _ in range(n)]
+    kv_lens = [max(0, x + rng.choice([0, 0, -2, rng.randint(0, 400)])) for x in q_lens]
+    if sum(q_lens) == 0:
+        q_lens[0], kv_lens[0] = 3, 5
+    q, k, v, plan = prompt_case(hq, hkv, d, dtype, q_lens, kv_lens, seed=seed)
+    prompt_reference(q, k, v, q_lens, kv_lens).check(plan.run(q, k, v), dtype)
+    groups = [rng.choice([1, 2, rng.randint(1, 40)]) for _ in range(rng.randint(1, 5))]
+    shared = [rng.choice([0, 15, 16, rng.randint(0, 900)]) for _ in groups]
+    lens = [max(0, s + rng.choice([0, 1, rng.randint(0, 300), -rng.randint(0, 900)])) for g, s in zip(groups, shared) for _ in range(g)]
+    q, kv, table = paged_case(hq, hkv, d, dtype, groups, shared, lens, seed=seed)
+    step = dense_attention.SharedPrefixAttention(kv, groups, i32(shared), hq)
+    decode_reference(q, kv.k_pool, kv.v_pool, table, lens).check(step.step(q), dtype)
+    assert ops.device_status() == 0
