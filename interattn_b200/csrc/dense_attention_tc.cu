@@ -301,7 +301,7 @@ __device__ __forceinline__ void weights(const uint32_t (&s)[32], uint64_t c, uin
 }
 
 struct Bars {
-  uint64_t full[8], empty[8], q_full[2], q_empty[2], s_full[2], p_full[2], o_full[2], stats, read, work_full[kWorkSlots],
+  uint64_t full[8], empty[8], q_full[2], q_empty[2], s_full[2], p_half[2], p_full[2], o_full[2], stats, read, work_full[kWorkSlots],
       work_empty[kWorkSlots], drain;
 };
 
@@ -627,14 +627,23 @@ template <int D, bool PAGED> struct MmaRole {
         const uint32_t vs = uniform((v.use + 1) % C::stages), old = uniform(!v.opens),
                        k16 = uniform(min(kKeys / 16, (v.keys + 15) >> 4));
         const uint64_t b = umma_desc(q0 + (uint32_t)C::ring + vs * C::kv_tile, kNextCols);
-        if (!wait(&bars->full[vs], ((v.use + 1) / C::stages) & 1) || !wait(&bars->p_full[me], p_count++ & 1)) break;
-        const bool both = more && first_ready();
+        if (!wait(&bars->full[vs], ((v.use + 1) / C::stages) & 1) || !wait(&bars->p_half[me], p_count & 1)) break;
         tc_fence_after();
         if (elect_one()) {
 #pragma unroll
-          for (int k = 0; k < kKeys / 16; ++k)  // 16 keys: 8 columns of packed weights, 16 rows of V
+          for (int k = 0; k < kKeys / 32; ++k)  // 16 keys: 8 columns of packed weights, 16 rows of V
             if (k < k16)
               umma_ts(tmem + 256 + me * 128, tmem + me * 128 + k * 8, b + k * kStepBytes / 16, kIdesc<D, true>, k > 0 ? 1u : old);
+        }
+        __syncwarp();
+        const bool both = more && first_ready();
+        if (!wait(&bars->p_full[me], p_count++ & 1)) break;
+        tc_fence_after();
+        if (elect_one()) {
+#pragma unroll
+          for (int k = kKeys / 32; k < kKeys / 16; ++k)
+            if (k < k16)
+              umma_ts(tmem + 256 + me * 128, tmem + me * 128 + k * 8, b + k * kStepBytes / 16, kIdesc<D, true>, 1u);
           umma_commit(&bars->o_full[me]);
           umma_commit(&bars->empty[vs]);
           if (both) issue_first(f);
@@ -741,8 +750,13 @@ __device__ __forceinline__ void softmax_role(const TcParams& p, Bars* bars, cons
         uint64_t sum[2] = {0, 0};
 #pragma unroll
         for (int i = 0; i < kKeys / 32; ++i) {
-          if (i * 32 >= columns) break;
-          weights(r[i], c2, mc2, sum, s_addr + 16 * i);
+          if (i == kKeys / 64) {  // the second product begins with the first half of the keys
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bars->p_half[w]);
+          }
+          if (i * 32 < columns) weights(r[i], c2, mc2, sum, s_addr + 16 * i);
         }
         float la, lb;
         unpair(add2(sum[0], sum[1]), la, lb);
@@ -751,7 +765,10 @@ __device__ __forceinline__ void softmax_role(const TcParams& p, Bars* bars, cons
         tc_fence_before();
       }
       __syncwarp();
-      if (lane == 0) mbar_arrive(&bars->p_full[w]);
+      if (lane == 0) {
+        if (!busy) mbar_arrive(&bars->p_half[w]);
+        mbar_arrive(&bars->p_full[w]);
+      }
     }
     if (!wait(&bars->o_full[w], (s_it - 1) & 1)) return;
     tc_fence_after();
@@ -913,7 +930,8 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tc_kernel(const __grid_con
       mbar_init(&bars.q_full[w], 1);
       mbar_init(&bars.q_empty[w], 2);
       mbar_init(&bars.s_full[w], 1);
-      mbar_init(&bars.p_full[w], 4);  // a lane of each warp
+      mbar_init(&bars.p_half[w], 4);  // a lane of each warp
+      mbar_init(&bars.p_full[w], 4);
       mbar_init(&bars.o_full[w], 1);
     }
     for (int i = 0; i < kWorkSlots; ++i) {
