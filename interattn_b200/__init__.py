@@ -3,6 +3,8 @@
 Public surface:
 
 * ``interattn_b200.ops``            - batched / paged operators over the C ABI
+* ``interattn_b200.dense_attention`` - attention over all keys: packed prompts, decode steps over shared prefixes
+* ``interattn_b200.page_cache``     - pages that sequences share: extend, write, fork, free, compact
 * ``interattn_b200.reference_api``  - the reference project's operator names and
   signatures (``_build_prompt_blocks``, ``_select_prompt_blocks``,
   ``_run_condition_block_selection_stats``,
