@@ -715,25 +715,20 @@ int ia_shared_prefix_plan(const int32_t* group_sizes, int n_groups, const ia_geo
   return IA_OK;
 }
 
-// partial outputs and their log-sum-exps: a slot per (item, CTA) that can occur
+// partial outputs and their log-sum-exps, and where the entities' units begin
 static int64_t carve_shared(int n_shared, const ia_geom& g, char* base, SharedParams* p) {
-  const int64_t slots_shared = n_shared > 0 ? (int64_t)n_shared * g.n_kv_heads + shared_ctas() : 0;
-  const int64_t slots_own = (int64_t)g.batch * g.n_kv_heads + shared_ctas();
+  const int64_t rows = 2 * (int64_t)g.batch * g.n_kv_heads * g.group_size + (int64_t)shared_ctas() * shared_row_block(g.dtype);
   int64_t off = 0;
   auto take = [&](int64_t bytes) {
     char* r = base ? base + off : nullptr;
     off += align256(bytes);
     return r;
   };
-  char* a[5] = {take(slots_shared * shared_row_block(g.dtype) * g.head_dim * 4), take(slots_shared * shared_row_block(g.dtype) * 4),
-                take(slots_own * g.group_size * g.head_dim * 4), take(slots_own * g.group_size * 4),
-                take(((int64_t)n_shared + g.batch + 1) * 8)};
+  char* a[3] = {take(rows * g.head_dim * 4), take(rows * 4), take(((int64_t)n_shared + g.batch + 1) * 8)};
   if (p) {
-    p->o_shared = (float*)a[0];
-    p->lse_shared = (float*)a[1];
-    p->o_own = (float*)a[2];
-    p->lse_own = (float*)a[3];
-    p->unit_begin = (long long*)a[4];
+    p->o = (float*)a[0];
+    p->lse = (float*)a[1];
+    p->unit_begin = (long long*)a[2];
   }
   return off;
 }

@@ -258,15 +258,13 @@ __global__ void __launch_bounds__(kThreads) shared_attention_kernel(const Shared
     const int32_t* table = p.block_table + (int64_t)lead.x * p.max_pages;
     const int from = lo + c.k * kKeys, to = max(from, min(lead.y, from + n * kKeys));
     const bool own = c.e >= p.n_shared;
-    const int64_t slot = (int64_t)(own ? c.e - p.n_shared : c.e) * p.n_kv_heads + c.h + cta;
-    const int slot_rows = own ? G : p.row_block;
+    const int64_t row0 = c.k == 0 ? item_rows(p, own, ent.first_seq, ent.n_seqs, c.h) : cta_rows(p, cta);
     const PagedKeys<float> key{(const float*)p.k_pool + c.h * p.head_stride, (const float*)p.v_pool + c.h * p.head_stride,
                                table, p.page_stride, D, p.n_pool_pages, p.max_pages};
     const float* q = (const float*)p.q + ((int64_t)ent.first_seq * hq + c.h * G) * D;
     const auto q_row = [&](int r) { return q + (int64_t)(r / G) * hq * D + r % G * D; };
     const auto limit = [&](int r) { return min(to, shared_seq_len(p, ent.first_seq + r / G)); };
-    const RowSink sink{(own ? p.o_own : p.o_shared) + slot * slot_rows * D, (own ? p.lse_own : p.lse_shared) + slot * slot_rows,
-                       (int64_t)G * D, D, G, G};
+    const RowSink sink{p.o + row0 * D, p.lse + row0, (int64_t)G * D, D, G, G};
     for (int j = (from >> 4) + threadIdx.x; j < (to + 15) >> 4; j += kThreads) {
       const int page = table[j];
       if (page < 0 || (p.n_pool_pages > 0 && page >= p.n_pool_pages)) atomicOr(p.status, DEV_STATUS_BAD_INDEX);
@@ -312,17 +310,19 @@ __global__ void __launch_bounds__(256) shared_merge_kernel(const SharedParams p,
     c0[i] = units > 0 ? share_owner(u0, total, ctas) : 0;
     n[i] = units > 0 ? share_owner(u0 + units - 1, total, ctas) - c0[i] + 1 : 0;
   }
-  const int64_t row0[2] = {(((int64_t)info.x * p.n_kv_heads + h + c0[0]) * p.row_block) + info.y * G + g,
-                           ((int64_t)seq * p.n_kv_heads + h + c0[1]) * G + g};
+  const SharedEntity ent = load_entity(p, info.x);
+  const int at[2] = {info.y * G + g, g};  // the row in its item
+  const int64_t first[2] = {item_rows(p, false, ent.first_seq, ent.n_seqs, h) + at[0], item_rows(p, true, seq, 1, h) + at[1]};
   float acc[D / 32], M = -INFINITY, L = 0.f;
 #pragma unroll
   for (int i = 0; i < D / 32; ++i) acc[i] = 0.f;
   for (int s0 = 0; s0 < n[0] + n[1]; s0 += 32) {
     const int mine = s0 + lane, count = min(32, n[0] + n[1] - s0);
     const bool own = mine >= n[0];
-    const int64_t row = own ? row0[1] + (int64_t)(mine - n[0]) * G : row0[0] + (int64_t)mine * p.row_block;
-    const float lse = lane < count ? __ldcg((own ? p.lse_own : p.lse_shared) + row) * kLog2e : -INFINITY;
-    const float* src = (own ? p.o_own : p.o_shared) + row * D;
+    const int segment = own ? mine - n[0] : mine;
+    const int64_t row = segment == 0 ? first[own] : cta_rows(p, c0[own] + segment) + at[own];
+    const float lse = lane < count ? __ldcg(p.lse + row) * kLog2e : -INFINITY;
+    const float* src = p.o + row * D;
     const float m = fmaxf(M, warp_max(lse)), base = m == -INFINITY ? 0.f : m;
     const float keep = exp2f(M - base), w = exp2f(lse - base);  // a segment without a visible key: weight 0, o is 0
     L = L * keep + warp_sum(w);

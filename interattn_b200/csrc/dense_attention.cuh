@@ -38,8 +38,8 @@ struct PromptTensors {
 // member may have left); an own part covers [split, seq_len) of its sequence.
 // An item is an (entity, kv head), its keys are cut into units of kUnit keys, and CTA c of P takes the units
 // [T c / P, T (c + 1) / P) of all T units laid end to end: equal shares whatever the lengths are, one run of keys per
-// CTA and item.  Each (item, CTA) leaves a normalised partial output and its log-sum-exp in the slot
-// item + c; both indexes only grow along the line of units, so no two segments share a slot.
+// CTA and item.  Each (item, CTA) leaves a normalised partial output and its log-sum-exp: the segment that begins the item in
+// the item's own rows, another in rows of the CTA - only the first segment of a CTA can begin inside an item.
 struct SharedEntity {
   int32_t first_seq, n_seqs;    // whose query rows
   int32_t group_first, group_n; // whose table rows may be read
@@ -51,14 +51,22 @@ struct SharedParams {
   const void *q, *k_pool, *v_pool;
   const int32_t *block_table, *seq_lens, *shared_lens;
   const SharedEntity* entities;  // [n_shared + batch]
-  float *o_shared, *lse_shared;  // slots of row_block rows
-  float *o_own, *lse_own;        // slots of `group` rows
+  float *o, *lse;                // partial rows: of the shared items, of the own items, row_block for every CTA
   long long* unit_begin;         // [n_shared + batch + 1] where the entities' units begin; written for the merge
   int* status;
   int64_t page_stride, head_stride;  // elements
   int32_t n_shared, batch, n_kv_heads, group, max_pages, n_pool_pages, row_block;
 };
 
+// where the partial rows of an item begin
+__device__ __forceinline__ int64_t item_rows(const SharedParams& p, bool own, int first_seq, int n_seqs, int head) {
+  const int64_t all = (int64_t)p.batch * p.n_kv_heads * p.group;
+  return own ? all + ((int64_t)first_seq * p.n_kv_heads + head) * p.group
+             : ((int64_t)first_seq * p.n_kv_heads + (int64_t)head * n_seqs) * p.group;
+}
+__device__ __forceinline__ int64_t cta_rows(const SharedParams& p, int cta) {
+  return 2 * (int64_t)p.batch * p.n_kv_heads * p.group + (int64_t)cta * p.row_block;
+}
 __device__ __forceinline__ int shared_split(const SharedParams& p, int group) {
   return max(0, min(p.shared_lens[group], p.max_pages * 16)) & ~15;
 }

@@ -69,9 +69,8 @@ struct Work {
   int limit0;         // prompt: keys that the first query token sees
   int n_keys;         // keys from key0 on that anyone sees
   int row;            // decode step: table row
-  short own;          // decode step: own part (slots of G rows)
-  short last;         // nothing follows
-  int64_t slot;
+  int last;           // nothing follows
+  int64_t out_row;    // decode step: where the partial rows begin
 };
 
 struct TcParams {
@@ -383,18 +382,16 @@ template <int D, bool PAGED> struct CopyRole {
       const int units = __shfl_sync(0xffffffffu, w_units, at), n = (int)min((int64_t)(units - cur.k), cur.left);
       wk.q_tok = __shfl_sync(0xffffffffu, w_first, at);
       wk.n_tok = __shfl_sync(0xffffffffu, w_n, at);
-      wk.own = cur.e >= s.n_shared;
-      if (wk.own) {
-        wk.row = wk.q_tok;
-      } else if (lead_of != cur.e) {
+      const bool own = cur.e >= s.n_shared;
+      if (!own && lead_of != cur.e) {
         lead_of = cur.e;
         lead = entity_lead(s, load_entity(s, cur.e), hi);
       }
-      if (!wk.own) wk.row = lead.x;
+      wk.row = own ? wk.q_tok : lead.x;
       wk.head = cur.h;
       wk.key0 = lo + cur.k * kKeys;
-      wk.n_keys = max(0, min(wk.own ? hi : lead.y, wk.key0 + n * kKeys) - wk.key0);
-      wk.slot = (int64_t)(wk.own ? cur.e - s.n_shared : cur.e) * s.n_kv_heads + cur.h + blockIdx.x;
+      wk.n_keys = max(0, min(own ? hi : lead.y, wk.key0 + n * kKeys) - wk.key0);
+      wk.out_row = cur.k == 0 ? item_rows(s, own, wk.q_tok, wk.n_tok, cur.h) : cta_rows(s, blockIdx.x);
       wk.order.split = wk.n_tok <= tpm;
       wk.order.keys[0] = wk.order.keys[1] = max(1, wk.n_keys);  // a tile of keys that nobody sees, where there are none
       cur.left -= n;
@@ -802,10 +799,9 @@ __device__ __forceinline__ void softmax_role(const TcParams& p, Bars* bars, cons
     float* lse_out;    // of this row
     int at;            // this row, in elements from `out`; -1: none
     if constexpr (PAGED) {
-      const int64_t first = wk.slot * (wk.own ? G : p.s.row_block);
-      out = (wk.own ? p.s.o_own : p.s.o_shared) + first * D;
+      out = p.s.o + wk.out_row * D;
       at = (tok * G + g) * D;
-      lse_out = (wk.own ? p.s.lse_own : p.s.lse_shared) + first + tok * G + g;
+      lse_out = p.s.lse + wk.out_row + tok * G + g;
     } else {
       const int64_t first = wk.q_tok * hq + wk.head * G;
       out = (Out*)p.t.out + first * D;

@@ -405,7 +405,7 @@ __global__ void __launch_bounds__(kMoveThreads) pages_write_kernel(const WritePa
         continue;
       }
       row = p.rows[lo];
-      good = (unsigned)row < (unsigned)st.n_rows;
+      good = (unsigned)row < (unsigned)st.n_rows && start >= 0 && end <= p.n_tokens;
       bool again = false;
       for (int i = lane; good && i < lo; i += 32) again |= p.rows[i] == row;
       good = good && !__any_sync(0xffffffffu, again);  // a row named twice: the first entry counts

@@ -247,3 +247,12 @@ def test_page_plan_waits_for_the_cluster_before_it_reads_a_peer():
         assert 0 < body.index("if constexpr (CTAS > 1) sync_all<CTAS>()") < body.index("scan<CTAS>(")
     scan = text[text.index("Sums scan("):]
     assert scan.index("sync_all<CTAS>()") < scan.index("peer_word(")
+
+
+def test_shared_workspace_does_not_grow_with_the_group_sizes(lib):
+    """Partial rows: one per query row and part, and one block per SM - also for many groups of one."""
+    for dtype in (_lib.IA_F32, _lib.IA_BF16):
+        g = geom(batch=2048, n_kv_heads=8, dtype=dtype)
+        for n_shared in (8, 2048):
+            rows = 2 * 2048 * 32 + 160 * 256
+            assert lib.ia_shared_prefix_workspace_bytes(n_shared, ctypes.byref(g)) <= rows * 65 * 4 + 8 * 4200 + 1024

@@ -172,6 +172,12 @@ def test_write_refuses_what_does_not_fit():
     assert float(cache.pools[0][0][page, :, 3:5].float().sum()) == 2 * 2 * 64
     page = int(cache.block_table[1, 0])
     assert torch.equal(cache.pools[0][0][page], want[0][0][page])
+    before = [(k.clone(), v.clone()) for k, v in cache.pools]
+    for starts in ([0, 31], [-1, 3], [-(2 ** 31), 2 ** 31 - 1], [5, 2], [2 ** 31 - 5, 2 ** 31 - 1]):      # not these tokens
+        cache.write(0, i32([0]), i32(starts), k, k)
+        ops.device_status()
+    for got, exp in zip(cache.pools, before):
+        assert torch.equal(got[0], exp[0]) and torch.equal(got[1], exp[1])
 
 
 def test_captured_and_on_another_stream():
