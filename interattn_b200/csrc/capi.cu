@@ -645,9 +645,14 @@ static int check_prompt_lens(const int32_t* q_lens, const int32_t* kv_lens, int 
 int64_t ia_prompt_plan_ints(const int32_t* q_lens, const int32_t* kv_lens, int n_seqs, int n_kv_heads, int group_size,
                             int head_dim, int dtype) {
   if (check_prompt_lens(q_lens, kv_lens, n_seqs, n_kv_heads, group_size, head_dim, dtype)) return -1;
-  const int64_t n = prompt_plan_ints(q_lens, n_seqs, n_kv_heads, group_size, dtype);
-  if (n < 0) fail(IA_ERR_UNSUPPORTED, "prompt_plan: too many pieces");
-  return n;
+  try {
+    const int64_t n = prompt_plan_ints(q_lens, kv_lens, n_seqs, n_kv_heads, group_size, dtype);
+    if (n < 0) fail(IA_ERR_UNSUPPORTED, "prompt_plan: too many pieces");
+    return n;
+  } catch (const std::exception&) {
+    fail(IA_ERR_UNSUPPORTED, "prompt_plan: out of host memory");
+    return -1;
+  }
 }
 
 int ia_prompt_plan(const int32_t* q_lens, const int32_t* kv_lens, int n_seqs, int n_kv_heads, int group_size, int head_dim,

@@ -7,7 +7,7 @@
 // maximum moves.  All of it in fp32.  A thread owns RPT rows x 4 keys of the logits and RPT rows x D / 16 output columns;
 // 16 neighbouring lanes share a row, so the row's statistics are four shuffles.  Rows of 132 floats keep the key reads of
 // 8 lanes on 32 banks.  A 4096-token prompt at 32 / 8 heads of 128: 39 TFLOP/s, bound by the FMA pipe and its operands from
-// shared memory; a decode step of single sequences: 1.1 TB/s, bound by reading the tile from shared memory in every warp.
+// shared memory.  Decode steps of up to kFewRows rows are bound by reading the cache and have a form of their own.
 #include <algorithm>
 #include <atomic>
 #include <cstring>
@@ -21,13 +21,12 @@
 namespace ia {
 namespace {
 
-constexpr int kThreads = 256, kKeys = 64, kPLd = kKeys + 4;
+constexpr int kThreads = 256, kKeys = 64, kPLd = kKeys + 4, kFewRows = 16;
 
-// At most 16 rows: a ring of three tiles is under way.  More rows: the products take the time, and K and V of
-// the next tile replace each as soon as it has been used.
+// K and V of the next tile replace each as soon as it has been used.
 template <int D, int RPT> struct Smem {
-  static constexpr int rows = 16 * RPT, ld = D + 4, stages = RPT == 1 ? 3 : 1;
-  static constexpr int q = 0, k = q + rows * ld, kv = kKeys * ld + kKeys * D, p = k + stages * kv, floats = p + rows * kPLd;
+  static constexpr int rows = 16 * RPT, ld = D + 4;
+  static constexpr int q = 0, k = q + rows * ld, v = k + kKeys * ld, p = v + kKeys * D, floats = p + rows * kPLd;
   static constexpr size_t bytes = (size_t)floats * 4 + rows * 8;  // + limits and flags
 };
 
@@ -60,7 +59,7 @@ __device__ void attend(float* sm, int n_rows, int lo, int hi, float scale_log2, 
   using S = Smem<D, RPT>;
   constexpr int ROWS = S::rows, LD = S::ld, NO = D / 64;
   const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
-  float *qs = sm + S::q, *ps = sm + S::p;
+  float *qs = sm + S::q, *ks = sm + S::k, *vs = sm + S::v, *ps = sm + S::p;
   int* lim = reinterpret_cast<int*>(sm + S::floats);
   int* bad = lim + ROWS;
   const float* any = q_row(0);
@@ -69,14 +68,10 @@ __device__ void attend(float* sm, int n_rows, int lo, int hi, float scale_log2, 
     const int row = i / (D / 4), c = i % (D / 4) * 4;
     cp_async16(qs + row * LD + c, row < n_rows ? q_row(row) + c : any, row < n_rows);
   }
-#pragma unroll
-  for (int st = 0; st < S::stages; ++st) {  // a group each for K and V of a tile
-    float* to = sm + S::k + st * S::kv;
-    if (lo + st * kKeys < hi) load_tile<false, D, LD>(to, any, lo + st * kKeys, hi, key);
-    cp_commit();
-    if (lo + st * kKeys < hi) load_tile<true, D, D>(to + kKeys * LD, any, lo + st * kKeys, hi, key);
-    cp_commit();
-  }
+  load_tile<false, D, LD>(ks, any, lo, hi, key);
+  cp_commit();
+  load_tile<true, D, D>(vs, any, lo, hi, key);
+  cp_commit();
   if (tid < ROWS) {
     lim[tid] = tid < n_rows ? limit(tid) : 0;
     bad[tid] = 0;
@@ -91,12 +86,9 @@ __device__ void attend(float* sm, int n_rows, int lo, int hi, float scale_log2, 
 #pragma unroll
       for (int b = 0; b < 4; ++b) o[i][a][b] = 0.f;
   }
-  int st = 0;
   for (int j0 = lo; j0 < hi; j0 += kKeys) {
-    float *ks = sm + S::k + st * S::kv, *vs = ks + kKeys * LD;
-    if (++st == S::stages) st = 0;
-    const int ahead = j0 + S::stages * kKeys;  // the tile that takes this one's place
-    cp_wait<2 * S::stages - 1>();
+    const int ahead = j0 + kKeys;
+    cp_wait<1>();
     __syncthreads();
     float s[RPT][4];
 #pragma unroll
@@ -149,7 +141,7 @@ __device__ void attend(float* sm, int n_rows, int lo, int hi, float scale_log2, 
 #pragma unroll
         for (int b = 0; b < 4; ++b) o[i][a][b] *= keep;
     }
-    cp_wait<2 * S::stages - 1>();
+    cp_wait<1>();
     __syncthreads();  // also: the row's weights are written
 #pragma unroll 2
     for (int n = 0; n < kKeys; n += 4) {
@@ -222,6 +214,156 @@ struct RowSink {  // rows r = token * group + g of one kv head
   __device__ __forceinline__ float* lse(int r) const { return l == nullptr ? nullptr : l + r / group * l_tok + r % group; }
 };
 
+// The decode step of a few rows (at most RP), where reading K and V is what takes the time: each warp has a ring of its own of
+// 8-key batches and takes every eighth batch, D / 32 dims a lane.  32 / RP keys make 32 dot products, whose partial sums 31
+// shuffles bring together so that lane k * RP + r ends up with the logit of key k and row r; weights go back the same way.
+// The warps' outputs meet in shared memory at the end.  What a row does not see is never multiplied with it.
+// 16 x 16000 shared keys at 8 kv heads of 128, 1 / 2 / 4 sequences of 4 rows each: 3.0 / 3.6 / 3.0 TB/s (the tiled form with
+// 16 rows, three tiles under way: 1.2 TB/s for any of them; 16 rows here whatever there are: 1.9 TB/s).  Bound by the
+// latency of a batch's chain - products, shuffles, exponential - with 8 warps an SM, and by the start of each segment.
+// The batch loop is not unrolled: unrolled over a page, fetching the instructions took 50 us of a small step's 70 us.
+constexpr int kWarps = kThreads / 32, kFewKeys = 8, kFewRing = 3 * 2 * kFewKeys * 128;  // floats of a warp's ring
+
+template <int D, int RP, typename QRow, typename Limit>
+__device__ void attend_few(float* sm, int n_rows, int lo, int hi, float scale_log2, const PagedKeys<float>& key, const QRow& q_row,
+                           const Limit& limit, const RowSink& sink) {
+  constexpr int V = D / 32, KB = 32 / RP, kBatch = 2 * kFewKeys * D, kStages = kFewRing / kBatch, kChunks = kFewKeys * D / 128;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, my_row = lane % RP, my_key = lane / RP;
+  float* ring = sm + warp * kFewRing;
+  __syncthreads();  // the piece before is done with the shared memory
+  const auto page_of = [&](int j) {  // the page that holds key j, -1 where there is none
+    if (j >= hi || (j >> 4) >= key.max_pages) return -1;
+    const int page = key.table[j >> 4];
+    return key.n_pages > 0 && page >= key.n_pages ? -1 : page;
+  };
+  const auto issue = [&](int j, int page, float* to) {  // a batch's K, then its V; zeros where there is no key
+    const int64_t at = (int64_t)max(page, 0) * key.page_stride + (int64_t)(j & 15) * D;
+#pragma unroll
+    for (int i = 0; i < kChunks; ++i) {
+      const int c = (i * 32 + lane) * 4;
+      const bool ok = page >= 0 && j + c / D < hi;
+      cp_async16(to + c, key.k + (ok ? at + c : 0), ok);
+      cp_async16(to + kFewKeys * D + c, key.v + (ok ? at + c : 0), ok);
+    }
+  };
+  constexpr int kStep = kWarps * kFewKeys;
+  int j0 = lo + warp * kFewKeys, put = 0, get = 0;
+#pragma unroll 1
+  for (int i = 0; i < kStages - 1; ++i) {
+    issue(j0 + i * kStep, page_of(j0 + i * kStep), ring + i * kBatch);
+    cp_commit();
+  }
+  put = kStages - 1;
+  int next = page_of(j0 + (kStages - 1) * kStep);
+  float q[RP][V], acc[RP][V], m = -INFINITY, l = 0.f;
+#pragma unroll
+  for (int r = 0; r < RP; ++r) {
+    if (r < n_rows) load_vec<V>(q_row(r) + lane * V, q[r]);
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      q[r][i] = r < n_rows ? q[r][i] * scale_log2 : 0.f;
+      acc[r][i] = 0.f;
+    }
+  }
+  const int my_limit = my_row < n_rows ? limit(my_row) : 0;
+#pragma unroll 1
+  for (; j0 < hi; j0 += kStep) {
+    __syncwarp();  // all lanes are done with the batch whose place is filled now
+    issue(j0 + (kStages - 1) * kStep, next, ring + put * kBatch);
+    cp_commit();
+    if (++put == kStages) put = 0;
+    next = page_of(j0 + kStages * kStep);
+    cp_wait<kStages - 1>();
+    __syncwarp();
+    const float *ks = ring + get * kBatch + lane * V, *vs = ks + kFewKeys * D;
+    if (++get == kStages) get = 0;
+#pragma unroll 1
+    for (int k0 = 0; k0 < kFewKeys; k0 += KB, ks += KB * D, vs += KB * D) {
+      float s[32];
+#pragma unroll
+      for (int i = 0; i < KB; ++i) {
+        float x[V];
+        load_vec<V>(ks + i * D, x);
+#pragma unroll
+        for (int r = 0; r < RP; ++r) {
+          s[i * RP + r] = q[r][0] * x[0];
+#pragma unroll
+          for (int d = 1; d < V; ++d) s[i * RP + r] += q[r][d] * x[d];
+        }
+      }
+#pragma unroll
+      for (int w = 16; w > 0; w >>= 1)  // w values are left, in either half of the lanes the half that belongs there
+#pragma unroll
+        for (int i = 0; i < w; ++i) {
+          const bool upper = lane & w;
+          const float give = upper ? s[i] : s[i + w], keep = upper ? s[i + w] : s[i];
+          s[i] = keep + __shfl_xor_sync(0xffffffffu, give, w);
+        }
+      const bool sees = j0 + k0 + my_key < my_limit;
+      const unsigned seen = __ballot_sync(0xffffffffu, sees);
+      const float t = sees ? s[0] : -INFINITY;
+      float top = t;
+#pragma unroll
+      for (int w = RP; w < 32; w <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+      const float m_new = fmaxf(m, top), base = m_new == -INFINITY ? 0.f : m_new;
+      const float keep = exp2f(m - base), weight = exp2f(t - base);
+      if (__any_sync(0xffffffffu, m_new != m)) {
+#pragma unroll
+        for (int r = 0; r < RP; ++r) {
+          const float kr = __shfl_sync(0xffffffffu, keep, r);
+#pragma unroll
+          for (int d = 0; d < V; ++d) acc[r][d] *= kr;
+        }
+        l *= keep;
+      }
+      m = m_new;
+      l += weight;
+#pragma unroll
+      for (int i = 0; i < KB; ++i) {
+        float x[V];
+        load_vec<V>(vs + i * D, x);
+#pragma unroll
+        for (int r = 0; r < RP; ++r) {
+          const float w = __shfl_sync(0xffffffffu, weight, i * RP + r);
+          if (seen >> (i * RP + r) & 1) {
+#pragma unroll
+            for (int d = 0; d < V; ++d) acc[r][d] += w * x[d];
+          }
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int w = RP; w < 32; w <<= 1) l += __shfl_xor_sync(0xffffffffu, l, w);
+  cp_wait<0>();
+  __syncthreads();  // every ring is done with
+  float *o = sm, *stats = sm + kWarps * RP * D;  // [warp][row][D], [warp][row](m, l)
+#pragma unroll
+  for (int r = 0; r < RP; ++r) store_vec<V>(o + (warp * RP + r) * D + lane * V, acc[r]);
+  if (lane < RP) {
+    stats[(warp * RP + lane) * 2] = m;
+    stats[(warp * RP + lane) * 2 + 1] = l;
+  }
+  __syncthreads();
+#pragma unroll 1
+  for (int i = tid; i < n_rows * D; i += kThreads) {
+    const int r = i / D, d = i % D;
+    float M = -INFINITY, L = 0.f, x = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) M = fmaxf(M, stats[(w * RP + r) * 2]);
+    const float base = M == -INFINITY ? 0.f : M;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const float f = exp2f(stats[(w * RP + r) * 2] - base);
+      L += stats[(w * RP + r) * 2 + 1] * f;
+      x += o[(w * RP + r) * D + d] * f;
+    }
+    const bool empty = limit(r) <= lo;
+    sink.row(r)[d] = empty ? 0.f : x / L;
+    if (d == 0) *sink.lse(r) = empty ? -INFINITY : (M + log2f(L)) * kLn2;
+  }
+}
+
 template <int D, int RPT>
 __global__ void __launch_bounds__(kThreads) prompt_attention_kernel(const PromptTensors t, const PromptItem* items) {
   extern __shared__ __align__(16) float sm[];
@@ -248,7 +390,7 @@ __global__ void __launch_bounds__(kThreads) shared_attention_kernel(const Shared
   grid_dependency_wait();
   grid_launch_dependents();
   const int G = p.group, hq = p.n_kv_heads * G, cta = blockIdx.x;
-  SharedCursor c = find_share<kKeys, kThreads>(p, cta, gridDim.x, scratch);
+  SharedCursor c = find_share<0, kThreads>(p, cta, gridDim.x, scratch);
   while (c.left > 0) {
     const SharedEntity ent = load_entity(p, c.e);
     int lo, hi;
@@ -256,7 +398,7 @@ __global__ void __launch_bounds__(kThreads) shared_attention_kernel(const Shared
     const int n = (int)min((int64_t)(c.units - c.k), c.left);
     const int2 lead = entity_lead(p, ent, hi);
     const int32_t* table = p.block_table + (int64_t)lead.x * p.max_pages;
-    const int from = lo + c.k * kKeys, to = max(from, min(lead.y, from + n * kKeys));
+    const int from = lo + c.k * ent.unit, to = max(from, min(lead.y, from + n * ent.unit));
     const bool own = c.e >= p.n_shared;
     const int64_t row0 = c.k == 0 ? item_rows(p, own, ent.first_seq, ent.n_seqs, c.h) : cta_rows(p, cta);
     const PagedKeys<float> key{(const float*)p.k_pool + c.h * p.head_stride, (const float*)p.v_pool + c.h * p.head_stride,
@@ -269,17 +411,22 @@ __global__ void __launch_bounds__(kThreads) shared_attention_kernel(const Shared
       const int page = table[j];
       if (page < 0 || (p.n_pool_pages > 0 && page >= p.n_pool_pages)) atomicOr(p.status, DEV_STATUS_BAD_INDEX);
     }
-    // a single sequence has at most 16 rows: the narrow form, which spends the threads on keys instead of empty rows
-    if (ent.n_seqs * G <= 16)
-      attend<D, 1>(sm, ent.n_seqs * G, from, to, kLog2e * rsqrtf((float)D), key, q_row, limit, sink);
-    else
-      attend<D, 8>(sm, ent.n_seqs * G, from, to, kLog2e * rsqrtf((float)D), key, q_row, limit, sink);
+    // Few rows: see attend_few.  More: the tile with the fewest empty rows; 16 groups of 8 / 16 sequences of 4 rows over
+    // 4000 keys 0.59 / 0.74 ms, with tiles of 128 rows 1.13 / 1.21 ms.
+    const int n_rows = ent.n_seqs * G;
+    const float scale = kLog2e * rsqrtf((float)D);
+    if (n_rows <= 4) attend_few<D, 4>(sm, n_rows, from, to, scale, key, q_row, limit, sink);
+    else if (n_rows <= 8) attend_few<D, 8>(sm, n_rows, from, to, scale, key, q_row, limit, sink);
+    else if (n_rows <= kFewRows) attend_few<D, kFewRows>(sm, n_rows, from, to, scale, key, q_row, limit, sink);
+    else if (n_rows <= 32) attend<D, 2>(sm, n_rows, from, to, scale, key, q_row, limit, sink);
+    else if (n_rows <= 64) attend<D, 4>(sm, n_rows, from, to, scale, key, q_row, limit, sink);
+    else attend<D, 8>(sm, n_rows, from, to, scale, key, q_row, limit, sink);
     c.left -= n;
     c.k = 0;
     if (++c.h == p.n_kv_heads) {
       c.h = 0;
       if (c.left > 0)  // some entity behind this one has units: they were counted
-        do c.units = entity_units<kKeys>(p, ++c.e);
+        do c.units = entity_units<0>(p, ++c.e);
         while (c.units == 0);
     }
   }
@@ -374,7 +521,7 @@ int launch_prompt(const PromptTensors& t, const PromptItem* items, int n_items, 
 template <int D> int launch_shared(const SharedParams& p, int ctas, cudaStream_t stream) {
   auto kern = shared_attention_kernel<D>;
   static SmemOnce once;
-  constexpr size_t bytes = std::max(Smem<D, 8>::bytes, Smem<D, 1>::bytes);
+  constexpr size_t bytes = std::max(Smem<D, 8>::bytes, (size_t)kWarps * kFewRing * 4);
   if (int s = once.allow((const void*)kern, bytes, "shared_attention_kernel")) return s;
   return launch(kern, (unsigned)ctas, bytes, stream, "shared_attention_kernel", p);
 }
@@ -432,72 +579,109 @@ int launch_shared_merge(const SharedParams& p, const int32_t* seq_info, int head
 // Words: a header of 8, where each CTA's items begin (ctas + 1 words, padded to whole items), the items.
 namespace {
 constexpr int kRowsFew = 32, kRowsFull = 128;
-constexpr int kPieceCost = 256;  // what starting and ending a piece costs, in keys
 struct PlanShape {
   int n_items, ctas, item_tokens;
   bool few_rows;
   int64_t ints() const { return 8 + (int64_t)(ctas + 1 + 7) / 8 * 8 + (int64_t)n_items * 8; }
 };
-int64_t count_items(const int32_t* q_lens, int n_seqs, int tokens) {
-  int64_t n = 0;
-  for (int i = 0; i < n_seqs; ++i) n += ((int64_t)q_lens[i] + tokens - 1) / tokens;
-  return n;
+struct PlanInput {
+  const int32_t *q_lens, *kv_lens;
+  int n_seqs, n_kv_heads, group, dtype;
+};
+int piece_keys(const PromptItem& it) { return std::max(0, std::min(it.limit0 + it.n_tok - 1, it.kv_len)); }
+// the pieces, the longest first, so that what is started last is short
+std::vector<PromptItem> make_pieces(const PlanInput& in, const PlanShape& s, int64_t* n_q, int64_t* n_kv) {
+  std::vector<PromptItem> items;
+  items.reserve(s.n_items);
+  int64_t q0 = 0, k0 = 0;
+  for (int i = 0; i < in.n_seqs; ++i) {
+    for (int t = 0; t < in.q_lens[i]; t += s.item_tokens)
+      for (int h = 0; h < in.n_kv_heads; ++h)
+        items.push_back(PromptItem{(int)(q0 + t), std::min(s.item_tokens, in.q_lens[i] - t), (int)k0,
+                                   in.kv_lens[i] - in.q_lens[i] + t + 1, in.kv_lens[i], h, {0, 0}});
+    q0 += in.q_lens[i];
+    k0 += in.kv_lens[i];
+  }
+  std::stable_sort(items.begin(), items.end(),
+                   [](const PromptItem& a, const PromptItem& b) { return piece_keys(a) > piece_keys(b); });
+  *n_q = q0;
+  *n_kv = k0;
+  return items;
 }
-bool plan_shape(const int32_t* q_lens, int n_seqs, int n_kv_heads, int group, int dtype, PlanShape* s) {
-  // query rows of a piece: large ones read K and V less often, small ones spread over more SMs
-  const int full = dtype == IA_F32 ? kRowsFull / group : 2 * (kRowsFull / group);
-  const int few = dtype == IA_F32 ? kRowsFew / group : kRowsFull / group;
-  int64_t items = count_items(q_lens, n_seqs, full) * n_kv_heads;
-  s->few_rows = items < 2 * sm_count();
-  s->item_tokens = s->few_rows ? few : full;
-  items = count_items(q_lens, n_seqs, s->item_tokens) * n_kv_heads;
-  if (items > 0x7fffffff / 64) return false;
-  s->n_items = (int)items;
-  s->ctas = dtype == IA_F32 ? (int)items : (int)std::min<int64_t>(items, sm_count());
+// What a piece costs, in quarters of what a key costs a large piece.  Starting and ending one takes as long as 256 keys
+// (tensor cores; a small one 192) or 32 (fp32; 16); a key of a small piece, half or a quarter of the rows, 1 / 2 or 3 / 8.
+int64_t piece_cost(const PromptItem& it, int dtype, bool few_rows) {
+  const int64_t n = piece_keys(it);
+  if (dtype == IA_F32) return few_rows ? n + n / 2 + 4 * 16 : 4 * n + 4 * 32;
+  return few_rows ? 2 * n + 4 * 192 : 4 * n + 4 * 256;
+}
+// The next longest piece goes to the SM with the least to do so far; returns what the busiest has to do.
+int64_t spread(const std::vector<PromptItem>& items, int ctas, int dtype, bool few_rows, std::vector<int>* cta_of) {
+  using Load = std::pair<int64_t, int>;
+  std::priority_queue<Load, std::vector<Load>, std::greater<Load>> loads;
+  for (int c = 0; c < ctas; ++c) loads.push({0, c});
+  int64_t most = 0;
+  for (const PromptItem& it : items) {
+    const Load at = loads.top();
+    loads.pop();
+    if (cta_of != nullptr) cta_of->push_back(at.second);
+    const int64_t load = at.first + piece_cost(it, dtype, few_rows);
+    most = std::max(most, load);
+    loads.push({load, at.second});
+  }
+  return most;
+}
+PlanShape shape_of(const PlanInput& in, bool few_rows, bool* fits) {
+  const int rows = kRowsFull / in.group;
+  PlanShape s;
+  s.few_rows = few_rows;
+  s.item_tokens = in.dtype == IA_F32 ? (few_rows ? kRowsFew / in.group : rows) : (few_rows ? rows : 2 * rows);
+  int64_t n = 0;
+  for (int i = 0; i < in.n_seqs; ++i) n += ((int64_t)in.q_lens[i] + s.item_tokens - 1) / s.item_tokens;
+  n *= in.n_kv_heads;
+  *fits = n <= 0x7fffffff / 64;
+  s.n_items = (int)n;
+  s.ctas = in.dtype == IA_F32 ? (int)n : (int)std::min<int64_t>(n, sm_count());
+  return s;
+}
+// Large pieces (128 rows in fp32, two tiles of 128 on the tensor cores) use what they read better, small ones (32, one tile)
+// spread a short batch over more SMs: the plan is made for both and the one whose busiest SM ends first is taken.  32 / 8
+// heads of 128, small and large pieces, us: fp32 one prompt of 600: 139 and 166, of 900: 301 and 242, 150, 30, 10, 400, 5 and
+// 77: 90 and 119, four of 300: 156 and 131; bf16 one of 600: 18.5 and 23.5, of 1700: 45 and 44, four of 300: 22.7 and 19.5,
+// three of 700: 37 and 31.  With four large pieces an SM the small ones gain nothing more (bf16 3000 and 2300: 148 and 138).
+bool plan_shape(const PlanInput& in, PlanShape* s) {
+  bool fits, fits_few;
+  *s = shape_of(in, false, &fits);
+  if (!fits || s->n_items >= 4 * sm_count()) return fits;
+  const PlanShape few = shape_of(in, true, &fits_few);
+  int64_t q, kv;
+  if (spread(make_pieces(in, few, &q, &kv), sm_count(), in.dtype, true, nullptr) <
+      spread(make_pieces(in, *s, &q, &kv), sm_count(), in.dtype, false, nullptr))
+    *s = few;
   return true;
 }
 }  // namespace
 
-int64_t prompt_plan_ints(const int32_t* q_lens, int n_seqs, int n_kv_heads, int group, int dtype) {
+int64_t prompt_plan_ints(const int32_t* q_lens, const int32_t* kv_lens, int n_seqs, int n_kv_heads, int group, int dtype) {
   PlanShape s;
-  return plan_shape(q_lens, n_seqs, n_kv_heads, group, dtype, &s) ? s.ints() : -1;
+  return plan_shape(PlanInput{q_lens, kv_lens, n_seqs, n_kv_heads, group, dtype}, &s) ? s.ints() : -1;
 }
 
 int make_prompt_plan(const int32_t* q_lens, const int32_t* kv_lens, int n_seqs, int n_kv_heads, int group, int head_dim, int dtype,
                      int32_t* plan, int64_t plan_ints) {
+  const PlanInput in{q_lens, kv_lens, n_seqs, n_kv_heads, group, dtype};
   PlanShape s;
-  if (!plan_shape(q_lens, n_seqs, n_kv_heads, group, dtype, &s) || plan_ints < s.ints())
-    return fail(IA_ERR_BAD_ARG, "prompt_plan: %lld words", (long long)plan_ints);
-  std::vector<PromptItem> items;
-  items.reserve(s.n_items);
-  int64_t q0 = 0, k0 = 0;
-  for (int i = 0; i < n_seqs; ++i) {
-    for (int t = 0; t < q_lens[i]; t += s.item_tokens)
-      for (int h = 0; h < n_kv_heads; ++h)
-        items.push_back(PromptItem{(int)(q0 + t), std::min(s.item_tokens, q_lens[i] - t), (int)k0,
-                                   kv_lens[i] - q_lens[i] + t + 1, kv_lens[i], h, {0, 0}});
-    q0 += q_lens[i];
-    k0 += kv_lens[i];
-  }
-  const auto keys = [](const PromptItem& it) { return std::max(0, std::min(it.limit0 + it.n_tok - 1, it.kv_len)); };
-  // the longest first, so that what is started last is short
-  std::stable_sort(items.begin(), items.end(), [&](const PromptItem& a, const PromptItem& b) { return keys(a) > keys(b); });
+  if (!plan_shape(in, &s) || plan_ints < s.ints()) return fail(IA_ERR_BAD_ARG, "prompt_plan: %lld words", (long long)plan_ints);
+  int64_t q0, k0;
+  const std::vector<PromptItem> items = make_pieces(in, s, &q0, &k0);
   std::vector<int> order(s.n_items), begin(s.ctas + 1, 0);
   if (dtype == IA_F32) {  // a CTA each, in this order
     for (int i = 0; i < s.n_items; ++i) order[i] = begin[i] = i;
     begin[s.ctas] = s.n_items;
-  } else {  // a list for each SM: the next longest piece goes to the SM with the least to do so far
-    std::vector<int> cta_of(s.n_items);
-    using Load = std::pair<int64_t, int>;
-    std::priority_queue<Load, std::vector<Load>, std::greater<Load>> loads;
-    for (int c = 0; c < s.ctas; ++c) loads.push({0, c});
-    for (int i = 0; i < s.n_items; ++i) {
-      const Load at = loads.top();
-      loads.pop();
-      cta_of[i] = at.second;
-      ++begin[at.second + 1];
-      loads.push({at.first + keys(items[i]) + kPieceCost, at.second});
-    }
+  } else {  // a list for each SM
+    std::vector<int> cta_of;
+    spread(items, s.ctas, dtype, s.few_rows, &cta_of);
+    for (const int c : cta_of) ++begin[c + 1];
     for (int c = 0; c < s.ctas; ++c) begin[c + 1] += begin[c];
     std::vector<int> next(begin.begin(), begin.end() - 1);
     for (int i = 0; i < s.n_items; ++i) order[next[cta_of[i]]++] = i;
@@ -528,16 +712,27 @@ void make_shared_plan(const int32_t* group_sizes, int n_groups, int batch, int g
   int32_t* info = plan + 8 + 8 * ((int64_t)n_shared + batch);
   std::fill(plan, plan + 8, 0);
   plan[0] = n_shared;
+  // A unit of many rows takes several times as long as one of few, and shares are equal in units: where there are entities
+  // of many rows, those of few get longer units.  16 groups of 8 / 16 / 32 sequences of 4 rows over 4000 keys with 1 to 256
+  // own ones: 0.59 / 0.74 / 1.47 ms, with 64 keys throughout 0.62 / 0.95 / 2.14 ms.  Without such entities 64 keys
+  // spread a short step over the most SMs.
+  bool wide = false;
+  for (int g = 0; g < n_groups; ++g) wide |= std::min(per, group_sizes[g]) * group > kFewRows;
+  const auto entity = [&](int first, int n, int group_first, int group_n, int g) {
+    const int rows = n * group;
+    const int unit = dtype != IA_F32 ? kTensorUnit : !wide ? kKeys : rows <= kFewRows ? 8 * kKeys : rows <= 32 ? 2 * kKeys : kKeys;
+    return SharedEntity{first, n, group_first, group_n, g, unit, {0, 0}};
+  };
   int seq = 0, e = 0;
   for (int g = 0; g < n_groups; ++g) {
     const int lead = seq;
     for (int m = 0; m < group_sizes[g]; m += per, ++e) {
       const int n = std::min(per, group_sizes[g] - m);
-      ent[e] = SharedEntity{lead + m, n, lead, group_sizes[g], g, {0, 0, 0}};
+      ent[e] = entity(lead + m, n, lead, group_sizes[g], g);
       for (int i = 0; i < n; ++i) {
         info[2 * (lead + m + i)] = e;
         info[2 * (lead + m + i) + 1] = i;
-        ent[n_shared + lead + m + i] = SharedEntity{lead + m + i, 1, lead + m + i, 1, g, {0, 0, 0}};
+        ent[n_shared + lead + m + i] = entity(lead + m + i, 1, lead + m + i, 1, g);
       }
     }
     seq += group_sizes[g];

@@ -36,15 +36,18 @@ struct PromptTensors {
 // part per sequence.  A shared part covers the keys [0, split) of its group, split = shared_len rounded down to whole
 // pages, read through the table row of the longest member (the first that holds the whole prefix, where one does: any
 // member may have left); an own part covers [split, seq_len) of its sequence.
-// An item is an (entity, kv head), its keys are cut into units of kUnit keys, and CTA c of P takes the units
+// An item is an (entity, kv head), its keys are cut into units (the tensor-core kernel: kUnit keys; fp32: as many as the
+// plan says for the entity, so that units of many and of few rows take about as long), and CTA c of P takes the units
 // [T c / P, T (c + 1) / P) of all T units laid end to end: equal shares whatever the lengths are, one run of keys per
 // CTA and item.  Each (item, CTA) leaves a normalised partial output and its log-sum-exp: the segment that begins the item in
 // the item's own rows, another in rows of the CTA - only the first segment of a CTA can begin inside an item.
+constexpr int kTensorUnit = 128;
 struct SharedEntity {
   int32_t first_seq, n_seqs;    // whose query rows
   int32_t group_first, group_n; // whose table rows may be read
   int32_t group;
-  int32_t reserved[3];
+  int32_t unit;                 // keys of a unit
+  int32_t reserved[2];
 };
 static_assert(sizeof(SharedEntity) == 32, "eight words of the plan");
 struct SharedParams {
@@ -107,11 +110,12 @@ __device__ __forceinline__ SharedEntity load_entity(const SharedParams& p, int e
   u.v[1] = reinterpret_cast<const int4*>(p.entities + e)[1];
   return u.e;
 }
-template <int kUnit> __device__ __forceinline__ int entity_units(const SharedParams& p, int e) {
+template <int kUnit> __device__ __forceinline__ int entity_units(const SharedParams& p, int e) {  // kUnit 0: the plan's
   const SharedEntity ent = load_entity(p, e);
   int lo, hi;
   entity_keys(p, e, ent, lo, hi);
-  return (hi - lo + kUnit - 1) / kUnit;
+  const int unit = kUnit > 0 ? kUnit : ent.unit;
+  return (hi - lo + unit - 1) / unit;
 }
 // no share is empty: between the first and the last CTA of an item every slot is written
 __device__ __forceinline__ int shares_of(int64_t total, int ctas) { return total < ctas ? (int)total : ctas; }
@@ -263,7 +267,8 @@ struct SmemOnce {  // a kernel's shared memory, allowed once per device
   std::atomic<uint64_t> done{0};
   int allow(const void* kern, size_t bytes, const char* what);
 };
-int64_t prompt_plan_ints(const int32_t* q_lens, int n_seqs, int n_kv_heads, int group, int dtype);  // -1: too large
+int64_t prompt_plan_ints(const int32_t* q_lens, const int32_t* kv_lens, int n_seqs, int n_kv_heads, int group,
+                         int dtype);  // -1: too large
 int make_prompt_plan(const int32_t* q_lens, const int32_t* kv_lens, int n_seqs, int n_kv_heads, int group, int head_dim, int dtype,
                      int32_t* plan, int64_t plan_ints);
 int shared_row_block(int dtype);  // query rows of a shared part, at most

@@ -36,7 +36,7 @@
 namespace ia {
 namespace {
 
-constexpr int kThreads = 352, kRows = 128, kKeys = 128, kWorkSlots = 8;
+constexpr int kThreads = 352, kRows = 128, kKeys = kTensorUnit, kWorkSlots = 8;
 constexpr int kCopyWarp = 8, kMmaWarp = 9;  // and 10
 
 template <int D> struct Tc {
@@ -468,7 +468,7 @@ template <int D, bool PAGED> struct CopyRole {
       if (lane == 0) mbar_arrive_expect_tx(full, (uint32_t)pages * (C::halves * 2048));
       __syncwarp();
       if (lane < pages) {
-        if (which == 0) {  // [64 keys][128 bytes] per half
+        if (which == 0) {  // [128 keys][128 bytes] per half
 #pragma unroll
           for (int h = 0; h < C::halves; ++h)
             tma_load_5d(smem_u32(dst + h * C::kv_block + lane * 2048), &p.tm_k, 0, 0, h, wk.head, page, full);

@@ -65,6 +65,18 @@ def test_prompt_plan_shares_the_work_evenly(lib):
     assert max(loads) <= 1.02 * sum(loads) / ctas + 256
 
 
+@pytest.mark.parametrize("dtype,lens,small", [
+    (_lib.IA_F32, [130], True), (_lib.IA_F32, [600], True), (_lib.IA_F32, [1000], False), (_lib.IA_F32, [300] * 4, False),
+    (_lib.IA_BF16, [600], True), (_lib.IA_BF16, [1000], True), (_lib.IA_BF16, [700] * 3, False), (_lib.IA_BF16, [9000], False),
+    (_lib.IA_F32, [300, 200, 100, 50], True), (_lib.IA_BF16, [300, 200, 100, 50], True)])
+def test_prompt_plan_takes_small_pieces_where_the_busiest_sm_then_ends_first(lib, dtype, lens, small):
+    """32 / 8 heads of 128 on 148 SMs; each of the two was timed."""
+    plan = prompt_plan(lib, lens, lens, 8, 4, 128, dtype)
+    rows = 4 * max(plan[plan[3] + 8 * i + 1] for i in range(plan[0]))
+    full = 128 if dtype == _lib.IA_F32 else 256
+    assert plan[2] == small and (rows <= full // 2) == small
+
+
 @pytest.mark.parametrize("change,word", [
     (dict(hkv=0), b"kv heads"), (dict(group=17), b"group size"), (dict(d=96), b"head_dim"), (dict(dtype=7), b"dtype"),
     (dict(q=[4, -1]), b"sequence 1"), (dict(kv=[4, -2]), b"sequence 1"), (dict(q=[1 << 30, 1]), b"tokens"),
@@ -133,6 +145,18 @@ def test_shared_plan_puts_every_sequence_into_one_shared_part(lib, dtype, groups
     for b, ent in enumerate(entities[n:]):
         assert ent[:4] == [b, 1, b, 1]
     assert lib.ia_shared_prefix_workspace_bytes(n, ctypes.byref(g)) > 0
+
+
+def test_shared_plan_fp32_units_follow_the_rows(lib):
+    """Keys of a unit: 64 where all entities are of few rows, longer for the few among many."""
+    def units(groups, group):
+        g = geom(batch=sum(groups), group_size=group, dtype=_lib.IA_F32)
+        words = lib.ia_shared_prefix_plan_ints(ints(groups), len(groups), ctypes.byref(g))
+        plan = (ctypes.c_int32 * words)()
+        _lib.check(lib.ia_shared_prefix_plan(ints(groups), len(groups), ctypes.byref(g), plan, words))
+        return {(plan[8 * e + 9] * group, plan[8 * e + 13]) for e in range(plan[0] + sum(groups))}
+    assert units([4, 1, 3], 4) == {(4, 64), (12, 64), (16, 64)}
+    assert units([1, 8, 16, 32, 40], 4) == {(4, 512), (32, 128), (64, 64), (128, 64)}
 
 
 def test_shared_refusals(lib):

@@ -197,6 +197,40 @@ def test_shared_prefix(hq, hkv, d, dtype, groups, shared, lens):
     decode_reference(q, kv.k_pool, kv.v_pool, table, lens).check(alone.step(q), dtype)
 
 
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("group", [1, 4, 5])
+@pytest.mark.parametrize("groups", [[1, 2, 3], [4, 1], [8, 5], [13, 1, 16], [17], [31, 3], [32, 1], [33]])
+def test_shared_prefix_fp32_row_counts(d, group, groups):
+    """Both sides of every row count at which the fp32 step changes its form; members of different lengths, one idle, one
+    inside the shared part, own parts from nothing to several units of the longest kind."""
+    n = sum(groups)
+    shared = [150 + 97 * g for g in range(len(groups))]
+    lens, first = [], 0
+    for size, split in zip(groups, shared):
+        lens += [[split + 41 * i, split, 1200 + i, split // 2, 0][(i + size) % 5] for i in range(size)]
+        first += size
+    q, kv, table = paged_case(2 * group, 2, d, F32, groups, shared, lens, seed=30)
+    step = dense_attention.SharedPrefixAttention(kv, groups, i32(shared), 2 * group)
+    out = step.step(q)
+    assert ops.device_status() == 0 and out.shape[0] == n
+    decode_reference(q, kv.k_pool, kv.v_pool, table, lens).check(out, F32)
+    assert torch.equal(step.step(q), out)
+
+
+@pytest.mark.parametrize("poison", [float("nan"), float("inf"), float("-inf")])
+@pytest.mark.parametrize("dtype,hq,groups", [(F32, 4, [1, 1]), (F32, 8, [1, 1]), (F32, 16, [1, 1]), (F32, 8, [5, 1]), (BF16, 8, [1, 1])])
+def test_shared_prefix_a_bad_value_spoils_exactly_the_rows_that_see_it(dtype, hq, groups, poison):
+    n = sum(groups)
+    shared, lens = [0] * len(groups), [100 + 13 * i for i in range(n)]
+    q, kv, table = paged_case(hq, 1, 64, dtype, groups, shared, lens, seed=31)
+    at = lens[0] - 1  # the first sequence's last token, and the place behind it
+    kv.v_pool[table[0, at // 16].long(), :, at % 16, 7] = poison
+    kv.v_pool[table[n - 1, lens[n - 1] // 16].long(), :, lens[n - 1] % 16:, 9] = poison
+    out = dense_attention.SharedPrefixAttention(kv, groups, i32(shared), hq).step(q)
+    bad = ~torch.isfinite(out)
+    assert bad[0, :, 7].all() and int(bad.sum()) == hq
+
+
 @pytest.mark.parametrize("hq,hkv,d,dtype", [(32, 8, 128, BF16), (8, 2, 64, F32)])
 def test_shared_prefix_long(hq, hkv, d, dtype):
     """Cut over all SMs; lengths that end inside tiles."""
