@@ -670,6 +670,20 @@ static bool strides_ok(int64_t tok, int64_t head, int head_dim, int size) {
   return tok >= head_dim && head >= head_dim && (tok * size) % 16 == 0 && (head * size) % 16 == 0;
 }
 
+// A piece's rows may be looked at again after they have been written, and other pieces read the same keys.
+static bool prompt_out_overlaps(const ia_prompt_tensors& t, int size) {
+  const int64_t hq = (int64_t)t.n_kv_heads * t.group_size;
+  const uintptr_t out = reinterpret_cast<uintptr_t>(t.out), out_end = out + (uintptr_t)(t.n_q_tokens * hq * t.head_dim * size);
+  const auto meets = [&](const void* p, int64_t tokens, int64_t heads, int64_t tok, int64_t head) {
+    const uintptr_t at = reinterpret_cast<uintptr_t>(p);
+    const uintptr_t end = at + (uintptr_t)(((tokens - 1) * tok + (heads - 1) * head + t.head_dim) * size);
+    return tokens > 0 && at < out_end && out < end;
+  };
+  return meets(t.q, t.n_q_tokens, hq, t.q_tok_stride, t.q_head_stride) ||
+         meets(t.k, t.n_kv_tokens, t.n_kv_heads, t.k_tok_stride, t.k_head_stride) ||
+         meets(t.v, t.n_kv_tokens, t.n_kv_heads, t.v_tok_stride, t.v_head_stride);
+}
+
 int ia_prompt_attention(const ia_prompt_tensors* t, const int32_t* plan_host, const int32_t* plan_device, ia_stream_t stream) {
   if (!t || !plan_host || !plan_device) return fail(IA_ERR_BAD_ARG, "prompt_attention: null argument");
   if (plan_host[4] != t->group_size * 1000 + t->head_dim || plan_host[5] != t->n_kv_heads * 16 + t->dtype)
@@ -687,6 +701,7 @@ int ia_prompt_attention(const ia_prompt_tensors* t, const int32_t* plan_host, co
       (t->n_kv_tokens > 0 && (!strides_ok(t->k_tok_stride, t->k_head_stride, t->head_dim, size) ||
                               !strides_ok(t->v_tok_stride, t->v_head_stride, t->head_dim, size))))
     return fail(IA_ERR_BAD_ARG, "prompt_attention: token and head strides are multiples of 16 bytes and hold a head");
+  if (prompt_out_overlaps(*t, size)) return fail(IA_ERR_BAD_ARG, "prompt_attention: the output may not overlap q, k or v");
   const PromptTensors p{t->q, t->k, t->v, t->out, t->lse, t->q_tok_stride, t->q_head_stride, t->k_tok_stride, t->k_head_stride,
                         t->v_tok_stride, t->v_head_stride, t->n_q_tokens, t->n_kv_tokens, t->n_kv_heads, t->group_size};
   const PromptItem* items = reinterpret_cast<const PromptItem*>(plan_device + plan_host[3]);

@@ -112,7 +112,7 @@ class PromptAttention:
     def run(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, out: Optional[torch.Tensor] = None,
             return_lse: bool = False):
         """q ``[sum(q_lens), Hq, D]``, k and v ``[sum(kv_lens), Hkv, D]`` (token and head strides of any multiple of 16 bytes)
-        -> ``[sum(q_lens), Hq, D]``, with ``return_lse`` also the log-sum-exp ``[sum(q_lens), Hq]`` f32 (-inf for a
+        -> ``[sum(q_lens), Hq, D]``, which may not overlap them; with ``return_lse`` also the log-sum-exp ``[sum(q_lens), Hq]`` f32 (-inf for a
         row without keys) that ``ops.finalize`` merges by."""
         for name, t, shape in (("q", q, self._q_shape), ("k", k, self._kv_shape), ("v", v, self._kv_shape)):
             if not self._fits(t, shape):
@@ -168,6 +168,7 @@ class SharedPrefixAttention:
             self._plan, self._parts = plan.to(self.device), int(plan[0])
             self._ws_bytes = int(lib.ia_shared_prefix_workspace_bytes(self._parts, ctypes.byref(self.geom)))
         self._call, self._index, self._q_shape = lib.ia_shared_prefix_decode, self.device.index, torch.Size(self._shape)
+        self._held = (kv.k_pool, kv.v_pool, kv.block_table, kv.seq_lens)  # kv's fields may be given other tensors
         self._args = (_ptr(kv.k_pool), _ptr(kv.v_pool), _ptr(kv.block_table), _ptr(kv.seq_lens), _ptr(shared_lens),
                       _ptr(self._plan), self._parts, ctypes.byref(self.geom))
 

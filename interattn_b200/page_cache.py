@@ -70,6 +70,7 @@ class PageCache:
             page_stride=k.stride(0), head_stride=k.stride(1), n_rows=int(block_table.shape[0]),
             max_pages=int(block_table.shape[1]), n_pages=int(k.shape[0]), n_pools=len(flat), n_kv_heads=int(k.shape[1]),
             head_dim=int(k.shape[3]), dtype=_DTYPES[k.dtype], reserved=0)
+        self._held = (flat, block_table, seq_lens, refs)  # the attributes may be given other tensors
         self._c, self._index = ctypes.byref(self._state), self.device.index
         self._lib = _lib.load()
         self._token_shape = (int(k.shape[1]), int(k.shape[3]))

@@ -100,7 +100,8 @@ def tensors(**kw):
     (dict(n_kv_heads=4), b"other heads"), (dict(head_dim=128), b"other heads"), (dict(dtype=_lib.IA_F32), b"other heads"),
     (dict(n_q_tokens=7), b"the plan has"), (dict(n_kv_tokens=9), b"the plan has"), (dict(q=None), b"null"), (dict(k=None), b"null"),
     (dict(out=8), b"aligned"), (dict(v=20), b"aligned"), (dict(q_tok_stride=33), b"strides"), (dict(k_head_stride=32), b"strides"),
-    (dict(v_tok_stride=130), b"strides")])
+    (dict(v_tok_stride=130), b"strides"), (dict(), b"overlap"), (dict(q=1 << 20, k=16 + 8 * 8 * 64 * 2 - 16, v=1 << 20), b"overlap"),
+    (dict(q=1 << 20, k=1 << 20, v=(1 << 20) - 7 * 256 - 2 * 64 * 2, out=(1 << 20) - 128), b"overlap")])
 def test_prompt_call_refusals(lib, change, word):
     plan = prompt_plan(lib, [4, 4], [4, 4], 2, 4, 64, _lib.IA_BF16)
     host = ints(plan[:8])

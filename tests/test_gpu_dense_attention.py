@@ -71,6 +71,15 @@ def test_prompt_strided_views(dtype, d):
     assert torch.equal(out, plan.run(heads_first, k, v))
 
 
+def test_prompt_output_may_not_overlap_what_is_read():
+    q, k, v, plan = prompt_case(2, 2, 64, BF16, [5, 9], [5, 9], seed=4)
+    for out in (q, k, v):
+        with pytest.raises(ValueError, match="overlap"):
+            plan.run(q, k, v, out=out)
+    both = torch.stack([q, q])
+    assert torch.equal(plan.run(both[0], k, v, out=both[1]), plan.run(q, k, v))
+
+
 @pytest.mark.parametrize("dtype,d,hq,hkv", [(BF16, 128, 8, 2), (BF16, 64, 2, 2), (F32, 64, 4, 2), (F32, 128, 2, 2)])
 @pytest.mark.parametrize("poison", [float("nan"), float("inf"), float("-inf"), 3.0e38])
 def test_prompt_rows_do_not_see_the_future_or_the_neighbour(dtype, d, hq, hkv, poison):
@@ -273,6 +282,19 @@ def test_shared_prefix_shorter_member_next_to_poison(dtype, d):
     want.out[[0, 2]], want.mean_abs[[0, 2]] = 0, 0
     out[[0, 2]] = 0
     want.check(out, dtype)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_shared_prefix_in_place_and_with_the_cache_s_fields_replaced(dtype):
+    groups, shared, lens = [3, 1], [64, 0], [70, 99, 64, 200]
+    q, kv, table = paged_case(8, 2, 64, dtype, groups, shared, lens, seed=33)
+    step = dense_attention.SharedPrefixAttention(kv, groups, i32(shared), 8)
+    want = step.step(q)
+    shape = kv.block_table.shape
+    kv.block_table, kv.seq_lens = None, None        # the step holds what it was given
+    other = torch.full(shape, 1 << 20, dtype=torch.int32, device="cuda")
+    assert step.step(q, out=q) is q and torch.equal(q, want)
+    assert ops.device_status() == 0 and other.shape == shape
 
 
 def test_shared_prefix_bad_entries_are_reported():
