@@ -9,8 +9,12 @@
 // through distributed shared memory).  Whatever moves data (the copies, the table rows of a fork, the remapped entries)
 // follows in a second launch on the whole GPU and reads what to do from the scratch that the first left.
 //
-// Measured: moving 1.14 GB of pages 182 us (0.97 of the copy peak), a plan over 18,400 pages 10 us, 64 forks of 8k tokens 19 us with
-// the free before them (the host's 18 us); the plan is a chain of dependent loads and barriers.
+// A warp looks at 128 consecutive counts at a time, so they are read once and in order, and pages are granted in two steps, free
+// page to rank and rank to list entry, so that they spread over all threads wherever in the pool they lie (with a run of pages
+// per thread, 256 rows' pages out of 65536 took 153 us instead of 17).
+//
+// Measured: moving 1.14 GB of pages 182 us (0.97 of the copy peak), a plan over 16,384 pages 9 us, 64 forks of 8k tokens 15 us with
+// the free before them; the plan is a chain of dependent loads and barriers.
 #include <algorithm>
 
 #include "dense_attention.cuh"
@@ -21,7 +25,11 @@ namespace {
 
 constexpr int kPage = 16;
 constexpr int kPlanCtas = 8, kPlanThreads = 1024;  // of the large plan; the small one is one CTA
-constexpr int kSmallList = 256, kSmallPool = 65536;
+// One CTA needs no cluster barrier, eight read the counts faster.  Handing out 4 pages to 4 / 256 rows and taking them back, one
+// CTA and eight, us: 1024 pages 8.0 / 12.1 and 14.0 / 16.2, 32768 pages 12.6 / 17.6 and 14.7 / 16.4, 65536 pages 17.2 / 21.7 and
+// 14.2 / 16.6, 262144 pages 46 / 50 and 19 / 20.  The compaction's plan with few pages to move: 4096 pages 6.1 and 8.7, 16384
+// pages 9.0 and 9.0, 32768 pages 12.7 and 8.8.  A list is short while a thread can hold its row against all before it.
+constexpr int kSmallList = 256, kSmallPool = 32768, kSmallCompact = 16384;
 constexpr int kMoveThreads = 256;
 
 // scratch: counters, then per entry of a list the inclusive sum of the pages wanted and what was granted, then the moves
@@ -112,18 +120,45 @@ template <int CTAS> __device__ Sums scan(int v, int* warp_sums, int* cta_sum) {
   return {before, total};
 }
 
-// how many of the pages [p0, p1) are free; four counts at a time where the array allows it
-__device__ __forceinline__ int count_free(const int* refs, int p0, int p1) {
-  int n = 0, g = p0;
-  if ((reinterpret_cast<uintptr_t>(refs + p0) & 15) == 0) {
-#pragma unroll 4
-    for (; g + 4 <= p1; g += 4) {
-      const int4 r = *reinterpret_cast<const int4*>(refs + g);
-      n += (r.x == 0) + (r.y == 0) + (r.z == 0) + (r.w == 0);
-    }
+// A warp takes a run of consecutive pages, 128 at a time, a lane four of them: run w of all is [p0, p1).
+struct Run { int p0, p1; };
+template <int CTAS> __device__ __forceinline__ Run run_of(int n_pages) {
+  constexpr int kWarps = CTAS * kPlanThreads / 32;
+  const int per = ((n_pages + kWarps - 1) / kWarps + 127) & ~127, w = cta_rank<CTAS>() * (kPlanThreads / 32) + (threadIdx.x >> 5);
+  const int64_t p0 = (int64_t)w * per;
+  return {(int)min((int64_t)n_pages, p0), (int)min((int64_t)n_pages, p0 + per)};
+}
+// bit c: page at + c is in use
+__device__ __forceinline__ int used_bits(const int* refs, int at, int end) {
+  if (at + 4 <= end && (reinterpret_cast<uintptr_t>(refs) & 15) == 0) {
+    const int4 r = *reinterpret_cast<const int4*>(refs + at);
+    return (r.x != 0) | (r.y != 0) << 1 | (r.z != 0) << 2 | (r.w != 0) << 3;
   }
-  for (; g < p1; ++g) n += refs[g] == 0;
+  int bits = 0;
+#pragma unroll
+  for (int c = 0; c < 4; ++c)
+    if (at + c < end && refs[at + c] != 0) bits |= 1 << c;
+  return bits;
+}
+// bit c: page at + c exists before `end`
+__device__ __forceinline__ int page_bits(int at, int end) { return (1 << max(0, min(4, end - at))) - 1; }
+__device__ __forceinline__ int count_used(const int* refs, Run run) {  // the lane's share
+  int n = 0;
+#pragma unroll 4
+  for (int g = run.p0 + (threadIdx.x & 31) * 4; g < run.p1; g += 128) n += __popc(used_bits(refs, g, run.p1));
   return n;
+}
+// of the lane's up to four bits: how many set bits lie before them in the warp, and how many there are
+__device__ __forceinline__ int2 rank_bits(int bits) {
+  const unsigned below = (1u << (threadIdx.x & 31)) - 1;
+  int2 r = {0, 0};
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    const unsigned m = __ballot_sync(0xffffffffu, bits >> c & 1);
+    r.x += __popc(m & below);
+    r.y += __popc(m);
+  }
+  return r;
 }
 
 // ---- who gets which page --------------------------------------------------------------------------------------------
@@ -139,7 +174,7 @@ struct PlanParams {
 template <int CTAS> __global__ void __launch_bounds__(kPlanThreads) pages_plan_kernel(const PlanParams p) {
   __shared__ int warp_sums[32];
   __shared__ int cta_sum;
-  __shared__ int named[CTAS == 1 ? kSmallList : 1];
+  __shared__ __align__(16) int named[CTAS == 1 ? kSmallList : 4];  // the rows, then the sums
   constexpr int kAll = CTAS * kPlanThreads;
   const State& st = p.st;
   const int me = cta_rank<CTAS>() * kPlanThreads + threadIdx.x;
@@ -147,16 +182,22 @@ template <int CTAS> __global__ void __launch_bounds__(kPlanThreads) pages_plan_k
   if constexpr (CTAS > 1) sync_all<CTAS>();  // the whole cluster runs before anyone reads a peer's shared memory
   grid_dependency_wait();
   if (p.fork) grid_launch_dependents();  // the copies follow; what follows an extend is not known here
-  // free pages; a thread counts a run of them
-  const int run = ((st.n_pages + kAll - 1) / kAll + 3) & ~3, p0 = min(st.n_pages, me * run), p1 = min(st.n_pages, p0 + run);
-  const int n_free = count_free(st.refs, p0, p1);
+  const Run run = run_of<CTAS>(st.n_pages);
+  int n_free = -count_used(st.refs, run);
+  if ((threadIdx.x & 31) == 0) n_free += run.p1 - run.p0;  // the lanes' sum is what counts
   // a row that the list names twice belongs to its first entry
   bool again = false;
   if constexpr (CTAS == 1) {
-    if (me < p.n) named[me] = p.rows[me];
+    if (me < kSmallList) named[me] = me < p.n ? p.rows[me] : 0;
     __syncthreads();
-    if (me < p.n)
-      for (int i = 0; i < me; ++i) again |= named[i] == named[me];
+    if (me < p.n) {
+      const int mine = named[me];
+#pragma unroll 4
+      for (int i = 0; i < (me | 31); i += 4) {
+        const int4 x = *reinterpret_cast<const int4*>(named + i);
+        again |= (i < me && x.x == mine) || (i + 1 < me && x.y == mine) || (i + 2 < me && x.z == mine) || (i + 3 < me && x.w == mine);
+      }
+    }
   } else {
     for (int i = i0; i < i1; ++i)
       if ((unsigned)p.rows[i] < (unsigned)st.n_rows) p.sc.owner[p.rows[i]] = 0x7fffffff;
@@ -202,6 +243,7 @@ template <int CTAS> __global__ void __launch_bounds__(kPlanThreads) pages_plan_k
     upto += need;
     const bool fits = upto <= free_pages.total;
     p.sc.upto[i] = upto;
+    if constexpr (CTAS == 1) named[i] = upto;
     if (!fits && p.sc.kept[i] >= 0) {
       p.sc.kept[i] = -1;
       report(st, IA_DEV_STATUS_NO_PAGES);
@@ -213,21 +255,38 @@ template <int CTAS> __global__ void __launch_bounds__(kPlanThreads) pages_plan_k
   // new lengths; all lengths were read before the barriers above
   for (int i = i0; i < i1; ++i)
     if (p.sc.kept[i] >= 0) st.lens[p.rows[i]] = p.sc.new_len[i];
-  // the free page of rank r goes to the entry whose sums enclose r
-  int rank = free_pages.before;
-  for (int g = p0; g < p1 && rank < grants.total; ++g) {
-    if (st.refs[g] != 0) continue;
-    int lo = 0, hi = p.n - 1;  // first entry with upto > rank
+  // the free page of rank r ...
+  int rank = __shfl_sync(0xffffffffu, free_pages.before, 0);
+  for (int g = run.p0; g < run.p1 && rank < grants.total; g += 128) {
+    const int at = g + (threadIdx.x & 31) * 4, bits = page_bits(at, run.p1) & ~used_bits(st.refs, at, run.p1);
+    const int2 r = rank_bits(bits);
+    int k = rank + r.x;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      if (!(bits >> c & 1)) continue;
+      if (k < grants.total) {
+        p.sc.moves[k].y = at + c;
+        st.refs[at + c] = 1;
+      }
+      ++k;
+    }
+    rank += r.y;
+  }
+  __threadfence();
+  sync_all<CTAS>();
+  // ... goes to the first entry whose sum is above r
+  for (int r = me; r < grants.total; r += kAll) {
+    const int page = __ldcg(&p.sc.moves[r].y);
+    int lo = 0, hi = p.n - 1;
     while (lo < hi) {
       const int mid = (lo + hi) >> 1;
-      if (__ldcg(p.sc.upto + mid) > rank) hi = mid;
+      if ((CTAS == 1 ? named[mid] : __ldcg(p.sc.upto + mid)) > r) hi = mid;
       else lo = mid + 1;
     }
-    const int before = lo > 0 ? __ldcg(p.sc.upto + lo - 1) : 0, at = __ldcg(p.sc.kept + lo) + rank - before;
-    st.table[(int64_t)p.rows[lo] * st.max_pages + at] = g;
-    st.refs[g] = 1;
-    if (p.fork) p.sc.moves[rank] = make_int2(st.table[(int64_t)p.other[lo] * st.max_pages + at], g);
-    ++rank;
+    const int before = lo > 0 ? (CTAS == 1 ? named[lo - 1] : __ldcg(p.sc.upto + lo - 1)) : 0;
+    const int at = __ldcg(p.sc.kept + lo) + r - before;
+    st.table[(int64_t)p.rows[lo] * st.max_pages + at] = page;
+    if (p.fork) p.sc.moves[r].x = st.table[(int64_t)p.other[lo] * st.max_pages + at];
   }
   if (me == 0) p.sc.n_moves[0] = p.fork ? grants.total : 0;
 }
@@ -237,29 +296,35 @@ struct CompactParams { State st; Scratch sc; };
 template <int CTAS> __global__ void __launch_bounds__(kPlanThreads) pages_compact_plan_kernel(const CompactParams p) {
   __shared__ int warp_sums[32];
   __shared__ int cta_sum;
-  constexpr int kAll = CTAS * kPlanThreads;
   const State& st = p.st;
   const Scratch& sc = p.sc;
   const int me = cta_rank<CTAS>() * kPlanThreads + threadIdx.x;
   if constexpr (CTAS > 1) sync_all<CTAS>();
   grid_dependency_wait();
   grid_launch_dependents();
-  const int run = ((st.n_pages + kAll - 1) / kAll + 3) & ~3, p0 = min(st.n_pages, me * run), p1 = min(st.n_pages, p0 + run);
-  const Sums all = scan<CTAS>(p1 - p0 - count_free(st.refs, p0, p1), warp_sums, &cta_sum);
+  const Run run = run_of<CTAS>(st.n_pages);
+  const Sums all = scan<CTAS>(count_used(st.refs, run), warp_sums, &cta_sum);
   const int n_live = all.total;
-  // live pages before n_live: the sum up to the boundary; holes below it and movers above it pair off by rank
-  int hole = p0 - all.before;
-  const int upto = max(p0, min(p1, n_live));
-  const Sums low = scan<CTAS>(upto - p0 - count_free(st.refs, p0, upto), warp_sums, &cta_sum);
-  int mover = all.before - min(all.before, low.total);
-  if (p0 < n_live && p1 > n_live) mover = 0;
-  for (int g = p0; g < p1; ++g) {
-    const bool is_live = st.refs[g] != 0;
-    if (g < n_live && !is_live) sc.moves[hole++].y = g;
-    if (g >= n_live && is_live) {
-      sc.remap[g] = mover;  // the move that takes this page
-      sc.moves[mover++].x = g;
+  // holes below n_live and movers at or past it pair off by rank
+  const Run low_run = {run.p0, max(run.p0, min(run.p1, n_live))};
+  const Sums low = scan<CTAS>(count_used(st.refs, low_run), warp_sums, &cta_sum);
+  const int live_before = __shfl_sync(0xffffffffu, all.before, 0), low_before = __shfl_sync(0xffffffffu, low.before, 0);
+  int hole = run.p0 - live_before, mover = live_before - low_before;
+  for (int g = run.p0; g < run.p1; g += 128) {
+    const int at = g + (threadIdx.x & 31) * 4, used = used_bits(st.refs, at, run.p1);
+    const int below = page_bits(at, min(run.p1, n_live)), holes = below & ~used, movers = used & ~below;
+    const int2 h = rank_bits(holes), m = rank_bits(movers);
+    int to = hole + h.x, from = mover + m.x;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      if (holes >> c & 1) sc.moves[to++].y = at + c;
+      if (movers >> c & 1) {
+        sc.remap[at + c] = from;  // the move that takes this page
+        sc.moves[from++].x = at + c;
+      }
     }
+    hole += h.y;
+    mover += m.y;
   }
   if (me == 0) {
     sc.n_moves[0] = n_live - low.total;
@@ -517,7 +582,7 @@ int launch_pages_compact(const ia_page_cache& c, cudaStream_t stream) {
   if (int s = state_of(c, &st)) return s;
   const Scratch sc = scratch_of(c);
   const CompactParams p{st, sc};
-  const int s = c.n_pages <= kSmallPool
+  const int s = c.n_pages <= kSmallCompact
                     ? launch(pages_compact_plan_kernel<1>, 1u, (unsigned)kPlanThreads, stream, "pages_compact_plan_kernel", p)
                     : launch(pages_compact_plan_kernel<kPlanCtas>, (unsigned)kPlanCtas, (unsigned)kPlanThreads, stream,
                              "pages_compact_plan_kernel", p, kPlanCtas);

@@ -95,6 +95,40 @@ def test_random_calls(seed):
     assert bool(status & _lib.IA_DEV_STATUS_BAD_INDEX) == model.bad and bool(status & _lib.IA_DEV_STATUS_NO_PAGES) == model.full
 
 
+@pytest.mark.parametrize("aligned", [True, False])
+@pytest.mark.parametrize("n_pages,n_rows", [(1, 3), (127, 5), (129, 256), (4099, 257), (16384, 30), (16385, 30), (32768, 256), (32769, 7),
+                                            (70001, 40)])
+def test_pools_and_lists_around_the_plans_sizes(n_pages, n_rows, aligned):
+    """Free pages scattered over the whole pool, also where the counts begin between 16-byte boundaries."""
+    rng = random.Random(n_pages + n_rows)
+    max_pages = max(1, 2 * n_pages // n_rows)
+    pool = torch.arange(n_pages, device="cuda", dtype=torch.float32).view(-1, 1, 1, 1).expand(n_pages, 1, PAGE, 64).contiguous()
+    refs = torch.zeros((n_pages + 1,), dtype=torch.int32, device="cuda")[0 if aligned else 1:][:n_pages]
+    cache = page_cache.PageCache([(pool, pool.clone())], torch.full((n_rows, max_pages), -1, dtype=torch.int32, device="cuda"),
+                                 i32([0] * n_rows), refs)
+    model = PagesModel(n_pages, n_rows, max_pages)
+    rows = list(range(n_rows))
+    for _ in range(2):
+        counts = [rng.randint(0, max(1, n_pages // n_rows) * 14) for _ in rows]
+        counts = [min(c, max_pages * PAGE - n) for c, n in zip(counts, model.lens)]
+        cache.extend(i32(rows), i32(counts)), model.extend(rows, counts)
+        gone = rng.sample(rows, n_rows // 2)
+        cache.free(i32(gone)), model.free(gone)
+        same(cache, model)
+    parents = [rng.choice([r for r in rows if r not in gone]) for _ in gone]
+    share = n_rows % 2 == 0
+    cache.fork(i32(parents), i32(gone), share=share), model.fork(parents, gone, share)
+    same(cache, model)
+    gone = rng.sample(rows, n_rows // 3)
+    cache.free(i32(gone)), model.free(gone)
+    cache.compact(), model.compact()
+    same(cache, model)
+    live = [p for p, r in enumerate(model.refs) if r]
+    want = torch.tensor(model.contents, device="cuda")[live].float()
+    assert all(torch.equal(x[live, 0, 0, 0], want) and torch.equal(x[live, 0, 15, 63], want) for x in cache.pools[0])
+    assert bool(ops.device_status() & _lib.IA_DEV_STATUS_NO_PAGES) == model.full and not model.bad
+
+
 def test_refused_entries_change_nothing():
     cache, model, pools = make(20, 6, 8)
     cache.extend(i32([0, 1]), i32([20, 40])), model.extend([0, 1], [20, 40])
