@@ -118,7 +118,7 @@ class PromptAttention:
             if not self._fits(t, shape):
                 self._refuse(name, t, shape)
         if out is None:
-            out = torch.empty(self._q_shape, dtype=self.dtype, device=self.device)
+            out = q.new_empty(self._q_shape)
         elif not self._fits(out, self._q_shape):
             self._refuse("out", out, self._q_shape)
         elif not out.is_contiguous():

@@ -73,7 +73,8 @@ class PageCache:
         self._held = (flat, block_table, seq_lens, refs)  # the attributes may be given other tensors
         self._c, self._index = ctypes.byref(self._state), self.device.index
         self._lib = _lib.load()
-        self._token_shape = (int(k.shape[1]), int(k.shape[3]))
+        self._token_shape, self._dtype = (int(k.shape[1]), int(k.shape[3])), k.dtype
+        self._pool_addresses = [(a.data_ptr(), b.data_ptr()) for a, b in self.pools]
 
     @staticmethod
     def empty(n_layers: int, n_pages: int, n_kv_heads: int, head_dim: int, n_rows: int, max_pages: int, *,
@@ -112,19 +113,19 @@ class PageCache:
     def write(self, layer: int, rows: torch.Tensor, starts: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> None:
         """Tokens ``[starts[i], starts[i + 1])`` of k and v ``[T, Hkv, D]`` (token and head strides of any multiple of 16 bytes)
         become the last tokens of ``rows[i]`` in this layer."""
-        k_pool, v_pool = self.pools[layer]
-        if k.shape != v.shape:
+        shape, ks, vs = k.shape, k.stride(), v.stride()
+        if shape != v.shape:
             raise ValueError("k and v hold the same tokens")
-        for name, t in (("k", k), ("v", v)):
-            if t.dim() != 3 or t.shape[1:] != self._token_shape or t.dtype is not k_pool.dtype or t.stride(2) != 1 \
-                    or t.get_device() != self._index:
+        if len(shape) != 3 or (shape[1], shape[2]) != self._token_shape or ks[2] != 1 or vs[2] != 1 \
+                or k.dtype is not self._dtype or v.dtype is not self._dtype or k.get_device() != self._index \
+                or v.get_device() != self._index:
+            for name, t in (("k", k), ("v", v)):
                 _need_cuda(t)
                 _same_device(self.device, **{name: t})
-                raise ValueError(f"{name} must be a [T, Hkv, D] tensor of the pools' dtype with contiguous heads")
+            raise ValueError("k and v must be [T, Hkv, D] tensors of the pools' dtype with contiguous heads")
         n = rows.numel()
-        (kt, kh, _), (vt, vh, _) = k.stride(), v.stride()
         self._call(self._lib.ia_pages_write, self._list("rows", rows), self._list("starts", starts, n + 1), n, k.data_ptr(),
-                   v.data_ptr(), kt, kh, vt, vh, k.shape[0], k_pool.data_ptr(), v_pool.data_ptr())
+                   v.data_ptr(), ks[0], ks[1], vs[0], vs[1], shape[0], *self._pool_addresses[layer])
 
     def fork(self, parents: torch.Tensor, children: torch.Tensor, *, share: bool = True) -> None:
         """``children[i]``, an empty row, becomes a copy of ``parents[i]`` as it was before the call.  With ``share`` the two
