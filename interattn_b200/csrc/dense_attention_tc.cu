@@ -46,7 +46,7 @@ template <int D> struct Tc {
   static constexpr int kv_block = kKeys * 128, kv_tile = halves * kv_block;
   static constexpr int stages = D == 128 ? 4 : 8;      // ring of K and V tiles
   static constexpr int out_warp = 4096;                 // a warp's 32 rows of 128 bytes on their way out
-  static constexpr size_t ring = 2 * (size_t)tile, tiles = ring + (size_t)stages * kv_tile, control = tiles + 8 * out_warp, smem = control + 3072;
+  static constexpr size_t ring = 2 * (size_t)tile, tiles = ring + (size_t)stages * kv_tile, control = tiles + 8 * out_warp, smem = control + 3 * 1024;
 };
 
 // The key tiles of a piece and who takes them.  Split: one row tile, key tile j goes to set (first + j) % 2 of softmax warps.
@@ -261,6 +261,11 @@ __device__ __forceinline__ void unpair(uint64_t v, float& lo, float& hi) { asm("
 __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
   uint64_t d;
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
   return d;
 }
 __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
@@ -812,49 +817,64 @@ __device__ __forceinline__ void softmax_role(const TcParams& p, Bars* bars, cons
     const int col0 = merge ? w * (D / 2) : 0, col1 = merge ? col0 + D / 2 : D;
     unsigned char* rows = out_base + warp * Tc<D>::out_warp;  // [32 rows][32 columns], 16-byte words swizzled
     constexpr int kWords = 32 * sizeof(Out) / 16;             // words of a row: 8 or 4
-    bool finite = true;
+    uint64_t not_finite[2] = {0, 0};  // sums of zero times what is written
     if (busy) {
+      int to[kWords];  // kWords neighbouring lanes write a row's run
+#pragma unroll
+      for (int i = 0; i < kWords; ++i) {
+        to[i] = __shfl_sync(0xffffffffu, at, i * (32 / kWords) + lane / kWords);
+        if (to[i] >= 0) to[i] += lane % kWords * (16 / (int)sizeof(Out));
+      }
+      const bool any_empty = __any_sync(0xffffffffu, empty);
+      const uint64_t scale2 = pair(scale, scale), its2 = pair(its_scale, its_scale);
 #pragma unroll 1
       for (int col = col0; col < col1; col += 32) {
-        float x[32];
+        uint64_t x[16];
         {
           uint32_t o[32];
           tmem_ld(o_addr + w * 128 + col, o);
           tmem_wait_ld(o);
 #pragma unroll
-          for (int k = 0; k < 32; ++k) x[k] = empty ? 0.f : __uint_as_float(o[k]) * scale;
+          for (int k = 0; k < 16; ++k) x[k] = mul2(pair(__uint_as_float(o[2 * k]), __uint_as_float(o[2 * k + 1])), scale2);
           if (merge) {
             tmem_ld(o_addr + (w ^ 1) * 128 + col, o);
             tmem_wait_ld(o);
 #pragma unroll
-            for (int k = 0; k < 32; ++k) x[k] = empty ? 0.f : fmaf(__uint_as_float(o[k]), its_scale, x[k]);
+            for (int k = 0; k < 16; ++k) x[k] = fma2(pair(__uint_as_float(o[2 * k]), __uint_as_float(o[2 * k + 1])), its2, x[k]);
           }
         }
+        if (any_empty) {
 #pragma unroll
-        for (int k = 0; k < 32; ++k) finite &= fabsf(x[k]) <= 3.4028235e38f;
+          for (int k = 0; k < 16; ++k) x[k] = empty ? 0 : x[k];
+        }
+#pragma unroll
+        for (int k = 0; k < 16; ++k) not_finite[k & 1] = fma2(x[k], 0, not_finite[k & 1]);
 #pragma unroll
         for (int k = 0; k < kWords; ++k) {
-          uint4 v;
-          if constexpr (PAGED)
-            v = make_uint4(__float_as_uint(x[4 * k]), __float_as_uint(x[4 * k + 1]), __float_as_uint(x[4 * k + 2]), __float_as_uint(x[4 * k + 3]));
-          else
-            v = make_uint4(pack_bf16(x[8 * k], x[8 * k + 1]), pack_bf16(x[8 * k + 2], x[8 * k + 3]), pack_bf16(x[8 * k + 4], x[8 * k + 5]),
-                           pack_bf16(x[8 * k + 6], x[8 * k + 7]));
-          *reinterpret_cast<uint4*>(rows + lane * 128 + ((k ^ (lane & 7)) << 4)) = v;
+          uint32_t v[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            float lo, hi;
+            if constexpr (PAGED) {
+              unpair(x[2 * k + i / 2], lo, hi);
+              v[i] = __float_as_uint(i & 1 ? hi : lo);
+            } else {
+              unpair(x[4 * k + i], lo, hi);
+              v[i] = pack_bf16(lo, hi);
+            }
+          }
+          *reinterpret_cast<uint4*>(rows + lane * 128 + ((k ^ (lane & 7)) << 4)) = make_uint4(v[0], v[1], v[2], v[3]);
         }
         __syncwarp();
-        // kWords neighbouring lanes write a row's run; all reads before the first write
-        uint4 v[kWords];
-        int to[kWords];
+        uint4 v[kWords];  // all reads before the first write
 #pragma unroll
         for (int i = 0; i < kWords; ++i) {
           const int r = i * (32 / kWords) + lane / kWords, k = lane % kWords;
-          to[i] = __shfl_sync(0xffffffffu, at, r);
           v[i] = *reinterpret_cast<const uint4*>(rows + r * 128 + ((k ^ (r & 7)) << 4));
         }
 #pragma unroll
         for (int i = 0; i < kWords; ++i)
-          if (to[i] >= 0) *reinterpret_cast<uint4*>(out + to[i] + col + lane % kWords * (16 / (int)sizeof(Out))) = v[i];
+          if (to[i] >= 0) *reinterpret_cast<uint4*>(out + to[i] + col) = v[i];
         __syncwarp();
       }
       if (valid && lse_out != nullptr && (!merge || me == 0)) *lse_out = lse;
@@ -866,7 +886,9 @@ __device__ __forceinline__ void softmax_role(const TcParams& p, Bars* bars, cons
       if (!wait(&bars->read, x_it & 1)) return;
       ++x_it;
     }
-    const unsigned bad = __ballot_sync(0xffffffffu, valid && !finite);
+    float nan_lo, nan_hi;
+    unpair(add2(not_finite[0], not_finite[1]), nan_lo, nan_hi);
+    const unsigned bad = __ballot_sync(0xffffffffu, valid && !(nan_lo + nan_hi == 0.f));
     if (bad != 0) {  // see exact_row
       using T = __nv_bfloat16;
       const auto redo = [&](const auto& key, const T* q, int64_t tok_stride, int64_t head_stride) {
@@ -911,7 +933,7 @@ template <int D, bool PAGED>
 __global__ void __launch_bounds__(kThreads, 1) attend_tc_kernel(const __grid_constant__ TcParams p) {
   using C = Tc<D>;
   extern __shared__ __align__(1024) unsigned char base[];
-  static_assert(sizeof(Control) <= 3072, "the whole of an SM's shared memory is spoken for");
+  static_assert(sizeof(Control) <= 3 * 1024, "the whole of an SM's shared memory is spoken for");
   Control& ctl = *reinterpret_cast<Control*>(base + C::control);
   Bars& bars = ctl.bars;
   const int warp = threadIdx.x >> 5;
