@@ -542,8 +542,11 @@ typedef struct ia_prompt_tensors {
                             16 bytes, head_dim elements contiguous */
   int32_t n_q_tokens, n_kv_tokens, n_kv_heads, group_size, head_dim, dtype;
 } ia_prompt_tensors;
-/* plan_host: the first 8 words of the plan (host memory); plan_device: all of it. */
-int ia_prompt_attention(const ia_prompt_tensors* tensors, const int32_t* plan_host, const int32_t* plan_device,
+/* plan_host: the first 8 words of the plan (host memory); plan_device: all of it.  workspace: 16-byte aligned,
+ * ia_prompt_workspace_bytes() of it (0: the plan cuts no keys, and null will do); calls that overlap on the GPU need their own. */
+int64_t ia_prompt_workspace_bytes(const int32_t* plan_host);
+int ia_prompt_attention(const ia_prompt_tensors* tensors, const int32_t* plan_host, const int32_t* plan_device, void* workspace,
+                        int64_t workspace_bytes,
                         ia_stream_t stream);
 
 /* One decode step in which consecutive sequences form groups whose first tokens lie in the same pages: those are read

@@ -145,7 +145,8 @@ SIGNATURES = {
     "ia_llama_argmax_parts": (c_int, [c_void_p, c_int, c_void_p, c_int, c_int, c_void_p, c_void_p]),
     "ia_prompt_plan_ints": (c_int64, [c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int]),
     "ia_prompt_plan": (c_int, [c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p, c_int64]),
-    "ia_prompt_attention": (c_int, [c_char_p, c_void_p, c_void_p, c_void_p]),   # the bytes of a PromptTensors
+    "ia_prompt_workspace_bytes": (c_int64, [c_void_p]),
+    "ia_prompt_attention": (c_int, [c_char_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p]),   # the bytes of a PromptTensors
     "ia_shared_prefix_plan_ints": (c_int64, [c_void_p, c_int, POINTER(Geom)]),
     "ia_shared_prefix_plan": (c_int, [c_void_p, c_int, POINTER(Geom), c_void_p, c_int64]),
     "ia_shared_prefix_workspace_bytes": (c_int64, [c_int, POINTER(Geom)]),

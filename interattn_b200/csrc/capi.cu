@@ -684,7 +684,16 @@ static bool prompt_out_overlaps(const ia_prompt_tensors& t, int size) {
          meets(t.v, t.n_kv_tokens, t.n_kv_heads, t.v_tok_stride, t.v_head_stride);
 }
 
-int ia_prompt_attention(const ia_prompt_tensors* t, const int32_t* plan_host, const int32_t* plan_device, ia_stream_t stream) {
+int64_t ia_prompt_workspace_bytes(const int32_t* plan_host) {
+  if (!plan_host) {
+    fail(IA_ERR_BAD_ARG, "prompt_workspace_bytes: null argument");
+    return -1;
+  }
+  return plan_host[2] < 2 ? 0 : (int64_t)plan_host[0] * kPartRows * (plan_host[4] % 1000 + 1) * 4;
+}
+
+int ia_prompt_attention(const ia_prompt_tensors* t, const int32_t* plan_host, const int32_t* plan_device, void* workspace,
+                        int64_t workspace_bytes, ia_stream_t stream) {
   if (!t || !plan_host || !plan_device) return fail(IA_ERR_BAD_ARG, "prompt_attention: null argument");
   if (plan_host[4] != t->group_size * 1000 + t->head_dim || plan_host[5] != t->n_kv_heads * 16 + t->dtype)
     return fail(IA_ERR_BAD_ARG, "prompt_attention: the plan was made for other heads or another dtype");
@@ -702,11 +711,22 @@ int ia_prompt_attention(const ia_prompt_tensors* t, const int32_t* plan_host, co
                               !strides_ok(t->v_tok_stride, t->v_head_stride, t->head_dim, size))))
     return fail(IA_ERR_BAD_ARG, "prompt_attention: token and head strides are multiples of 16 bytes and hold a head");
   if (prompt_out_overlaps(*t, size)) return fail(IA_ERR_BAD_ARG, "prompt_attention: the output may not overlap q, k or v");
+  const int64_t need = ia_prompt_workspace_bytes(plan_host);
+  if (need > 0 && (!workspace || !aligned16(workspace) || workspace_bytes < need))
+    return fail(IA_ERR_BAD_ARG, "prompt_attention: workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)need);
+  const bool parts = plan_host[2] >= 2;
+  float* part_o = parts ? static_cast<float*>(workspace) : nullptr;
+  float* part_lse = parts ? part_o + (int64_t)plan_host[0] * kPartRows * t->head_dim : nullptr;
   const PromptTensors p{t->q, t->k, t->v, t->out, t->lse, t->q_tok_stride, t->q_head_stride, t->k_tok_stride, t->k_head_stride,
-                        t->v_tok_stride, t->v_head_stride, t->n_q_tokens, t->n_kv_tokens, t->n_kv_heads, t->group_size};
+                        t->v_tok_stride, t->v_head_stride, t->n_q_tokens, t->n_kv_tokens, t->n_kv_heads, t->group_size,
+                        part_o, part_lse};
   const PromptItem* items = reinterpret_cast<const PromptItem*>(plan_device + plan_host[3]);
-  if (t->dtype == IA_BF16) return launch_prompt_tc(p, t->head_dim, items, plan_device + 8, plan_host[1], (cudaStream_t)stream);
-  return launch_prompt_f32(p, t->head_dim, items, plan_host[0], plan_host[2] != 0, (cudaStream_t)stream);
+  const int s = t->dtype == IA_BF16
+                    ? launch_prompt_tc(p, t->head_dim, items, plan_device + 8, plan_host[1], (cudaStream_t)stream)
+                    : launch_prompt_f32(p, t->head_dim, items, plan_host[0], plan_host[2] != 0, (cudaStream_t)stream);
+  if (s || !parts) return s;
+  return launch_prompt_merge(p, t->head_dim, t->dtype, reinterpret_cast<const PromptPiece*>(items + plan_host[0]), plan_host[2] - 2,
+                             (cudaStream_t)stream);
 }
 
 static int check_groups(const int32_t* group_sizes, int n_groups, const ia_geom* g) {

@@ -377,8 +377,10 @@ __global__ void __launch_bounds__(kThreads) prompt_attention_kernel(const Prompt
   const float* q = (const float*)t.q + it.q_tok * t.q_tok_stride + (int64_t)it.head * G * t.q_head_stride;
   const auto q_row = [&](int r) { return q + r / G * t.q_tok_stride + r % G * t.q_head_stride; };
   const auto limit = [&](int r) { return max(0, min(it.limit0 + r / G, it.kv_len)); };
-  const RowSink sink{(float*)t.out + ((int64_t)it.q_tok * hq + it.head * G) * D,
-                     t.lse == nullptr ? nullptr : t.lse + (int64_t)it.q_tok * hq + it.head * G, (int64_t)hq * D, D, hq, G};
+  const RowSink whole{(float*)t.out + ((int64_t)it.q_tok * hq + it.head * G) * D,
+                      t.lse == nullptr ? nullptr : t.lse + (int64_t)it.q_tok * hq + it.head * G, (int64_t)hq * D, D, hq, G};
+  const int64_t row0 = (int64_t)it.slot * kPartRows;
+  const RowSink sink = t.part_o == nullptr ? whole : RowSink{t.part_o + row0 * D, t.part_lse + row0, (int64_t)G * D, D, G, G};
   attend<D, RPT>(sm, it.n_tok * G, 0, limit(it.n_tok * G - 1), kLog2e * rsqrtf((float)D), key, q_row, limit, sink);
 }
 
@@ -432,9 +434,63 @@ __global__ void __launch_bounds__(kThreads) shared_attention_kernel(const Shared
   }
 }
 
-// out[row] = sum_s o_s 2^(lse_s - M) / sum_s 2^(lse_s - M) over the segments of the row's shared and own item, a warp per
-// query row.  Lane i fetches the i-th log-sum-exp, so the weights are there before the first partial row, whose loads
-// then do not depend on one another.
+// out[row] = sum_s o_s 2^(lse_s - M) / sum_s 2^(lse_s - M) over partial rows, a warp per output row.  Lane i fetches the i-th
+// log-sum-exp, so the weights are there before the first partial row, whose loads then do not depend on one another.
+template <int D> struct Merged {
+  float acc[D / 32], M = -INFINITY, L = 0.f;
+  __device__ __forceinline__ Merged() {
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) acc[i] = 0.f;
+  }
+  // `count` more, lane i's in row `row`
+  __device__ __forceinline__ void add(const float* o, const float* lses, int64_t row, int count) {
+    const int lane = threadIdx.x & 31;
+    const float lse = lane < count ? __ldcg(lses + row) * kLog2e : -INFINITY;
+    const float* src = o + row * D;
+    const float m = fmaxf(M, warp_max(lse)), base = m == -INFINITY ? 0.f : m;
+    const float keep = exp2f(M - base), w = exp2f(lse - base);  // a part without a visible key: weight 0, o is 0
+    L = L * keep + warp_sum(w);
+    M = m;
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) acc[i] *= keep;
+#pragma unroll 8
+    for (int s = 0; s < count; ++s) {
+      const float ws = __shfl_sync(0xffffffffu, w, s);
+      const float* from = (const float*)__shfl_sync(0xffffffffu, (unsigned long long)src, s) + lane * (D / 32);
+      if constexpr (D == 128) {
+        const float4 x = __ldcg(reinterpret_cast<const float4*>(from));
+        acc[0] += ws * x.x; acc[1] += ws * x.y; acc[2] += ws * x.z; acc[3] += ws * x.w;
+      } else {
+        const float2 x = __ldcg(reinterpret_cast<const float2*>(from));
+        acc[0] += ws * x.x; acc[1] += ws * x.y;
+      }
+    }
+  }
+  template <typename T> __device__ __forceinline__ void store(T* to) {
+    const float inv = L == 0.f ? 0.f : 1.f / L;  // no keys: zeros
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) acc[i] *= inv;
+    store_vec<D / 32>(to + (threadIdx.x & 31) * (D / 32), acc);
+  }
+};
+
+template <typename T, int D>
+__global__ void __launch_bounds__(256) prompt_merge_kernel(const PromptTensors t, const PromptPiece* pieces, int blocks) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = blockIdx.x % blocks * 8 + warp;
+  const PromptPiece piece = pieces[blockIdx.x / blocks];
+  grid_dependency_wait();
+  grid_launch_dependents();
+  const int G = t.group, hq = t.n_kv_heads * G;
+  if (r >= piece.n_tok * G) return;
+  Merged<D> merged;
+  for (int s = 0; s < piece.parts; s += 32)
+    merged.add(t.part_o, t.part_lse, (int64_t)(piece.slot + s + lane) * kPartRows + r, min(32, piece.parts - s));
+  const int64_t row = (int64_t)(piece.q_tok + r / G) * hq + piece.head * G + r % G;
+  if (t.lse != nullptr && lane == 0) t.lse[row] = merged.L == 0.f ? -INFINITY : (merged.M + log2f(merged.L)) * kLn2;
+  merged.store((T*)t.out + row * D);
+}
+
+// The segments of a row's shared and own item.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) shared_merge_kernel(const SharedParams p, const int2* seq_info, int ctas, T* out) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -460,39 +516,15 @@ __global__ void __launch_bounds__(256) shared_merge_kernel(const SharedParams p,
   const SharedEntity ent = load_entity(p, info.x);
   const int at[2] = {info.y * G + g, g};  // the row in its item
   const int64_t first[2] = {item_rows(p, false, ent.first_seq, ent.n_seqs, h) + at[0], item_rows(p, true, seq, 1, h) + at[1]};
-  float acc[D / 32], M = -INFINITY, L = 0.f;
-#pragma unroll
-  for (int i = 0; i < D / 32; ++i) acc[i] = 0.f;
+  Merged<D> merged;
   for (int s0 = 0; s0 < n[0] + n[1]; s0 += 32) {
-    const int mine = s0 + lane, count = min(32, n[0] + n[1] - s0);
+    const int mine = s0 + lane;
     const bool own = mine >= n[0];
     const int segment = own ? mine - n[0] : mine;
     const int64_t row = segment == 0 ? first[own] : cta_rows(p, c0[own] + segment) + at[own];
-    const float lse = lane < count ? __ldcg(p.lse + row) * kLog2e : -INFINITY;
-    const float* src = p.o + row * D;
-    const float m = fmaxf(M, warp_max(lse)), base = m == -INFINITY ? 0.f : m;
-    const float keep = exp2f(M - base), w = exp2f(lse - base);  // a segment without a visible key: weight 0, o is 0
-    L = L * keep + warp_sum(w);
-    M = m;
-#pragma unroll
-    for (int i = 0; i < D / 32; ++i) acc[i] *= keep;
-#pragma unroll 8
-    for (int s = 0; s < count; ++s) {
-      const float ws = __shfl_sync(0xffffffffu, w, s);
-      const float* from = (const float*)__shfl_sync(0xffffffffu, (unsigned long long)src, s) + lane * (D / 32);
-      if constexpr (D == 128) {
-        const float4 x = __ldcg(reinterpret_cast<const float4*>(from));
-        acc[0] += ws * x.x; acc[1] += ws * x.y; acc[2] += ws * x.z; acc[3] += ws * x.w;
-      } else {
-        const float2 x = __ldcg(reinterpret_cast<const float2*>(from));
-        acc[0] += ws * x.x; acc[1] += ws * x.y;
-      }
-    }
+    merged.add(p.o, p.lse, row, min(32, n[0] + n[1] - s0));
   }
-  const float inv = n[0] + n[1] == 0 || M == -INFINITY ? 0.f : 1.f / L;  // a sequence without keys: zeros
-#pragma unroll
-  for (int i = 0; i < D / 32; ++i) acc[i] *= inv;
-  store_vec<D / 32>(out + ((int64_t)seq * hq + head) * D + lane * (D / 32), acc);
+  merged.store(out + ((int64_t)seq * hq + head) * D);
 }
 
 template <typename... Args, typename... Given>
@@ -524,6 +556,11 @@ template <int D> int launch_shared(const SharedParams& p, int ctas, cudaStream_t
   constexpr size_t bytes = std::max(Smem<D, 8>::bytes, (size_t)kWarps * kFewRing * 4);
   if (int s = once.allow((const void*)kern, bytes, "shared_attention_kernel")) return s;
   return launch(kern, (unsigned)ctas, bytes, stream, "shared_attention_kernel", p);
+}
+template <typename T, int D>
+int launch_parts(const PromptTensors& t, const PromptPiece* pieces, int n_pieces, cudaStream_t stream) {
+  constexpr int rows = std::is_same_v<T, float> ? 32 : kPartRows, blocks = rows / 8;  // rows of a small piece
+  return launch(prompt_merge_kernel<T, D>, (unsigned)(n_pieces * blocks), 0, stream, "prompt_merge_kernel", t, pieces, blocks);
 }
 template <typename T, int D>
 int launch_merge(const SharedParams& p, const int2* seq_info, int ctas, T* out, cudaStream_t stream) {
@@ -561,6 +598,12 @@ int launch_prompt_f32(const PromptTensors& t, int head_dim, const PromptItem* it
   return few_rows ? launch_prompt<64, 2>(t, items, n_items, stream) : launch_prompt<64, 8>(t, items, n_items, stream);
 }
 
+int launch_prompt_merge(const PromptTensors& t, int head_dim, int dtype, const PromptPiece* pieces, int n_pieces, cudaStream_t stream) {
+  if (dtype == IA_F32) return head_dim == 128 ? launch_parts<float, 128>(t, pieces, n_pieces, stream) : launch_parts<float, 64>(t, pieces, n_pieces, stream);
+  return head_dim == 128 ? launch_parts<__nv_bfloat16, 128>(t, pieces, n_pieces, stream)
+                         : launch_parts<__nv_bfloat16, 64>(t, pieces, n_pieces, stream);
+}
+
 int launch_shared_f32(const SharedParams& p, int head_dim, int ctas, cudaStream_t stream) {
   return head_dim == 128 ? launch_shared<128>(p, ctas, stream) : launch_shared<64>(p, ctas, stream);
 }
@@ -576,13 +619,16 @@ int launch_shared_merge(const SharedParams& p, const int32_t* seq_info, int head
 }
 
 // ---- the prompt's plan ----------------------------------------------------------------------------------------------
-// Words: a header of 8, where each CTA's items begin (ctas + 1 words, padded to whole items), the items.
+// Words: a header of 8, where each CTA's items begin (ctas + 1 words, padded to whole items), the items, and the pieces where
+// they are cut.
 namespace {
 constexpr int kRowsFew = 32, kRowsFull = 128;
 struct PlanShape {
   int n_items, ctas, item_tokens;
   bool few_rows;
-  int64_t ints() const { return 8 + (int64_t)(ctas + 1 + 7) / 8 * 8 + (int64_t)n_items * 8; }
+  int chunk = 0, n_pieces = 0;  // keys of a part, 0: not cut
+  int64_t first() const { return 8 + (int64_t)(ctas + 1 + 7) / 8 * 8; }
+  int64_t ints() const { return first() + ((int64_t)n_items + n_pieces) * 8; }
 };
 struct PlanInput {
   const int32_t *q_lens, *kv_lens;
@@ -598,7 +644,7 @@ std::vector<PromptItem> make_pieces(const PlanInput& in, const PlanShape& s, int
     for (int t = 0; t < in.q_lens[i]; t += s.item_tokens)
       for (int h = 0; h < in.n_kv_heads; ++h)
         items.push_back(PromptItem{(int)(q0 + t), std::min(s.item_tokens, in.q_lens[i] - t), (int)k0,
-                                   in.kv_lens[i] - in.q_lens[i] + t + 1, in.kv_lens[i], h, {0, 0}});
+                                   in.kv_lens[i] - in.q_lens[i] + t + 1, in.kv_lens[i], h, 0, 0});
     q0 += in.q_lens[i];
     k0 += in.kv_lens[i];
   }
@@ -607,6 +653,21 @@ std::vector<PromptItem> make_pieces(const PlanInput& in, const PlanShape& s, int
   *n_q = q0;
   *n_kv = k0;
   return items;
+}
+// The parts of the pieces, the longest first, and which piece they make up.
+std::vector<PromptItem> cut_pieces(const std::vector<PromptItem>& whole, int chunk, std::vector<PromptPiece>* pieces) {
+  std::vector<PromptItem> parts;
+  for (const PromptItem& it : whole) {
+    const int n = std::max(1, (piece_keys(it) + chunk - 1) / chunk);
+    if (pieces) pieces->push_back(PromptPiece{it.q_tok, it.n_tok, it.head, (int)parts.size(), n, {0, 0, 0}});
+    for (int i = 0; i < n; ++i) {
+      const int lo = i * chunk;
+      parts.push_back(PromptItem{it.q_tok, it.n_tok, it.kv_tok + lo, it.limit0 - lo, std::min(it.kv_len - lo, chunk), it.head, (int)parts.size(), 0});
+    }
+  }
+  std::stable_sort(parts.begin(), parts.end(),
+                   [](const PromptItem& a, const PromptItem& b) { return piece_keys(a) > piece_keys(b); });
+  return parts;
 }
 // What a piece costs, in quarters of what a key costs a large piece.  Starting and ending one takes as long as 256 keys
 // (tensor cores; a small one 192) or 32 (fp32; 16); a key of a small piece, half or a quarter of the rows, 1 / 2 or 3 / 8.
@@ -653,11 +714,37 @@ bool plan_shape(const PlanInput& in, PlanShape* s) {
   bool fits, fits_few;
   *s = shape_of(in, false, &fits);
   if (!fits || s->n_items >= 4 * sm_count()) return fits;
-  const PlanShape few = shape_of(in, true, &fits_few);
+  PlanShape few = shape_of(in, true, &fits_few);
   int64_t q, kv;
-  if (spread(make_pieces(in, few, &q, &kv), sm_count(), in.dtype, true, nullptr) <
-      spread(make_pieces(in, *s, &q, &kv), sm_count(), in.dtype, false, nullptr))
+  const std::vector<PromptItem> small = make_pieces(in, few, &q, &kv);
+  const int sms = sm_count();
+  const int64_t few_cost = spread(small, sms, in.dtype, true, nullptr);
+  int64_t best = spread(make_pieces(in, *s, &q, &kv), sms, in.dtype, false, nullptr);
+  if (few_cost < best) {
+    best = few_cost;
     *s = few;
+  }
+  // Few rows and many keys: small pieces whose keys are cut, for one or two parts an SM.  Merging them takes as long as starting
+  // a large piece or two.
+  int64_t keys = 0, ideal = 0;
+  for (const PromptItem& it : small) {
+    keys += piece_keys(it);
+    ideal += piece_cost(it, in.dtype, true);
+  }
+  if (small.empty() || best * sms < ideal + ideal / 3) return true;
+  for (int waves = 1; waves <= 2; ++waves) {
+    const int chunk = (int)((keys / (sms * waves) + 128) / 128 * 128);
+    if (chunk >= piece_keys(small[0])) continue;
+    const std::vector<PromptItem> parts = cut_pieces(small, chunk, nullptr);
+    const int64_t cost = spread(parts, sms, in.dtype, true, nullptr) + (in.dtype == IA_F32 ? 2 * 4 * 32 : 4 * 256);
+    if (cost >= best) continue;
+    best = cost;
+    few.chunk = chunk;
+    few.n_pieces = (int)small.size();
+    few.n_items = (int)parts.size();
+    few.ctas = in.dtype == IA_F32 ? few.n_items : std::min(few.n_items, sms);
+    *s = few;
+  }
   return true;
 }
 }  // namespace
@@ -673,7 +760,9 @@ int make_prompt_plan(const int32_t* q_lens, const int32_t* kv_lens, int n_seqs, 
   PlanShape s;
   if (!plan_shape(in, &s) || plan_ints < s.ints()) return fail(IA_ERR_BAD_ARG, "prompt_plan: %lld words", (long long)plan_ints);
   int64_t q0, k0;
-  const std::vector<PromptItem> items = make_pieces(in, s, &q0, &k0);
+  std::vector<PromptItem> items = make_pieces(in, s, &q0, &k0);
+  std::vector<PromptPiece> pieces;
+  if (s.chunk > 0) items = cut_pieces(items, s.chunk, &pieces);
   std::vector<int> order(s.n_items), begin(s.ctas + 1, 0);
   if (dtype == IA_F32) {  // a CTA each, in this order
     for (int i = 0; i < s.n_items; ++i) order[i] = begin[i] = i;
@@ -686,12 +775,13 @@ int make_prompt_plan(const int32_t* q_lens, const int32_t* kv_lens, int n_seqs, 
     std::vector<int> next(begin.begin(), begin.end() - 1);
     for (int i = 0; i < s.n_items; ++i) order[next[cta_of[i]]++] = i;
   }
-  const int64_t first = s.ints() - (int64_t)s.n_items * 8;
-  const int32_t head[8] = {s.n_items, s.ctas, s.few_rows, (int32_t)first, group * 1000 + head_dim, n_kv_heads * 16 + dtype,
-                           (int32_t)q0, (int32_t)k0};
+  const int64_t first = s.first();
+  const int32_t head[8] = {s.n_items, s.ctas, s.chunk > 0 ? 2 + s.n_pieces : (int)s.few_rows, (int32_t)first, group * 1000 + head_dim,
+                           n_kv_heads * 16 + dtype, (int32_t)q0, (int32_t)k0};
   std::copy(head, head + 8, plan);
   for (int64_t i = 8; i < first; ++i) plan[i] = begin[std::min<int64_t>(i - 8, s.ctas)];
   for (int i = 0; i < s.n_items; ++i) std::memcpy(plan + first + 8 * (int64_t)i, &items[order[i]], sizeof(PromptItem));
+  if (!pieces.empty()) std::memcpy(plan + first + 8 * (int64_t)s.n_items, pieces.data(), pieces.size() * sizeof(PromptPiece));
   return IA_OK;
 }
 

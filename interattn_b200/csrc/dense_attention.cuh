@@ -18,9 +18,19 @@ struct PromptItem {
   int32_t limit0;   // visible keys of the first query token; may be <= 0
   int32_t kv_len;
   int32_t head;     // kv head
-  int32_t reserved[2];
+  int32_t slot;     // a part of the keys: which kPartRows rows of the workspace it fills
+  int32_t reserved;
 };
 static_assert(sizeof(PromptItem) == 32, "read as two 16-byte words");
+// Few query rows and many keys: the keys of a piece are cut into parts of about equal length, items whose sequence is the
+// part, and the parts' outputs and log-sum-exps are merged.
+struct PromptPiece {
+  int32_t q_tok, n_tok, head;
+  int32_t slot, parts;  // its parts fill the slots [slot, slot + parts)
+  int32_t reserved[3];
+};
+static_assert(sizeof(PromptPiece) == 32, "eight words of the plan");
+constexpr int kPartRows = 128;
 
 // Tensors of a prompt call; strides in elements, the D elements of one (token, head) contiguous.
 struct PromptTensors {
@@ -29,6 +39,7 @@ struct PromptTensors {
   float* lse;       // [q tokens, n_q_heads], may be null
   int64_t q_tok_stride, q_head_stride, k_tok_stride, k_head_stride, v_tok_stride, v_head_stride;
   int32_t n_q_tok, n_kv_tok, n_kv_heads, group;
+  float *part_o, *part_lse;  // [slots, kPartRows, D] and [slots, kPartRows]; null: pieces are not cut
 };
 
 // ---- the decode step of sequences that share a prefix ---------------------------------------------------------------
@@ -278,6 +289,7 @@ void make_shared_plan(const int32_t* group_sizes, int n_groups, int batch, int g
 
 int launch_prompt_f32(const PromptTensors& t, int head_dim, const PromptItem* items, int n_items, bool few_rows,
                       cudaStream_t stream);
+int launch_prompt_merge(const PromptTensors& t, int head_dim, int dtype, const PromptPiece* pieces, int n_pieces, cudaStream_t stream);
 int launch_shared_f32(const SharedParams& p, int head_dim, int ctas, cudaStream_t stream);
 int launch_prompt_tc(const PromptTensors& t, int head_dim, const PromptItem* items, const int32_t* cta_begin, int ctas,
                      cudaStream_t stream);

@@ -70,7 +70,7 @@ struct Work {
   int n_keys;         // keys from key0 on that anyone sees
   int row;            // decode step: table row
   int last;           // nothing follows
-  int64_t out_row;    // decode step: where the partial rows begin
+  int64_t out_row;    // where the partial rows begin, if there are any
 };
 
 struct TcParams {
@@ -424,6 +424,7 @@ template <int D, bool PAGED> struct CopyRole {
       wk.key0 = item.kv_tok;
       wk.limit0 = item.limit0;
       wk.n_keys = item.kv_len;
+      wk.out_row = (int64_t)item.slot * kPartRows;
       wk.order.split = item.n_tok <= tpm;
       wk.order.keys[0] = max(1, row_limit<false>(p, wk, min(item.n_tok, tpm) - 1));
       wk.order.keys[1] = max(1, row_limit<false>(p, wk, item.n_tok - 1));
@@ -672,10 +673,10 @@ template <int D, bool PAGED> struct MmaRole {
 };
 
 // ---- softmax warps ----------------------------------------------------------------------------------------------------
-template <int D, bool PAGED>
+template <int D, bool PAGED, bool PARTS>
 __device__ __forceinline__ void softmax_role(const TcParams& p, Bars* bars, const Work* ring, uint32_t tmem, unsigned char* out_base,
                                              float2 (*stats)[kRows]) {
-  using Out = std::conditional_t<PAGED, float, __nv_bfloat16>;
+  using Out = std::conditional_t<PAGED || PARTS, float, __nv_bfloat16>;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, w = warp >> 2, row = (warp & 3) * 32 + lane;
   const int G = p.group, tpm = kRows / G, row_tok = row / G, g = row % G;
   const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
@@ -807,6 +808,10 @@ __device__ __forceinline__ void softmax_role(const TcParams& p, Bars* bars, cons
       out = p.s.o + wk.out_row * D;
       at = (tok * G + g) * D;
       lse_out = p.s.lse + wk.out_row + tok * G + g;
+    } else if constexpr (PARTS) {
+      out = p.t.part_o + wk.out_row * D;
+      at = (tok * G + g) * D;
+      lse_out = p.t.part_lse + wk.out_row + tok * G + g;
     } else {
       const int64_t first = wk.q_tok * hq + wk.head * G;
       out = (Out*)p.t.out + first * D;
@@ -855,7 +860,7 @@ __device__ __forceinline__ void softmax_role(const TcParams& p, Bars* bars, cons
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             float lo, hi;
-            if constexpr (PAGED) {
+            if constexpr (PAGED || PARTS) {
               unpair(x[2 * k + i / 2], lo, hi);
               v[i] = __float_as_uint(i & 1 ? hi : lo);
             } else {
@@ -929,7 +934,7 @@ struct Control {
   uint32_t tmem;
 };
 
-template <int D, bool PAGED>
+template <int D, bool PAGED, bool PARTS>
 __global__ void __launch_bounds__(kThreads, 1) attend_tc_kernel(const __grid_constant__ TcParams p) {
   using C = Tc<D>;
   extern __shared__ __align__(1024) unsigned char base[];
@@ -976,7 +981,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tc_kernel(const __grid_con
   SharedCursor cur{};
   if constexpr (PAGED) cur = find_share<kKeys, kThreads>(p.s, blockIdx.x, gridDim.x, reinterpret_cast<unsigned long long*>(ctl.stats));
   if (warp < kCopyWarp) {
-    softmax_role<D, PAGED>(p, &bars, ctl.ring, tmem, base + C::tiles, ctl.stats);
+    softmax_role<D, PAGED, PARTS>(p, &bars, ctl.ring, tmem, base + C::tiles, ctl.stats);
   } else {
     if (warp == kCopyWarp) CopyRole<D, PAGED>(p, &bars, ctl.ring, base, cur).run();
     if (warp >= kMmaWarp) MmaRole<D, PAGED>(p, &bars, ctl.ring, smem_u32(base), uniform(tmem), uniform(warp - kMmaWarp)).run();
@@ -1027,8 +1032,8 @@ int encode_q(CUtensorMap* tm, const void* q, int head_dim, int group, int n_kv_h
                    {64, group, kRows / group, 1, 1});
 }
 
-template <int D, bool PAGED> int launch_tc(const TcParams& p, int grid, cudaStream_t stream) {
-  auto kern = attend_tc_kernel<D, PAGED>;
+template <int D, bool PAGED, bool PARTS = false> int launch_tc(const TcParams& p, int grid, cudaStream_t stream) {
+  auto kern = attend_tc_kernel<D, PAGED, PARTS>;
   static SmemOnce once;
   if (int s = once.allow((const void*)kern, Tc<D>::smem, "attend_tc_kernel")) return s;
   const cudaError_t e = launch_overlapped(kern, (unsigned)grid, (unsigned)kThreads, Tc<D>::smem, stream, p);
@@ -1059,6 +1064,7 @@ int launch_prompt_tc(const PromptTensors& t, int head_dim, const PromptItem* ite
     if (int s = encode<4>(&p.tm_k, t.k, dims, ks, box)) return s;
     if (int s = encode<4>(&p.tm_v, t.v, dims, vs, box)) return s;
   }
+  if (t.part_o != nullptr) return head_dim == 128 ? launch_tc<128, false, true>(p, ctas, stream) : launch_tc<64, false, true>(p, ctas, stream);
   return head_dim == 128 ? launch_tc<128, false>(p, ctas, stream) : launch_tc<64, false>(p, ctas, stream);
 }
 

@@ -62,7 +62,8 @@ class PromptAttention:
     where it is infinite or NaN.
 
     The lengths are host values; the work is cut and spread over the GPU once, here, and the object serves every layer
-    and any number of streams and captured graphs: it holds nothing that a call writes."""
+    and any number of streams and captured graphs: it holds nothing that a call writes.  Where there are few queries and
+    many keys the keys are cut too, and ``run`` takes a workspace from torch's allocator."""
 
     def __init__(self, q_lens: Sequence[int], n_q_heads: int, n_kv_heads: int, head_dim: int, *,
                  kv_lens: Optional[Sequence[int]] = None, dtype: torch.dtype = torch.bfloat16, device="cuda"):
@@ -92,6 +93,7 @@ class PromptAttention:
             _lib.check(lib.ia_prompt_plan(*args, _ptr(self._host), words))
             self._plan = self._host.to(self.device)
         self._host = self._host[:8].clone()
+        self._ws_bytes = int(lib.ia_prompt_workspace_bytes(_ptr(self._host)))
         # run() is called once per layer: what it passes and checks against is made here
         self._call, self._index = lib.ia_prompt_attention, self.device.index
         self._plan_args = (self._host.data_ptr(), self._plan.data_ptr())
@@ -127,8 +129,10 @@ class PromptAttention:
         (qt, qh, _), (kt, kh, _), (vt, vh, _) = q.stride(), k.stride(), v.stride()
         tensors = _PROMPT_TENSORS(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(),
                                   qt, qh, kt, kh, vt, vh, *self._sizes)
+        ws = torch.empty((self._ws_bytes,), dtype=torch.uint8, device=self.device) if self._ws_bytes else None
         with device_guard(self._index):
-            _lib.check(self._call(tensors, *self._plan_args, _raw_stream(self._index)))
+            _lib.check(self._call(tensors, *self._plan_args, 0 if ws is None else ws.data_ptr(), self._ws_bytes,
+                                  _raw_stream(self._index)))
         return (out, lse) if return_lse else out
 
 

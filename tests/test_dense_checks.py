@@ -37,15 +37,31 @@ def prompt_plan(lib, q_lens, kv_lens, hkv, group, d, dtype):
 @pytest.mark.parametrize("dtype", [_lib.IA_F32, _lib.IA_BF16])
 @pytest.mark.parametrize("hkv,group", [(2, 4), (1, 1), (3, 3), (1, 16), (8, 5)])
 @pytest.mark.parametrize("q_lens,kv_lens", [([1], [1]), ([], []), ([0, 5, 0], [7, 5, 0]), ([1000, 3, 64, 129], [1000, 300, 10, 129]),
-                                            ([5000] * 7, [9000] * 7)])
+                                            ([5000] * 7, [9000] * 7), ([3], [20000]), ([40, 1, 0], [5000, 9001, 77]),
+                                            ([70], [200])])
 def test_prompt_plan_holds_every_token_and_head_once(lib, dtype, hkv, group, q_lens, kv_lens):
     plan = prompt_plan(lib, q_lens, kv_lens, hkv, group, 128, dtype)
     n_items, ctas, _, first = plan[:4]
     begin = plan[8:8 + ctas + 1]
     assert begin[0] == 0 and begin[-1] == n_items and all(a <= b for a, b in zip(begin, begin[1:]))
+    items = [plan[first + 8 * i:first + 8 * i + 7] for i in range(n_items)]
+    if plan[2] >= 2:    # keys are cut: put the parts of every piece together again
+        parts, items = {it[6]: it for it in items}, []
+        assert sorted(parts) == list(range(n_items))
+        for i in range(plan[2] - 2):
+            q_tok, n_tok, head, slot, n, *_ = plan[first + 8 * (n_items + i):first + 8 * (n_items + i) + 8]
+            mine = [parts[slot + k] for k in range(n)]
+            for a, b in zip(mine, mine[1:]):
+                assert a[2] + a[4] == b[2] and a[3] - a[4] == b[3] and a[4] % 128 == 0
+            assert all((it[0], it[1], it[5]) == (q_tok, n_tok, head) for it in mine)
+            assert all(min(it[3] + n_tok - 1, it[4]) > 0 for it in mine[1:])
+            _, _, kv_tok, limit0, *_ = mine[0]
+            whole = sum(it[4] for it in mine)
+            seq = next(s for s in range(len(q_lens)) if sum(q_lens[:s]) <= q_tok < sum(q_lens[:s + 1]))
+            assert whole >= min(kv_lens[seq], limit0 + n_tok - 1) and whole <= kv_lens[seq]
+            items.append([q_tok, n_tok, kv_tok, limit0, kv_lens[seq], head])
     seen = set()
-    for i in range(n_items):
-        q_tok, n_tok, kv_tok, limit0, kv_len, head = plan[first + 8 * i:first + 8 * i + 6]
+    for q_tok, n_tok, kv_tok, limit0, kv_len, head, *_ in items:
         seq = next(s for s in range(len(q_lens)) if sum(q_lens[:s]) <= q_tok < sum(q_lens[:s + 1]))
         assert 0 < n_tok * group <= 256 and kv_tok == sum(kv_lens[:seq]) and kv_len == kv_lens[seq]
         assert limit0 == kv_lens[seq] - q_lens[seq] + (q_tok - sum(q_lens[:seq])) + 1
@@ -105,9 +121,16 @@ def tensors(**kw):
 def test_prompt_call_refusals(lib, change, word):
     plan = prompt_plan(lib, [4, 4], [4, 4], 2, 4, 64, _lib.IA_BF16)
     host = ints(plan[:8])
-    assert lib.ia_prompt_attention(tensors(**change), host, 16, None) < 0
+    assert lib.ia_prompt_attention(tensors(**change), host, 16, None, 0, None) < 0
     assert word in lib.ia_last_error_string()
-    assert lib.ia_prompt_attention(tensors(), host, None, None) < 0
+    assert lib.ia_prompt_attention(tensors(), host, None, None, 0, None) < 0
+    plan = prompt_plan(lib, [4, 4], [9000, 9000], 2, 4, 64, _lib.IA_BF16)     # few queries, many keys: cut
+    host, fit = ints(plan[:8]), tensors(out=1 << 30, k=1 << 20, v=1 << 20, n_kv_tokens=18000)
+    need = lib.ia_prompt_workspace_bytes(host)
+    assert need > 0 and lib.ia_prompt_workspace_bytes(None) == -1
+    for ws, size in ((None, need), (16, need - 1), (24, need)):
+        assert lib.ia_prompt_attention(fit, host, 16, ws, size, None) < 0
+        assert b"workspace" in lib.ia_last_error_string()
 
 
 def test_packed_arguments_match_the_struct():

@@ -45,6 +45,66 @@ def test_prompt(hq, hkv, d, dtype, q_lens, kv_lens):
     assert torch.equal(plan.run(q, k, v), out)      # the same bits again, and without the log-sum-exp
 
 
+@pytest.mark.parametrize("hq,hkv,d,dtype", GEOMETRIES)
+@pytest.mark.parametrize("q_lens,kv_lens", [
+    ([3], [9000]), ([1, 17, 0], [5000, 3001, 64]), ([64, 5], [2100, 4000]), ([100, 1], [2600, 4099]),
+    ([4, 9], [3, 6000]),                           # one whose first query sees nothing
+])
+def test_prompt_few_queries_many_keys(hq, hkv, d, dtype, q_lens, kv_lens):
+    """The keys of a piece are cut and the parts merged."""
+    q, k, v, plan = prompt_case(hq, hkv, d, dtype, q_lens, kv_lens, seed=40)
+    assert plan._ws_bytes > 0
+    k = (k.float() * torch.linspace(0.05, 3.0, k.shape[0], device="cuda")[:, None, None]).to(dtype)
+    ref = prompt_reference(q, k, v, q_lens, kv_lens)
+    out, lse = plan.run(q, k, v, return_lse=True)
+    assert ops.device_status() == 0
+    ref.check(out, dtype)
+    ref.check_lse(lse)
+    assert torch.equal(plan.run(q, k, v), out)
+
+
+@pytest.mark.parametrize("dtype,d", [(BF16, 128), (BF16, 64), (F32, 64)])
+@pytest.mark.parametrize("poison", [float("nan"), float("inf"), float("-inf")])
+@pytest.mark.parametrize("back", [1, 3, 40])
+def test_prompt_cut_keys_bad_places(dtype, d, poison, back):
+    """A bad value that only the last `back` queries see, and a neighbour's keys behind the end."""
+    q_lens, kv_lens = [50, 2], [6000, 3000]
+    q, k, v, plan = prompt_case(4, 2, d, dtype, q_lens, kv_lens, seed=41)
+    want = plan.run(q, k, v)
+    v[6000 - back, 1, 5] = poison
+    k[6000:], v[6000:] = poison, poison
+    out = plan.run(q, k, v)
+    assert plan._ws_bytes > 0 and ops.device_status() == 0
+    bad = ~torch.isfinite(out[:50])
+    assert bad[50 - back:, 2:, 5].all() and int(bad.sum()) == back * 2
+    ref = want[:50].float()
+    assert torch.equal(out[:50 - back], want[:50 - back]) or torch.allclose(out[:50 - back].float(), ref[:50 - back], rtol=2 ** -7, atol=2 ** -9)
+
+
+def test_prompt_cut_keys_captured_and_on_two_streams():
+    q_lens, kv_lens = [5, 60], [7000, 2000]
+    q, k, v, plan = prompt_case(8, 2, 128, BF16, q_lens, kv_lens, seed=42)
+    assert plan._ws_bytes > 0
+    want, q2 = plan.run(q, k, v), torch.randn_like(q)
+    want2 = plan.run(q2, k, v)
+    inputs = [q.clone(), q.clone()]
+    graphs = []
+    for x in inputs:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            y = plan.run(x, k, v)
+        graphs.append((g, y))
+    inputs[1].copy_(q2)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(20):
+        for (g, _y), s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(graphs[0][1], want) and torch.equal(graphs[1][1], want2)
+
+
 @pytest.mark.parametrize("hq,hkv,d,dtype", [(8, 2, 128, BF16), (8, 2, 64, BF16), (4, 4, 64, F32)])
 def test_prompt_of_many_tiles(hq, hkv, d, dtype):
     """Enough pieces that a CTA takes several, with a rising score that moves the running maximum often."""
