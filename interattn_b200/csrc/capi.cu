@@ -723,10 +723,10 @@ int ia_prompt_attention(const ia_prompt_tensors* t, const int32_t* plan_host, co
   const PromptItem* items = reinterpret_cast<const PromptItem*>(plan_device + plan_host[3]);
   const int s = t->dtype == IA_BF16
                     ? launch_prompt_tc(p, t->head_dim, items, plan_device + 8, plan_host[1], (cudaStream_t)stream)
-                    : launch_prompt_f32(p, t->head_dim, items, plan_host[0], plan_host[2] != 0, (cudaStream_t)stream);
+                    : launch_prompt_f32(p, t->head_dim, items, plan_host[0], (plan_host[2] & 1) != 0, (cudaStream_t)stream);
   if (s || !parts) return s;
-  return launch_prompt_merge(p, t->head_dim, t->dtype, reinterpret_cast<const PromptPiece*>(items + plan_host[0]), plan_host[2] - 2,
-                             (cudaStream_t)stream);
+  return launch_prompt_merge(p, t->head_dim, t->dtype, reinterpret_cast<const PromptPiece*>(items + plan_host[0]), plan_host[2] / 2,
+                             (plan_host[2] & 1) != 0, (cudaStream_t)stream);
 }
 
 static int check_groups(const int32_t* group_sizes, int n_groups, const ia_geom* g) {

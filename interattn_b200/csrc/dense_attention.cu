@@ -558,8 +558,8 @@ template <int D> int launch_shared(const SharedParams& p, int ctas, cudaStream_t
   return launch(kern, (unsigned)ctas, bytes, stream, "shared_attention_kernel", p);
 }
 template <typename T, int D>
-int launch_parts(const PromptTensors& t, const PromptPiece* pieces, int n_pieces, cudaStream_t stream) {
-  constexpr int rows = std::is_same_v<T, float> ? 32 : kPartRows, blocks = rows / 8;  // rows of a small piece
+int launch_parts(const PromptTensors& t, const PromptPiece* pieces, int n_pieces, bool few_rows, cudaStream_t stream) {
+  const int blocks = (std::is_same_v<T, float> && few_rows ? 32 : kPartRows) / 8;
   return launch(prompt_merge_kernel<T, D>, (unsigned)(n_pieces * blocks), 0, stream, "prompt_merge_kernel", t, pieces, blocks);
 }
 template <typename T, int D>
@@ -598,10 +598,13 @@ int launch_prompt_f32(const PromptTensors& t, int head_dim, const PromptItem* it
   return few_rows ? launch_prompt<64, 2>(t, items, n_items, stream) : launch_prompt<64, 8>(t, items, n_items, stream);
 }
 
-int launch_prompt_merge(const PromptTensors& t, int head_dim, int dtype, const PromptPiece* pieces, int n_pieces, cudaStream_t stream) {
-  if (dtype == IA_F32) return head_dim == 128 ? launch_parts<float, 128>(t, pieces, n_pieces, stream) : launch_parts<float, 64>(t, pieces, n_pieces, stream);
-  return head_dim == 128 ? launch_parts<__nv_bfloat16, 128>(t, pieces, n_pieces, stream)
-                         : launch_parts<__nv_bfloat16, 64>(t, pieces, n_pieces, stream);
+int launch_prompt_merge(const PromptTensors& t, int head_dim, int dtype, const PromptPiece* pieces, int n_pieces, bool few_rows,
+                        cudaStream_t stream) {
+  if (dtype == IA_F32)
+    return head_dim == 128 ? launch_parts<float, 128>(t, pieces, n_pieces, few_rows, stream)
+                           : launch_parts<float, 64>(t, pieces, n_pieces, few_rows, stream);
+  return head_dim == 128 ? launch_parts<__nv_bfloat16, 128>(t, pieces, n_pieces, few_rows, stream)
+                         : launch_parts<__nv_bfloat16, 64>(t, pieces, n_pieces, few_rows, stream);
 }
 
 int launch_shared_f32(const SharedParams& p, int head_dim, int ctas, cudaStream_t stream) {
@@ -710,40 +713,44 @@ PlanShape shape_of(const PlanInput& in, bool few_rows, bool* fits) {
 // heads of 128, small and large pieces, us: fp32 one prompt of 600: 139 and 166, of 900: 301 and 242, 150, 30, 10, 400, 5 and
 // 77: 90 and 119, four of 300: 156 and 131; bf16 one of 600: 18.5 and 23.5, of 1700: 45 and 44, four of 300: 22.7 and 19.5,
 // three of 700: 37 and 31.  With four large pieces an SM the small ones gain nothing more (bf16 3000 and 2300: 148 and 138).
+// Keys whole and cut, us: one token behind 16000: fp32 1742 and 111, bf16 146 and 30; 100 behind 8000: 893 and 476, 80 and 38;
+// eight times 4 behind 3000: 334 and 179, 43 and 36; one fp32 prompt of 600: 137 and 114.
 bool plan_shape(const PlanInput& in, PlanShape* s) {
   bool fits, fits_few;
   *s = shape_of(in, false, &fits);
   if (!fits || s->n_items >= 4 * sm_count()) return fits;
-  PlanShape few = shape_of(in, true, &fits_few);
-  int64_t q, kv;
-  const std::vector<PromptItem> small = make_pieces(in, few, &q, &kv);
+  const PlanShape shapes[2] = {*s, shape_of(in, true, &fits_few)};
   const int sms = sm_count();
-  const int64_t few_cost = spread(small, sms, in.dtype, true, nullptr);
-  int64_t best = spread(make_pieces(in, *s, &q, &kv), sms, in.dtype, false, nullptr);
-  if (few_cost < best) {
-    best = few_cost;
-    *s = few;
-  }
-  // Few rows and many keys: small pieces whose keys are cut, for one or two parts an SM.  Merging them takes as long as starting
-  // a large piece or two.
-  int64_t keys = 0, ideal = 0;
-  for (const PromptItem& it : small) {
-    keys += piece_keys(it);
-    ideal += piece_cost(it, in.dtype, true);
-  }
-  if (small.empty() || best * sms < ideal + ideal / 3) return true;
-  for (int waves = 1; waves <= 2; ++waves) {
-    const int chunk = (int)((keys / (sms * waves) + 128) / 128 * 128);
-    if (chunk >= piece_keys(small[0])) continue;
-    const std::vector<PromptItem> parts = cut_pieces(small, chunk, nullptr);
-    const int64_t cost = spread(parts, sms, in.dtype, true, nullptr) + (in.dtype == IA_F32 ? 2 * 4 * 32 : 4 * 256);
-    if (cost >= best) continue;
+  int64_t q, kv, best = 0, ideal[2] = {0, 0}, keys[2] = {0, 0};
+  std::vector<PromptItem> whole[2];
+  for (int few = 0; few < 2; ++few) {
+    whole[few] = make_pieces(in, shapes[few], &q, &kv);
+    for (const PromptItem& it : whole[few]) {
+      keys[few] += piece_keys(it);
+      ideal[few] += piece_cost(it, in.dtype, few != 0);
+    }
+    const int64_t cost = spread(whole[few], sms, in.dtype, few != 0, nullptr);
+    if (few != 0 && cost >= best) continue;
     best = cost;
-    few.chunk = chunk;
-    few.n_pieces = (int)small.size();
-    few.n_items = (int)parts.size();
-    few.ctas = in.dtype == IA_F32 ? few.n_items : std::min(few.n_items, sms);
-    *s = few;
+    *s = shapes[few];
+  }
+  // Few rows and many keys: the keys are cut, for one or two parts an SM.  Merging them takes as long as starting a large piece or
+  // two.  A slot of the workspace holds one row tile, so on the tensor cores only small pieces are cut.
+  for (int few = in.dtype == IA_F32 ? 0 : 1; few < 2; ++few) {
+    if (whole[few].empty() || best * sms < ideal[few] + ideal[few] / 3) continue;
+    for (int waves = 1; waves <= 2; ++waves) {
+      const int chunk = (int)((keys[few] / (sms * waves) + 128) / 128 * 128);
+      if (chunk >= piece_keys(whole[few][0])) continue;
+      const std::vector<PromptItem> parts = cut_pieces(whole[few], chunk, nullptr);
+      const int64_t cost = spread(parts, sms, in.dtype, few != 0, nullptr) + (in.dtype == IA_F32 ? 2 * 4 * 32 : 4 * 256);
+      if (cost >= best) continue;
+      best = cost;
+      *s = shapes[few];
+      s->chunk = chunk;
+      s->n_pieces = (int)whole[few].size();
+      s->n_items = (int)parts.size();
+      s->ctas = in.dtype == IA_F32 ? s->n_items : std::min(s->n_items, sms);
+    }
   }
   return true;
 }
@@ -776,7 +783,7 @@ int make_prompt_plan(const int32_t* q_lens, const int32_t* kv_lens, int n_seqs, 
     for (int i = 0; i < s.n_items; ++i) order[next[cta_of[i]]++] = i;
   }
   const int64_t first = s.first();
-  const int32_t head[8] = {s.n_items, s.ctas, s.chunk > 0 ? 2 + s.n_pieces : (int)s.few_rows, (int32_t)first, group * 1000 + head_dim,
+  const int32_t head[8] = {s.n_items, s.ctas, (s.chunk > 0 ? 2 * s.n_pieces : 0) + s.few_rows, (int32_t)first, group * 1000 + head_dim,
                            n_kv_heads * 16 + dtype, (int32_t)q0, (int32_t)k0};
   std::copy(head, head + 8, plan);
   for (int64_t i = 8; i < first; ++i) plan[i] = begin[std::min<int64_t>(i - 8, s.ctas)];

@@ -289,7 +289,8 @@ void make_shared_plan(const int32_t* group_sizes, int n_groups, int batch, int g
 
 int launch_prompt_f32(const PromptTensors& t, int head_dim, const PromptItem* items, int n_items, bool few_rows,
                       cudaStream_t stream);
-int launch_prompt_merge(const PromptTensors& t, int head_dim, int dtype, const PromptPiece* pieces, int n_pieces, cudaStream_t stream);
+int launch_prompt_merge(const PromptTensors& t, int head_dim, int dtype, const PromptPiece* pieces, int n_pieces, bool few_rows,
+                        cudaStream_t stream);
 int launch_shared_f32(const SharedParams& p, int head_dim, int ctas, cudaStream_t stream);
 int launch_prompt_tc(const PromptTensors& t, int head_dim, const PromptItem* items, const int32_t* cta_begin, int ctas,
                      cudaStream_t stream);

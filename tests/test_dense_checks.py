@@ -48,7 +48,7 @@ def test_prompt_plan_holds_every_token_and_head_once(lib, dtype, hkv, group, q_l
     if plan[2] >= 2:    # keys are cut: put the parts of every piece together again
         parts, items = {it[6]: it for it in items}, []
         assert sorted(parts) == list(range(n_items))
-        for i in range(plan[2] - 2):
+        for i in range(plan[2] // 2):
             q_tok, n_tok, head, slot, n, *_ = plan[first + 8 * (n_items + i):first + 8 * (n_items + i) + 8]
             mine = [parts[slot + k] for k in range(n)]
             for a, b in zip(mine, mine[1:]):
@@ -82,7 +82,7 @@ def test_prompt_plan_shares_the_work_evenly(lib):
 
 
 @pytest.mark.parametrize("dtype,lens,small", [
-    (_lib.IA_F32, [130], True), (_lib.IA_F32, [600], True), (_lib.IA_F32, [1000], False), (_lib.IA_F32, [300] * 4, False),
+    (_lib.IA_F32, [130], True), (_lib.IA_F32, [1000], False), (_lib.IA_F32, [300] * 4, False),
     (_lib.IA_BF16, [600], True), (_lib.IA_BF16, [1000], True), (_lib.IA_BF16, [700] * 3, False), (_lib.IA_BF16, [9000], False),
     (_lib.IA_F32, [300, 200, 100, 50], True), (_lib.IA_BF16, [300, 200, 100, 50], True)])
 def test_prompt_plan_takes_small_pieces_where_the_busiest_sm_then_ends_first(lib, dtype, lens, small):
@@ -91,6 +91,17 @@ def test_prompt_plan_takes_small_pieces_where_the_busiest_sm_then_ends_first(lib
     rows = 4 * max(plan[plan[3] + 8 * i + 1] for i in range(plan[0]))
     full = 128 if dtype == _lib.IA_F32 else 256
     assert plan[2] == small and (rows <= full // 2) == small
+
+
+@pytest.mark.parametrize("dtype,lens,prior,cut", [
+    (_lib.IA_F32, [1], [16000], True), (_lib.IA_BF16, [1], [16000], True), (_lib.IA_F32, [100], [8000], True),
+    (_lib.IA_BF16, [100], [2000], True), (_lib.IA_F32, [600], [0], True), (_lib.IA_BF16, [4] * 8, [3000] * 8, True),
+    (_lib.IA_F32, [1000], [0], False), (_lib.IA_BF16, [600], [0], False), (_lib.IA_BF16, [500], [16000], False),
+    (_lib.IA_F32, [500], [16000], False), (_lib.IA_BF16, [64] * 8, [1000] * 8, False)])
+def test_prompt_plan_cuts_keys_where_few_pieces_have_many(lib, dtype, lens, prior, cut):
+    """32 / 8 heads of 128 on 148 SMs; both sides were timed."""
+    plan = prompt_plan(lib, lens, [a + b for a, b in zip(lens, prior)], 8, 4, 128, dtype)
+    assert (plan[2] >= 2) == cut and (lib.ia_prompt_workspace_bytes(ints(plan[:8])) > 0) == cut
 
 
 @pytest.mark.parametrize("change,word", [
