@@ -739,7 +739,7 @@ bool plan_shape(const PlanInput& in, PlanShape* s) {
   for (int few = in.dtype == IA_F32 ? 0 : 1; few < 2; ++few) {
     if (whole[few].empty() || best * sms < ideal[few] + ideal[few] / 3) continue;
     for (int waves = 1; waves <= 2; ++waves) {
-      const int chunk = (int)((keys[few] / (sms * waves) + 128) / 128 * 128);
+      const int chunk = (int)(std::min<int64_t>(keys[few] / (sms * waves) + 128, 1 << 30) / 128 * 128);
       if (chunk >= piece_keys(whole[few][0])) continue;
       const std::vector<PromptItem> parts = cut_pieces(whole[few], chunk, nullptr);
       const int64_t cost = spread(parts, sms, in.dtype, few != 0, nullptr) + (in.dtype == IA_F32 ? 2 * 4 * 32 : 4 * 256);

@@ -72,6 +72,14 @@ def test_prompt_plan_holds_every_token_and_head_once(lib, dtype, hkv, group, q_l
     assert len(seen) == sum(q_lens) * hkv
 
 
+def test_prompt_plan_of_the_longest_sequence(lib):
+    """2^30 keys for each of 300 small pieces: what would be an SM's share of them is past 32 bits."""
+    plan = prompt_plan(lib, [300], [1 << 30], 30, 4, 128, _lib.IA_BF16)
+    items = [plan[plan[3] + 8 * i:plan[3] + 8 * i + 6] for i in range(plan[0])]
+    assert all(0 < it[4] <= 1 << 30 and 0 <= it[2] < 1 << 30 and it[3] > 0 for it in items)
+    assert sum(it[1] * it[4] for it in items) == 300 * 30 << 30
+
+
 def test_prompt_plan_shares_the_work_evenly(lib):
     lens = [32768, 100, 5000, 17]
     plan = prompt_plan(lib, lens, lens, 8, 4, 128, _lib.IA_BF16)
