@@ -13,6 +13,9 @@
 // page to rank and rank to list entry, so that they spread over all threads wherever in the pool they lie (with a run of pages
 // per thread, 256 rows' pages out of 65536 took 153 us instead of 17).
 //
+// A write goes to the end of whatever its row holds, so it has to know when that is not where its tokens belong: the scratch keeps
+// for every row whether its last extend was refused, and how many of its tokens lie in pages that a fork shared (see Guard).
+//
 // Measured: moving 1.14 GB of pages 182 us (0.97 of the copy peak), a plan over 16,384 pages 9 us, 64 forks of 8k tokens 15 us with
 // the free before them; the plan is a chain of dependent loads and barriers.
 #include <algorithm>
@@ -32,12 +35,20 @@ constexpr int kPlanCtas = 8, kPlanThreads = 1024;  // of the large plan; the sma
 constexpr int kSmallList = 256, kSmallPool = 32768, kSmallCompact = 16384;
 constexpr int kMoveThreads = 256;
 
-// scratch: counters, then per entry of a list the inclusive sum of the pages wanted and what was granted, then the moves
+// What a write to the row may not touch; all zero at first.
+struct Guard {
+  int shared;   // the row's first tokens, whole pages, that a fork shared: not while another count holds the page
+  int refused;  // the row's last extend that asked for tokens was refused: nothing
+};
+// scratch: the rows' guards, which outlive a call; counters, then per entry of a list the inclusive sum of the pages wanted and
+// what was granted, then the moves
 struct Scratch {
+  Guard* guard;      // [n_rows]
   int* n_moves;      // [4]: moves, live pages, unused
   int* owner;        // [n_rows] first entry of the list that names the row
   int* upto;         // [n_entries] inclusive sums
-  int* kept;         // [n_entries] pages of the row before, or taken over from the parent; -1: the entry was refused
+  int* kept;         // [n_entries] pages of the row before, or taken over from the parent; -1: the entry was refused, -2: it names
+                     // no row, or one that an entry before it names
   int* new_len;      // [n_entries]
   int2* moves;       // [n_pages] (from, to)
   int* remap;        // [n_pages]
@@ -49,9 +60,9 @@ int64_t scratch_layout(char* base, int64_t n_rows, int64_t n_pages, Scratch* s) 
     off += (bytes + 255) / 256 * 256;
     return r;
   };
-  char* a[7] = {take(16),         take(n_rows * 4),  take(n_rows * 4), take(n_rows * 4),
-                take(n_rows * 4), take(n_pages * 8), take(n_pages * 4)};  // no list is longer than the table
-  if (s) *s = Scratch{(int*)a[0], (int*)a[1], (int*)a[2], (int*)a[3], (int*)a[4], (int2*)a[5], (int*)a[6]};
+  char* a[8] = {take(n_rows * 8), take(16),         take(n_rows * 4),  take(n_rows * 4),
+                take(n_rows * 4), take(n_rows * 4), take(n_pages * 8), take(n_pages * 4)};  // no list is longer than the table
+  if (s) *s = Scratch{(Guard*)a[0], (int*)a[1], (int*)a[2], (int*)a[3], (int*)a[4], (int*)a[5], (int2*)a[6], (int*)a[7]};
   return off;
 }
 
@@ -211,11 +222,12 @@ template <int CTAS> __global__ void __launch_bounds__(kPlanThreads) pages_plan_k
   int wanted = 0;
   for (int i = i0; i < i1; ++i) {
     const int row = p.rows[i], other = p.other[i];
-    int kept = -1, need = 0;
+    int kept = -2, need = 0;
     if constexpr (CTAS > 1)
       if ((unsigned)row < (unsigned)st.n_rows) again = __ldcg(p.sc.owner + row) != i;
     if ((unsigned)row < (unsigned)st.n_rows && !again) {
       const int len = len_of(st, row);
+      kept = -1;
       if (p.fork) {
         if ((unsigned)other < (unsigned)st.n_rows && other != row && len == 0) {
           const int parent = len_of(st, other);
@@ -253,8 +265,17 @@ template <int CTAS> __global__ void __launch_bounds__(kPlanThreads) pages_plan_k
   __threadfence();
   const Sums grants = scan<CTAS>(granted, warp_sums, &cta_sum);  // also: the sums above are visible to all
   // new lengths; all lengths were read before the barriers above
-  for (int i = i0; i < i1; ++i)
-    if (p.sc.kept[i] >= 0) st.lens[p.rows[i]] = p.sc.new_len[i];
+  for (int i = i0; i < i1; ++i) {
+    const int row = p.rows[i], kept = p.sc.kept[i];
+    if (kept >= 0) st.lens[row] = p.sc.new_len[i];
+    if (!p.fork) {
+      if (kept >= -1 && p.other[i] != 0) p.sc.guard[row].refused = kept < 0;
+    } else if (kept >= 0) {  // a parent of whole pages is no child, and all its entries say the same
+      const int shared = p.share ? kept * kPage : 0;
+      p.sc.guard[row] = Guard{shared, 0};
+      if (shared > 0) p.sc.guard[p.other[i]].shared = shared;
+    }
+  }
   // the free page of rank r ...
   int rank = __shfl_sync(0xffffffffu, free_pages.before, 0);
   for (int g = run.p0; g < run.p1 && rank < grants.total; g += 128) {
@@ -410,7 +431,7 @@ __global__ void __launch_bounds__(kMoveThreads) pages_compact_kernel(const MoveP
 }
 
 // One CTA per entry: whoever takes the row's length away gives its pages back, so a row named twice is freed once.
-struct FreeParams { State st; const int* rows; };
+struct FreeParams { State st; Guard* guard; const int* rows; };
 __global__ void __launch_bounds__(512) pages_free_kernel(const FreeParams p) {
   __shared__ int len_s;
   const State& st = p.st;
@@ -420,7 +441,10 @@ __global__ void __launch_bounds__(512) pages_free_kernel(const FreeParams p) {
     if (threadIdx.x == 0) report(st, DEV_STATUS_BAD_INDEX);
     return;
   }
-  if (threadIdx.x == 0) len_s = max(0, min(atomicExch(st.lens + row, 0), st.max_pages * kPage));
+  if (threadIdx.x == 0) {
+    len_s = max(0, min(atomicExch(st.lens + row, 0), st.max_pages * kPage));
+    p.guard[row] = Guard{0, 0};
+  }
   __syncthreads();
   for (int j = threadIdx.x; j < pages_of(len_s); j += 512) {
     int* entry = st.table + (int64_t)row * st.max_pages + j;
@@ -437,6 +461,7 @@ __global__ void __launch_bounds__(512) pages_free_kernel(const FreeParams p) {
 // ---- writing --------------------------------------------------------------------------------------------------------
 struct WriteParams {
   State st;
+  const Guard* guard;
   const int *rows, *starts;  // [n], [n + 1]
   int n, n_tokens;
   const char *k, *v;
@@ -475,8 +500,18 @@ __global__ void __launch_bounds__(kMoveThreads) pages_write_kernel(const WritePa
       for (int i = lane; good && i < lo; i += 32) again |= p.rows[i] == row;
       good = good && !__any_sync(0xffffffffu, again);  // a row named twice: the first entry counts
       if (good) {
+        const Guard g = p.guard[row];
         first = len_of(st, row) - (end - start);
-        good = first >= 0;
+        good = first >= 0 && g.refused == 0;
+        const int shared = min(g.shared, first + end - start);
+        if (good && first < shared) {  // no page of these may be another row's too
+          bool held = false;
+          for (int j = first / kPage + lane; j < pages_of(shared); j += 32) {
+            const int page = st.table[(int64_t)row * st.max_pages + j];
+            held |= (unsigned)page < (unsigned)st.n_pages && st.refs[page] > 1;
+          }
+          good = !__any_sync(0xffffffffu, held);
+        }
       }
       if (!good && lane == 0) report(st, DEV_STATUS_BAD_INDEX);
     }
@@ -574,7 +609,7 @@ int launch_pages_fork(const ia_page_cache& c, const int32_t* parents, const int3
 int launch_pages_free(const ia_page_cache& c, const int32_t* rows, int n, cudaStream_t stream) {
   State st;
   if (int s = state_of(c, &st)) return s;
-  return launch(pages_free_kernel, (unsigned)n, 512u, stream, "pages_free_kernel", FreeParams{st, rows});
+  return launch(pages_free_kernel, (unsigned)n, 512u, stream, "pages_free_kernel", FreeParams{st, scratch_of(c).guard, rows});
 }
 
 int launch_pages_compact(const ia_page_cache& c, cudaStream_t stream) {
@@ -599,7 +634,7 @@ int launch_pages_write(const ia_page_cache& c, const int32_t* rows, const int32_
   const int64_t warps = w.n_tokens, ctas = (warps + kMoveThreads / 32 - 1) / (kMoveThreads / 32);
   return launch(pages_write_kernel, (unsigned)std::min<int64_t>(ctas, sm_count() * 8), (unsigned)kMoveThreads, stream,
                 "pages_write_kernel",
-                WriteParams{st, rows, starts, n, w.n_tokens, (const char*)w.k, (const char*)w.v, (char*)w.k_pool, (char*)w.v_pool,
+                WriteParams{st, scratch_of(c).guard, rows, starts, n, w.n_tokens, (const char*)w.k, (const char*)w.v, (char*)w.k_pool, (char*)w.v_pool,
                             w.k_tok_stride * size, w.k_head_stride * size, w.v_tok_stride * size, w.v_head_stride * size,
                             c.page_stride * size, c.head_stride * size, c.n_kv_heads, c.head_dim * size / 16});
 }

@@ -8,7 +8,8 @@ admits, forks and frees sequences can run ahead of the GPU or be captured into a
 Free pages are handed out lowest first, in the order of the list, so the same calls give the same tables every time.
 What goes wrong on the device is refused for the list entry concerned and reported in ``ops.device_status()``:
 ``IA_DEV_STATUS_BAD_INDEX`` (a row or count out of range, a row named twice, a child that is not empty) or
-``IA_DEV_STATUS_NO_PAGES`` (the entries from the first one that does not fit on were left as they were).
+``IA_DEV_STATUS_NO_PAGES`` (the entries from the first one that does not fit on were left as they were).  What was refused stays
+refused in the calls that run ahead of that news: a row whose ``extend`` was refused takes no ``write`` until one is served.
 """
 
 from __future__ import annotations
@@ -62,7 +63,7 @@ class PageCache:
         if size < 0:
             _lib.check(_lib.IA_ERR_BAD_ARG)
         self._addresses = torch.tensor([p.data_ptr() for p in flat], dtype=torch.int64, device=self.device)
-        self._scratch = torch.empty((size + 256,), dtype=torch.uint8, device=self.device)
+        self._scratch = torch.zeros((size + 256,), dtype=torch.uint8, device=self.device)
         scratch = self._scratch.data_ptr()
         self._state = _lib.PageCacheState(
             block_table=block_table.data_ptr(), seq_lens=seq_lens.data_ptr(), refs=refs.data_ptr(),
@@ -112,7 +113,8 @@ class PageCache:
 
     def write(self, layer: int, rows: torch.Tensor, starts: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> None:
         """Tokens ``[starts[i], starts[i + 1])`` of k and v ``[T, Hkv, D]`` (token and head strides of any multiple of 16 bytes)
-        become the last tokens of ``rows[i]`` in this layer."""
+        become the last tokens of ``rows[i]`` in this layer.  Refused for a row whose last ``extend`` was refused, and where a
+        token would fall into a whole page that a fork shared while others still hold it."""
         shape, ks, vs = k.shape, k.stride(), v.stride()
         if shape != v.shape:
             raise ValueError("k and v hold the same tokens")
