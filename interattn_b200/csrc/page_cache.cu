@@ -40,10 +40,9 @@ struct Guard {
   int shared;   // the row's first tokens, whole pages, that a fork shared: not while another count holds the page
   int refused;  // the row's last extend that asked for tokens was refused: nothing
 };
-// scratch: the rows' guards, which outlive a call; counters, then per entry of a list the inclusive sum of the pages wanted and
-// what was granted, then the moves
+// scratch: counters, then per entry of a list the inclusive sum of the pages wanted and what was granted, then the moves; the rows'
+// guards, which outlive a call
 struct Scratch {
-  Guard* guard;      // [n_rows]
   int* n_moves;      // [4]: moves, live pages, unused
   int* owner;        // [n_rows] first entry of the list that names the row
   int* upto;         // [n_entries] inclusive sums
@@ -52,6 +51,7 @@ struct Scratch {
   int* new_len;      // [n_entries]
   int2* moves;       // [n_pages] (from, to)
   int* remap;        // [n_pages]
+  Guard* guard;      // [n_rows]
 };
 int64_t scratch_layout(char* base, int64_t n_rows, int64_t n_pages, Scratch* s) {
   int64_t off = 0;
@@ -60,9 +60,9 @@ int64_t scratch_layout(char* base, int64_t n_rows, int64_t n_pages, Scratch* s) 
     off += (bytes + 255) / 256 * 256;
     return r;
   };
-  char* a[8] = {take(n_rows * 8), take(16),         take(n_rows * 4),  take(n_rows * 4),
-                take(n_rows * 4), take(n_rows * 4), take(n_pages * 8), take(n_pages * 4)};  // no list is longer than the table
-  if (s) *s = Scratch{(Guard*)a[0], (int*)a[1], (int*)a[2], (int*)a[3], (int*)a[4], (int*)a[5], (int2*)a[6], (int*)a[7]};
+  char* a[8] = {take(16),         take(n_rows * 4),  take(n_rows * 4),  take(n_rows * 4),
+                take(n_rows * 4), take(n_pages * 8), take(n_pages * 4), take(n_rows * 8)};  // no list is longer than the table
+  if (s) *s = Scratch{(int*)a[0], (int*)a[1], (int*)a[2], (int*)a[3], (int*)a[4], (int2*)a[5], (int*)a[6], (Guard*)a[7]};
   return off;
 }
 
@@ -219,10 +219,12 @@ template <int CTAS> __global__ void __launch_bounds__(kPlanThreads) pages_plan_k
     __threadfence();
     sync_all<CTAS>();
   }
-  int wanted = 0;
+  int wanted = 0, row = 0, other = 0, kept = 0;  // of the thread's entry, if it has one only
   for (int i = i0; i < i1; ++i) {
-    const int row = p.rows[i], other = p.other[i];
-    int kept = -2, need = 0;
+    row = p.rows[i];
+    other = p.other[i];
+    kept = -2;
+    int need = 0;
     if constexpr (CTAS > 1)
       if ((unsigned)row < (unsigned)st.n_rows) again = __ldcg(p.sc.owner + row) != i;
     if ((unsigned)row < (unsigned)st.n_rows && !again) {
@@ -256,8 +258,9 @@ template <int CTAS> __global__ void __launch_bounds__(kPlanThreads) pages_plan_k
     const bool fits = upto <= free_pages.total;
     p.sc.upto[i] = upto;
     if constexpr (CTAS == 1) named[i] = upto;
-    if (!fits && p.sc.kept[i] >= 0) {
-      p.sc.kept[i] = -1;
+    if (per > 1) kept = p.sc.kept[i];
+    if (!fits && kept >= 0) {
+      p.sc.kept[i] = kept = -1;
       report(st, IA_DEV_STATUS_NO_PAGES);
     }
     if (fits) granted += need;
@@ -265,17 +268,8 @@ template <int CTAS> __global__ void __launch_bounds__(kPlanThreads) pages_plan_k
   __threadfence();
   const Sums grants = scan<CTAS>(granted, warp_sums, &cta_sum);  // also: the sums above are visible to all
   // new lengths; all lengths were read before the barriers above
-  for (int i = i0; i < i1; ++i) {
-    const int row = p.rows[i], kept = p.sc.kept[i];
-    if (kept >= 0) st.lens[row] = p.sc.new_len[i];
-    if (!p.fork) {
-      if (kept >= -1 && p.other[i] != 0) p.sc.guard[row].refused = kept < 0;
-    } else if (kept >= 0) {  // a parent of whole pages is no child, and all its entries say the same
-      const int shared = p.share ? kept * kPage : 0;
-      p.sc.guard[row] = Guard{shared, 0};
-      if (shared > 0) p.sc.guard[p.other[i]].shared = shared;
-    }
-  }
+  for (int i = i0; i < i1; ++i)
+    if (p.sc.kept[i] >= 0) st.lens[p.rows[i]] = p.sc.new_len[i];
   // the free page of rank r ...
   int rank = __shfl_sync(0xffffffffu, free_pages.before, 0);
   for (int g = run.p0; g < run.p1 && rank < grants.total; g += 128) {
@@ -310,6 +304,20 @@ template <int CTAS> __global__ void __launch_bounds__(kPlanThreads) pages_plan_k
     if (p.fork) p.sc.moves[r].x = st.table[(int64_t)p.other[lo] * st.max_pages + at];
   }
   if (me == 0) p.sc.n_moves[0] = p.fork ? grants.total : 0;
+  for (int i = i0; i < i1; ++i) {  // here no barrier waits for these stores
+    if (per > 1) {
+      row = p.rows[i];
+      other = p.other[i];
+      kept = p.sc.kept[i];
+    }
+    if (!p.fork) {
+      if (kept >= -1 && other != 0) p.sc.guard[row].refused = kept < 0;
+    } else if (kept >= 0) {  // a parent of whole pages is no child, and all its entries say the same
+      const int shared = p.share ? kept * kPage : 0;
+      p.sc.guard[row] = Guard{shared, 0};
+      if (shared > 0) p.sc.guard[other].shared = shared;
+    }
+  }
 }
 
 // Live pages at or past the number of live pages move into the holes below it, in order.
@@ -496,12 +504,13 @@ __global__ void __launch_bounds__(kMoveThreads) pages_write_kernel(const WritePa
       }
       row = p.rows[lo];
       good = (unsigned)row < (unsigned)st.n_rows && start >= 0 && end <= p.n_tokens;
+      const int len = good ? len_of(st, row) : 0;
+      const Guard g = good ? p.guard[row] : Guard{0, 0};
       bool again = false;
       for (int i = lane; good && i < lo; i += 32) again |= p.rows[i] == row;
       good = good && !__any_sync(0xffffffffu, again);  // a row named twice: the first entry counts
       if (good) {
-        const Guard g = p.guard[row];
-        first = len_of(st, row) - (end - start);
+        first = len - (end - start);
         good = first >= 0 && g.refused == 0;
         const int shared = min(g.shared, first + end - start);
         if (good && first < shared) {  // no page of these may be another row's too
