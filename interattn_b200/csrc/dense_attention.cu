@@ -436,8 +436,11 @@ __global__ void __launch_bounds__(kThreads) shared_attention_kernel(const Shared
 
 // out[row] = sum_s o_s 2^(lse_s - M) / sum_s 2^(lse_s - M) over partial rows, a warp per output row.  Lane i fetches the i-th
 // log-sum-exp, so the weights are there before the first partial row, whose loads then do not depend on one another.
+// A part with a log-sum-exp of -infinity is one that the row sees nothing of, and zeros, or one whose logits are all -infinity, and
+// NaN.  Neither weighs anything, so its row is not multiplied but left out; only where every part is of this kind does
+// a NaN among them count: infinity minus infinity, as if the keys had not been cut.
 template <int D> struct Merged {
-  float acc[D / 32], M = -INFINITY, L = 0.f;
+  float acc[D / 32], M = -INFINITY, L = 0.f, weightless = 0.f;
   __device__ __forceinline__ Merged() {
 #pragma unroll
     for (int i = 0; i < D / 32; ++i) acc[i] = 0.f;
@@ -448,28 +451,41 @@ template <int D> struct Merged {
     const float lse = lane < count ? __ldcg(lses + row) * kLog2e : -INFINITY;
     const float* src = o + row * D;
     const float m = fmaxf(M, warp_max(lse)), base = m == -INFINITY ? 0.f : m;
-    const float keep = exp2f(M - base), w = exp2f(lse - base);  // a part without a visible key: weight 0, o is 0
+    const float keep = exp2f(M - base), w = exp2f(lse - base);
+    const unsigned none = __ballot_sync(0xffffffffu, lane < count && lse == -INFINITY);
     L = L * keep + warp_sum(w);
     M = m;
 #pragma unroll
     for (int i = 0; i < D / 32; ++i) acc[i] *= keep;
+    if (none == 0) {
 #pragma unroll 8
-    for (int s = 0; s < count; ++s) {
-      const float ws = __shfl_sync(0xffffffffu, w, s);
-      const float* from = (const float*)__shfl_sync(0xffffffffu, (unsigned long long)src, s) + lane * (D / 32);
-      if constexpr (D == 128) {
-        const float4 x = __ldcg(reinterpret_cast<const float4*>(from));
-        acc[0] += ws * x.x; acc[1] += ws * x.y; acc[2] += ws * x.z; acc[3] += ws * x.w;
-      } else {
-        const float2 x = __ldcg(reinterpret_cast<const float2*>(from));
-        acc[0] += ws * x.x; acc[1] += ws * x.y;
-      }
+      for (int s = 0; s < count; ++s) add_row(src, w, s, false);
+    } else {  // apart: the usual case keeps its short loop
+#pragma unroll 4
+      for (int s = 0; s < count; ++s) add_row(src, w, s, none >> s & 1);
     }
   }
-  template <typename T> __device__ __forceinline__ void store(T* to) {
-    const float inv = L == 0.f ? 0.f : 1.f / L;  // no keys: zeros
+  // lane s's row by its weight
+  __device__ __forceinline__ void add_row(const float* src, float w, int s, bool none) {
+    constexpr int V = D / 32;
+    const float ws = __shfl_sync(0xffffffffu, w, s);
+    const float* from = (const float*)__shfl_sync(0xffffffffu, (unsigned long long)src, s) + (threadIdx.x & 31) * V;
+    float x[V];
+    if constexpr (D == 128) {
+      const float4 v = __ldcg(reinterpret_cast<const float4*>(from));
+      x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+    } else {
+      const float2 v = __ldcg(reinterpret_cast<const float2*>(from));
+      x[0] = v.x; x[1] = v.y;
+    }
+    if (none) weightless += x[0];
 #pragma unroll
-    for (int i = 0; i < D / 32; ++i) acc[i] *= inv;
+    for (int i = 0; i < V; ++i) acc[i] += ws * (none ? 0.f : x[i]);
+  }
+  template <typename T> __device__ __forceinline__ void store(T* to) {
+    const float inv = L == 0.f ? 0.f : 1.f / L;
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) acc[i] = L == 0.f ? weightless : acc[i] * inv;  // no keys: zeros
     store_vec<D / 32>(to + (threadIdx.x & 31) * (D / 32), acc);
   }
 };

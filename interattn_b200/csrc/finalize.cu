@@ -4,7 +4,8 @@
 // (llama/script/analysis/condition_block_gen/methods/condition_block_triton_impl/legacy.py:765-794),
 // written for normalised partials: with o_s = acc_s / l_s and
 // lse_s = m_s + log l_s,  out = sum_s o_s e^{lse_s - M} / sum_s e^{lse_s - M},
-// M = max_s lse_s.  A part with lse = -inf carries nothing; a row whose parts
+// M = max_s lse_s.  A part with lse = -inf carries nothing, whatever its row holds (NaN
+// where all its logits are -inf); a row whose parts
 // are all empty gives 0 (the reference clamps the denominator to 1e-30).
 // One warp per output row; the partials are a few hundred bytes per row, so
 // this kernel is launch-latency bound.
@@ -40,12 +41,12 @@ condition_block_stage2_reduce_kernel(const float* __restrict__ o_partial,
   const float* o = o_partial + (int64_t)row * n_parts * D + lane * VEC;
   for (int g = 0; g < n_groups; ++g)
     for (int s = 0; s < n_parts; ++s) {
-      const float w = expf(lse[g * group_stride + s] - ref);  // exp(-inf) = 0 for an empty part
+      const float part = lse[g * group_stride + s], w = expf(part - ref);  // exp(-inf) = 0 for an empty part
       float v[VEC];
       load_vec<VEC>(o + g * group_stride + (int64_t)s * D, v);
       den += w;
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) acc[i] = fmaf(w, v[i], acc[i]);
+      for (int i = 0; i < VEC; ++i) acc[i] = fmaf(w, part == -INFINITY ? 0.f : v[i], acc[i]);
     }
   const float inv = 1.f / fmaxf(den, 1e-30f);
 #pragma unroll
