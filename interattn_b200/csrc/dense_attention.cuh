@@ -201,24 +201,48 @@ __device__ __forceinline__ SharedCursor find_share(const SharedParams& p, int ct
 // The tiled kernels multiply masked places by a weight of zero, and zero times an infinity or a NaN is a NaN.  A row whose
 // result is not finite is therefore looked at again: if a value row that the row's tiles held but the row does not see is
 // not finite, the row is redone here from the keys it sees.  Key(j) gives the addresses of key and value row j.
-template <typename T, int D> __device__ __forceinline__ bool row_not_finite(const T* v) {
+template <typename T, int D> __device__ __forceinline__ bool row_not_finite(const T* v) {  // by one thread
   bool bad = false;
-  for (int d = threadIdx.x & 31; d < D; d += 32) bad |= !(fabsf(to_f32(v[d])) <= 3.4028235e38f);
-  return __any_sync(0xffffffffu, bad);
-}
-// the last key in [lo, hi) whose value row is not finite, or -1; by a whole warp
-template <typename T, int D, typename Key> __device__ int last_not_finite(int lo, int hi, const Key& key) {
-  int last = -1;
-  for (int j = lo; j < hi; ++j) {
-    const T *k, *v;
-    if (key(j, k, v) && row_not_finite<T, D>(v)) last = j;
+#pragma unroll 4
+  for (int d = 0; d < D; d += 4) {
+    float x[4];
+    load_vec<4>(v + d, x);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) bad |= !(fabsf(x[e]) <= 3.4028235e38f);
   }
+  return bad;
+}
+// The last key in [lo, hi) whose value row is not finite, or -1, by a whole warp, a lane a key.  Where several warps share the search,
+// this one takes the 32 keys from lo + first on and every `step` after.
+template <typename T, int D, typename Key> __device__ __forceinline__ int last_not_finite(int lo, int hi, const Key& key, int first = 0, int step = 32) {
+  int last = -1;
+  for (int64_t j = (int64_t)lo + first + (threadIdx.x & 31); j < hi; j += step) {
+    const T *k, *v;
+    if (key((int)j, k, v) && row_not_finite<T, D>(v)) last = (int)j;
+  }
+#pragma unroll  // not one instruction: with it here the assembler finds no registers for the fp32 kernel
+  for (int o = 16; o > 0; o >>= 1) last = max(last, __shfl_xor_sync(0xffffffffu, last, o));
   return last;
 }
-// softmax(q . k_j * scale) v_j over [lo, hi) by a whole warp; lane l ends up with the dims l, l + 32, ...
-template <typename T, int D, typename Key>
-__device__ void exact_row(const T* q, int lo, int hi, float scale_log2, const Key& key, float (&o)[D / 32], float& m,
+template <int N> __device__ __forceinline__ void unpack16(const uint4& w, float (&x)[N]) {
+  const uint32_t r[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (N == 8) {
+      x[2 * i] = bf16lo(r[i]);
+      x[2 * i + 1] = bf16hi(r[i]);
+    } else {
+      x[i] = __uint_as_float(r[i]);
+    }
+  }
+}
+// softmax(q . k_j * scale) v_j over [lo, hi) by a whole warp: a lane takes every 32nd key's logit, then the dims l, l + 32, ... of the
+// values.  Bound by the latency of its loads: kAhead of them are on their way together, as many as the kernel has registers for.  A
+// row whose every dim is NaN stays so: it ends there.
+template <typename T, int D, int kAhead, typename Key>
+__device__ __forceinline__ void exact_row(const T* q, int lo, int hi, float scale_log2, const Key& key, float (&o)[D / 32], float& m,
                           float& l) {
+  constexpr int kVec = 16 / sizeof(T), kLoads = D / kVec < kAhead ? D / kVec : kAhead;
   const int lane = threadIdx.x & 31;
   float qv[D / 32];
 #pragma unroll
@@ -228,21 +252,60 @@ __device__ void exact_row(const T* q, int lo, int hi, float scale_log2, const Ke
   }
   m = -INFINITY;
   l = 0.f;
-  for (int j = lo; j < hi; ++j) {
-    const T *k, *v;
-    if (!key(j, k, v)) continue;
+#pragma unroll 1
+  for (int64_t j0 = lo; j0 < hi; j0 += 32) {
+    const T *k = q, *v = q;
+    const bool seen = j0 + lane < hi && key((int)j0 + lane, k, v);
     float s = 0.f;
 #pragma unroll
-    for (int i = 0; i < D / 32; ++i) s += qv[i] * to_f32(k[lane + 32 * i]);
-    s = warp_sum(s);
-    const float m_new = fmaxf(m, s);
+    for (int d0 = 0; d0 < D; d0 += kLoads * kVec) {
+      uint4 raw[kLoads];
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) raw[i] = seen ? *reinterpret_cast<const uint4*>(k + d0 + i * kVec) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        float x[kVec];
+        unpack16(raw[i], x);
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) {
+          const int d = d0 + i * kVec + e;
+          s += __shfl_sync(0xffffffffu, qv[d / 32], d % 32) * x[e];
+        }
+      }
+    }
+    if (!seen) s = -INFINITY;
+    const float m_new = fmaxf(m, warp_max(s));
     const float base = m_new == -INFINITY ? 0.f : m_new;
     const float keep = exp2f(m - base), w = exp2f(s - base);
-    l = l * keep + w;
+    l = l * keep + (seen ? w : 0.f);
 #pragma unroll
-    for (int i = 0; i < D / 32; ++i) o[i] = o[i] * keep + w * to_f32(v[lane + 32 * i]);
+    for (int i = 0; i < D / 32; ++i) o[i] *= keep;
+    const unsigned which = __ballot_sync(0xffffffffu, seen);
+#pragma unroll 1
+    for (int s0 = 0; s0 < 32; s0 += kAhead) {
+      T x[kAhead][D / 32];
+#pragma unroll
+      for (int s1 = 0; s1 < kAhead; ++s1) {
+        const T* from = (const T*)__shfl_sync(0xffffffffu, (unsigned long long)v, s0 + s1);
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) x[s1][i] = from[lane + 32 * i];  // of a key that is not seen: the query, unused
+      }
+#pragma unroll
+      for (int s1 = 0; s1 < kAhead; ++s1) {
+        const float ws = __shfl_sync(0xffffffffu, w, s0 + s1);
+        if (which >> (s0 + s1) & 1) {
+#pragma unroll
+          for (int i = 0; i < D / 32; ++i) o[i] += ws * to_f32(x[s1][i]);
+        }
+      }
+    }
     m = m_new;
+    bool lost = true;
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) lost &= o[i] != o[i];
+    if (__all_sync(0xffffffffu, lost)) break;
   }
+  l = warp_sum(l);
 }
 
 template <typename T> struct PackedKeys {  // the keys of one sequence and kv head

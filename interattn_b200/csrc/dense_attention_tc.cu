@@ -673,10 +673,12 @@ template <int D, bool PAGED> struct MmaRole {
 };
 
 // ---- softmax warps ----------------------------------------------------------------------------------------------------
+template <bool PAGED, bool PARTS> using OutOf = std::conditional_t<PAGED || PARTS, float, __nv_bfloat16>;
+
 template <int D, bool PAGED, bool PARTS>
 __device__ __forceinline__ void softmax_role(const TcParams& p, Bars* bars, const Work* ring, uint32_t tmem, unsigned char* out_base,
-                                             float2 (*stats)[kRows]) {
-  using Out = std::conditional_t<PAGED || PARTS, float, __nv_bfloat16>;
+                                             float2 (*stats)[kRows], int* flagged) {
+  using Out = OutOf<PAGED, PARTS>;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, w = warp >> 2, row = (warp & 3) * 32 + lane;
   const int G = p.group, tpm = kRows / G, row_tok = row / G, g = row % G;
   const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
@@ -711,7 +713,7 @@ __device__ __forceinline__ void softmax_role(const TcParams& p, Bars* bars, cons
     const int least = __reduce_min_sync(0xffffffffu, valid ? limit : 0x7fffffff);  // below it nothing is masked
     float m = -INFINITY, l = 0.f;
     for (int j = begin; j < total; j += stride) {
-            if (!wait(&bars->s_full[w], s_it & 1)) return;
+      if (!wait(&bars->s_full[w], s_it & 1)) return;
       ++s_it;
       if (busy) {
         tc_fence_after();
@@ -894,35 +896,7 @@ __device__ __forceinline__ void softmax_role(const TcParams& p, Bars* bars, cons
     float nan_lo, nan_hi;
     unpair(add2(not_finite[0], not_finite[1]), nan_lo, nan_hi);
     const unsigned bad = __ballot_sync(0xffffffffu, valid && !(nan_lo + nan_hi == 0.f));
-    if (bad != 0) {  // see exact_row
-      using T = __nv_bfloat16;
-      const auto redo = [&](const auto& key, const T* q, int64_t tok_stride, int64_t head_stride) {
-        const int last = last_not_finite<T, D>(least, PAGED ? wk.n_keys : total * kKeys, key);
-        for (int r = 0; r < 32; ++r) {
-          const int lim = __shfl_sync(0xffffffffu, limit, r), to = __shfl_sync(0xffffffffu, at, r);
-          const int q_tok = __shfl_sync(0xffffffffu, tok, r), q_head = __shfl_sync(0xffffffffu, g, r);
-          if (!((bad >> r) & 1) || last < lim) continue;
-          float x[D / 32], mx, lx;
-          exact_row<T, D>(q + q_tok * tok_stride + q_head * head_stride, 0, lim, c, key, x, mx, lx);
-#pragma unroll
-          for (int i = 0; i < D / 32; ++i)
-            if (lane + 32 * i >= col0 && lane + 32 * i < col1) from_f32(out[to + lane + 32 * i], x[i] / lx);
-        }
-      };
-      __syncwarp();
-      if constexpr (PAGED) {
-        const PagedKeys<T> key{(const T*)p.s.k_pool + wk.head * p.s.head_stride, (const T*)p.s.v_pool + wk.head * p.s.head_stride,
-                               p.s.block_table + (int64_t)wk.row * p.s.max_pages + (wk.key0 >> 4), p.s.page_stride, D,
-                               p.s.n_pool_pages, p.s.max_pages - (wk.key0 >> 4)};
-        redo(key, (const T*)p.s.q + (wk.q_tok * hq + wk.head * G) * D, hq * D, D);
-      } else {
-        const PackedKeys<T> key{(const T*)p.t.k + wk.key0 * p.t.k_tok_stride + wk.head * p.t.k_head_stride,
-                                (const T*)p.t.v + wk.key0 * p.t.v_tok_stride + wk.head * p.t.v_head_stride, p.t.k_tok_stride,
-                                p.t.v_tok_stride, p.t.n_kv_tok - wk.key0};
-        redo(key, (const T*)p.t.q + (int64_t)wk.q_tok * p.t.q_tok_stride + (int64_t)wk.head * G * p.t.q_head_stride, p.t.q_tok_stride,
-             p.t.q_head_stride);
-      }
-    }
+    if (bad != 0 && lane == 0) *flagged = 1;  // see redo_rows
     done();
   }
 }
@@ -932,7 +906,111 @@ struct Control {
   Work ring[kWorkSlots];
   float2 stats[2][kRows];  // (m, l) of either set, for the merge
   uint32_t tmem;
+  int flagged;             // some row came out non-finite
 };
+
+// ---- rows that came out non-finite ------------------------------------------------------------------------------------
+// See exact_row.  How long this takes grows with the rows times their keys, so it waits until the CTA's last piece is done and no
+// role waits for another within a limit.  The pieces are gone through once more: which of their rows are not finite, which is
+// the last bad value row that one of them held but does not see, and the rows that do not see it again, a warp each.  An 8192-token
+// prompt of the Llama-3-8B heads whose last value is infinite: 18.7 ms instead of 0.57 (63 tokens of the last piece, eight SMs busy);
+// with a NaN at every 1000th token 1.2 ms, at all of them 1.9 ms; 4 x 4800 tokens behind 150,000 each, the last of each
+// infinite: 267 ms instead of 12.
+struct Redo {
+  unsigned rows[2 * kRows / 32];  // a bit a row
+  int least, last;                // least limit of these rows; last bad key
+};
+template <int D, bool PAGED, bool PARTS, typename Key>
+__device__ __forceinline__ void redo_piece(const TcParams& p, const Work& wk, int end, const Key& key, const __nv_bfloat16* q, int64_t q_tok_stride,
+                           int64_t q_head_stride, OutOf<PAGED, PARTS>* out, int64_t out_tok_stride, Redo* redo) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, G = p.group, rows = wk.n_tok * G;
+  constexpr int kWarps = kThreads / 32;
+  __syncthreads();  // the piece before is done with the shared words
+  if (threadIdx.x < 2 * kRows / 32) redo->rows[threadIdx.x] = 0;
+  if (threadIdx.x == 0) {
+    redo->least = 0x7fffffff;
+    redo->last = -1;
+  }
+  __syncthreads();
+  for (int r = warp; r < rows; r += kWarps) {
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) bad |= !(fabsf(to_f32(out[r / G * out_tok_stride + r % G * D + lane + 32 * i])) <= 3.4028235e38f);
+    if (!__any_sync(0xffffffffu, bad) || lane != 0) continue;
+    atomicOr(&redo->rows[r / 32], 1u << (r & 31));
+    atomicMin(&redo->least, row_limit<PAGED>(p, wk, r / G));
+  }
+  __syncthreads();
+  if (redo->least >= end) return;
+  const int last = last_not_finite<__nv_bfloat16, D>(redo->least, end, key, warp * 32, kThreads);
+  if (lane == 0) atomicMax(&redo->last, last);
+  __syncthreads();
+  for (int r = warp; r < rows; r += kWarps) {
+    const int limit = row_limit<PAGED>(p, wk, r / G);
+    if (!(redo->rows[r / 32] >> (r & 31) & 1) || redo->last < limit) continue;
+    float x[D / 32], m, l;
+    exact_row<__nv_bfloat16, D, 16>(q + r / G * q_tok_stride + r % G * q_head_stride, 0, limit, kLog2e * rsqrtf((float)D), key, x, m, l);
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) from_f32(out[r / G * out_tok_stride + r % G * D + lane + 32 * i], x[i] / l);
+  }
+}
+template <int D, bool PAGED, bool PARTS>
+__device__ __noinline__ void redo_rows(const TcParams& p, unsigned long long* scratch, Redo* redo) {
+  using T = __nv_bfloat16;
+  const int G = p.group;
+  Work wk{};
+  if constexpr (PAGED) {
+    const SharedParams& s = p.s;
+    const int64_t hq = (int64_t)G * s.n_kv_heads;
+    SharedCursor c = find_share<kKeys, kThreads>(s, blockIdx.x, gridDim.x, scratch);
+    while (c.left > 0) {
+      const SharedEntity ent = load_entity(s, c.e);
+      int lo, hi;
+      entity_keys(s, c.e, ent, lo, hi);
+      const int n = (int)min((int64_t)(c.units - c.k), c.left);
+      const bool own = c.e >= s.n_shared;
+      const int2 lead = own ? make_int2(ent.first_seq, hi) : entity_lead(s, ent, hi);
+      wk.q_tok = ent.first_seq;
+      wk.n_tok = ent.n_seqs;
+      wk.key0 = lo + c.k * kKeys;
+      wk.n_keys = max(0, min(lead.y, wk.key0 + n * kKeys) - wk.key0);
+      const int64_t row0 = c.k == 0 ? item_rows(s, own, ent.first_seq, ent.n_seqs, c.h) : cta_rows(s, blockIdx.x);
+      const PagedKeys<T> key{(const T*)s.k_pool + c.h * s.head_stride, (const T*)s.v_pool + c.h * s.head_stride,
+                             s.block_table + (int64_t)lead.x * s.max_pages + (wk.key0 >> 4), s.page_stride, D, s.n_pool_pages,
+                             s.max_pages - (wk.key0 >> 4)};
+      redo_piece<D, PAGED, PARTS>(p, wk, wk.n_keys, key, (const T*)s.q + (wk.q_tok * hq + c.h * G) * D, hq * D, D, s.o + row0 * D,
+                                  (int64_t)G * D, redo);
+      c.left -= n;
+      c.k = 0;
+      if (++c.h == s.n_kv_heads) {
+        c.h = 0;
+        if (c.left > 0)  // some entity behind this one has units: they were counted
+          do c.units = entity_units<kKeys>(s, ++c.e);
+          while (c.units == 0);
+      }
+    }
+  } else {
+    const PromptTensors& t = p.t;
+    const int64_t hq = (int64_t)G * t.n_kv_heads;
+    for (int i = p.cta_begin[blockIdx.x]; i < p.cta_begin[blockIdx.x + 1]; ++i) {
+      const PromptItem item = p.items[i];
+      wk.n_tok = item.n_tok;
+      wk.limit0 = item.limit0;
+      wk.n_keys = item.kv_len;
+      const PackedKeys<T> key{(const T*)t.k + item.kv_tok * t.k_tok_stride + item.head * t.k_head_stride,
+                              (const T*)t.v + item.kv_tok * t.v_tok_stride + item.head * t.v_head_stride, t.k_tok_stride,
+                              t.v_tok_stride, t.n_kv_tok - item.kv_tok};
+      const int end = (max(1, row_limit<false>(p, wk, item.n_tok - 1)) + kKeys - 1) / kKeys * kKeys;  // of the tiles that it held
+      const T* q = (const T*)t.q + item.q_tok * t.q_tok_stride + (int64_t)item.head * G * t.q_head_stride;
+      if constexpr (PARTS)
+        redo_piece<D, PAGED, PARTS>(p, wk, end, key, q, t.q_tok_stride, t.q_head_stride, t.part_o + (int64_t)item.slot * kPartRows * D,
+                                    (int64_t)G * D, redo);
+      else
+        redo_piece<D, PAGED, PARTS>(p, wk, end, key, q, t.q_tok_stride, t.q_head_stride,
+                                    (T*)t.out + (item.q_tok * hq + item.head * G) * D, hq * D, redo);
+    }
+  }
+}
 
 template <int D, bool PAGED, bool PARTS>
 __global__ void __launch_bounds__(kThreads, 1) attend_tc_kernel(const __grid_constant__ TcParams p) {
@@ -966,6 +1044,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tc_kernel(const __grid_con
       mbar_init(&bars.work_empty[i], 10);  // eight softmax warps and two MMA threads
     }
     mbar_init(&bars.drain, 2);
+    ctl.flagged = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == kMmaWarp) {
@@ -981,7 +1060,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tc_kernel(const __grid_con
   SharedCursor cur{};
   if constexpr (PAGED) cur = find_share<kKeys, kThreads>(p.s, blockIdx.x, gridDim.x, reinterpret_cast<unsigned long long*>(ctl.stats));
   if (warp < kCopyWarp) {
-    softmax_role<D, PAGED, PARTS>(p, &bars, ctl.ring, tmem, base + C::tiles, ctl.stats);
+    softmax_role<D, PAGED, PARTS>(p, &bars, ctl.ring, tmem, base + C::tiles, ctl.stats, &ctl.flagged);
   } else {
     if (warp == kCopyWarp) CopyRole<D, PAGED>(p, &bars, ctl.ring, base, cur).run();
     if (warp >= kMmaWarp) MmaRole<D, PAGED>(p, &bars, ctl.ring, smem_u32(base), uniform(tmem), uniform(warp - kMmaWarp)).run();
@@ -992,6 +1071,8 @@ __global__ void __launch_bounds__(kThreads, 1) attend_tc_kernel(const __grid_con
   tc_fence_after();
   if (warp == kMmaWarp)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+  if (ctl.flagged != 0)
+    redo_rows<D, PAGED, PARTS>(p, reinterpret_cast<unsigned long long*>(ctl.stats), reinterpret_cast<Redo*>(base));
 }
 
 // ---- host -------------------------------------------------------------------------------------------------------------
