@@ -641,7 +641,7 @@ int launch_shared_merge(const SharedParams& p, const int32_t* seq_info, int head
 // Words: a header of 8, where each CTA's items begin (ctas + 1 words, padded to whole items), the items, and the pieces where
 // they are cut.
 namespace {
-constexpr int kRowsFew = 32, kRowsFull = 128;
+constexpr int kRowsFew = 32, kRowsFull = 128, kMostParts = 32;  // parts an SM, at most
 struct PlanShape {
   int n_items, ctas, item_tokens;
   bool few_rows;
@@ -711,6 +711,18 @@ int64_t spread(const std::vector<PromptItem>& items, int ctas, int dtype, bool f
   }
   return most;
 }
+struct PlanTotals { int64_t cost, longest; };  // of all pieces, and of the costliest
+PlanTotals totals_of(const PlanInput& in, const PlanShape& s) {
+  PlanTotals t{0, 0};
+  for (int i = 0; i < in.n_seqs; ++i)
+    for (int64_t at = 0; at < in.q_lens[i]; at += s.item_tokens) {
+      const int n = (int)std::min<int64_t>(s.item_tokens, in.q_lens[i] - at);
+      const int64_t cost = piece_cost(PromptItem{0, n, 0, (int)(in.kv_lens[i] - in.q_lens[i] + at + 1), in.kv_lens[i], 0, 0, 0}, in.dtype, s.few_rows);
+      t.cost += cost * in.n_kv_heads;
+      t.longest = std::max(t.longest, cost);
+    }
+  return t;
+}
 PlanShape shape_of(const PlanInput& in, bool few_rows, bool* fits) {
   const int rows = kRowsFull / in.group;
   PlanShape s;
@@ -724,19 +736,44 @@ PlanShape shape_of(const PlanInput& in, bool few_rows, bool* fits) {
   s.ctas = in.dtype == IA_F32 ? (int)n : (int)std::min<int64_t>(n, sm_count());
   return s;
 }
+// What merging parts costs: as much as starting a large piece or two, and past two parts an SM the traffic of their rows through
+// memory, out and back, at an SM's share of the copy peak.
+int64_t merge_cost(const std::vector<PromptItem>& parts, int sms, const PlanInput& in) {
+  int64_t rows = 0;
+  for (const PromptItem& it : parts) rows += (int64_t)it.n_tok * in.group;
+  const int64_t more = std::max<int64_t>(0, rows / sms - 2 * kPartRows);
+  return in.dtype == IA_F32 ? 2 * 4 * 32 + more / 3 : 4 * 256 + 5 * more;
+}
 // Large pieces (128 rows in fp32, two tiles of 128 on the tensor cores) use what they read better, small ones (32, one tile)
 // spread a short batch over more SMs: the plan is made for both and the one whose busiest SM ends first is taken.  32 / 8
 // heads of 128, small and large pieces, us: fp32 one prompt of 600: 139 and 166, of 900: 301 and 242, 150, 30, 10, 400, 5 and
 // 77: 90 and 119, four of 300: 156 and 131; bf16 one of 600: 18.5 and 23.5, of 1700: 45 and 44, four of 300: 22.7 and 19.5,
-// three of 700: 37 and 31.  With four large pieces an SM the small ones gain nothing more (bf16 3000 and 2300: 148 and 138).
+// three of 700: 37 and 31, 3000 and 2300: 148 and 138.
 // Keys whole and cut, us: one token behind 16000: fp32 1742 and 111, bf16 146 and 30; 100 behind 8000: 893 and 476, 80 and 38;
 // eight times 4 behind 3000: 334 and 179, 43 and 36; one fp32 prompt of 600: 137 and 114.
+//
+// With four large pieces an SM or more either kind keeps the SMs busy, so the one whose pieces cost less in all is taken: the large
+// ones unless most are nearly empty.  On the tensor cores the small ones have to save an eighth: what they read twice counts
+// then.  That is all there is to decide where the costliest piece is at most a third of an SM's work (handing out the longest
+// first, the busiest SM then has at most a third too much), or where there are so many pieces that parts of all of them would take
+// more than 0.3 GB of workspace; else the search goes on as with few.  Large and whole against what is taken, us, one token each
+// behind 500 keys: 74 sequences fp32 516 and 193 (small), bf16 39.6 and 39.9 (small); one of them behind 16000: 3903 and 409 (cut),
+// 147 and 67 (cut).  bf16: 100 pieces of 64 behind 200, one behind 30000: 524 and 170 (cut); 512 behind 16000 beside 11 behind
+// 188: 317 and 220 (small); a prompt of 2000 and 100 of 30: 56.7 and, small, 59.2 (large is taken).
 bool plan_shape(const PlanInput& in, PlanShape* s) {
   bool fits, fits_few;
   *s = shape_of(in, false, &fits);
-  if (!fits || s->n_items >= 4 * sm_count()) return fits;
+  const bool many = s->n_items >= 4 * sm_count();
+  const auto must_save = [&](int64_t cost) { return many && in.dtype != IA_F32 ? cost / 8 : 0; };
   const PlanShape shapes[2] = {*s, shape_of(in, true, &fits_few)};
   const int sms = sm_count();
+  if (!fits || !fits_few) return fits;
+  if (many) {
+    const PlanTotals totals[2] = {totals_of(in, shapes[0]), totals_of(in, shapes[1])};
+    const int few = totals[1].cost < totals[0].cost - must_save(totals[0].cost);
+    *s = shapes[few];
+    if (3 * sms * totals[few].longest <= totals[few].cost || shapes[0].n_items > kMostParts * sms) return true;
+  }
   int64_t q, kv, best = 0, ideal[2] = {0, 0}, keys[2] = {0, 0};
   std::vector<PromptItem> whole[2];
   for (int few = 0; few < 2; ++few) {
@@ -746,19 +783,20 @@ bool plan_shape(const PlanInput& in, PlanShape* s) {
       ideal[few] += piece_cost(it, in.dtype, few != 0);
     }
     const int64_t cost = spread(whole[few], sms, in.dtype, few != 0, nullptr);
-    if (few != 0 && cost >= best) continue;
+    if (few != 0 && cost >= best - must_save(best)) continue;
     best = cost;
     *s = shapes[few];
   }
-  // Few rows and many keys: the keys are cut, for one or two parts an SM.  Merging them takes as long as starting a large piece or
-  // two.  A slot of the workspace holds one row tile, so on the tensor cores only small pieces are cut.
+  // Few rows and many keys: the keys are cut, for one or two parts an SM.  A slot of the workspace holds one row tile, so on the
+  // tensor cores only small pieces are cut.
   for (int few = in.dtype == IA_F32 ? 0 : 1; few < 2; ++few) {
     if (whole[few].empty() || best * sms < ideal[few] + ideal[few] / 3) continue;
     for (int waves = 1; waves <= 2; ++waves) {
       const int chunk = (int)(std::min<int64_t>(keys[few] / (sms * waves) + 128, 1 << 30) / 128 * 128);
       if (chunk >= piece_keys(whole[few][0])) continue;
       const std::vector<PromptItem> parts = cut_pieces(whole[few], chunk, nullptr);
-      const int64_t cost = spread(parts, sms, in.dtype, few != 0, nullptr) + (in.dtype == IA_F32 ? 2 * 4 * 32 : 4 * 256);
+      if ((int64_t)parts.size() > (int64_t)kMostParts * sms) continue;
+      const int64_t cost = spread(parts, sms, in.dtype, few != 0, nullptr) + merge_cost(parts, sms, in);
       if (cost >= best) continue;
       best = cost;
       *s = shapes[few];

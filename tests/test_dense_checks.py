@@ -112,6 +112,44 @@ def test_prompt_plan_cuts_keys_where_few_pieces_have_many(lib, dtype, lens, prio
     assert (plan[2] >= 2) == cut and (lib.ia_prompt_workspace_bytes(ints(plan[:8])) > 0) == cut
 
 
+def busiest_and_mean(plan):
+    n_items, ctas, _, first = plan[:4]
+    keys = [max(0, min(plan[first + 8 * i + 3] + plan[first + 8 * i + 1] - 1, plan[first + 8 * i + 4])) for i in range(n_items)]
+    return max(sum(keys[a:b]) for a, b in zip(plan[8:8 + ctas], plan[9:9 + ctas])), sum(keys) / 148, max(keys)
+
+
+@pytest.mark.parametrize("n", [73, 74, 75, 150, 400])
+def test_prompt_plan_of_one_long_sequence_among_many(lib, n):
+    """One token each, one behind 100000 keys: no SM walks them alone, on either side of four pieces an SM."""
+    for dtype in (_lib.IA_BF16, _lib.IA_F32):
+        plan = prompt_plan(lib, [1] * n, [100000] + [500] * (n - 1), 8, 4, 128, dtype)
+        busiest, mean, longest = busiest_and_mean(plan)
+        assert plan[2] >= 2 and plan[2] & 1 and longest < 100000
+        assert max(busiest if dtype == _lib.IA_BF16 else longest, mean) <= 1.4 * mean
+    plan = prompt_plan(lib, [1] * 40, [16000] + [500] * 39, 16, 4, 128, _lib.IA_BF16)
+    busiest, mean, _ = busiest_and_mean(plan)
+    assert busiest <= 1.4 * mean
+
+
+@pytest.mark.parametrize("n", [73, 74, 300, 2000])
+def test_prompt_plan_takes_small_pieces_for_few_rows_however_many_there_are(lib, n):
+    """A single token's four rows never get a tile of 128 in fp32, nor two of them in bf16."""
+    for dtype in (_lib.IA_F32, _lib.IA_BF16):
+        assert prompt_plan(lib, [1] * n, [500] * n, 8, 4, 128, dtype)[2] & 1
+
+
+@pytest.mark.parametrize("dtype,q_lens,prior,small,cut", [
+    (_lib.IA_F32, [10] * 150, [0] * 150, True, False), (_lib.IA_F32, [20] * 150, [0] * 150, False, False),
+    (_lib.IA_F32, [70] * 100, [0] * 100, False, False), (_lib.IA_BF16, [70] * 100, [0] * 100, False, False),
+    (_lib.IA_BF16, [40] * 150, [1000] * 150, False, False), (_lib.IA_BF16, [2000] + [30] * 100, [0] * 101, False, False),
+    (_lib.IA_BF16, [512] * 12, [16000] + [188] * 11, True, False), (_lib.IA_BF16, [64] * 100, [30000] + [200] * 99, True, True)])
+def test_prompt_plan_where_there_are_many_pieces(lib, dtype, q_lens, prior, small, cut):
+    """32 / 8 heads of 128 on 148 SMs; both sides were timed."""
+    plan = prompt_plan(lib, q_lens, [a + b for a, b in zip(q_lens, prior)], 8, 4, 128, dtype)
+    assert bool(plan[2] & 1) == small and (plan[2] >= 2) == cut
+    assert lib.ia_prompt_workspace_bytes(ints(plan[:8])) <= 32 * 148 * 128 * 129 * 4
+
+
 @pytest.mark.parametrize("change,word", [
     (dict(hkv=0), b"kv heads"), (dict(group=17), b"group size"), (dict(d=96), b"head_dim"), (dict(dtype=7), b"dtype"),
     (dict(q=[4, -1]), b"sequence 1"), (dict(kv=[4, -2]), b"sequence 1"), (dict(q=[1 << 30, 1]), b"tokens"),
