@@ -591,9 +591,10 @@ int64_t ia_pages_scratch_bytes(int n_rows, int n_pages);
  * ia_pages_write. */
 int ia_pages_extend(const ia_page_cache* cache, const int32_t* rows, const int32_t* n_tokens, int n, ia_stream_t stream);
 /* Keys and values of one layer: tokens [starts[i], starts[i + 1]) of k, v [n_tokens, n_kv_heads, head_dim] become the last
- * tokens of rows[i].  starts int32 [n + 1] ascending.  Strides in elements, multiples of 16 bytes.  An entry is refused with
- * IA_DEV_STATUS_BAD_INDEX, and nothing of it written, if the row's last ia_pages_extend that asked for tokens was refused, or if a
- * token would fall into a whole page that ia_pages_fork shared and that is still counted more than once. */
+ * tokens of rows[i].  starts int32 [n + 1]; tokens before the first and from the last on are nobody's.  Strides in elements, multiples
+ * of 16 bytes.  Refused with IA_DEV_STATUS_BAD_INDEX, and not written: the whole call, if a start lies below the one before it; an
+ * entry, if it lies outside the tokens, if the row's last ia_pages_extend that asked for tokens was refused, or if a token would
+ * fall into a whole page that ia_pages_fork shared and that is still counted more than once. */
 int ia_pages_write(const ia_page_cache* cache, const int32_t* rows, const int32_t* starts, int n, const void* k, const void* v,
                    int64_t k_tok_stride, int64_t k_head_stride, int64_t v_tok_stride, int64_t v_head_stride, int n_tokens,
                    void* k_pool, void* v_pool, ia_stream_t stream);

@@ -485,15 +485,32 @@ __global__ void __launch_bounds__(kMoveThreads) pages_write_kernel(const WritePa
   const int lane = threadIdx.x & 31;
   const int warps = gridDim.x * (kMoveThreads / 32), me = blockIdx.x * (kMoveThreads / 32) + (threadIdx.x >> 5);
   const int words = p.n_heads * p.run_words;
+  // Whose a token is is found by halves, which asks for starts that do not fall.  One CTA reports, also what no token would meet.
+  const int mine = lane < p.n ? p.starts[lane] : 0x7fffffff;  // the whole list, if a warp holds it (4 rows 3.08 us, by halves 3.27)
+  bool falls = false, outside = false;
+  for (int i = threadIdx.x; i < p.n; i += kMoveThreads) {
+    const int a = p.starts[i], b = p.starts[i + 1];
+    falls |= a > b;
+    outside |= a < 0 || b > p.n_tokens;
+  }
+  if (outside && blockIdx.x == 0) report(st, DEV_STATUS_BAD_INDEX);
+  if (__syncthreads_or(falls)) {
+    if (blockIdx.x == 0 && threadIdx.x == 0) report(st, DEV_STATUS_BAD_INDEX);
+    return;
+  }
   int entry = -1, row = 0, start = 0, end = 0, first = 0;  // the entry at hand: tokens [start, end), positions from `first`
   bool good = false;
   for (int t = me; t < p.n_tokens; t += warps) {
     if (entry < 0 || t < start || t >= end) {
       int lo = 0, hi = p.n - 1;  // last entry with starts[entry] <= t
-      while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (p.starts[mid] <= t) lo = mid;
-        else hi = mid - 1;
+      if (p.n <= 32) {
+        lo = max(0, __popc(__ballot_sync(0xffffffffu, mine <= t)) - 1);
+      } else {
+        while (lo < hi) {
+          const int mid = (lo + hi + 1) >> 1;
+          if (p.starts[mid] <= t) lo = mid;
+          else hi = mid - 1;
+        }
       }
       entry = lo;
       start = p.starts[lo];

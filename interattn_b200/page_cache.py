@@ -113,8 +113,9 @@ class PageCache:
 
     def write(self, layer: int, rows: torch.Tensor, starts: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> None:
         """Tokens ``[starts[i], starts[i + 1])`` of k and v ``[T, Hkv, D]`` (token and head strides of any multiple of 16 bytes)
-        become the last tokens of ``rows[i]`` in this layer.  Refused for a row whose last ``extend`` was refused, and where a
-        token would fall into a whole page that a fork shared while others still hold it."""
+        become the last tokens of ``rows[i]`` in this layer; tokens before the first start and from the last on belong to no row.
+        Refused for a row whose last ``extend`` was refused, where a token would fall into a whole page that a fork shared
+        while others still hold it, outside the tokens, and for all rows if a start lies below the one before it."""
         shape, ks, vs = k.shape, k.stride(), v.stride()
         if shape != v.shape:
             raise ValueError("k and v hold the same tokens")

@@ -208,3 +208,55 @@ def test_captured_loop_with_a_refused_row():
     put(want, cache, 0, 33, k[0], v[0]), put(want, cache, 1, 32, k[1], v[1])
     unchanged(cache, want)
     assert cache.seq_lens.tolist() == [34, 33, 64, 0] and ops.device_status() == 0
+
+
+TOP = 2 ** 31 - 1
+
+
+@pytest.mark.parametrize("starts", [[0, 40, 20, 60], [0, 10, 5, 60], [5, 2, 2, 2], [60, 60, 60, 59], [0, 0, -5, 10], [0, 60, 0, 60],
+                                    [TOP, -TOP - 1, 0, 60]])
+def test_starts_that_fall_are_refused_as_a_whole(starts):
+    """Which tokens such a list means cannot be said: nothing is written, and it is reported."""
+    cache = make(40, 4, 8)
+    cache.extend(i32([0, 1, 2]), i32([40, 40, 40]))
+    want = copies(cache)
+    write_all(cache, [0, 1, 2], starts, *tokens(60))
+    assert ops.device_status() == BAD
+    unchanged(cache, want)
+
+
+@pytest.mark.parametrize("starts,good", [([0, 20, 40, 61], 2), ([-1, 20, 40, 60], [1, 2]), ([0, 30, 60, TOP], 2), ([61, 61, 61, 61], []),
+                                         ([TOP - 5, TOP - 3, TOP - 1, TOP], []), ([-TOP - 1, -9, -9, 20], [])])
+def test_starts_outside_the_tokens_are_reported(starts, good):
+    """Also where no token belongs to such an entry; the others are written."""
+    good = list(range(good)) if isinstance(good, int) else good
+    cache = make(40, 4, 8)
+    cache.extend(i32([0, 1, 2]), i32([40, 40, 40]))
+    want = copies(cache)
+    k, v = tokens(60)
+    write_all(cache, [0, 1, 2], starts, k, v)
+    assert ops.device_status() == BAD
+    for i in good:
+        for t in range(starts[i], starts[i + 1]):
+            put(want, cache, i, 40 - starts[i + 1] + t, k[t], v[t])
+    unchanged(cache, want)
+
+
+def test_tokens_before_the_first_and_behind_the_last_start_are_left_out():
+    n = 700                                                    # more entries than a CTA has threads
+    cache = make(1500, n, 2)
+    cache.extend(i32(range(n)), i32([3] * n))
+    want = copies(cache)
+    k, v = tokens(2 * n + 9)
+    starts = [4 + 2 * i for i in range(n + 1)]
+    write_all(cache, list(range(n)), starts, k, v)
+    for kp, vp in want:
+        for pool, x in ((kp, k), (vp, v)):
+            pages = cache.block_table[:, 0].long()
+            pool[pages, :, 1], pool[pages, :, 2] = x[4:4 + 2 * n:2], x[5:5 + 2 * n:2]
+    unchanged(cache, want)
+    assert ops.device_status() == 0
+    starts[650] = starts[649] - 1
+    write_all(cache, list(range(n)), starts, v, k)
+    assert ops.device_status() == BAD
+    unchanged(cache, want)
