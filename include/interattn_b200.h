@@ -539,7 +539,7 @@ typedef struct ia_prompt_tensors {
   void* out;             /* [q tokens, query heads, head_dim] contiguous, 16-byte aligned */
   float* lse;            /* [q tokens, query heads] natural log-sum-exp, -inf for rows without keys; may be null */
   int64_t q_tok_stride, q_head_stride, k_tok_stride, k_head_stride, v_tok_stride, v_head_stride; /* elements; multiples of
-                            16 bytes, head_dim elements contiguous */
+                            16 bytes (of one token or one head: any), head_dim elements contiguous */
   int32_t n_q_tokens, n_kv_tokens, n_kv_heads, group_size, head_dim, dtype;
 } ia_prompt_tensors;
 /* plan_host: the first 8 words of the plan (host memory); plan_device: all of it.  workspace: 16-byte aligned,

@@ -670,6 +670,12 @@ static bool strides_ok(int64_t tok, int64_t head, int head_dim, int size) {
   return tok >= head_dim && head >= head_dim && (tok * size) % 16 == 0 && (head * size) % 16 == 0;
 }
 
+// The stride of a dimension of one element is never stepped by and may be anything; here it becomes one that passes.
+static void settle_strides(int64_t tokens, int64_t heads, int head_dim, int64_t* tok, int64_t* head) {
+  if (tokens == 1) *tok = head_dim;
+  if (heads == 1) *head = head_dim;
+}
+
 // A piece's rows may be looked at again after they have been written, and other pieces read the same keys.
 static bool prompt_out_overlaps(const ia_prompt_tensors& t, int size) {
   const int64_t hq = (int64_t)t.n_kv_heads * t.group_size;
@@ -692,9 +698,11 @@ int64_t ia_prompt_workspace_bytes(const int32_t* plan_host) {
   return plan_host[2] < 2 ? 0 : (int64_t)plan_host[0] * kPartRows * (plan_host[4] % 1000 + 1) * 4;
 }
 
-int ia_prompt_attention(const ia_prompt_tensors* t, const int32_t* plan_host, const int32_t* plan_device, void* workspace,
+int ia_prompt_attention(const ia_prompt_tensors* tensors, const int32_t* plan_host, const int32_t* plan_device, void* workspace,
                         int64_t workspace_bytes, ia_stream_t stream) {
-  if (!t || !plan_host || !plan_device) return fail(IA_ERR_BAD_ARG, "prompt_attention: null argument");
+  if (!tensors || !plan_host || !plan_device) return fail(IA_ERR_BAD_ARG, "prompt_attention: null argument");
+  ia_prompt_tensors settled = *tensors;
+  ia_prompt_tensors* const t = &settled;
   if (plan_host[4] != t->group_size * 1000 + t->head_dim || plan_host[5] != t->n_kv_heads * 16 + t->dtype)
     return fail(IA_ERR_BAD_ARG, "prompt_attention: the plan was made for other heads or another dtype");
   if (plan_host[6] != t->n_q_tokens || plan_host[7] != t->n_kv_tokens)
@@ -706,6 +714,9 @@ int ia_prompt_attention(const ia_prompt_tensors* t, const int32_t* plan_host, co
   if (!aligned16(t->q) || !aligned16(t->k) || !aligned16(t->v) || !aligned16(t->out))
     return fail(IA_ERR_BAD_ARG, "prompt_attention: tensors must be 16-byte aligned");
   const int size = t->dtype == IA_BF16 ? 2 : 4;
+  settle_strides(t->n_q_tokens, (int64_t)t->n_kv_heads * t->group_size, t->head_dim, &t->q_tok_stride, &t->q_head_stride);
+  settle_strides(t->n_kv_tokens, t->n_kv_heads, t->head_dim, &t->k_tok_stride, &t->k_head_stride);
+  settle_strides(t->n_kv_tokens, t->n_kv_heads, t->head_dim, &t->v_tok_stride, &t->v_head_stride);
   if (!strides_ok(t->q_tok_stride, t->q_head_stride, t->head_dim, size) ||
       (t->n_kv_tokens > 0 && (!strides_ok(t->k_tok_stride, t->k_head_stride, t->head_dim, size) ||
                               !strides_ok(t->v_tok_stride, t->v_head_stride, t->head_dim, size))))
@@ -859,6 +870,8 @@ int ia_pages_write(const ia_page_cache* c, const int32_t* rows, const int32_t* s
   if (!aligned16(k) || !aligned16(v) || !aligned16(k_pool) || !aligned16(v_pool))
     return fail(IA_ERR_BAD_ARG, "pages_write: tensors must be 16-byte aligned");
   const int size = c->dtype == IA_BF16 ? 2 : 4;
+  settle_strides(n_tokens, c->n_kv_heads, c->head_dim, &k_tok_stride, &k_head_stride);
+  settle_strides(n_tokens, c->n_kv_heads, c->head_dim, &v_tok_stride, &v_head_stride);
   if (!strides_ok(k_tok_stride, k_head_stride, c->head_dim, size) || !strides_ok(v_tok_stride, v_head_stride, c->head_dim, size))
     return fail(IA_ERR_BAD_ARG, "pages_write: token and head strides are multiples of 16 bytes and hold a head");
   return launch_pages_write(*c, rows, starts, n,

@@ -190,6 +190,24 @@ def test_prompt_call_refusals(lib, change, word):
         assert b"workspace" in lib.ia_last_error_string()
 
 
+def test_strides_that_nothing_steps_by_are_not_looked_at(lib):
+    """Of one token or one head: torch gives such a dimension any stride.  The call gets past the checks, as far as the next one."""
+    plan = prompt_plan(lib, [1], [1], 2, 4, 64, _lib.IA_BF16)
+    odd = dict(n_q_tokens=1, n_kv_tokens=1, q_tok_stride=1, k_tok_stride=7, v_tok_stride=0)
+    assert lib.ia_prompt_attention(tensors(**odd), ints(plan[:8]), 16, None, 0, None) < 0
+    assert b"overlap" in lib.ia_last_error_string()
+    plan = prompt_plan(lib, [8], [8], 1, 1, 64, _lib.IA_BF16)
+    odd = dict(n_kv_heads=1, group_size=1, q_head_stride=1, k_head_stride=3, v_head_stride=0)
+    assert lib.ia_prompt_attention(tensors(**odd), ints(plan[:8]), 16, None, 0, None) < 0
+    assert b"overlap" in lib.ia_last_error_string()
+    plan = prompt_plan(lib, [8], [8], 1, 4, 64, _lib.IA_BF16)     # one kv head, but four query heads
+    assert lib.ia_prompt_attention(tensors(**{**odd, "group_size": 4}), ints(plan[:8]), 16, None, 0, None) < 0
+    assert b"strides" in lib.ia_last_error_string()
+    for cache, strides, n in ((cache_state(n_kv_heads=1), (1, 64, 128, 64), 4), (cache_state(), (128, 1, 128, 64), 1)):
+        assert lib.ia_pages_write(cache, 16, 16, 1, 16, 16, *strides, n, 16, 16, None) < 0
+        assert b"strides" in lib.ia_last_error_string()
+
+
 def test_packed_arguments_match_the_struct():
     assert len(dense_attention._PROMPT_TENSORS(*range(17))) == struct.calcsize("=5Q6q6i") == ctypes.sizeof(_lib.PromptTensors)
     p = _lib.PromptTensors.from_buffer_copy(dense_attention._PROMPT_TENSORS(*range(17)))
