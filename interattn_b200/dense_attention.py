@@ -44,9 +44,10 @@ def _same_device(device: torch.device, **tensors) -> None:
 
 
 def _host_lens(name: str, lens) -> torch.Tensor:
-    t = torch.as_tensor(lens, dtype=torch.int64, device="cpu")
-    if t.dim() != 1 or (t.numel() and (int(t.min()) < 0 or int(t.max()) > 0x7fffffff)):
-        raise ValueError(f"{name} is a list of lengths, one per sequence, none negative")
+    given = torch.as_tensor(lens, device="cpu")
+    t = given.to(torch.int64)
+    if t.dim() != 1 or not torch.equal(t.to(given.dtype), given) or (t.numel() and (int(t.min()) < 0 or int(t.max()) > 0x7fffffff)):
+        raise ValueError(f"{name} is a list of lengths, whole numbers, one per sequence, none negative")
     return t.to(torch.int32).contiguous()
 
 

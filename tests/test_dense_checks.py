@@ -340,6 +340,19 @@ def test_python_refusals():
                 page_cache.PageCache(**{**good, **change})
 
 
+@pytest.mark.parametrize("lens", [[4.5], [4.0, 2.25], torch.tensor([3.0, float("nan")]), [float("inf")], [[4]], 4, torch.tensor([1 << 31]), [-0.5]])
+def test_lengths_are_whole_numbers(lens):
+    """Nothing is rounded on the way in."""
+    with pytest.raises(ValueError, match="lengths"):
+        dense_attention.PromptAttention(lens, 8, 2, 64)
+    with pytest.raises(ValueError, match="lengths"):
+        dense_attention.PromptAttention([4], 8, 2, 64, kv_lens=lens)
+    assert dense_attention._host_lens("x", []).shape == (0,)
+    for good in ((3, 0), torch.tensor([3, 0], dtype=torch.int16), [3.0, 0.0], torch.tensor([3, 0]).double()):
+        got = dense_attention._host_lens("x", good)
+        assert got.dtype == torch.int32 and got.tolist() == [3, 0]
+
+
 # ---- read from the sources: a GPU test would see the lack of these by hanging ------------------------------------------
 
 def source(name):
