@@ -37,6 +37,17 @@ def device_guard(index: int):
     return _NO_GUARD if index == _current_device() else torch.cuda.device(index)
 
 
+def stream_for(index: int, known: set, *held: torch.Tensor) -> int:
+    """The device's current stream, for kernels that read `held`, which the streams in `known` wait for already: torch's
+    allocator hears of another one, so that memory whose owner is dropped waits for it too."""
+    raw = _raw_stream(index)
+    if raw not in known:
+        for t in held:
+            t.record_stream(torch.cuda.current_stream(index))
+        known.add(raw)
+    return raw
+
+
 def _same_device(device: torch.device, **tensors) -> None:
     for name, t in tensors.items():
         if t is not None and t.device != device:
@@ -63,8 +74,8 @@ class PromptAttention:
     where it is infinite or NaN.
 
     The lengths are host values; the work is cut and spread over the GPU once, here, and the object serves every layer
-    and any number of streams and captured graphs: it holds nothing that a call writes.  Where there are few queries and
-    many keys the keys are cut too, and ``run`` takes a workspace from torch's allocator."""
+    and any number of streams and captured graphs (keep it as long as these): it holds nothing that a call writes.  Where
+    there are few queries and many keys the keys are cut too, and ``run`` takes a workspace from torch's allocator."""
 
     def __init__(self, q_lens: Sequence[int], n_q_heads: int, n_kv_heads: int, head_dim: int, *,
                  kv_lens: Optional[Sequence[int]] = None, dtype: torch.dtype = torch.bfloat16, device="cuda"):
@@ -97,6 +108,7 @@ class PromptAttention:
         self._ws_bytes = int(lib.ia_prompt_workspace_bytes(_ptr(self._host)))
         # run() is called once per layer: what it passes and checks against is made here
         self._call, self._index = lib.ia_prompt_attention, self.device.index
+        self._streams = {_raw_stream(self._index)}
         self._plan_args = (self._host.data_ptr(), self._plan.data_ptr())
         self._sizes = (self.n_q_tokens, self.n_kv_tokens, self.n_kv_heads, group, self.head_dim, _DTYPES[dtype])
         self._q_shape = torch.Size((self.n_q_tokens, self.n_q_heads, self.head_dim))
@@ -133,7 +145,7 @@ class PromptAttention:
         ws = torch.empty((self._ws_bytes,), dtype=torch.uint8, device=self.device) if self._ws_bytes else None
         with device_guard(self._index):
             _lib.check(self._call(tensors, *self._plan_args, 0 if ws is None else ws.data_ptr(), self._ws_bytes,
-                                  _raw_stream(self._index)))
+                                  stream_for(self._index, self._streams, self._plan)))
         return (out, lse) if return_lse else out
 
 
@@ -147,8 +159,8 @@ class SharedPrefixAttention:
     not read and its output is zeros).  ``kv.prefix_lens`` is not used.
 
     ``step`` reads the lengths and tables on the device, allocates its workspace and output from torch's allocator and
-    does not synchronise: it can be captured, and calls on several streams do not meet.  The tensors of ``kv`` and
-    ``shared_lens`` are bound at construction: update them in place."""
+    does not synchronise: it can be captured (keep the object as long as the graph), and calls on several streams do not
+    meet.  The tensors of ``kv`` and ``shared_lens`` are bound at construction: update them in place."""
 
     def __init__(self, kv: PagedKV, group_sizes: Sequence[int], shared_lens: torch.Tensor, n_q_heads: int):
         if n_q_heads <= 0 or n_q_heads % kv.n_kv_heads != 0:
@@ -173,6 +185,7 @@ class SharedPrefixAttention:
             self._plan, self._parts = plan.to(self.device), int(plan[0])
             self._ws_bytes = int(lib.ia_shared_prefix_workspace_bytes(self._parts, ctypes.byref(self.geom)))
         self._call, self._index, self._q_shape = lib.ia_shared_prefix_decode, self.device.index, torch.Size(self._shape)
+        self._streams = {_raw_stream(self._index)}
         self._held = (kv.k_pool, kv.v_pool, kv.block_table, kv.seq_lens)  # kv's fields may be given other tensors
         self._args = (_ptr(kv.k_pool), _ptr(kv.v_pool), _ptr(kv.block_table), _ptr(kv.seq_lens), _ptr(shared_lens),
                       _ptr(self._plan), self._parts, ctypes.byref(self.geom))
@@ -188,7 +201,7 @@ class SharedPrefixAttention:
         ws = torch.empty((self._ws_bytes,), dtype=torch.uint8, device=self.device)
         with device_guard(self._index):
             _lib.check(self._call(q.data_ptr(), *self._args, ws.data_ptr(), self._ws_bytes, out.data_ptr(),
-                                  _raw_stream(self._index)))
+                                  stream_for(self._index, self._streams, self._plan)))
         return out
 
     def _refuse(self, name: str, t: torch.Tensor) -> None:

@@ -20,7 +20,7 @@ from typing import Optional, Sequence, Tuple
 import torch
 
 from . import _lib
-from .dense_attention import _raw_stream, _same_device, device_guard
+from .dense_attention import _raw_stream, _same_device, device_guard, stream_for
 from .ops import PagedKV, _DTYPES, _need_cuda
 
 PAGE = 16
@@ -62,8 +62,9 @@ class PageCache:
         size = int(_lib.load().ia_pages_scratch_bytes(int(block_table.shape[0]), int(k.shape[0])))
         if size < 0:
             _lib.check(_lib.IA_ERR_BAD_ARG)
-        self._addresses = torch.tensor([p.data_ptr() for p in flat], dtype=torch.int64, device=self.device)
+        # the copy of the addresses waits for its stream, so the scratch too is ready for any other
         self._scratch = torch.zeros((size + 256,), dtype=torch.uint8, device=self.device)
+        self._addresses = torch.tensor([p.data_ptr() for p in flat], dtype=torch.int64, device=self.device)
         scratch = self._scratch.data_ptr()
         self._state = _lib.PageCacheState(
             block_table=block_table.data_ptr(), seq_lens=seq_lens.data_ptr(), refs=refs.data_ptr(),
@@ -73,6 +74,7 @@ class PageCache:
             head_dim=int(k.shape[3]), dtype=_DTYPES[k.dtype], reserved=0)
         self._held = (flat, block_table, seq_lens, refs)  # the attributes may be given other tensors
         self._c, self._index = ctypes.byref(self._state), self.device.index
+        self._streams = {_raw_stream(self._index)}
         self._lib = _lib.load()
         self._token_shape, self._dtype = (int(k.shape[1]), int(k.shape[3])), k.dtype
         self._pool_addresses = [(a.data_ptr(), b.data_ptr()) for a, b in self.pools]
@@ -104,7 +106,7 @@ class PageCache:
 
     def _call(self, function, *args) -> None:
         with device_guard(self._index):
-            _lib.check(function(self._c, *args, _raw_stream(self._index)))
+            _lib.check(function(self._c, *args, stream_for(self._index, self._streams, self._scratch, self._addresses)))
 
     def extend(self, rows: torch.Tensor, n_tokens: torch.Tensor) -> None:
         """``rows[i]`` becomes ``n_tokens[i]`` tokens longer and gets the pages for them."""
