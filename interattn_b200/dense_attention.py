@@ -115,7 +115,8 @@ class PromptAttention:
         self._kv_shape = torch.Size((self.n_kv_tokens, self.n_kv_heads, self.head_dim))
 
     def _fits(self, t: torch.Tensor, shape: torch.Size) -> bool:
-        return t.shape == shape and t.dtype is self.dtype and t.get_device() == self._index and t.stride(2) == 1
+        return t.shape == shape and t.dtype is self.dtype and t.get_device() == self._index \
+            and (t.stride(2) == 1 or t.numel() == 0)
 
     def _refuse(self, name: str, t: torch.Tensor, shape: torch.Size) -> None:
         _need_cuda(t)

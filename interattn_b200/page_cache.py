@@ -121,7 +121,7 @@ class PageCache:
         shape, ks, vs = k.shape, k.stride(), v.stride()
         if shape != v.shape:
             raise ValueError("k and v hold the same tokens")
-        if len(shape) != 3 or (shape[1], shape[2]) != self._token_shape or ks[2] != 1 or vs[2] != 1 \
+        if len(shape) != 3 or (shape[1], shape[2]) != self._token_shape or ((ks[2] != 1 or vs[2] != 1) and shape[0] != 0) \
                 or k.dtype is not self._dtype or v.dtype is not self._dtype or k.get_device() != self._index \
                 or v.get_device() != self._index:
             for name, t in (("k", k), ("v", v)):
