@@ -1080,13 +1080,16 @@ typedef CUresult (*EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void
                              const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion,
                              CUtensorMapFloatOOBfill);
 EncodeFn encoder() {
-  static EncodeFn fn = nullptr;  // every thread would store the same pointer
+  static std::atomic<EncodeFn> known{nullptr};  // any thread may be the first; all would store the same pointer
+  EncodeFn fn = known.load(std::memory_order_relaxed);
   if (fn == nullptr) {
     void* sym = nullptr;
     cudaDriverEntryPointQueryResult found;
     if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &sym, cudaEnableDefault, &found) == cudaSuccess &&
-        found == cudaDriverEntryPointSuccess)
+        found == cudaDriverEntryPointSuccess) {
       fn = reinterpret_cast<EncodeFn>(sym);
+      known.store(fn, std::memory_order_relaxed);
+    }
   }
   return fn;
 }

@@ -25,7 +25,7 @@ from typing import Optional, Sequence
 import torch
 
 from . import _lib
-from .ops import PagedKV, _DTYPES, _need_cuda, _ptr, _q_geom
+from .ops import PagedKV, _DTYPES, _need_cuda, _ptr
 
 
 _raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
