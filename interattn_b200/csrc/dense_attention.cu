@@ -461,7 +461,7 @@ template <int D> struct Merged {
 #pragma unroll 8
       for (int s = 0; s < count; ++s) add_row(src, w, s, false);
     } else {  // apart: the usual case keeps its short loop
-#pragma unroll 4
+#pragma unroll 1
       for (int s = 0; s < count; ++s) add_row(src, w, s, none >> s & 1);
     }
   }

@@ -37,15 +37,12 @@ def device_guard(index: int):
     return _NO_GUARD if index == _current_device() else torch.cuda.device(index)
 
 
-def stream_for(index: int, known: set, *held: torch.Tensor) -> int:
-    """The device's current stream, for kernels that read `held`, which the streams in `known` wait for already: torch's
-    allocator hears of another one, so that memory whose owner is dropped waits for it too."""
-    raw = _raw_stream(index)
-    if raw not in known:
-        for t in held:
-            t.record_stream(torch.cuda.current_stream(index))
-        known.add(raw)
-    return raw
+def wait_for(stream: int, known: set, index: int, *held: torch.Tensor) -> None:
+    """torch's allocator hears of a stream, the device's current one, whose kernels read `held`: memory whose owner is dropped waits
+    for it too, as it does for those in `known`."""
+    for t in held:
+        t.record_stream(torch.cuda.current_stream(index))
+    known.add(stream)
 
 
 def _same_device(device: torch.device, **tensors) -> None:
@@ -144,9 +141,11 @@ class PromptAttention:
         tensors = _PROMPT_TENSORS(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(),
                                   qt, qh, kt, kh, vt, vh, *self._sizes)
         ws = torch.empty((self._ws_bytes,), dtype=torch.uint8, device=self.device) if self._ws_bytes else None
+        stream = _raw_stream(self._index)
+        if stream not in self._streams:
+            wait_for(stream, self._streams, self._index, self._plan)
         with device_guard(self._index):
-            _lib.check(self._call(tensors, *self._plan_args, 0 if ws is None else ws.data_ptr(), self._ws_bytes,
-                                  stream_for(self._index, self._streams, self._plan)))
+            _lib.check(self._call(tensors, *self._plan_args, 0 if ws is None else ws.data_ptr(), self._ws_bytes, stream))
         return (out, lse) if return_lse else out
 
 
@@ -200,9 +199,11 @@ class SharedPrefixAttention:
         elif out.shape != self._q_shape or out.dtype is not self._dtype or out.get_device() != self._index or not out.is_contiguous():
             self._refuse("out", out)
         ws = torch.empty((self._ws_bytes,), dtype=torch.uint8, device=self.device)
+        stream = _raw_stream(self._index)
+        if stream not in self._streams:
+            wait_for(stream, self._streams, self._index, self._plan)
         with device_guard(self._index):
-            _lib.check(self._call(q.data_ptr(), *self._args, ws.data_ptr(), self._ws_bytes, out.data_ptr(),
-                                  stream_for(self._index, self._streams, self._plan)))
+            _lib.check(self._call(q.data_ptr(), *self._args, ws.data_ptr(), self._ws_bytes, out.data_ptr(), stream))
         return out
 
     def _refuse(self, name: str, t: torch.Tensor) -> None:

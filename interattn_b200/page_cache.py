@@ -20,7 +20,7 @@ from typing import Optional, Sequence, Tuple
 import torch
 
 from . import _lib
-from .dense_attention import _raw_stream, _same_device, device_guard, stream_for
+from .dense_attention import _raw_stream, _same_device, device_guard, wait_for
 from .ops import PagedKV, _DTYPES, _need_cuda
 
 PAGE = 16
@@ -105,8 +105,11 @@ class PageCache:
         return t.data_ptr()
 
     def _call(self, function, *args) -> None:
+        stream = _raw_stream(self._index)
+        if stream not in self._streams:
+            wait_for(stream, self._streams, self._index, self._scratch, self._addresses)
         with device_guard(self._index):
-            _lib.check(function(self._c, *args, stream_for(self._index, self._streams, self._scratch, self._addresses)))
+            _lib.check(function(self._c, *args, stream))
 
     def extend(self, rows: torch.Tensor, n_tokens: torch.Tensor) -> None:
         """``rows[i]`` becomes ``n_tokens[i]`` tokens longer and gets the pages for them."""
