@@ -6,8 +6,8 @@
 // registers through shared memory into the second product, the accumulator is rescaled by exp(m_old - m_new) when the
 // maximum moves.  All of it in fp32.  A thread owns RPT rows x 4 keys of the logits and RPT rows x D / 16 output columns;
 // 16 neighbouring lanes share a row, so the row's statistics are four shuffles.  Rows of 132 floats keep the key reads of
-// 8 lanes on 32 banks.  A 4096-token prompt at 32 / 8 heads of 128: 39 TFLOP/s, bound by the FMA pipe and its operands from
-// shared memory.  Decode steps of up to kFewRows rows are bound by reading the cache and have a form of their own.
+// 8 lanes on 32 banks.  A 4096-token prompt at 32 / 8 heads of 128: 38 TFLOP/s, bound by latency: two warps a scheduler, which wait
+// for operands from shared memory, with the FMA pipe busy for 57 % of the cycles and shared memory for 49 %.  Decode steps of up to kFewRows rows are bound by reading the cache and have a form of their own.
 #include <algorithm>
 #include <atomic>
 #include <cstring>
@@ -866,7 +866,8 @@ void make_shared_plan(const int32_t* group_sizes, int n_groups, int batch, int g
   // A unit of many rows takes several times as long as one of few, and shares are equal in units: where there are entities
   // of many rows, those of few get longer units.  16 groups of 8 / 16 / 32 sequences of 4 rows over 4000 keys with 1 to 256
   // own ones: 0.59 / 0.74 / 1.47 ms, with 64 keys throughout 0.62 / 0.95 / 2.14 ms.  Without such entities 64 keys
-  // spread a short step over the most SMs.
+  // spread a short step over the most SMs.  The tensor-core kernel's unit is its key tile whatever the rows, so there shares are not
+  // equal in time where entities of two row tiles stand beside own parts (64 sequences of 8 rows over 128k keys).
   bool wide = false;
   for (int g = 0; g < n_groups; ++g) wide |= std::min(per, group_sizes[g]) * group > kFewRows;
   const auto entity = [&](int first, int n, int group_first, int group_n, int g) {

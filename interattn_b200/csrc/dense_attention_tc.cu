@@ -24,9 +24,10 @@
 // holds a warp until the tensor core takes the instruction, so what one decides and waits for between them is hidden behind
 // the other's.  Tensor memory: S_0, S_1, O_0, O_1 of 128 columns each.
 //
-// Measured at the Llama-3-8B heads: one 32k prompt 7.6 ms as a burst (1.16 PFLOP/s, 0.69 of the measured GEMM peak; 9.0 ms when the
-// power cap holds the clock), bound by a tile's chain of products and exponentials; a decode step of 64 sequences in eight
-// groups, 955 MB, 227 us in this kernel (0.65 of the copy peak), a key tile taking 1.6 us an SM once the ring runs.
+// Measured at the Llama-3-8B heads, in a queue of passes: one 32k prompt 9.0 ms (0.97 PFLOP/s, 0.57 of the measured GEMM peak as a burst
+// and 0.69 of the sustained one; the power cap holds the clock), one of 8k 0.57 ms, bound by a tile's chain of products and
+// exponentials; a decode step of 64 sequences in eight groups, 955 MB, 234 us in this kernel (0.63 of the copy peak), a key
+// tile taking 1.6 us an SM once the ring runs.
 #include <type_traits>
 
 #include <cuda.h>  // CUtensorMap (types only; the encoder is fetched through the runtime)
