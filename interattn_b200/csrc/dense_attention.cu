@@ -202,7 +202,6 @@ __device__ void attend(float* sm, int n_rows, int lo, int hi, float scale_log2, 
     exact_row<float, D, 2>(q_row(row), lo, lim[row], scale_log2, key, x, mx, lx);
 #pragma unroll
     for (int i = 0; i < D / 32; ++i) sink.row(row)[(tid & 31) + 32 * i] = x[i] / lx;
-    if ((tid & 31) == 0 && sink.lse(row) != nullptr) *sink.lse(row) = (mx + log2f(lx)) * kLn2;
   }
 }
 

@@ -238,7 +238,8 @@ template <int N> __device__ __forceinline__ void unpack16(const uint4& w, float 
 }
 // softmax(q . k_j * scale) v_j over [lo, hi) by a whole warp: a lane takes every 32nd key's logit, then the dims l, l + 32, ... of the
 // values.  Bound by the latency of its loads: kAhead of them are on their way together, as many as the kernel has registers for.  A
-// row whose every dim is NaN stays so: it ends there.
+// row whose every dim is NaN stays so: it ends there, with m and l of the keys so far.  (The log-sum-exp needs no second look:
+// what a row does not see never got into its logits.)
 template <typename T, int D, int kAhead, typename Key>
 __device__ __forceinline__ void exact_row(const T* q, int lo, int hi, float scale_log2, const Key& key, float (&o)[D / 32], float& m,
                           float& l) {

@@ -108,3 +108,19 @@ def test_cut_keys_with_a_bad_value_in_every_part(dtype):
     assert torch.equal(bad, want[:, None].expand_as(bad)) and ops.device_status() == 0
     ref.out[bad], ref.mean_abs[bad] = 0, 0
     ref.check(torch.where(bad.cuda(), 0, out[:60]), dtype)
+
+
+@pytest.mark.parametrize("dtype,d", [(BF16, 128), (BF16, 64), (F32, 64), (F32, 128)])
+@pytest.mark.parametrize("q_lens,kv_lens", [([160], [160]), ([20], [9000]), ([900, 30], [900, 200])])
+def test_log_sum_exps_do_not_depend_on_the_values(dtype, d, q_lens, kv_lens):
+    """Rows that are NaN throughout, beside a bad value that they do not see: done again or not, their log-sum-exps are the keys'."""
+    q, k, v = on_gpu((sum(q_lens), 4, d), dtype, 10), on_gpu((sum(kv_lens), 2, d), dtype, 11), on_gpu((sum(kv_lens), 2, d), dtype, 12)
+    plan = dense_attention.PromptAttention(q_lens, 4, 2, d, kv_lens=kv_lens, dtype=dtype)
+    n, m = q_lens[0], kv_lens[0]
+    v[10], v[m - 1] = float("nan"), float("inf")
+    out, lse = plan.run(q, k, v, return_lse=True)
+    ref = rows_reference(q[:n], k[:m], v[:m].nan_to_num(0, 0, 0), list(range(n)), [m - n + r + 1 for r in range(n)])
+    ref.check_lse(lse[:n])
+    sees = torch.tensor([m - n + r + 1 > 10 for r in range(n)], device="cuda")
+    assert bool(torch.isnan(out[:n][sees].float()).all()) and bool(torch.isfinite(out[:n][~sees].float()).all())
+    assert bool(torch.isfinite(lse).all()) and ops.device_status() == 0
