@@ -100,7 +100,7 @@ def test_write_after_extend_met_the_table_s_end(n_pages, length):
 @pytest.mark.parametrize("n_pages", SIZES)
 def test_write_after_extend_was_refused_behind_another(n_pages):
     """A row that wants no page itself is refused with those behind the first that does not fit; bad rows and second mentions are not
-    what a row's own entry is judged by."""
+    what decides about a row's own entry."""
     cache = make(n_pages, 6, 8, taken=n_pages - 4)
     cache.extend(i32([0, 1, 2]), i32([16, 20, 5]))
     want = copies(cache)
